@@ -732,6 +732,192 @@ int mlxrocm_switch_glu(
     size_t workspace_bytes,
     mlxrocm_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Attention, its paged cache, and drafted tokens                            */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * What stands between a layer's projections when a model is served or tuned (the reference
+ * computes it with fast::ScaledDotProductAttention, mlx/fast.cpp, and leaves caches and drafts
+ * to its callers).
+ *
+ * A sequence has `length` tokens, of which the last Lq are the queries; the token at position p
+ * sees the tokens j with
+ *     0 <= j <= p   and   (p - j < window  or  j < keep)
+ * (a window that is no shorter than the sequence: plain causal attention).  Queries at
+ * negative positions -- a sequence with fewer than Lq tokens, padded in front -- see nothing and
+ * give zeros.  Hq query heads share Hkv key heads, Hq / Hkv in a row each.  D: a multiple of 8 up
+ * to 256.  Scores, sums and results are formed in 32 bits; with 16-bit types the probabilities are
+ * rounded to the type for their product with v.  What a row does not see does not reach it,
+ * whatever it holds (infinities and NaN too).
+ *
+ * lengths: [B] on the device, clamped to 0 .. most keys.  strides: host array, in elements, three
+ * for each operand in the order [sequence, head, token] (the last dimension is dense); operands
+ * and strides are aligned to 16 bytes, else MLXROCM_UNSUPPORTED.  workspace: device scratch used
+ * only during the call, 16-byte aligned, of _workspace_size bytes (0: it may be NULL).
+ *
+ * mlxrocm_window_attention: q [B, Hq, Lq, D], k and v [B, Hkv, Lk, D], out as q.  lengths may be
+ * NULL (Lk each).  strides: of q, k, v, out.  lse: NULL, or [B, Hq, Lq] floats that the gradients
+ * need.
+ * mlxrocm_window_attention_vjp: the gradients dq, dk, dv of q, k, v from dout, that of out.
+ * strides: of q, k, v, out, dout, dq, dk, dv.  Sums are taken in a fixed order.
+ */
+size_t mlxrocm_window_attention_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype);
+int mlxrocm_window_attention(
+    const void* q,
+    const void* k,
+    const void* v,
+    void* out,
+    float* lse,
+    const int32_t* lengths,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+size_t mlxrocm_window_attention_vjp_workspace_size(int B, int Hq, int Lq);
+int mlxrocm_window_attention_vjp(
+    const void* q,
+    const void* k,
+    const void* v,
+    const void* out,
+    const float* lse,
+    const void* dout,
+    void* dq,
+    void* dk,
+    void* dv,
+    const int32_t* lengths,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+
+/*
+ * The same over a cache of pages: k_pages and v_pages [pages, Hkv, page_size, D], key j of
+ * sequence b in row j % page_size of page table[b][j / page_size].  page_size: a multiple of 16.
+ * table: [B, table_width] on the device, its entries clamped to pages that exist; the keys of a
+ * sequence are bounded by table_width * page_size (max_keys of the workspace size).  strides:
+ * of q [sequence, head, token], k_pages and v_pages [page, head, row], out, and of a row of table
+ * (13 in all).
+ * mlxrocm_paged_cache_update: k and v [B, Hkv, L, D] into those pages, as the last L of each
+ * sequence's lengths[b] tokens; what lies before position 0, or on a page that does not exist, is
+ * left out.  strides: of k, v, k_pages, v_pages and of a row of table.
+ */
+size_t mlxrocm_paged_attention_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int D, int max_keys, int window, int keep, int dtype);
+int mlxrocm_paged_attention(
+    const void* q,
+    const void* k_pages,
+    const void* v_pages,
+    const int32_t* table,
+    const int32_t* lengths,
+    void* out,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int D,
+    int pages,
+    int page_size,
+    int table_width,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+int mlxrocm_paged_cache_update(
+    const void* k,
+    const void* v,
+    void* k_pages,
+    void* v_pages,
+    const int32_t* table,
+    const int32_t* lengths,
+    int B,
+    int Hkv,
+    int L,
+    int D,
+    int pages,
+    int page_size,
+    int table_width,
+    const int64_t* strides,
+    int dtype,
+    mlxrocm_stream_t stream);
+
+/*
+ * The launches that either attention makes of a shape (keys: Lk, or table_width * page_size),
+ * written to plan without touching a device, as mlxrocm_qmm_plan does.
+ */
+int mlxrocm_attention_plan(
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int keys,
+    int D,
+    int window,
+    int keep,
+    int dtype,
+    char* plan,
+    size_t plan_bytes);
+
+/*
+ * Verification of drafted tokens.  Draft i of a sequence is taken while
+ *     accept[i] * probs[i][draft[i]] < target[i][draft[i]]
+ * (the product exact; probs NULL: drafts are certain, 1).  At the first, n, that is not, a token
+ * is drawn from max(target[n] - probs[n], 0) -- without probs from target[n] less the draft
+ * itself; from target[n] if that is zero throughout -- and from target[n] if all were taken.
+ * The draw is by whole numbers, so it does not depend on the order of any sum: weight w counts
+ * c = floor(min(w, 1) 2^40), and with N their total the token is the first whose running sum
+ * exceeds min(floor(sample * N), N - 1).  A row without any weight gives -1.
+ *
+ * draft [B, K], target [B, K + 1, V] and probs [B, K, V] of dtype with strides {target sequence,
+ * target row, probs sequence, probs row} in elements (host array), accept [B, K], sample [B] in
+ * [0, 1), lengths [B] (drafts of each sequence, clamped to 0 .. K) or NULL.
+ * tokens [B, K + 1]: the drafts that were taken, the token drawn, then -1; accepted [B]: n.
+ * A draft that is no token of the vocabulary is not taken.  V: up to 2^22.
+ */
+size_t mlxrocm_verify_draft_workspace_size(int B, int V);
+int mlxrocm_verify_draft(
+    const int32_t* draft,
+    const void* target,
+    const void* probs,
+    const float* accept,
+    const float* sample,
+    const int32_t* lengths,
+    int32_t* tokens,
+    int32_t* accepted,
+    int B,
+    int K,
+    int V,
+    const int64_t* strides,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+
 /*
  * Gated-MLP decode: out = silu(x @ dequant(w_gate).T) * (x @ dequant(w_up).T),
  * both projections in one launch over the shared x, then one elementwise pass.

@@ -23,6 +23,7 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _p = ctypes.c_void_p
+_f = ctypes.c_float
 
 # name -> (restype, argtypes); the list the symbol-export test walks.
 SIGNATURES = {
@@ -53,6 +54,19 @@ SIGNATURES = {
         _i,
         [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _i, _i, _p],
     ),
+    "mlxrocm_window_attention_workspace_size": (_sz, [_i] * 9),
+    "mlxrocm_window_attention": (_i, [_p] * 6 + [_i] * 6 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
+    "mlxrocm_window_attention_vjp_workspace_size": (_sz, [_i] * 3),
+    "mlxrocm_window_attention_vjp": (
+        _i,
+        [_p] * 10 + [_i] * 6 + [_p, _f] + [_i] * 3 + [_p, _sz, _p],
+    ),
+    "mlxrocm_paged_attention_workspace_size": (_sz, [_i] * 9),
+    "mlxrocm_paged_attention": (_i, [_p] * 6 + [_i] * 8 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
+    "mlxrocm_paged_cache_update": (_i, [_p] * 6 + [_i] * 7 + [_p, _i, _p]),
+    "mlxrocm_attention_plan": (_i, [_i] * 9 + [ctypes.c_char_p, _sz]),
+    "mlxrocm_verify_draft_workspace_size": (_sz, [_i] * 2),
+    "mlxrocm_verify_draft": (_i, [_p] * 8 + [_i] * 3 + [_p, _i, _p, _sz, _p]),
     "mlxrocm_switch_glu_workspace_size": (_sz, [_i] * 8),
     "mlxrocm_switch_glu": (_i, [_p] * 2 + [_i] + [_p] * 10 + [_i] * 8 + [_p, _sz, _p]),
     "mlxrocm_qmm_swiglu_workspace_size": (_sz, [_i, _i, _i]),
@@ -224,6 +238,14 @@ def gather_qmm_plan(M, N, K, n_indices, x_batches, n_experts, group_size=64, bit
     buf = ctypes.create_string_buffer(1024)
     rc = lib.mlxrocm_gather_qmm_plan(M, N, K, n_indices, x_batches, n_experts, group_size, bits,
                                      dtype, int(transpose), workspace_bytes, buf, len(buf))
+    return rc, buf.value.decode()
+
+
+def attention_plan(B, Hq, Hkv, Lq, keys, D, window=1 << 30, keep=0, dtype=BFLOAT16):
+    """(status, plan) of window_attention or paged_attention: the kernels a call would launch,
+    e.g. "attention_few(dim=128,rows=16,splits=2)+attention_join"."""
+    buf = ctypes.create_string_buffer(512)
+    rc = load().mlxrocm_attention_plan(B, Hq, Hkv, Lq, keys, D, window, keep, dtype, buf, len(buf))
     return rc, buf.value.decode()
 
 

@@ -1,0 +1,427 @@
+// attention.h -- what the attention kernels share: their arguments, which keys a
+// query sees, where the rows of keys, values and queries lie, fragments of the
+// matrix instructions and tiles in LDS.
+//
+// For one sequence and one key head the G query heads that share it and the Lq new
+// tokens are taken together as R = G Lq rows: row r is token i = r / G of query head
+// hk G + r % G, at position p = length - Lq + i of the sequence.  It sees key j where
+//   0 <= j <= p  and  (p - j < window or j < keep),
+// nothing if p < 0 (padding in front of a short sequence).  Every key that is read is
+// so read once for all heads that share it, and the sums over those heads that the
+// gradients of keys and values need are sums over rows.
+//
+// Every product is formed with the queries (forward, dq) or the keys (dk, dv) as the
+// columns of the matrix instruction's result: a lane then holds one column, so running
+// maxima, sums and rescaling are plain per-lane arithmetic, and the probabilities are
+// where the next product wants its second operand: a result has in register i of lane l
+// (32x32) row 8 (i / 4) + 4 (l / 32) + i % 4 of column l % 32, and an operand has 8
+// values along the contraction.  The order in which a sum over keys is taken is free, so
+// registers 8 q .. 8 q + 7 of a lane serve as those 8 values without moving: they stand
+// for keys 16 q + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}, h = l / 32, and the other
+// operand is read from LDS in that order.
+#pragma once
+
+#include "mfma_dequant.h"
+#include "mfma_loads.h"
+
+namespace mlxrocm {
+
+struct AttentionArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse; // [B, Hq, Lq]: log2 of the sum of exp(score), for the gradients; may be null
+  const int* lengths; // [B], or null: every sequence has `keys`
+  const int* table;   // [B, table_stride], or null: contiguous keys
+  int64_t table_stride;
+  int B, Hq, Hkv, G, Lq, D;
+  int keys;      // most keys a sequence can have
+  int page;      // rows of a page (table), and what divides by it
+  uint32_t page_magic;
+  int pages;
+  // strides in elements; of k and v: [sequence or page, head, row]
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3]; // [sequence, head, token]
+  float scale_log2; // |scale| log2(e)
+  uint32_t q_sign;  // 0x80008000 (16-bit types), 0x80000000 (float32) where scale < 0
+  int window, keep;
+  int splits;
+  float* part_out; // [splits, B Hkv, R, D], not yet divided by the sums
+  float2* part_ml; // [splits, B Hkv, R]: maximum (log2 units) and sum
+};
+
+// The gradients' further operands.
+struct AttentionGradArgs {
+  AttentionArgs a; // out: the forward's result, lse: its sums
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* delta; // [B, Hq, Lq]: sum over D of dout * out
+  int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+  float scale;
+};
+
+// Whether the few-rows kernel takes a call (else the tiles of 128 rows).
+constexpr int kFewRows = 64;
+
+// One unit for each type: by the dtype of a call
+int launch_attention_few_f32(const AttentionArgs& a, hipStream_t s);
+int launch_attention_few_f16(const AttentionArgs& a, hipStream_t s);
+int launch_attention_few_bf16(const AttentionArgs& a, hipStream_t s);
+int launch_attention_rows_f32(const AttentionArgs& a, hipStream_t s);
+int launch_attention_rows_f16(const AttentionArgs& a, hipStream_t s);
+int launch_attention_rows_bf16(const AttentionArgs& a, hipStream_t s);
+int launch_attention_join(const AttentionArgs& a, int dtype, hipStream_t s);
+int launch_attention_grad_f32(const AttentionGradArgs& g, hipStream_t s);
+int launch_attention_grad_f16(const AttentionGradArgs& g, hipStream_t s);
+int launch_attention_grad_bf16(const AttentionGradArgs& g, hipStream_t s);
+
+#ifdef __HIPCC__
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+// 8 consecutive values along a contraction, as one lane of an operand holds them.
+template <typename T>
+struct Frag {
+  uint32_t w[4];
+};
+template <>
+struct Frag<float> {
+  float w[8];
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 frag_bits(const Frag<T>& f) {
+  return make_uint4(f.w[0], f.w[1], f.w[2], f.w[3]);
+}
+
+// c + a b over 16 values of the contraction (8 in each half of the wave): one
+// instruction for the 16-bit types; float32 takes eight of two values each.
+template <typename T>
+__device__ __forceinline__ floatx16 mma32(const Frag<T>& a, const Frag<T>& b, floatx16 c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w[j], b.w[j], c, 0, 0, 0);
+    }
+    return c;
+  } else if constexpr (std::is_same<T, bf16_t>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// The same for 16 x 16 results over 32 values of the contraction.
+template <typename T>
+__device__ __forceinline__ floatx4 mma16(const Frag<T>& a, const Frag<T>& b, floatx4 c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.w[j], b.w[j], c, 0, 0, 0);
+    }
+    return c;
+  } else {
+    return mfma16<T>(frag_bits<T>(a), frag_bits<T>(b), c);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> zero_frag() {
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(f.w) / 4); ++i) {
+    f.w[i] = 0;
+  }
+  return f;
+}
+
+// 8 consecutive elements of memory (16-byte aligned)
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* p) {
+  Frag<T> f;
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 4) {
+    const uint4 b = *reinterpret_cast<const uint4*>(p + 4);
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f.w[i] = __uint_as_float(u[i]);
+    }
+  } else {
+    f.w[0] = a.x;
+    f.w[1] = a.y;
+    f.w[2] = a.z;
+    f.w[3] = a.w;
+  }
+  return f;
+}
+
+// Negated where scale < 0 (exact), so that maxima are taken of what is exponentiated.
+template <typename T>
+__device__ __forceinline__ void flip(Frag<T>& f, uint32_t sign) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(f.w) / 4); ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f.w[i] = __uint_as_float(__float_as_uint(f.w[i]) ^ sign);
+    } else {
+      f.w[i] ^= sign;
+    }
+  }
+}
+
+// Probabilities (or their gradients) as an operand.  For the 16-bit types this is where
+// they are rounded to the type of the values they multiply: the matrix instruction takes
+// both operands in one type, and a probability's relative error of 2^-9 (2^-12) is that of
+// the value beside it.  Sums of probabilities are taken before it, in 32 bits.
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_of(const float* p) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f.w[i] = p[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f.w[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+    }
+  }
+  return f;
+}
+
+// 4 values to consecutive elements (aligned to all of them)
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const floatx4& v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  }
+}
+
+__device__ __forceinline__ bool not_finite(float v) {
+  return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+}
+
+// The fragment with zeros for infinities and NaN.
+template <typename T>
+__device__ __forceinline__ void drop_not_finite(Frag<T>& f) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(f.w) / 4); ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f.w[i] = not_finite(f.w[i]) ? 0.0f : f.w[i];
+    } else {
+      constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+      uint32_t w = f.w[i];
+      w = (w & kExp) == kExp ? w & 0xffff0000u : w;
+      w = (w & (kExp << 16)) == (kExp << 16) ? w & 0xffffu : w;
+      f.w[i] = w;
+    }
+  }
+}
+
+// This lane's value and that of lane ^ 32, in either order.
+__device__ __forceinline__ float2 both_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_halves(float v) {
+  const float2 r = both_halves(v);
+  return fmaxf(r.x, r.y);
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const float2 r = both_halves(v);
+  return r.x + r.y;
+}
+
+// ---- which keys ----------------------------------------------------------------
+// The rows of one tile of rows that see anything are first .. last; the keys they see lie
+// in [0, a_end) (the ones that are kept) and [w_begin, w_end), cut into tiles of KT keys.
+struct KeyRange {
+  int a_end, w_begin, w_end;
+  int a_tiles, tiles;
+};
+
+__device__ __forceinline__ KeyRange
+keys_of(const AttentionArgs& a, int length, int first_row, int last_row, int kt) {
+  const int p_lo = length - a.Lq + first_row / a.G;
+  const int p_hi = length - a.Lq + last_row / a.G;
+  KeyRange r;
+  r.w_end = p_hi + 1;
+  r.w_begin = max(0, p_lo - a.window + 1);
+  r.a_end = min(a.keep, p_hi + 1);
+  if (r.a_end >= r.w_begin) { // one range
+    r.a_end = 0;
+    r.w_begin = 0;
+  }
+  r.a_tiles = (r.a_end + kt - 1) / kt;
+  r.tiles = r.a_tiles + (r.w_end - r.w_begin + kt - 1) / kt;
+  return r;
+}
+
+// Keys [begin, end) of tile t; end - begin <= kt
+__device__ __forceinline__ void tile_of(const KeyRange& r, int t, int kt, int* begin, int* end) {
+  const bool a = t < r.a_tiles;
+  *begin = a ? t * kt : r.w_begin + (t - r.a_tiles) * kt;
+  *end = min(*begin + kt, a ? r.a_end : r.w_end);
+}
+
+// Whether a tile's keys [begin, end) are all seen by, or all hidden from, positions lo .. hi
+__device__ __forceinline__ bool all_seen(
+    int begin, int end, int lo, int hi, int window, int keep) {
+  return end - 1 <= lo && (hi - begin < window || end <= keep);
+}
+__device__ __forceinline__ bool none_seen(
+    int begin, int end, int lo, int hi, int window, int keep) {
+  return begin > hi || (lo - (end - 1) >= window && begin >= keep);
+}
+
+// Divides by the page size: page_magic = 2^32 / page + 1 overshoots by one at most.
+__device__ __forceinline__ int page_of(const AttentionArgs& a, int j, int* in_page) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(j), a.page_magic));
+  int r = j - q * a.page;
+  if (r < 0) {
+    --q;
+    r += a.page;
+  }
+  *in_page = r;
+  return q;
+}
+
+// Offsets of key j's row in k and in v: through the page table, whose entries are clamped to
+// pages that exist, or along contiguous keys.
+struct KeyRow {
+  int64_t k, v;
+};
+template <bool PAGED>
+__device__ __forceinline__ KeyRow key_row(const AttentionArgs& a, int b, int hk, int j) {
+  int64_t first = b;
+  int at = j;
+  if constexpr (PAGED) {
+    int in_page;
+    const int page = page_of(a, j, &in_page);
+    const int id = a.table[b * a.table_stride + page];
+    first = min(max(id, 0), a.pages - 1);
+    at = in_page;
+  }
+  KeyRow r;
+  r.k = first * a.k_strides[0] + hk * a.k_strides[1] + at * a.k_strides[2];
+  r.v = first * a.v_strides[0] + hk * a.v_strides[1] + at * a.v_strides[2];
+  return r;
+}
+
+// Length of a sequence, within the keys that it can have
+__device__ __forceinline__ int length_of(const AttentionArgs& a, int b) {
+  return a.lengths == nullptr ? a.keys : min(max(a.lengths[b], 0), a.keys);
+}
+
+// Offset of row r's token in a [sequence, head, token] tensor
+__device__ __forceinline__ int64_t row_offset(
+    const int64_t (&strides)[3], int b, int hk, int G, int r) {
+  const int i = r / G;
+  return b * strides[0] + (hk * G + (r - i * G)) * strides[1] + i * strides[2];
+}
+
+// Which (sequence, key head) and which of its `per` pieces a workgroup has.  Workgroups go
+// to the 8 dies in turn, and each die has an L2 of its own: eight heads side by side, one
+// on each die, so that all that read a head's keys find them in one L2.
+__device__ __forceinline__ void piece_of(int heads, int per, int* head, int* piece) {
+  const int block = blockIdx.x;
+  const int group = block / (8 * per);
+  const int rest = block - group * 8 * per;
+  const int width = min(8, heads - group * 8);
+  *head = group * 8 + rest % width;
+  *piece = rest / width;
+}
+
+// ---- tiles in LDS -----------------------------------------------------------------
+// `rows` rows of DT elements in 16-byte units, unit u of row r at place u ^ swizzle(r) of the
+// row: eight rows read at one column (load_rows) fall into eight different places, and four
+// rows read 32 bytes wide (load_cols) too.  DT = 96 of 16 bits has 12 units, which no
+// exclusive or permutes; its rows lie 48 banks apart as they are.
+template <typename T, int DT>
+struct Tile {
+  static constexpr int kUnit = 16 / sizeof(T);
+  static constexpr int kUnits = DT / kUnit;
+
+  static __device__ __forceinline__ int swizzle(int row) {
+    return kUnits % 8 == 0 ? ((row & 3) << 1 | (row >> 2 & 1)) : 0;
+  }
+  static __device__ __forceinline__ int at(int row, int unit) {
+    return row * DT + (unit ^ swizzle(row)) * kUnit;
+  }
+  // elements 8 chunk .. 8 chunk + 7 of a row
+  static __device__ __forceinline__ Frag<T> load_rows(const T* tile, int row, int chunk) {
+    if constexpr (sizeof(T) == 4) {
+      Frag<T> f;
+      const float4 a = *reinterpret_cast<const float4*>(tile + at(row, 2 * chunk));
+      const float4 b = *reinterpret_cast<const float4*>(tile + at(row, 2 * chunk + 1));
+      f.w[0] = a.x;
+      f.w[1] = a.y;
+      f.w[2] = a.z;
+      f.w[3] = a.w;
+      f.w[4] = b.x;
+      f.w[5] = b.y;
+      f.w[6] = b.z;
+      f.w[7] = b.w;
+      return f;
+    } else {
+      return load_frag<T>(tile + at(row, chunk));
+    }
+  }
+  // element d + lane % 32 of rows row + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}: the transposing
+  // read takes four rows of 16 columns from 16 lanes' addresses and gives each lane a column
+  static __device__ __forceinline__ Frag<T> load_cols(const T* tile, int row, int d, int lane) {
+    Frag<T> f;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+      const int c = d + (lane & 31);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = row + 8 * (j / 4) + 4 * h + j % 4;
+        f.w[j] = tile[at(r, c / 4) + c % 4];
+      }
+    } else {
+      const int c = d + (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = row + 8 * half + 4 * h + (lane >> 2 & 3);
+        const T* p = tile + at(r, c / 8) + (c & 4);
+        const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) shortx4*)(p));
+        const uint2 u = __builtin_bit_cast(uint2, x);
+        f.w[2 * half] = u.x;
+        f.w[2 * half + 1] = u.y;
+      }
+    }
+    return f;
+  }
+  static __device__ __forceinline__ float value(const T* tile, int row, int d) {
+    return to_f32(tile[at(row, d / kUnit) + d % kUnit]);
+  }
+};
+
+__device__ const uint4 kNoData = {0, 0, 0, 0}; // what columns past D are filled from
+
+// 64 lanes x 16 bytes from each lane's own address to LDS, lane by lane from `at` (uniform);
+// vmcnt counts them (the wait state behind the write of M0: see dma16).
+__device__ __forceinline__ void dma16_from(uint32_t at, const void* p) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(p), "s"(at)
+               : "memory");
+}
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+#endif // __HIPCC__
+
+} // namespace mlxrocm

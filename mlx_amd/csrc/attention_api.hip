@@ -1,0 +1,420 @@
+// attention_api.hip -- the entry points of attention: checks, the choice of kernel and of the
+// number of runs that the keys are cut into.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.h"
+
+namespace mlxrocm {
+
+namespace {
+
+constexpr int kMostKeys = 1 << 30; // positions and their differences stay in 32 bits
+constexpr int kMostSplits = 64;
+
+bool few(const AttentionArgs& a) {
+  return static_cast<int64_t>(a.G) * a.Lq <= kFewRows;
+}
+
+int64_t heads_of(const AttentionArgs& a) {
+  return static_cast<int64_t>(a.B) * a.Hkv;
+}
+
+// Runs that the keys of a row are cut into: as many as give the chip work, with some tiles left
+// to each.
+int splits_of(const AttentionArgs& a) {
+  const int64_t span =
+      std::min<int64_t>(a.keys, static_cast<int64_t>(a.window) + a.keep + a.Lq);
+  int64_t splits;
+  if (few(a)) {
+    splits = std::min<int64_t>((1024 + heads_of(a) - 1) / heads_of(a), span / 256);
+  } else {
+    const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads_of(a);
+    splits = std::min<int64_t>(512 / blocks, span / 512);
+  }
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(splits, 1), kMostSplits));
+}
+
+size_t round256(size_t n) {
+  return (n + 255) / 256 * 256;
+}
+
+size_t workspace_of(const AttentionArgs& a) {
+  const int splits = splits_of(a);
+  if (splits == 1) {
+    return 0;
+  }
+  const size_t rows = static_cast<size_t>(splits) * a.B * a.Hq * a.Lq;
+  return round256(rows * a.D * sizeof(float)) + rows * sizeof(float2);
+}
+
+// Shapes alone; `name` for messages
+int check_shape(const char* name, const AttentionArgs& a, int dtype) {
+  if (!valid_dtype(dtype)) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] unknown dtype %d", name, dtype);
+  }
+  if (a.B < 0 || a.Hq < 0 || a.Hkv < 0 || a.Lq < 0 || a.keys < 0 || a.D <= 0) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] negative dimension", name);
+  }
+  if (a.D % 8 != 0 || a.D > 256) {
+    return fail(
+        MLXROCM_INVALID_ARGUMENT, "[%s] head dimension %d is not a multiple of 8 up to 256", name,
+        a.D);
+  }
+  if (a.Hkv == 0 ? a.Hq != 0 : a.Hq % a.Hkv != 0) {
+    return fail(
+        MLXROCM_INVALID_ARGUMENT, "[%s] %d query heads cannot share %d key heads", name, a.Hq,
+        a.Hkv);
+  }
+  if (a.window < 1 || a.keep < 0) {
+    return fail(
+        MLXROCM_INVALID_ARGUMENT, "[%s] window %d must be positive and keep %d not negative", name,
+        a.window, a.keep);
+  }
+  // what indexes the launch and the rows in 32 bits
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
+  if (a.keys > kMostKeys || rows > kMostKeys ||
+      ((rows + 15) / 16 * kMostSplits + a.keys / 128 + 1) * a.B * a.Hkv > INT32_MAX) {
+    return fail(MLXROCM_UNSUPPORTED, "[%s] the problem exceeds the grid", name);
+  }
+  return MLXROCM_OK;
+}
+
+int check_operand(
+    const char* name, const char* what, const void* p, const int64_t (&strides)[3], int dtype) {
+  if (p == nullptr) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer: %s", name, what);
+  }
+  const int64_t unit = 16 / static_cast<int64_t>(dtype_size(dtype));
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || strides[0] % unit != 0 ||
+      strides[1] % unit != 0 || strides[2] % unit != 0) {
+    return fail(MLXROCM_UNSUPPORTED, "[%s] %s is not aligned to 16 bytes", name, what);
+  }
+  return MLXROCM_OK;
+}
+
+#define TRY(expr)          \
+  do {                     \
+    const int rc_ = expr;  \
+    if (rc_ != MLXROCM_OK) \
+      return rc_;          \
+  } while (0)
+
+void take(int64_t (&to)[3], const int64_t* from) {
+  to[0] = from[0];
+  to[1] = from[1];
+  to[2] = from[2];
+}
+
+void set_scale(AttentionArgs& a, float scale, int dtype) {
+  // (no score is worth less than 1e-30 log2 units: a scale of zero would make NaN of the -inf of
+  // masked scores)
+  a.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  a.q_sign = std::signbit(scale) ? (dtype == MLXROCM_FLOAT32 ? 0x80000000u : 0x80008000u) : 0u;
+}
+
+AttentionArgs shape_of(
+    int B, int Hq, int Hkv, int Lq, int keys, int D, int window, int keep) {
+  AttentionArgs a{};
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.G = Hkv > 0 ? Hq / Hkv : 0;
+  a.Lq = Lq;
+  a.keys = keys;
+  a.D = D;
+  a.window = std::min(window, kMostKeys);
+  a.keep = std::min(keep, kMostKeys);
+  return a;
+}
+
+bool empty(const AttentionArgs& a) {
+  return a.B == 0 || a.Hq == 0 || a.Lq == 0;
+}
+
+int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t bytes,
+        hipStream_t s) {
+  a.splits = splits_of(a);
+  if (a.splits > 1 && !rehearsing()) {
+    const size_t need = workspace_of(a);
+    if (workspace == nullptr || bytes < need) {
+      return fail(
+          MLXROCM_INVALID_ARGUMENT, "[%s] workspace of %zu bytes, %zu needed", name, bytes, need);
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+      return fail(MLXROCM_INVALID_ARGUMENT, "[%s] workspace is not aligned to 16 bytes", name);
+    }
+    const size_t rows = static_cast<size_t>(a.splits) * a.B * a.Hq * a.Lq;
+    a.part_out = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(
+        static_cast<char*>(workspace) + round256(rows * a.D * sizeof(float)));
+  }
+  if (few(a)) {
+    TRY(dtype == MLXROCM_FLOAT32       ? launch_attention_few_f32(a, s)
+            : dtype == MLXROCM_FLOAT16 ? launch_attention_few_f16(a, s)
+                                       : launch_attention_few_bf16(a, s));
+  } else {
+    TRY(dtype == MLXROCM_FLOAT32       ? launch_attention_rows_f32(a, s)
+            : dtype == MLXROCM_FLOAT16 ? launch_attention_rows_f16(a, s)
+                                       : launch_attention_rows_bf16(a, s));
+  }
+  return a.splits > 1 ? launch_attention_join(a, dtype, s) : static_cast<int>(MLXROCM_OK);
+}
+
+} // namespace
+
+} // namespace mlxrocm
+
+extern "C" size_t mlxrocm_window_attention_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype) {
+  using namespace mlxrocm;
+  const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
+  return check_shape("window_attention", a, dtype) != MLXROCM_OK || empty(a) ? 0
+                                                                             : workspace_of(a);
+}
+
+extern "C" int mlxrocm_window_attention(
+    const void* q,
+    const void* k,
+    const void* v,
+    void* out,
+    float* lse,
+    const int32_t* lengths,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream) {
+  mlxrocm::ApiRange api_range("mlxrocm_window_attention");
+  using namespace mlxrocm;
+  const char* name = "window_attention";
+  AttentionArgs a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
+  TRY(check_shape(name, a, dtype));
+  if (empty(a)) {
+    return MLXROCM_OK;
+  }
+  if (!std::isfinite(scale) || strides == nullptr) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] scale is not finite or strides are null", name);
+  }
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.lengths = lengths;
+  take(a.q_strides, strides);
+  take(a.k_strides, strides + 3);
+  take(a.v_strides, strides + 6);
+  take(a.out_strides, strides + 9);
+  TRY(check_operand(name, "q", q, a.q_strides, dtype));
+  TRY(check_operand(name, "out", out, a.out_strides, dtype));
+  if (Lk > 0) {
+    TRY(check_operand(name, "k", k, a.k_strides, dtype));
+    TRY(check_operand(name, "v", v, a.v_strides, dtype));
+  }
+  set_scale(a, scale, dtype);
+  return run(name, a, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t mlxrocm_window_attention_vjp_workspace_size(int B, int Hq, int Lq) {
+  return static_cast<size_t>(std::max(B, 0)) * std::max(Hq, 0) * std::max(Lq, 0) * sizeof(float);
+}
+
+extern "C" int mlxrocm_window_attention_vjp(
+    const void* q,
+    const void* k,
+    const void* v,
+    const void* out,
+    const float* lse,
+    const void* dout,
+    void* dq,
+    void* dk,
+    void* dv,
+    const int32_t* lengths,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream) {
+  mlxrocm::ApiRange api_range("mlxrocm_window_attention_vjp");
+  using namespace mlxrocm;
+  const char* name = "window_attention_vjp";
+  AttentionGradArgs g{};
+  AttentionArgs& a = g.a;
+  a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
+  TRY(check_shape(name, a, dtype));
+  if (B == 0 || Hq == 0 || (Lq == 0 && Lk == 0)) {
+    return MLXROCM_OK;
+  }
+  if (!std::isfinite(scale) || strides == nullptr) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] scale is not finite or strides are null", name);
+  }
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = const_cast<void*>(out);
+  a.lse = const_cast<float*>(lse);
+  a.lengths = lengths;
+  a.splits = 1;
+  g.dout = dout;
+  g.dq = dq;
+  g.dk = dk;
+  g.dv = dv;
+  g.delta = static_cast<float*>(workspace);
+  g.scale = scale;
+  take(a.q_strides, strides);
+  take(a.k_strides, strides + 3);
+  take(a.v_strides, strides + 6);
+  take(a.out_strides, strides + 9);
+  take(g.dout_strides, strides + 12);
+  take(g.dq_strides, strides + 15);
+  take(g.dk_strides, strides + 18);
+  take(g.dv_strides, strides + 21);
+  if (Lq > 0) {
+    TRY(check_operand(name, "q", q, a.q_strides, dtype));
+    TRY(check_operand(name, "out", out, a.out_strides, dtype));
+    TRY(check_operand(name, "dout", dout, g.dout_strides, dtype));
+    TRY(check_operand(name, "dq", dq, g.dq_strides, dtype));
+    if (lse == nullptr) {
+      return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer: lse", name);
+    }
+    const size_t need = mlxrocm_window_attention_vjp_workspace_size(B, Hq, Lq);
+    if (workspace == nullptr || workspace_bytes < need) {
+      return fail(
+          MLXROCM_INVALID_ARGUMENT, "[%s] workspace of %zu bytes, %zu needed", name,
+          workspace_bytes, need);
+    }
+  }
+  if (Lk > 0) {
+    TRY(check_operand(name, "k", k, a.k_strides, dtype));
+    TRY(check_operand(name, "v", v, a.v_strides, dtype));
+    TRY(check_operand(name, "dk", dk, g.dk_strides, dtype));
+    TRY(check_operand(name, "dv", dv, g.dv_strides, dtype));
+  }
+  set_scale(a, scale, dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return dtype == MLXROCM_FLOAT32    ? launch_attention_grad_f32(g, s)
+      : dtype == MLXROCM_FLOAT16 ? launch_attention_grad_f16(g, s)
+                                 : launch_attention_grad_bf16(g, s);
+}
+
+extern "C" size_t mlxrocm_paged_attention_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int D, int max_keys, int window, int keep, int dtype) {
+  using namespace mlxrocm;
+  const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, max_keys, D, window, keep);
+  return check_shape("paged_attention", a, dtype) != MLXROCM_OK || empty(a) ? 0 : workspace_of(a);
+}
+
+extern "C" int mlxrocm_paged_attention(
+    const void* q,
+    const void* k_pages,
+    const void* v_pages,
+    const int32_t* table,
+    const int32_t* lengths,
+    void* out,
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int D,
+    int pages,
+    int page_size,
+    int table_width,
+    const int64_t* strides,
+    float scale,
+    int window,
+    int keep,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream) {
+  mlxrocm::ApiRange api_range("mlxrocm_paged_attention");
+  using namespace mlxrocm;
+  const char* name = "paged_attention";
+  if (page_size <= 0 || page_size % 16 != 0) {
+    return fail(
+        MLXROCM_INVALID_ARGUMENT, "[%s] page size %d is not a multiple of 16", name, page_size);
+  }
+  if (pages < 0 || table_width < 0) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] negative dimension", name);
+  }
+  const int64_t keys = static_cast<int64_t>(table_width) * page_size;
+  if (keys > kMostKeys) {
+    return fail(MLXROCM_UNSUPPORTED, "[%s] the problem exceeds the grid", name);
+  }
+  AttentionArgs a =
+      shape_of(B, Hq, Hkv, Lq, pages == 0 ? 0 : static_cast<int>(keys), D, window, keep);
+  TRY(check_shape(name, a, dtype));
+  if (empty(a)) {
+    return MLXROCM_OK;
+  }
+  if (!std::isfinite(scale) || strides == nullptr) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] scale is not finite or strides are null", name);
+  }
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.out = out;
+  a.lengths = lengths;
+  a.table = table;
+  a.page = page_size;
+  a.page_magic = static_cast<uint32_t>((uint64_t{1} << 32) / page_size + 1);
+  a.pages = pages;
+  take(a.q_strides, strides);
+  take(a.k_strides, strides + 3);
+  take(a.v_strides, strides + 6);
+  take(a.out_strides, strides + 9);
+  a.table_stride = strides[12];
+  TRY(check_operand(name, "q", q, a.q_strides, dtype));
+  TRY(check_operand(name, "out", out, a.out_strides, dtype));
+  if (lengths == nullptr) {
+    return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer: lengths", name);
+  }
+  if (a.keys > 0) {
+    TRY(check_operand(name, "k_pages", k_pages, a.k_strides, dtype));
+    TRY(check_operand(name, "v_pages", v_pages, a.v_strides, dtype));
+    if (table == nullptr) {
+      return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer: table", name);
+    }
+  }
+  set_scale(a, scale, dtype);
+  return run(name, a, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int mlxrocm_attention_plan(
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int keys,
+    int D,
+    int window,
+    int keep,
+    int dtype,
+    char* plan,
+    size_t plan_bytes) {
+  using namespace mlxrocm;
+  RehearsalScope rehearsal(plan, plan_bytes);
+  AttentionArgs a = shape_of(B, Hq, Hkv, Lq, keys, D, window, keep);
+  TRY(check_shape("attention_plan", a, dtype));
+  return empty(a) ? static_cast<int>(MLXROCM_OK)
+                  : run("attention_plan", a, dtype, nullptr, 0, nullptr);
+}

@@ -1,0 +1,422 @@
+// attention_few.h -- attention of up to 64 rows (a token, or a few, for all heads that
+// share a key head): bound by reading the keys and values once.
+//
+// The keys of a (sequence, key head) are cut into `splits` runs of tiles of 32, a workgroup
+// each, and within a workgroup its four waves take tiles in turn, each with a running maximum
+// and sum of its own; nothing waits for another wave until all keys are read.  The waves'
+// results are joined in LDS, those of the runs by the join kernel.
+//
+// Keys and values go from memory straight into the operands of the 16x16 matrix instruction:
+//   S^T = K Q^T    a lane has 16 bytes of key l % 16
+//   O^T = V^T P^T  a lane has E consecutive columns (E (l % 16) on) of the 8 values whose
+//                  probabilities it holds; two keys' dwords are interleaved by v_perm, and the
+//                  e-th instruction makes the columns E m + e.  So a load covers whole rows of v.
+#pragma once
+
+#include "attention.h"
+
+namespace mlxrocm {
+
+namespace {
+
+constexpr int kFewKeys = 32; // keys of a tile
+
+template <typename T, int DT>
+struct FewShape {
+  static constexpr int kE = DT == 64 ? 4 : DT == 96 ? 6 : 8; // columns of a lane
+  static constexpr int kGroups = DT == 256 ? 2 : 1;          // of 16 kE columns
+  static constexpr int kDwords = kE * sizeof(T) / 4;
+};
+
+// The keys of one tile as this lane's operands need them.
+template <typename T, int DT>
+struct FewTile {
+  using S = FewShape<T, DT>;
+  Frag<T> k[2][DT / 32];
+  uint32_t v[S::kGroups][8][S::kDwords];
+};
+
+template <int N>
+__device__ __forceinline__ void load_dwords(const void* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 x = *(reinterpret_cast<const uint4*>(p) + i / 4);
+      w[i] = x.x;
+      w[i + 1] = x.y;
+      w[i + 2] = x.z;
+      w[i + 3] = x.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint2 x = *(reinterpret_cast<const uint2*>(p) + i / 2);
+      w[i] = x.x;
+      w[i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i] = *(reinterpret_cast<const uint32_t*>(p) + i);
+    }
+  }
+}
+
+// Loads keys [begin, end) of which the first is a multiple of 16; keys before `low` or from `end`
+// on are replaced by the nearest that is read anyway.
+template <typename T, int DT, bool PAGED>
+__device__ __forceinline__ void load_tile(
+    const AttentionArgs& a, int b, int hk, int begin, int low, int end, int lane,
+    FewTile<T, DT>& tile) {
+  using S = FewShape<T, DT>;
+  const T* kp = static_cast<const T*>(a.k);
+  const T* vp = static_cast<const T*>(a.v);
+  const int m = lane & 15;
+  const int g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    // the 16 keys of one operand lie in one page
+    const int first = min(begin + 16 * t, (end - 1) & ~15);
+    const KeyRow r = key_row<PAGED>(a, b, hk, first);
+    const int least = max(low - first, 0);
+    const int most = end - 1 - first;
+    const T* k = kp + r.k + min(max(m, least), most) * a.k_strides[2];
+#pragma unroll
+    for (int c = 0; c < DT / 32; ++c) {
+      const int d = 32 * c + 8 * g;
+      tile.k[t][c] = d < a.D ? load_frag<T>(k + d) : zero_frag<T>();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T* v = vp + r.v + min(max(4 * g + i, least), most) * a.v_strides[2];
+#pragma unroll
+      for (int n = 0; n < S::kGroups; ++n) {
+        const int d = (16 * n + m) * S::kE;
+        if (d < a.D) {
+          load_dwords<S::kDwords>(v + d, tile.v[n][4 * t + i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < S::kDwords; ++e) {
+            tile.v[n][4 * t + i][e] = 0;
+          }
+        }
+      }
+    }
+  }
+}
+
+// Column e of the lane's columns over its 8 keys
+template <typename T, int DT>
+__device__ __forceinline__ Frag<T> column(
+    const uint32_t (&v)[8][FewShape<T, DT>::kDwords], int e) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f.w[j] = __uint_as_float(v[j][e]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f.w[j] = __builtin_amdgcn_perm(
+          v[2 * j + 1][e / 2], v[2 * j][e / 2], e % 2 != 0 ? 0x07060302u : 0x05040100u);
+    }
+  }
+  return f;
+}
+
+// max or sum over the four lanes that hold a column's keys
+__device__ __forceinline__ float max_quarters(float v) {
+  const uint32_t u = __float_as_uint(max_halves(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+  const uint32_t u = __float_as_uint(sum_halves(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// NT: tiles of 16 rows
+template <typename T, int DT, int NT, bool PAGED>
+__global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs a) {
+  using S = FewShape<T, DT>;
+  constexpr int KT = kFewKeys;
+  __shared__ float join_o[4][16][DT + 4];
+  __shared__ float join_m[4][16], join_l[4][16];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4;
+  int head, split;
+  piece_of(a.B * a.Hkv, a.splits, &head, &split);
+  const int b = head / a.Hkv;
+  const int hk = head - b * a.Hkv;
+  const int R = a.G * a.Lq;
+  const int length = length_of(a, b);
+  const int first_row = max(0, a.Lq - length) * a.G;
+  const bool any = length > 0; // then first_row < R
+
+  KeyRange range = {};
+  int t0 = 0, t1 = 0;
+  if (any) {
+    range = keys_of(a, length, first_row, R - 1, KT);
+    // whole groups of 16 keys, which lie in one page
+    const int low = range.w_begin & ~15;
+    range.tiles = range.a_tiles + (range.w_end - low + KT - 1) / KT;
+    t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / a.splits);
+    t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / a.splits);
+  }
+  const int p0 = length - a.Lq;
+  const int p_lo = p0 + first_row / a.G;
+  const int p_hi = p0 + a.Lq - 1;
+
+  Frag<T> q[NT][DT / 32];
+  int p[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = min(max(16 * n + (lane & 15), first_row), R - 1);
+    p[n] = p0 + row / a.G;
+    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.G, row);
+#pragma unroll
+    for (int c = 0; c < DT / 32; ++c) {
+      const int d = 32 * c + 8 * g;
+      q[n][c] = d < a.D && any ? load_frag<T>(src + d) : zero_frag<T>();
+      flip<T>(q[n][c], a.q_sign);
+    }
+  }
+
+  floatx4 o[NT][S::kGroups][S::kE];
+  float m[NT], l[NT];
+  // (a masked value that is not finite: see attention_rows_kernel)
+  for (int careful = 0;; careful = 1) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+        for (int e = 0; e < S::kE; ++e) {
+          o[n][x][e] = floatx4{};
+        }
+      }
+    }
+    for (int t = t0 + wave; t < t1; t += 4) {
+      const bool kept = t < range.a_tiles;
+      const int low = kept ? 0 : range.w_begin;
+      const int begin = kept ? t * KT : (range.w_begin & ~15) + (t - range.a_tiles) * KT;
+      const int end = min(begin + KT, kept ? range.a_end : range.w_end);
+      FewTile<T, DT> tile;
+      load_tile<T, DT, PAGED>(a, b, hk, begin, low, end, lane, tile);
+      const bool whole = begin >= low && end - begin == KT &&
+          all_seen(begin, end, p_lo, p_hi, a.window, a.keep);
+      Frag<T> w[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        floatx4 s[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          s[x] = floatx4{};
+#pragma unroll
+          for (int c = 0; c < DT / 32; ++c) {
+            s[x] = mma16<T>(tile.k[x][c], q[n][c], s[x]);
+          }
+        }
+        if (!whole) {
+          const int last = min(p[n], end - 1);
+          const int seen_from = p[n] - a.window + 1;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = begin + 16 * (i / 4) + 4 * g + i % 4;
+            const bool sees = j >= low && j <= last && (j >= seen_from || j < a.keep);
+            s[i / 4][i % 4] = sees ? s[i / 4][i % 4] : -INFINITY;
+          }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+          top = fmaxf(top, s[i / 4][i % 4]);
+        }
+        top *= a.scale_log2;
+        if (__any(top > m[n])) {
+          const float now = fmaxf(m[n], max_quarters(top));
+          const float by = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
+          m[n] = now;
+          l[n] *= by;
+#pragma unroll
+          for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+            for (int e = 0; e < S::kE; ++e) {
+              o[n][x][e] *= by;
+            }
+          }
+        }
+        const float less = m[n] == -INFINITY ? 0.0f : m[n];
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.scale_log2, -less));
+          l[n] += e[i];
+        }
+        w[n] = frag_of<T>(e);
+      }
+      const bool apart = careful != 0 && !whole;
+#pragma unroll
+      for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+        for (int e = 0; e < S::kE; ++e) {
+          Frag<T> f = column<T, DT>(tile.v[x], e);
+          if (apart) {
+            drop_not_finite<T>(f);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[n][x][e] = mma16<T>(f, w[n], o[n][x][e]);
+          }
+        }
+      }
+      if (apart) {
+        for (int j = max(begin, low); j < end; ++j) {
+          const T* v = static_cast<const T*>(a.v) + key_row<PAGED>(a, b, hk, j).v;
+#pragma unroll
+          for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+            for (int e = 0; e < S::kE; ++e) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int d = (16 * x + 4 * g + i) * S::kE + e;
+                const float value = d < a.D ? to_f32(v[d]) : 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const bool sees =
+                      j <= p[n] && (j >= p[n] - a.window + 1 || j < a.keep);
+                  o[n][x][e][i] += sees && not_finite(value) ? value : 0.0f;
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+        for (int e = 0; e < S::kE; ++e) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            odd = odd || not_finite(o[n][x][e][i]);
+          }
+        }
+      }
+    }
+    if (careful != 0 || !__any(odd)) {
+      break;
+    }
+  }
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float sum = sum_quarters(l[n]);
+    __syncthreads(); // the tile of rows before has been joined
+    if (g == 0) {
+      join_m[wave][lane] = m[n];
+      join_l[wave][lane] = sum;
+    }
+#pragma unroll
+    for (int x = 0; x < S::kGroups; ++x) {
+#pragma unroll
+      for (int e = 0; e < S::kE; ++e) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          join_o[wave][lane & 15][(16 * x + 4 * g + i) * S::kE + e] = o[n][x][e][i];
+        }
+      }
+    }
+    __syncthreads();
+    // 16 threads for a row
+    const int at = threadIdx.x >> 4;
+    const int row = 16 * n + at;
+    if (row < R) {
+      float top = join_m[0][at];
+#pragma unroll
+      for (int x = 1; x < 4; ++x) {
+        top = fmaxf(top, join_m[x][at]);
+      }
+      const float less = top == -INFINITY ? 0.0f : top;
+      float by[4], total = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        by[x] = join_m[x][at] == less ? 1.0f : __builtin_amdgcn_exp2f(join_m[x][at] - less);
+        total += by[x] * join_l[x][at];
+      }
+      const bool seeing = any && row >= first_row;
+      const float over = total == 0.0f ? 0.0f : 1.0f / total;
+      const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R + row;
+      T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row);
+      for (int d = 4 * (threadIdx.x & 15); d < a.D; d += 64) {
+        floatx4 sum4 = {};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 v = *reinterpret_cast<const float4*>(&join_o[x][at][d]);
+          sum4 += by[x] * floatx4{v.x, v.y, v.z, v.w};
+        }
+        if (a.splits > 1) {
+          *reinterpret_cast<float4*>(a.part_out + part * a.D + d) =
+              make_float4(sum4[0], sum4[1], sum4[2], sum4[3]);
+        } else {
+          store4<T>(out + d, seeing ? sum4 * over : floatx4{});
+        }
+      }
+      if ((threadIdx.x & 15) == 0) {
+        if (a.splits > 1) {
+          a.part_ml[part] = make_float2(top, seeing ? total : 0.0f);
+        } else if (a.lse != nullptr) {
+          const int i = row / a.G;
+          a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
+              seeing ? top + log2f(total) : 0.0f;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int DT, int NT>
+int launch_few_rows(const AttentionArgs& a, hipStream_t s) {
+  MLXROCM_REHEARSE("attention_few(dim=%d,rows=%d,splits=%d)", DT, 16 * NT, a.splits);
+  const dim3 grid(static_cast<unsigned>(a.B * a.Hkv * a.splits));
+  if (a.table != nullptr) {
+    attention_few_kernel<T, DT, NT, true><<<grid, 256, 0, s>>>(a);
+  } else {
+    attention_few_kernel<T, DT, NT, false><<<grid, 256, 0, s>>>(a);
+  }
+  MLXROCM_HIP_TRY(hipGetLastError());
+  return static_cast<int>(MLXROCM_OK);
+}
+
+template <typename T, int DT>
+int launch_few_of(const AttentionArgs& a, hipStream_t s) {
+  const int rows = a.G * a.Lq;
+  return rows <= 16 ? launch_few_rows<T, DT, 1>(a, s)
+      : rows <= 32  ? launch_few_rows<T, DT, 2>(a, s)
+                    : launch_few_rows<T, DT, 4>(a, s);
+}
+
+template <typename T>
+int launch_few_typed(const AttentionArgs& a, hipStream_t s) {
+  if (a.D <= 64) {
+    return launch_few_of<T, 64>(a, s);
+  } else if (a.D == 96) { // six columns of a lane end at 96 only
+    return launch_few_of<T, 96>(a, s);
+  } else if (a.D <= 128) {
+    return launch_few_of<T, 128>(a, s);
+  }
+  return launch_few_of<T, 256>(a, s);
+}
+
+} // namespace
+
+} // namespace mlxrocm
