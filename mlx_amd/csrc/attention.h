@@ -45,6 +45,7 @@ struct AttentionArgs {
   float scale_log2; // |scale| log2(e)
   uint32_t q_sign;  // 0x80008000 (16-bit types), 0x80000000 (float32) where scale < 0
   int window, keep;
+  int near; // the rows of one load lie within 32-bit offsets: of keys (1), of queries (2)
   int splits;
   float* part_out; // [splits, B Hkv, R, D], not yet divided by the sums
   float2* part_ml; // [splits, B Hkv, R]: maximum (log2 units) and sum
@@ -243,9 +244,11 @@ __device__ __forceinline__ float sum_halves(float v) {
 
 // ---- which keys ----------------------------------------------------------------
 // The rows of one tile of rows that see anything are first .. last; the keys they see lie
-// in [0, a_end) (the ones that are kept) and [w_begin, w_end), cut into tiles of KT keys.
+// in [0, a_end) (the ones that are kept) and [w_low, w_end), cut into tiles of KT keys.  Tiles
+// begin at multiples of 16, whose keys lie in one page: the first of the second range with some
+// keys that nobody sees.
 struct KeyRange {
-  int a_end, w_begin, w_end;
+  int a_end, w_low, w_end;
   int a_tiles, tiles;
 };
 
@@ -255,22 +258,34 @@ keys_of(const AttentionArgs& a, int length, int first_row, int last_row, int kt)
   const int p_hi = length - a.Lq + last_row / a.G;
   KeyRange r;
   r.w_end = p_hi + 1;
-  r.w_begin = max(0, p_lo - a.window + 1);
+  r.w_low = max(0, p_lo - a.window + 1);
   r.a_end = min(a.keep, p_hi + 1);
-  if (r.a_end >= r.w_begin) { // one range
+  if (r.a_end >= r.w_low) { // one range
     r.a_end = 0;
-    r.w_begin = 0;
+    r.w_low = 0;
   }
   r.a_tiles = (r.a_end + kt - 1) / kt;
-  r.tiles = r.a_tiles + (r.w_end - r.w_begin + kt - 1) / kt;
+  r.tiles = r.a_tiles + (r.w_end - (r.w_low & ~15) + kt - 1) / kt;
   return r;
 }
 
-// Keys [begin, end) of tile t; end - begin <= kt
-__device__ __forceinline__ void tile_of(const KeyRange& r, int t, int kt, int* begin, int* end) {
+// Keys of tile t: kt from `begin` on, of which [low, end) belong to it
+struct KeyTile {
+  int begin, low, end;
+};
+__device__ __forceinline__ KeyTile tile_of(const KeyRange& r, int t, int kt) {
   const bool a = t < r.a_tiles;
-  *begin = a ? t * kt : r.w_begin + (t - r.a_tiles) * kt;
-  *end = min(*begin + kt, a ? r.a_end : r.w_end);
+  KeyTile k;
+  k.begin = a ? t * kt : (r.w_low & ~15) + (t - r.a_tiles) * kt;
+  k.low = a ? 0 : r.w_low;
+  k.end = min(k.begin + kt, a ? r.a_end : r.w_end);
+  return k;
+}
+// Whether positions lo .. hi see all of a tile
+__device__ __forceinline__ bool
+whole_tile(const AttentionArgs& a, const KeyTile& k, int kt, int lo, int hi) {
+  return k.begin >= k.low && k.end - k.begin == kt && k.end - 1 <= lo &&
+      (hi - k.begin < a.window || k.end <= a.keep);
 }
 
 // Whether a tile's keys [begin, end) are all seen by, or all hidden from, positions lo .. hi
@@ -342,20 +357,23 @@ __device__ __forceinline__ void piece_of(int heads, int per, int* head, int* pie
 }
 
 // ---- tiles in LDS -----------------------------------------------------------------
-// `rows` rows of DT elements in 16-byte units, unit u of row r at place u ^ swizzle(r) of the
-// row: eight rows read at one column (load_rows) fall into eight different places, and four
-// rows read 32 bytes wide (load_cols) too.  DT = 96 of 16 bits has 12 units, which no
-// exclusive or permutes; its rows lie 48 banks apart as they are.
+// Rows of DT elements in 16-byte units, a power of two of places for them, unit u of row r at
+// place u ^ swizzle(r): eight rows read at one column (load_rows) fall into eight different
+// places, and four rows read 32 bytes wide (load_cols) too.
 template <typename T, int DT>
 struct Tile {
   static constexpr int kUnit = 16 / sizeof(T);
-  static constexpr int kUnits = DT / kUnit;
+  static constexpr int kPitch = DT == 96 ? 128 : DT;
+  static constexpr int kPlaces = kPitch / kUnit;
+  static constexpr int kRowsOfLoad = 64 / kPlaces; // that the 64 lanes of one load cover
+  static constexpr int kRowsOfPass = 4 * kRowsOfLoad; // ... and those of a workgroup's four waves
 
   static __device__ __forceinline__ int swizzle(int row) {
-    return kUnits % 8 == 0 ? ((row & 3) << 1 | (row >> 2 & 1)) : 0;
+    // (with 64 places a pass is four rows: a lane then loads the same column in each)
+    return kPlaces == 64 ? (row & 3) << 1 : (row & 3) << 1 | (row >> 2 & 1);
   }
   static __device__ __forceinline__ int at(int row, int unit) {
-    return row * DT + (unit ^ swizzle(row)) * kUnit;
+    return row * kPitch + (unit ^ swizzle(row)) * kUnit;
   }
   // elements 8 chunk .. 8 chunk + 7 of a row
   static __device__ __forceinline__ Frag<T> load_rows(const T* tile, int row, int chunk) {
@@ -407,8 +425,6 @@ struct Tile {
     return to_f32(tile[at(row, d / kUnit) + d % kUnit]);
   }
 };
-
-__device__ const uint4 kNoData = {0, 0, 0, 0}; // what columns past D are filled from
 
 // 64 lanes x 16 bytes from each lane's own address to LDS, lane by lane from `at` (uniform);
 // vmcnt counts them (the wait state behind the write of M0: see dma16).

@@ -106,6 +106,18 @@ void take(int64_t (&to)[3], const int64_t* from) {
   to[2] = from[2];
 }
 
+// Whether the rows that one load covers (eight at most) lie within 31 bits of bytes of the first
+bool near(const int64_t (&strides)[3], int dtype, int G) {
+  const int64_t most = INT32_MAX / static_cast<int64_t>(dtype_size(dtype));
+  const auto within = [&](int64_t n) { return n > -most / 16 && n < most / 16; };
+  return within(strides[2]) && (G == 1 || within(strides[1])) && strides[1] >= 0 &&
+      strides[2] >= 0;
+}
+
+void set_near(AttentionArgs& a, int dtype) {
+  a.near = near(a.k_strides, dtype, 1) && near(a.v_strides, dtype, 1) ? 1 : 0;
+}
+
 void set_scale(AttentionArgs& a, float scale, int dtype) {
   // (no score is worth less than 1e-30 log2 units: a scale of zero would make NaN of the -inf of
   // masked scores)
@@ -135,6 +147,7 @@ bool empty(const AttentionArgs& a) {
 int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t bytes,
         hipStream_t s) {
   a.splits = splits_of(a);
+  set_near(a, dtype);
   if (a.splits > 1 && !rehearsing()) {
     const size_t need = workspace_of(a);
     if (workspace == nullptr || bytes < need) {
@@ -310,6 +323,11 @@ extern "C" int mlxrocm_window_attention_vjp(
     TRY(check_operand(name, "dv", dv, g.dv_strides, dtype));
   }
   set_scale(a, scale, dtype);
+  set_near(a, dtype);
+  if ((a.G & (a.G - 1)) == 0 && near(a.q_strides, dtype, a.G) &&
+      near(g.dout_strides, dtype, a.G)) {
+    a.near |= 2;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == MLXROCM_FLOAT32    ? launch_attention_grad_f32(g, s)
       : dtype == MLXROCM_FLOAT16 ? launch_attention_grad_f16(g, s)

@@ -161,9 +161,6 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
   int t0 = 0, t1 = 0;
   if (any) {
     range = keys_of(a, length, first_row, R - 1, KT);
-    // whole groups of 16 keys, which lie in one page
-    const int low = range.w_begin & ~15;
-    range.tiles = range.a_tiles + (range.w_end - low + KT - 1) / KT;
     t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / a.splits);
     t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / a.splits);
   }
@@ -203,14 +200,13 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
       }
     }
     for (int t = t0 + wave; t < t1; t += 4) {
-      const bool kept = t < range.a_tiles;
-      const int low = kept ? 0 : range.w_begin;
-      const int begin = kept ? t * KT : (range.w_begin & ~15) + (t - range.a_tiles) * KT;
-      const int end = min(begin + KT, kept ? range.a_end : range.w_end);
+      const KeyTile at = tile_of(range, t, KT);
+      const int begin = at.begin;
+      const int low = at.low;
+      const int end = at.end;
       FewTile<T, DT> tile;
       load_tile<T, DT, PAGED>(a, b, hk, begin, low, end, lane, tile);
-      const bool whole = begin >= low && end - begin == KT &&
-          all_seen(begin, end, p_lo, p_hi, a.window, a.keep);
+      const bool whole = whole_tile(a, at, KT, p_lo, p_hi);
       Frag<T> w[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {

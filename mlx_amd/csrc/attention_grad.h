@@ -19,11 +19,11 @@ namespace {
 
 // ---- dq: workgroups of 128 rows, as the forward -----------------------------------------
 template <typename T, int DT>
-__global__ __launch_bounds__(256) void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
+__global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
-  constexpr int kBoth = 2 * S::kTileBytes / sizeof(T);
+  constexpr int kBoth = 2 * S::kTile;
   __shared__ __align__(16) T lds[2 * kBoth];
   const AttentionArgs& a = ga.a;
 
@@ -89,6 +89,10 @@ __global__ __launch_bounds__(256) void attention_dq_kernel(const AttentionGradAr
     }
   }
 
+  if (a.D < L::kPitch) {
+    clear_lds<T>(lds, 2 * kBoth);
+  }
+  KeyStream<T, DT, false> keys(a, b, hk, length, wave, lane);
   floatx16 dq[DT / 32];
   // (a masked key that is not finite: see attention_rows_kernel)
   for (int careful = 0;; careful = 1) {
@@ -96,29 +100,25 @@ __global__ __launch_bounds__(256) void attention_dq_kernel(const AttentionGradAr
     for (int d = 0; d < DT / 32; ++d) {
       dq[d] = floatx16{};
     }
-    int begin, end;
     if (range.tiles > 0) {
-      tile_of(range, 0, KT, &begin, &end);
-      fetch_keys<T, DT, false>(a, b, hk, begin, end, lds, lds + kBoth / 2);
+      keys.fetch(tile_of(range, 0, KT).begin, lds, lds + kBoth / 2);
     }
     for (int t = 0; t < range.tiles; ++t) {
       wait_loads();
       __syncthreads();
       const T* k_tile = lds + (t & 1) * kBoth;
       const T* v_tile = k_tile + kBoth / 2;
-      tile_of(range, t, KT, &begin, &end);
+      const KeyTile tile = tile_of(range, t, KT);
       if (t + 1 < range.tiles) {
-        int b1, e1;
-        tile_of(range, t + 1, KT, &b1, &e1);
         T* next = lds + ((t + 1) & 1) * kBoth;
-        fetch_keys<T, DT, false>(a, b, hk, b1, e1, next, next + kBoth / 2);
+        keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
       }
-      if (!works || none_seen(begin, end, p_lo, p_hi, a.window, a.keep)) {
+      const int begin = tile.begin;
+      if (!works || none_seen(begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
         continue;
       }
-      const bool whole =
-          end - begin == KT && all_seen(begin, end, p_lo, p_hi, a.window, a.keep);
-      const int last = min(p, end - 1);
+      const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
+      const int last = min(p, tile.end - 1);
       const bool apart = careful != 0 && !whole;
 #pragma unroll
       for (int g = 0; g < KT / 32; ++g) {
@@ -138,7 +138,8 @@ __global__ __launch_bounds__(256) void attention_dq_kernel(const AttentionGradAr
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int j = begin + 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            ds[i] = j <= last && (j >= seen_from || j < a.keep) ? ds[i] : 0.0f;
+            const bool sees = j >= tile.low && j <= last && (j >= seen_from || j < a.keep);
+            ds[i] = sees ? ds[i] : 0.0f;
           }
         }
         const Frag<T> w[2] = {frag_of<T>(ds), frag_of<T>(ds + 8)};
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(256) void attention_dq_kernel(const AttentionGradAr
         }
       }
       if (apart) {
-        for (int n = 0; n < end - begin; ++n) {
+        for (int n = max(tile.low - begin, 0); n < tile.end - begin; ++n) {
           const int j = begin + n;
           const bool sees = j <= p && (j >= seen_from || j < a.keep);
 #pragma unroll
@@ -214,40 +215,66 @@ struct StatsTile {
   int p[N];
 };
 
-// Fetches rows [begin, end) of q and dout; rows past them repeat the last one.
+// Fetches tiles of rows of q and dout to LDS (see KeyStream).  Where a power of two of heads
+// share a key head, a lane's rows lie at the same offsets from the first of each load.
 template <typename T, int DT>
-__device__ __forceinline__ void fetch_rows(
-    const AttentionGradArgs& ga, int b, int hk, int begin, int end, T* q_tile, T* d_tile) {
+struct RowStream {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
-  const AttentionArgs& a = ga.a;
-  const T* q = static_cast<const T*>(a.q);
-  const T* dout = static_cast<const T*>(ga.dout);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-  for (int n = 0; n < S::kPasses; ++n) {
-    const int u = n * 256 + threadIdx.x;
-    const int row = u / L::kUnits;
-    const int d = ((u % L::kUnits) ^ L::swizzle(row)) * L::kUnit;
-    const int r = min(begin + row, end - 1);
-    const bool in = d < a.D;
-    const uint32_t to = (n * 256 + wave * 64) * 16;
-    dma16_from(
-        lds_address(q_tile) + to,
-        in ? static_cast<const void*>(q + row_offset(a.q_strides, b, hk, a.G, r) + d) : &kNoData);
-    dma16_from(
-        lds_address(d_tile) + to,
-        in ? static_cast<const void*>(dout + row_offset(ga.dout_strides, b, hk, a.G, r) + d)
-           : &kNoData);
+  const AttentionGradArgs& ga;
+  int b, hk, end, wave;
+  int d;
+  uint32_t q_off, d_off;
+
+  __device__ __forceinline__ RowStream(
+      const AttentionGradArgs& args, int b_, int hk_, int end_, int wave_, int lane)
+      : ga(args), b(b_), hk(hk_), end(end_), wave(wave_) {
+    const int row = lane / L::kPlaces;
+    const int i = row / ga.a.G;
+    const int g = row - i * ga.a.G;
+    d = ((lane % L::kPlaces) ^ L::swizzle(wave * L::kRowsOfLoad + row)) * L::kUnit;
+    q_off = static_cast<uint32_t>(
+        (g * ga.a.q_strides[1] + i * ga.a.q_strides[2] + d) * sizeof(T));
+    d_off = static_cast<uint32_t>(
+        (g * ga.dout_strides[1] + i * ga.dout_strides[2] + d) * sizeof(T));
   }
-}
+  // Rows from `begin` on (a multiple of G); rows past the end repeat the last one
+  __device__ __forceinline__ void fetch(int begin, T* q_tile, T* d_tile) const {
+    const AttentionArgs& a = ga.a;
+    const T* q = static_cast<const T*>(a.q);
+    const T* dout = static_cast<const T*>(ga.dout);
+    const bool inside = begin + S::kKeys <= end && (a.near & 2) != 0;
+#pragma unroll
+    for (int n = 0; n < S::kPasses; ++n) {
+      const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+      const uint32_t to = row * L::kPitch * sizeof(T);
+      if (inside) {
+        const T* qp = q + row_offset(a.q_strides, b, hk, a.G, begin + row);
+        const T* dp = dout + row_offset(ga.dout_strides, b, hk, a.G, begin + row);
+        if (d < a.D) {
+          dma16(lds_address(q_tile) + to, q_off, qp);
+          dma16(lds_address(d_tile) + to, d_off, dp);
+        }
+      } else {
+        const int r =
+            min(begin + row + static_cast<int>(threadIdx.x & 63) / L::kPlaces, end - 1);
+        if (d < a.D) {
+          dma16_from(
+              lds_address(q_tile) + to, q + row_offset(a.q_strides, b, hk, a.G, r) + d);
+          dma16_from(
+              lds_address(d_tile) + to, dout + row_offset(ga.dout_strides, b, hk, a.G, r) + d);
+        }
+      }
+    }
+  }
+};
 
 template <typename T, int DT>
-__global__ __launch_bounds__(256) void attention_dkv_kernel(const AttentionGradArgs ga, int blocks) {
+__global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_dkv_kernel(const AttentionGradArgs ga, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int RT = S::kKeys; // rows of a tile
-  constexpr int kBoth = 2 * S::kTileBytes / sizeof(T);
+  constexpr int kBoth = 2 * S::kTile;
   // this lane's key and value: in registers, but for 256 floats, which are read again for
   // each tile (with both results they would need all 512 registers)
   constexpr bool kHeld = DT * sizeof(T) <= 512;
@@ -308,6 +335,10 @@ __global__ __launch_bounds__(256) void attention_dkv_kernel(const AttentionGradA
     return RowStats{a.lse[n], ga.delta[n], p0 + i};
   };
 
+  if (a.D < L::kPitch) {
+    clear_lds<T>(lds, 2 * kBoth);
+  }
+  const RowStream<T, DT> rows(ga, b, hk, end_row, wave, lane);
   floatx16 dk[DT / 32], dv[DT / 32];
   // (a masked row that is not finite: see attention_rows_kernel)
   for (int careful = 0;; careful = 1) {
@@ -321,8 +352,7 @@ __global__ __launch_bounds__(256) void attention_dkv_kernel(const AttentionGradA
       if (threadIdx.x < RT) {
         mine = stats_of(0);
       }
-      fetch_rows<T, DT>(
-          ga, b, hk, begin_row, min(begin_row + RT, end_row), lds, lds + kBoth / 2);
+      rows.fetch(begin_row, lds, lds + kBoth / 2);
     }
     for (int t = 0; t < tiles; ++t) {
       StatsTile<RT>& st = stats[t & 1];
@@ -342,8 +372,7 @@ __global__ __launch_bounds__(256) void attention_dkv_kernel(const AttentionGradA
           mine = stats_of(t + 1);
         }
         T* next = lds + ((t + 1) & 1) * kBoth;
-        fetch_rows<T, DT>(
-            ga, b, hk, begin + RT, min(begin + 2 * RT, end_row), next, next + kBoth / 2);
+        rows.fetch(begin + RT, next, next + kBoth / 2);
       }
       const int p_lo = st.p[0];
       const int p_hi = st.p[count - 1];

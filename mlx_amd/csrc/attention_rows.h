@@ -25,39 +25,93 @@ template <typename T, int DT>
 struct RowsShape {
   // keys of a tile: 16 KB of K and as much of V, 32 keys at least
   static constexpr int kKeys = DT * sizeof(T) <= 256 ? 64 : 32;
-  static constexpr int kTileBytes = kKeys * DT * sizeof(T);
-  static constexpr int kPasses = kTileBytes / (256 * 16); // loads of a thread per tile
+  static constexpr int kTile = kKeys * Tile<T, DT>::kPitch; // elements
+  static constexpr int kPasses = kKeys / Tile<T, DT>::kRowsOfPass;
 };
 
-// Fetches the rows of keys [begin, end) of k and v to LDS; rows past them repeat the last one,
-// so that nothing is read that no row sees.
-template <typename T, int DT, bool PAGED>
-__device__ __forceinline__ void fetch_keys(
-    const AttentionArgs& a, int b, int hk, int begin, int end, T* k_tile, T* v_tile) {
-  using S = RowsShape<T, DT>;
-  using L = Tile<T, DT>;
-  const T* k = static_cast<const T*>(a.k);
-  const T* v = static_cast<const T*>(a.v);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-  for (int n = 0; n < S::kPasses; ++n) {
-    const int u = n * 256 + threadIdx.x;
-    const int row = u / L::kUnits;
-    const int d = ((u % L::kUnits) ^ L::swizzle(row)) * L::kUnit;
-    const KeyRow r = key_row<PAGED>(a, b, hk, min(begin + row, end - 1));
-    const bool in = d < a.D;
-    const uint32_t to = (n * 256 + wave * 64) * 16;
-    dma16_from(lds_address(k_tile) + to, in ? static_cast<const void*>(k + r.k + d) : &kNoData);
-    dma16_from(lds_address(v_tile) + to, in ? static_cast<const void*>(v + r.v + d) : &kNoData);
+// Columns past D are not loaded: they are zero from the start.
+template <typename T>
+__device__ __forceinline__ void clear_lds(T* lds, int elements) {
+  for (int i = threadIdx.x * (16 / sizeof(T)); i < elements; i += 256 * (16 / sizeof(T))) {
+    *reinterpret_cast<uint4*>(lds + i) = make_uint4(0, 0, 0, 0);
   }
+  __syncthreads();
 }
 
+// Fetches tiles of keys and values to LDS, 16 bytes a lane, four waves beside each other.  What
+// differs between lanes is kept as 32-bit offsets, what differs between tiles is the same for all
+// lanes (the 16 keys from a multiple of 16 on are in one page): a load takes no vector arithmetic.
 template <typename T, int DT, bool PAGED>
-__global__ __launch_bounds__(256) void attention_rows_kernel(const AttentionArgs a, int blocks) {
+struct KeyStream {
+  using S = RowsShape<T, DT>;
+  using L = Tile<T, DT>;
+  const AttentionArgs& a;
+  int b, hk, length, wave;
+  int d;                 // this lane's column
+  uint32_t k_off, v_off; // bytes from the first row of a load
+  int ids = 0;           // PAGED: lane i has the page of keys 16 i .. 16 i + 15 of a tile
+
+  __device__ __forceinline__ KeyStream(
+      const AttentionArgs& args, int b_, int hk_, int length_, int wave_, int lane)
+      : a(args), b(b_), hk(hk_), length(length_), wave(wave_) {
+    const int row = lane / L::kPlaces;
+    d = ((lane % L::kPlaces) ^ L::swizzle(wave * L::kRowsOfLoad + row)) * L::kUnit;
+    k_off = static_cast<uint32_t>((row * a.k_strides[2] + d) * sizeof(T));
+    v_off = static_cast<uint32_t>((row * a.v_strides[2] + d) * sizeof(T));
+  }
+  // The pages of the tile from `begin` on, before the loads of the one before it
+  __device__ __forceinline__ void look_up(int begin) {
+    if constexpr (PAGED) {
+      int in_page;
+      const int lane = threadIdx.x & 63;
+      const int j = min(begin + 16 * (lane & (S::kKeys / 16 - 1)), a.keys - 1);
+      ids = min(max(a.table[b * a.table_stride + page_of(a, j, &in_page)], 0), a.pages - 1);
+    }
+  }
+  __device__ __forceinline__ void fetch(int begin, T* k_tile, T* v_tile) const {
+    const T* k = static_cast<const T*>(a.k) + hk * a.k_strides[1];
+    const T* v = static_cast<const T*>(a.v) + hk * a.v_strides[1];
+    const bool inside = begin + S::kKeys <= length && (a.near & 1) != 0;
+    if (inside) {
+#pragma unroll
+      for (int n = 0; n < S::kPasses; ++n) {
+        const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+        int64_t first = b;
+        int at = begin + row;
+        if constexpr (PAGED) {
+          first = __builtin_amdgcn_readlane(ids, row / 16);
+          page_of(a, at, &at);
+        }
+        const T* kp = k + first * a.k_strides[0] + at * a.k_strides[2];
+        const T* vp = v + first * a.v_strides[0] + at * a.v_strides[2];
+        const uint32_t to = row * L::kPitch * sizeof(T);
+        if (d < a.D) {
+          dma16(lds_address(k_tile) + to, k_off, kp);
+          dma16(lds_address(v_tile) + to, v_off, vp);
+        }
+      }
+    } else { // keys past the end repeat the last one
+#pragma unroll
+      for (int n = 0; n < S::kPasses; ++n) {
+        const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+        const int j = begin + row + static_cast<int>(threadIdx.x & 63) / L::kPlaces;
+        const KeyRow r = key_row<PAGED>(a, b, 0, min(j, length - 1));
+        const uint32_t to = row * L::kPitch * sizeof(T);
+        if (d < a.D) {
+          dma16_from(lds_address(k_tile) + to, k + r.k + d);
+          dma16_from(lds_address(v_tile) + to, v + r.v + d);
+        }
+      }
+    }
+  }
+};
+
+template <typename T, int DT, bool PAGED>
+__global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_rows_kernel(const AttentionArgs a, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
-  constexpr int kBoth = 2 * S::kTileBytes / sizeof(T); // K and V
+  constexpr int kBoth = 2 * S::kTile; // K and V
   __shared__ __align__(16) T lds[2 * kBoth];
 
   const int lane = threadIdx.x & 63;
@@ -111,6 +165,10 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(const AttentionArgs
 
   floatx16 o[DT / 32];
   float m, l; // of this lane's half of the keys: the maximum is common, the sum is its own
+  if (a.D < L::kPitch) {
+    clear_lds<T>(lds, 2 * kBoth);
+  }
+  KeyStream<T, DT, PAGED> keys(a, b, hk, length, wave, lane);
   // A masked value that is not finite would reach rows that do not see it, as 0 * inf: where a
   // result is not finite the rows are done again, those values apart from the products.
   for (int careful = 0;; careful = 1) {
@@ -120,24 +178,25 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(const AttentionArgs
     }
     m = -INFINITY;
     l = 0.0f;
-    int begin, end;
     if (t0 < t1) {
-      tile_of(range, t0, KT, &begin, &end);
-      fetch_keys<T, DT, PAGED>(a, b, hk, begin, end, lds, lds + kBoth / 2);
+      const int begin = tile_of(range, t0, KT).begin;
+      keys.look_up(begin);
+      keys.fetch(begin, lds, lds + kBoth / 2);
+      keys.look_up(tile_of(range, t0 + 1, KT).begin);
     }
     for (int t = t0; t < t1; ++t) {
       wait_loads();
       __syncthreads();
       const T* k_tile = lds + ((t - t0) & 1) * kBoth;
       const T* v_tile = k_tile + kBoth / 2;
-      tile_of(range, t, KT, &begin, &end);
+      const KeyTile tile = tile_of(range, t, KT);
       if (t + 1 < t1) {
-        int b1, e1;
-        tile_of(range, t + 1, KT, &b1, &e1);
         T* next = lds + ((t + 1 - t0) & 1) * kBoth;
-        fetch_keys<T, DT, PAGED>(a, b, hk, b1, e1, next, next + kBoth / 2);
+        keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
+        keys.look_up(tile_of(range, t + 2, KT).begin);
       }
-      if (!works || none_seen(begin, end, p_lo, p_hi, a.window, a.keep)) {
+      const int begin = tile.begin;
+      if (!works || none_seen(begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
         continue;
       }
       floatx16 s[KT / 32];
@@ -149,16 +208,16 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(const AttentionArgs
           s[g] = mma32<T>(L::load_rows(k_tile, 32 * g + (lane & 31), 2 * c + h), q[c], s[g]);
         }
       }
-      const bool whole =
-          end - begin == KT && all_seen(begin, end, p_lo, p_hi, a.window, a.keep);
+      const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
       if (!whole) {
-        const int last = min(p, end - 1);
+        const int last = min(p, tile.end - 1);
 #pragma unroll
         for (int g = 0; g < KT / 32; ++g) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int j = begin + 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            s[g][i] = j <= last && (j >= seen_from || j < a.keep) ? s[g][i] : -INFINITY;
+            const bool sees = j >= tile.low && j <= last && (j >= seen_from || j < a.keep);
+            s[g][i] = sees ? s[g][i] : -INFINITY;
           }
         }
       }
@@ -209,7 +268,7 @@ __global__ __launch_bounds__(256) void attention_rows_kernel(const AttentionArgs
         }
       }
       if (apart) {
-        for (int n = 0; n < end - begin; ++n) {
+        for (int n = max(tile.low - begin, 0); n < tile.end - begin; ++n) {
           const int j = begin + n;
           const bool sees = j <= p && (j >= seen_from || j < a.keep);
 #pragma unroll
