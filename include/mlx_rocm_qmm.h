@@ -785,7 +785,8 @@ int mlxrocm_window_attention(
     void* workspace,
     size_t workspace_bytes,
     mlxrocm_stream_t stream);
-size_t mlxrocm_window_attention_vjp_workspace_size(int B, int Hq, int Lq);
+size_t mlxrocm_window_attention_vjp_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype);
 int mlxrocm_window_attention_vjp(
     const void* q,
     const void* k,
@@ -867,9 +868,21 @@ int mlxrocm_paged_cache_update(
     mlxrocm_stream_t stream);
 
 /*
- * The launches that either attention makes of a shape (keys: Lk, or table_width * page_size),
- * written to plan without touching a device, as mlxrocm_qmm_plan does.
+ * The launches that either attention makes of a shape (keys: Lk, or table_width * page_size), and
+ * those of the gradients, written to plan without touching a device, as mlxrocm_qmm_plan does.
  */
+int mlxrocm_window_attention_vjp_plan(
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    int window,
+    int keep,
+    int dtype,
+    char* plan,
+    size_t plan_bytes);
 int mlxrocm_attention_plan(
     int B,
     int Hq,

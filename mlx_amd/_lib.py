@@ -56,7 +56,7 @@ SIGNATURES = {
     ),
     "mlxrocm_window_attention_workspace_size": (_sz, [_i] * 9),
     "mlxrocm_window_attention": (_i, [_p] * 6 + [_i] * 6 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
-    "mlxrocm_window_attention_vjp_workspace_size": (_sz, [_i] * 3),
+    "mlxrocm_window_attention_vjp_workspace_size": (_sz, [_i] * 9),
     "mlxrocm_window_attention_vjp": (
         _i,
         [_p] * 10 + [_i] * 6 + [_p, _f] + [_i] * 3 + [_p, _sz, _p],
@@ -64,6 +64,7 @@ SIGNATURES = {
     "mlxrocm_paged_attention_workspace_size": (_sz, [_i] * 9),
     "mlxrocm_paged_attention": (_i, [_p] * 6 + [_i] * 8 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
     "mlxrocm_paged_cache_update": (_i, [_p] * 6 + [_i] * 7 + [_p, _i, _p]),
+    "mlxrocm_window_attention_vjp_plan": (_i, [_i] * 9 + [ctypes.c_char_p, _sz]),
     "mlxrocm_attention_plan": (_i, [_i] * 9 + [ctypes.c_char_p, _sz]),
     "mlxrocm_verify_draft_workspace_size": (_sz, [_i] * 2),
     "mlxrocm_verify_draft": (_i, [_p] * 8 + [_i] * 3 + [_p, _i, _p, _sz, _p]),
@@ -246,6 +247,14 @@ def attention_plan(B, Hq, Hkv, Lq, keys, D, window=1 << 30, keep=0, dtype=BFLOAT
     e.g. "attention_few(dim=128,rows=16,splits=2)+attention_join"."""
     buf = ctypes.create_string_buffer(512)
     rc = load().mlxrocm_attention_plan(B, Hq, Hkv, Lq, keys, D, window, keep, dtype, buf, len(buf))
+    return rc, buf.value.decode()
+
+
+def attention_vjp_plan(B, Hq, Hkv, Lq, Lk, D, window=1 << 30, keep=0, dtype=BFLOAT16):
+    """The same for the gradients of window_attention."""
+    buf = ctypes.create_string_buffer(512)
+    rc = load().mlxrocm_window_attention_vjp_plan(
+        B, Hq, Hkv, Lq, Lk, D, window, keep, dtype, buf, len(buf))
     return rc, buf.value.decode()
 
 

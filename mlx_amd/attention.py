@@ -131,13 +131,15 @@ class _WindowAttentionVjp(torch.autograd.Function):
         dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
         B, Hq, Lq, D = q.shape
         Hkv, Lk = k.shape[1:3]
-        size = lib.mlxrocm_window_attention_vjp_workspace_size(B, Hq, Lq)
+        code = _DTYPE_CODE[q.dtype]
+        size = lib.mlxrocm_window_attention_vjp_workspace_size(
+            B, Hq, Hkv, Lq, Lk, D, *ctx.args[1:], code)
         workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
         _lib.check(lib.mlxrocm_window_attention_vjp(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
             dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             None if lengths is None else lengths.data_ptr(), B, Hq, Hkv, Lq, Lk, D,
-            _array(_strides(q, k, v, out, dout, dq, dk, dv)), *ctx.args, _DTYPE_CODE[q.dtype],
+            _array(_strides(q, k, v, out, dout, dq, dk, dv)), *ctx.args, code,
             workspace.data_ptr(), size, _stream_ptr(q)))
         return dq, dk, dv, None, None, None, None
 

@@ -45,10 +45,25 @@ struct AttentionArgs {
   float scale_log2; // |scale| log2(e)
   uint32_t q_sign;  // 0x80008000 (16-bit types), 0x80000000 (float32) where scale < 0
   int window, keep;
+  int g_log2; // of a power of two of heads (near & 2)
   int near; // the rows of one load lie within 32-bit offsets: of keys (1), of queries (2)
   int splits;
   float* part_out; // [splits, B Hkv, R, D], not yet divided by the sums
   float2* part_ml; // [splits, B Hkv, R]: maximum (log2 units) and sum
+};
+
+// How the gradients' sums are cut, for work enough at once: those of dq over keys, those of dk and
+// dv over rows.  The blocks of the keys that every later row sees (under a window) have many more
+// rows than the others.
+struct GradPlan {
+  int dq_splits;
+  int wide_blocks; // blocks of kept keys, with wide_splits runs each; the others have splits
+  int wide_splits, splits;
+  int blocks; // of keys
+  __host__ __device__ int pieces() const {
+    return wide_blocks * wide_splits + (blocks - wide_blocks) * splits;
+  }
+  __host__ __device__ bool dkv_split() const { return wide_splits > 1 || splits > 1; }
 };
 
 // The gradients' further operands.
@@ -61,7 +76,12 @@ struct AttentionGradArgs {
   float* delta; // [B, Hq, Lq]: sum over D of dout * out
   int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
   float scale;
+  GradPlan plan;
+  float* part_dq;  // [splits, B Hkv, R, D] where dq is split
+  float* part_dkv; // [piece, key of the block, 2, D] where dk and dv are
 };
+
+constexpr int kGradBlock = 128; // rows or keys of a workgroup
 
 // Whether the few-rows kernel takes a call (else the tiles of 128 rows).
 constexpr int kFewRows = 64;
@@ -74,6 +94,7 @@ int launch_attention_rows_f32(const AttentionArgs& a, hipStream_t s);
 int launch_attention_rows_f16(const AttentionArgs& a, hipStream_t s);
 int launch_attention_rows_bf16(const AttentionArgs& a, hipStream_t s);
 int launch_attention_join(const AttentionArgs& a, int dtype, hipStream_t s);
+int launch_attention_grad_join(const AttentionGradArgs& g, int dtype, hipStream_t s);
 int launch_attention_grad_f32(const AttentionGradArgs& g, hipStream_t s);
 int launch_attention_grad_f16(const AttentionGradArgs& g, hipStream_t s);
 int launch_attention_grad_bf16(const AttentionGradArgs& g, hipStream_t s);
@@ -210,20 +231,15 @@ __device__ __forceinline__ bool not_finite(float v) {
   return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
 }
 
-// The fragment with zeros for infinities and NaN.
+// The values of a dword with zeros for infinities and NaN.
 template <typename T>
-__device__ __forceinline__ void drop_not_finite(Frag<T>& f) {
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(f.w) / 4); ++i) {
-    if constexpr (sizeof(T) == 4) {
-      f.w[i] = not_finite(f.w[i]) ? 0.0f : f.w[i];
-    } else {
-      constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
-      uint32_t w = f.w[i];
-      w = (w & kExp) == kExp ? w & 0xffff0000u : w;
-      w = (w & (kExp << 16)) == (kExp << 16) ? w & 0xffffu : w;
-      f.w[i] = w;
-    }
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+  if constexpr (sizeof(T) == 4) {
+    return not_finite(__uint_as_float(w)) ? 0 : w;
+  } else {
+    constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+    w = (w & kExp) == kExp ? w & 0xffff0000u : w;
+    return (w & (kExp << 16)) == (kExp << 16) ? w & 0xffffu : w;
   }
 }
 
@@ -240,6 +256,28 @@ __device__ __forceinline__ float max_halves(float v) {
 __device__ __forceinline__ float sum_halves(float v) {
   const float2 r = both_halves(v);
   return r.x + r.y;
+}
+
+// N products whose LDS operands are read AHEAD products ahead: use(i, operand) and what it does
+// beside the product stay in their order.  Left alone, the compiler reads an operand, waits for
+// it, multiplies and reads the next: that takes the fewest registers.
+template <typename T, int N, int AHEAD = 4, typename Read, typename Use>
+__device__ __forceinline__ void read_ahead(const Read& read, const Use& use) {
+  constexpr int kAhead = sizeof(T) == 4 ? 1 : N < AHEAD ? N : AHEAD;
+  Frag<T> ring[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    ring[i] = read(i);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    use(i, ring[i % kAhead]);
+    if (i + kAhead < N) {
+      ring[i % kAhead] = read(i + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // ---- which keys ----------------------------------------------------------------
@@ -297,6 +335,20 @@ __device__ __forceinline__ bool none_seen(
     int begin, int end, int lo, int hi, int window, int keep) {
   return begin > hi || (lo - (end - 1) >= window && begin >= keep);
 }
+
+// Which of its keys a lane sees, n = key - begin - (its own first): counted from there, each
+// comparison is with a constant and no key's number takes a register.
+struct Seen {
+  int low, last, from, keep;
+  __device__ __forceinline__ Seen(const AttentionArgs& a, const KeyTile& t, int p, int own)
+      : low(t.low - t.begin - own),
+        last(min(p, t.end - 1) - t.begin - own),
+        from(p - a.window + 1 - t.begin - own),
+        keep(a.keep - t.begin - own) {}
+  __device__ __forceinline__ bool operator()(int n) const {
+    return n >= low && n <= last && (n >= from || n < keep);
+  }
+};
 
 // Divides by the page size: page_magic = 2^32 / page + 1 overshoots by one at most.
 __device__ __forceinline__ int page_of(const AttentionArgs& a, int j, int* in_page) {
@@ -375,12 +427,20 @@ struct Tile {
   static __device__ __forceinline__ int at(int row, int unit) {
     return row * kPitch + (unit ^ swizzle(row)) * kUnit;
   }
-  // elements 8 chunk .. 8 chunk + 7 of a row
-  static __device__ __forceinline__ Frag<T> load_rows(const T* tile, int row, int chunk) {
+  // Elements 16 c + 8 h .. 16 c + 8 h + 7 of row `row` + lane % 32, h = lane / 32; row: a multiple of
+  // 32.  Written so that few addresses differ by more than an offset in the instruction: a
+  // unit's three low bits are exclusive ored with what depends on the lane alone.
+  static __device__ __forceinline__ Frag<T> load_rows(const T* tile, int row, int c, int lane) {
+    const int r = lane & 31;
+    const int h = lane >> 5;
+    constexpr int kOf8 = 8 / kUnit; // units of 8 elements
+    const int t = (kOf8 * h) ^ swizzle(r);
+    const int unit = 2 * kOf8 * c;
+    const T* p = tile + row * kPitch + (unit & ~7) * kUnit + r * kPitch;
     if constexpr (sizeof(T) == 4) {
       Frag<T> f;
-      const float4 a = *reinterpret_cast<const float4*>(tile + at(row, 2 * chunk));
-      const float4 b = *reinterpret_cast<const float4*>(tile + at(row, 2 * chunk + 1));
+      const float4 a = *reinterpret_cast<const float4*>(p + ((unit & 7) ^ t) * kUnit);
+      const float4 b = *reinterpret_cast<const float4*>(p + ((unit & 7) ^ t ^ 1) * kUnit);
       f.w[0] = a.x;
       f.w[1] = a.y;
       f.w[2] = a.z;
@@ -391,11 +451,12 @@ struct Tile {
       f.w[7] = b.w;
       return f;
     } else {
-      return load_frag<T>(tile + at(row, chunk));
+      return load_frag<T>(p + ((unit & 7) ^ t) * kUnit);
     }
   }
-  // element d + lane % 32 of rows row + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}: the transposing
-  // read takes four rows of 16 columns from 16 lanes' addresses and gives each lane a column
+  // element d + lane % 32 of rows row + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}; row: a multiple of
+  // 16, d of 32.  The transposing read takes four rows of 16 columns from 16 lanes' addresses and
+  // gives each lane a column.
   static __device__ __forceinline__ Frag<T> load_cols(const T* tile, int row, int d, int lane) {
     Frag<T> f;
     const int h = lane >> 5;
@@ -407,13 +468,15 @@ struct Tile {
         f.w[j] = tile[at(r, c / 4) + c % 4];
       }
     } else {
-      const int c = d + (lane & 16) + 4 * (lane & 3);
+      const int y = lane >> 2 & 3;
+      const int t = ((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ swizzle(4 * h + y);
+      const int unit = d / 8;
+      const T* p = tile + row * kPitch + (unit & ~7) * kUnit + (4 * h + y) * kPitch +
+          ((unit & 7) ^ t) * kUnit + 4 * (lane & 1);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int r = row + 8 * half + 4 * h + (lane >> 2 & 3);
-        const T* p = tile + at(r, c / 8) + (c & 4);
         const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) shortx4*)(p));
+            (__attribute__((address_space(3))) shortx4*)(p + half * 8 * kPitch));
         const uint2 u = __builtin_bit_cast(uint2, x);
         f.w[2 * half] = u.x;
         f.w[2 * half + 1] = u.y;
@@ -436,6 +499,65 @@ __device__ __forceinline__ void dma16_from(uint32_t at, const void* p) {
 }
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// ---- what is not finite ------------------------------------------------------------
+// A masked value that is not finite would reach rows that do not see it: 0 * inf.  Tiles that not
+// all rows see are looked through for such values (the exponent's bits, plus one, carry into the
+// sign's place).  Where there are any, the product takes zeros for them, and when the result
+// is stored they are added to it for the rows that do see them.  (Added twice they change nothing.)
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  constexpr uint32_t kOne = sizeof(T) == 4           ? 0x00800000u
+      : std::is_same<T, bf16_t>::value ? 0x00800080u
+                                       : 0x04000400u;
+  constexpr uint32_t kMagnitude = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  return (w & kMagnitude) + kOne;
+}
+template <typename T>
+__device__ __forceinline__ bool is_odd(uint32_t bits) {
+  return (bits & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u)) != 0;
+}
+
+// Whether this thread's 256th of a tile in LDS has one
+template <typename T, int ELEMENTS>
+__device__ __forceinline__ bool odd_values(const T* tile) {
+  constexpr int kUnit = 16 / sizeof(T);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < ELEMENTS / (256 * kUnit); ++i) {
+    const uint4 w =
+        *reinterpret_cast<const uint4*>(tile + (i * 256 + static_cast<int>(threadIdx.x)) * kUnit);
+    bits |= odd_bits<T>(w.x) | odd_bits<T>(w.y) | odd_bits<T>(w.z) | odd_bits<T>(w.w);
+  }
+  return is_odd<T>(bits);
+}
+
+// This thread's 256th of a tile, with zeros for what is not finite
+template <typename T, int ELEMENTS>
+__device__ __forceinline__ void copy_finite(const T* from, T* to) {
+  constexpr int kUnit = 16 / sizeof(T);
+  for (int i = threadIdx.x * kUnit; i < ELEMENTS; i += 256 * kUnit) {
+    const uint4 w = *reinterpret_cast<const uint4*>(from + i);
+    *reinterpret_cast<uint4*>(to + i) = make_uint4(
+        finite_part<T>(w.x), finite_part<T>(w.y), finite_part<T>(w.z), finite_part<T>(w.w));
+  }
+}
+
+// p[at] += x in the type of p
+template <typename T>
+__device__ __forceinline__ void add_to(T* p, float x) {
+  *p = from_f32<T>(to_f32(*p) + x);
+}
+
+// Stores of this workgroup are behind, its threads may add to them
+__device__ __forceinline__ void after_stores() {
+  __threadfence_block();
+  __syncthreads();
+}
+
+__device__ __forceinline__ bool sees_key(const AttentionArgs& a, int p, int j) {
+  return j <= p && (p - j < a.window || j < a.keep);
 }
 
 #endif // __HIPCC__

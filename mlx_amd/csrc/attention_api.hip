@@ -22,7 +22,7 @@ int64_t heads_of(const AttentionArgs& a) {
 
 // Runs that the keys of a row are cut into: as many as give the chip work, with some tiles left
 // to each.
-int splits_of(const AttentionArgs& a) {
+int splits_of(const AttentionArgs& a, int dtype) {
   const int64_t span =
       std::min<int64_t>(a.keys, static_cast<int64_t>(a.window) + a.keep + a.Lq);
   int64_t splits;
@@ -30,7 +30,7 @@ int splits_of(const AttentionArgs& a) {
     splits = std::min<int64_t>((1024 + heads_of(a) - 1) / heads_of(a), span / 256);
   } else {
     const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads_of(a);
-    splits = std::min<int64_t>(512 / blocks, span / 512);
+    splits = std::min<int64_t>(512 / blocks, span / (dtype == MLXROCM_FLOAT32 ? 64 : 512));
   }
   return static_cast<int>(std::min<int64_t>(std::max<int64_t>(splits, 1), kMostSplits));
 }
@@ -39,14 +39,60 @@ size_t round256(size_t n) {
   return (n + 255) / 256 * 256;
 }
 
-size_t workspace_of(const AttentionArgs& a) {
-  const int splits = splits_of(a);
+size_t workspace_of(const AttentionArgs& a, int dtype) {
+  const int splits = splits_of(a, dtype);
   if (splits == 1) {
     return 0;
   }
   const size_t rows = static_cast<size_t>(splits) * a.B * a.Hq * a.Lq;
   return round256(rows * a.D * sizeof(float)) + rows * sizeof(float2);
 }
+
+// The cuts of the gradients' sums: parts of some tiles each, and a thousand workgroups if there
+// are as many.
+GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
+  GradPlan p{};
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
+  const int64_t row_blocks = (rows + kGradBlock - 1) / kGradBlock;
+  p.blocks = (a.keys + kGradBlock - 1) / kGradBlock;
+  // float32's matrix instruction takes 16 times as long: less is enough for a part
+  const int64_t least = dtype == MLXROCM_FLOAT32 ? 64 : 1024;
+  const int64_t reach = static_cast<int64_t>(a.window) + kGradBlock; // tokens
+  const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
+  const auto parts = [&](int64_t blocks, int64_t length) {
+    const int64_t wanted = (1024 + blocks * heads_of(a) - 1) / std::max<int64_t>(blocks * heads_of(a), 1);
+    return static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({wanted, length / least, int64_t{kMostSplits}})));
+  };
+  p.dq_splits = row_blocks > 0 ? parts(row_blocks, span) : 1;
+  const int64_t seen_by = std::min<int64_t>(a.Lq, reach) * a.G;
+  if (a.window < a.keys && seen_by < rows) {
+    p.wide_blocks = static_cast<int>(std::min<int64_t>(
+        p.blocks, (static_cast<int64_t>(a.keep) + kGradBlock - 1) / kGradBlock));
+  }
+  p.splits = p.blocks > 0 ? parts(p.blocks, seen_by) : 1;
+  // runs no longer than the others'
+  p.wide_splits = p.wide_blocks == 0
+      ? p.splits
+      : static_cast<int>(std::min<int64_t>(
+            kMostSplits, std::max<int64_t>(1, rows * p.splits / std::max<int64_t>(seen_by, 1))));
+  return p;
+}
+
+// delta, then the partial sums of dq, then those of dk and dv
+struct GradWorkspace {
+  size_t part_dq, part_dkv, total;
+  GradWorkspace(const AttentionArgs& a, const GradPlan& p) {
+    const size_t rows = static_cast<size_t>(a.B) * a.Hq * a.Lq;
+    part_dq = round256(rows * sizeof(float));
+    part_dkv = part_dq +
+        (p.dq_splits > 1 ? round256(rows * a.D * p.dq_splits * sizeof(float)) : 0);
+    total = part_dkv +
+        (p.dkv_split() ? static_cast<size_t>(heads_of(a)) * p.pieces() * kGradBlock * 2 * a.D *
+                 sizeof(float)
+                       : 0);
+  }
+};
 
 // Shapes alone; `name` for messages
 int check_shape(const char* name, const AttentionArgs& a, int dtype) {
@@ -146,10 +192,10 @@ bool empty(const AttentionArgs& a) {
 
 int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t bytes,
         hipStream_t s) {
-  a.splits = splits_of(a);
+  a.splits = splits_of(a, dtype);
   set_near(a, dtype);
   if (a.splits > 1 && !rehearsing()) {
-    const size_t need = workspace_of(a);
+    const size_t need = workspace_of(a, dtype);
     if (workspace == nullptr || bytes < need) {
       return fail(
           MLXROCM_INVALID_ARGUMENT, "[%s] workspace of %zu bytes, %zu needed", name, bytes, need);
@@ -174,6 +220,14 @@ int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t b
   return a.splits > 1 ? launch_attention_join(a, dtype, s) : static_cast<int>(MLXROCM_OK);
 }
 
+int run_grad(const AttentionGradArgs& g, int dtype, hipStream_t s) {
+  TRY(dtype == MLXROCM_FLOAT32       ? launch_attention_grad_f32(g, s)
+          : dtype == MLXROCM_FLOAT16 ? launch_attention_grad_f16(g, s)
+                                     : launch_attention_grad_bf16(g, s));
+  return g.plan.dq_splits > 1 || g.plan.dkv_split() ? launch_attention_grad_join(g, dtype, s)
+                                                    : static_cast<int>(MLXROCM_OK);
+}
+
 } // namespace
 
 } // namespace mlxrocm
@@ -183,7 +237,7 @@ extern "C" size_t mlxrocm_window_attention_workspace_size(
   using namespace mlxrocm;
   const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
   return check_shape("window_attention", a, dtype) != MLXROCM_OK || empty(a) ? 0
-                                                                             : workspace_of(a);
+                                                                             : workspace_of(a, dtype);
 }
 
 extern "C" int mlxrocm_window_attention(
@@ -238,8 +292,13 @@ extern "C" int mlxrocm_window_attention(
   return run(name, a, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t mlxrocm_window_attention_vjp_workspace_size(int B, int Hq, int Lq) {
-  return static_cast<size_t>(std::max(B, 0)) * std::max(Hq, 0) * std::max(Lq, 0) * sizeof(float);
+extern "C" size_t mlxrocm_window_attention_vjp_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype) {
+  using namespace mlxrocm;
+  const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
+  return check_shape("window_attention_vjp", a, dtype) != MLXROCM_OK
+      ? 0
+      : GradWorkspace(a, grad_plan_of(a, dtype)).total;
 }
 
 extern "C" int mlxrocm_window_attention_vjp(
@@ -291,7 +350,6 @@ extern "C" int mlxrocm_window_attention_vjp(
   g.dq = dq;
   g.dk = dk;
   g.dv = dv;
-  g.delta = static_cast<float*>(workspace);
   g.scale = scale;
   take(a.q_strides, strides);
   take(a.k_strides, strides + 3);
@@ -309,12 +367,22 @@ extern "C" int mlxrocm_window_attention_vjp(
     if (lse == nullptr) {
       return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer: lse", name);
     }
-    const size_t need = mlxrocm_window_attention_vjp_workspace_size(B, Hq, Lq);
-    if (workspace == nullptr || workspace_bytes < need) {
+  }
+  g.plan = grad_plan_of(a, dtype);
+  const GradWorkspace parts(a, g.plan);
+  if (parts.total > 0) {
+    if (workspace == nullptr || workspace_bytes < parts.total) {
       return fail(
           MLXROCM_INVALID_ARGUMENT, "[%s] workspace of %zu bytes, %zu needed", name,
-          workspace_bytes, need);
+          workspace_bytes, parts.total);
     }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+      return fail(MLXROCM_INVALID_ARGUMENT, "[%s] workspace is not aligned to 16 bytes", name);
+    }
+    char* at = static_cast<char*>(workspace);
+    g.delta = static_cast<float*>(workspace);
+    g.part_dq = reinterpret_cast<float*>(at + parts.part_dq);
+    g.part_dkv = reinterpret_cast<float*>(at + parts.part_dkv);
   }
   if (Lk > 0) {
     TRY(check_operand(name, "k", k, a.k_strides, dtype));
@@ -327,18 +395,18 @@ extern "C" int mlxrocm_window_attention_vjp(
   if ((a.G & (a.G - 1)) == 0 && near(a.q_strides, dtype, a.G) &&
       near(g.dout_strides, dtype, a.G)) {
     a.near |= 2;
+    a.g_log2 = __builtin_ctz(a.G);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == MLXROCM_FLOAT32    ? launch_attention_grad_f32(g, s)
-      : dtype == MLXROCM_FLOAT16 ? launch_attention_grad_f16(g, s)
-                                 : launch_attention_grad_bf16(g, s);
+  TRY(run_grad(g, dtype, s));
+  return MLXROCM_OK;
 }
 
 extern "C" size_t mlxrocm_paged_attention_workspace_size(
     int B, int Hq, int Hkv, int Lq, int D, int max_keys, int window, int keep, int dtype) {
   using namespace mlxrocm;
   const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, max_keys, D, window, keep);
-  return check_shape("paged_attention", a, dtype) != MLXROCM_OK || empty(a) ? 0 : workspace_of(a);
+  return check_shape("paged_attention", a, dtype) != MLXROCM_OK || empty(a) ? 0 : workspace_of(a, dtype);
 }
 
 extern "C" int mlxrocm_paged_attention(
@@ -435,4 +503,26 @@ extern "C" int mlxrocm_attention_plan(
   TRY(check_shape("attention_plan", a, dtype));
   return empty(a) ? static_cast<int>(MLXROCM_OK)
                   : run("attention_plan", a, dtype, nullptr, 0, nullptr);
+}
+
+extern "C" int mlxrocm_window_attention_vjp_plan(
+    int B,
+    int Hq,
+    int Hkv,
+    int Lq,
+    int Lk,
+    int D,
+    int window,
+    int keep,
+    int dtype,
+    char* plan,
+    size_t plan_bytes) {
+  using namespace mlxrocm;
+  RehearsalScope rehearsal(plan, plan_bytes);
+  AttentionGradArgs g{};
+  g.a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
+  TRY(check_shape("window_attention_vjp_plan", g.a, dtype));
+  g.plan = grad_plan_of(g.a, dtype);
+  return B == 0 || Hq == 0 || (Lq == 0 && Lk == 0) ? static_cast<int>(MLXROCM_OK)
+                                                   : run_grad(g, dtype, nullptr);
 }

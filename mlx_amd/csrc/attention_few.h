@@ -142,8 +142,10 @@ template <typename T, int DT, int NT, bool PAGED>
 __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs a) {
   using S = FewShape<T, DT>;
   constexpr int KT = kFewKeys;
-  __shared__ float join_o[4][16][DT + 4];
-  __shared__ float join_m[4][16], join_l[4][16];
+  __shared__ struct { // the waves' results of 16 rows, while they are joined
+    float o[4][16][DT + 4];
+    float m[4][16], l[4][16];
+  } join;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -185,132 +187,105 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
 
   floatx4 o[NT][S::kGroups][S::kE];
   float m[NT], l[NT];
-  // (a masked value that is not finite: see attention_rows_kernel)
-  for (int careful = 0;; careful = 1) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m[n] = -INFINITY;
-      l[n] = 0.0f;
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < S::kGroups; ++x) {
+    for (int x = 0; x < S::kGroups; ++x) {
 #pragma unroll
-        for (int e = 0; e < S::kE; ++e) {
-          o[n][x][e] = floatx4{};
-        }
+      for (int e = 0; e < S::kE; ++e) {
+        o[n][x][e] = floatx4{};
       }
     }
-    for (int t = t0 + wave; t < t1; t += 4) {
-      const KeyTile at = tile_of(range, t, KT);
-      const int begin = at.begin;
-      const int low = at.low;
-      const int end = at.end;
-      FewTile<T, DT> tile;
-      load_tile<T, DT, PAGED>(a, b, hk, begin, low, end, lane, tile);
-      const bool whole = whole_tile(a, at, KT, p_lo, p_hi);
-      Frag<T> w[NT];
+  }
+  bool odd = false; // some value was left out of the products
+  for (int t = t0 + wave; t < t1; t += 4) {
+    const KeyTile at = tile_of(range, t, KT);
+    const int begin = at.begin;
+    const int low = at.low;
+    const int end = at.end;
+    FewTile<T, DT> tile;
+    load_tile<T, DT, PAGED>(a, b, hk, begin, low, end, lane, tile);
+    const bool whole = whole_tile(a, at, KT, p_lo, p_hi);
+    Frag<T> w[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        floatx4 s[2];
+    for (int n = 0; n < NT; ++n) {
+      floatx4 s[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[x] = floatx4{};
+      for (int x = 0; x < 2; ++x) {
+        s[x] = floatx4{};
 #pragma unroll
-          for (int c = 0; c < DT / 32; ++c) {
-            s[x] = mma16<T>(tile.k[x][c], q[n][c], s[x]);
-          }
+        for (int c = 0; c < DT / 32; ++c) {
+          s[x] = mma16<T>(tile.k[x][c], q[n][c], s[x]);
         }
-        if (!whole) {
-          const int last = min(p[n], end - 1);
-          const int seen_from = p[n] - a.window + 1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int j = begin + 16 * (i / 4) + 4 * g + i % 4;
-            const bool sees = j >= low && j <= last && (j >= seen_from || j < a.keep);
-            s[i / 4][i % 4] = sees ? s[i / 4][i % 4] : -INFINITY;
-          }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) {
-          top = fmaxf(top, s[i / 4][i % 4]);
-        }
-        top *= a.scale_log2;
-        if (__any(top > m[n])) {
-          const float now = fmaxf(m[n], max_quarters(top));
-          const float by = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
-          m[n] = now;
-          l[n] *= by;
-#pragma unroll
-          for (int x = 0; x < S::kGroups; ++x) {
-#pragma unroll
-            for (int e = 0; e < S::kE; ++e) {
-              o[n][x][e] *= by;
-            }
-          }
-        }
-        const float less = m[n] == -INFINITY ? 0.0f : m[n];
-        float e[8];
+      }
+      if (!whole) {
+        const Seen sees(a, at, p[n], 4 * g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.scale_log2, -less));
-          l[n] += e[i];
-        }
-        w[n] = frag_of<T>(e);
-      }
-      const bool apart = careful != 0 && !whole;
-#pragma unroll
-      for (int x = 0; x < S::kGroups; ++x) {
-#pragma unroll
-        for (int e = 0; e < S::kE; ++e) {
-          Frag<T> f = column<T, DT>(tile.v[x], e);
-          if (apart) {
-            drop_not_finite<T>(f);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            o[n][x][e] = mma16<T>(f, w[n], o[n][x][e]);
-          }
+          s[i / 4][i % 4] = sees(16 * (i / 4) + i % 4) ? s[i / 4][i % 4] : -INFINITY;
         }
       }
-      if (apart) {
-        for (int j = max(begin, low); j < end; ++j) {
-          const T* v = static_cast<const T*>(a.v) + key_row<PAGED>(a, b, hk, j).v;
+      float top = s[0][0];
 #pragma unroll
-          for (int x = 0; x < S::kGroups; ++x) {
+      for (int i = 1; i < 8; ++i) {
+        top = fmaxf(top, s[i / 4][i % 4]);
+      }
+      top *= a.scale_log2;
+      if (__any(top > m[n])) {
+        const float now = fmaxf(m[n], max_quarters(top));
+        const float by = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - now);
+        m[n] = now;
+        l[n] *= by;
 #pragma unroll
-            for (int e = 0; e < S::kE; ++e) {
+        for (int x = 0; x < S::kGroups; ++x) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d = (16 * x + 4 * g + i) * S::kE + e;
-                const float value = d < a.D ? to_f32(v[d]) : 0.0f;
+          for (int e = 0; e < S::kE; ++e) {
+            o[n][x][e] *= by;
+          }
+        }
+      }
+      const float less = m[n] == -INFINITY ? 0.0f : m[n];
+      float e[8];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  const bool sees =
-                      j <= p[n] && (j >= p[n] - a.window + 1 || j < a.keep);
-                  o[n][x][e][i] += sees && not_finite(value) ? value : 0.0f;
-                }
-              }
-            }
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.scale_log2, -less));
+        l[n] += e[i];
+      }
+      w[n] = frag_of<T>(e);
+    }
+    // (rows of one position see the same keys, and those alone are loaded)
+    if (a.Lq > 1 && !whole) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int x = 0; x < S::kGroups * 8; ++x) {
+#pragma unroll
+        for (int e = 0; e < S::kDwords; ++e) {
+          bits |= odd_bits<T>(tile.v[x / 8][x % 8][e]);
+        }
+      }
+      if (__any(is_odd<T>(bits))) {
+        odd = true;
+#pragma unroll
+        for (int x = 0; x < S::kGroups * 8; ++x) {
+#pragma unroll
+          for (int e = 0; e < S::kDwords; ++e) {
+            tile.v[x / 8][x % 8][e] = finite_part<T>(tile.v[x / 8][x % 8][e]);
           }
         }
       }
     }
-    bool odd = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int x = 0; x < S::kGroups; ++x) {
 #pragma unroll
-      for (int x = 0; x < S::kGroups; ++x) {
+      for (int e = 0; e < S::kE; ++e) {
+        const Frag<T> f = column<T, DT>(tile.v[x], e);
 #pragma unroll
-        for (int e = 0; e < S::kE; ++e) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            odd = odd || not_finite(o[n][x][e][i]);
-          }
+        for (int n = 0; n < NT; ++n) {
+          o[n][x][e] = mma16<T>(f, w[n], o[n][x][e]);
         }
       }
-    }
-    if (careful != 0 || !__any(odd)) {
-      break;
     }
   }
 
@@ -319,8 +294,8 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
     const float sum = sum_quarters(l[n]);
     __syncthreads(); // the tile of rows before has been joined
     if (g == 0) {
-      join_m[wave][lane] = m[n];
-      join_l[wave][lane] = sum;
+      join.m[wave][lane] = m[n];
+      join.l[wave][lane] = sum;
     }
 #pragma unroll
     for (int x = 0; x < S::kGroups; ++x) {
@@ -328,7 +303,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
       for (int e = 0; e < S::kE; ++e) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          join_o[wave][lane & 15][(16 * x + 4 * g + i) * S::kE + e] = o[n][x][e][i];
+          join.o[wave][lane & 15][(16 * x + 4 * g + i) * S::kE + e] = o[n][x][e][i];
         }
       }
     }
@@ -337,17 +312,17 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
     const int at = threadIdx.x >> 4;
     const int row = 16 * n + at;
     if (row < R) {
-      float top = join_m[0][at];
+      float top = join.m[0][at];
 #pragma unroll
       for (int x = 1; x < 4; ++x) {
-        top = fmaxf(top, join_m[x][at]);
+        top = fmaxf(top, join.m[x][at]);
       }
       const float less = top == -INFINITY ? 0.0f : top;
       float by[4], total = 0.0f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        by[x] = join_m[x][at] == less ? 1.0f : __builtin_amdgcn_exp2f(join_m[x][at] - less);
-        total += by[x] * join_l[x][at];
+        by[x] = join.m[x][at] == less ? 1.0f : __builtin_amdgcn_exp2f(join.m[x][at] - less);
+        total += by[x] * join.l[x][at];
       }
       const bool seeing = any && row >= first_row;
       const float over = total == 0.0f ? 0.0f : 1.0f / total;
@@ -357,7 +332,7 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
         floatx4 sum4 = {};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float4 v = *reinterpret_cast<const float4*>(&join_o[x][at][d]);
+          const float4 v = *reinterpret_cast<const float4*>(&join.o[x][at][d]);
           sum4 += by[x] * floatx4{v.x, v.y, v.z, v.w};
         }
         if (a.splits > 1) {
@@ -374,6 +349,27 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
           const int i = row / a.G;
           a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
               seeing ? top + log2f(total) : 0.0f;
+        }
+      }
+    }
+  }
+  if (a.Lq > 1 && __syncthreads_or(odd)) {
+    after_stores();
+    const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
+    const int d = threadIdx.x;
+    for (int t = t0; t < t1 && d < a.D; ++t) {
+      const KeyTile at = tile_of(range, t, KT);
+      for (int j = max(at.begin, at.low); j < at.end; ++j) {
+        const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
+        for (int r = first_row; not_finite(x) && r < R; ++r) {
+          if (!sees_key(a, p0 + r / a.G, j)) {
+            continue;
+          }
+          if (a.splits > 1) {
+            add_to(a.part_out + (part + r) * a.D + d, x);
+          } else {
+            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, r) + d, x);
+          }
         }
       }
     }

@@ -17,9 +17,29 @@ namespace mlxrocm {
 
 namespace {
 
+// A lane's column of a partial sum
+template <int DT>
+__device__ __forceinline__ void store_part(
+    float* to, const floatx16 (&x)[DT / 32], bool any, int D, int h) {
+#pragma unroll
+  for (int d = 0; d < DT / 32; ++d) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = 32 * d + 8 * i + 4 * h;
+      if (c < D) {
+        *reinterpret_cast<float4*>(to + c) = any
+            ? make_float4(x[d][4 * i], x[d][4 * i + 1], x[d][4 * i + 2], x[d][4 * i + 3])
+            : make_float4(0, 0, 0, 0);
+      }
+    }
+  }
+}
+
 // ---- dq: workgroups of 128 rows, as the forward -----------------------------------------
 template <typename T, int DT>
-__global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(DT * sizeof(T) <= 256 ? 2 : 1, DT * sizeof(T) <= 256 ? 2 : 1)))
+void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
@@ -30,9 +50,11 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5;
+  const int splits = ga.plan.dq_splits;
   int head, piece;
-  piece_of(a.B * a.Hkv, blocks, &head, &piece);
-  const int block = blocks - 1 - piece;
+  piece_of(a.B * a.Hkv, blocks * splits, &head, &piece);
+  const int block = blocks - 1 - piece / splits;
+  const int split = piece % splits;
   const int b = head / a.Hkv;
   const int hk = head - b * a.Hkv;
   const int R = a.G * a.Lq;
@@ -47,16 +69,19 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
 
   const bool any = lo <= hi && length > 0;
   const KeyRange range = any ? keys_of(a, length, lo, hi, KT) : KeyRange{};
+  const int t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / splits);
   const int w_lo = max(r0, first_row);
   const int w_hi = min(r0 + 31, R - 1);
   const bool works = w_lo <= w_hi && length > 0;
   const int p0 = length - a.Lq;
+  const int b_lo = p0 + lo / a.G; // the workgroup's, and the wave's
+  const int b_hi = p0 + hi / a.G;
   const int p_lo = p0 + w_lo / a.G;
   const int p_hi = p0 + w_hi / a.G;
   const int from = min(max(row, lo), hi);
   const int i_from = from / a.G;
   const int p = p0 + i_from;
-  const int seen_from = p - a.window + 1;
 
   Frag<T> q[DT / 16], dout[DT / 16];
   float lse = 0.0f, delta = 0.0f;
@@ -84,7 +109,7 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
     const int64_t at =
         (static_cast<int64_t>(b) * a.Hq + hk * a.G + from - i_from * a.G) * a.Lq + i_from;
     lse = a.lse[at];
-    if (seeing && h == 0) {
+    if (seeing && h == 0 && split == 0) {
       ga.delta[at] = delta;
     }
   }
@@ -94,40 +119,48 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
   }
   KeyStream<T, DT, false> keys(a, b, hk, length, wave, lane);
   floatx16 dq[DT / 32];
-  // (a masked key that is not finite: see attention_rows_kernel)
-  for (int careful = 0;; careful = 1) {
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d) {
-      dq[d] = floatx16{};
-    }
-    if (range.tiles > 0) {
-      keys.fetch(tile_of(range, 0, KT).begin, lds, lds + kBoth / 2);
-    }
-    for (int t = 0; t < range.tiles; ++t) {
-      wait_loads();
+  for (int d = 0; d < DT / 32; ++d) {
+    dq[d] = floatx16{};
+  }
+  if (t0 < t1) {
+    keys.fetch(tile_of(range, t0, KT).begin, lds, lds + kBoth / 2);
+  }
+  bool odd = false; // some key was left out of the products
+  for (int t = t0; t < t1; ++t) {
+    wait_loads();
+    __syncthreads();
+    const T* k_tile = lds + ((t - t0) & 1) * kBoth;
+    const T* v_tile = k_tile + kBoth / 2;
+    T* next = lds + ((t + 1 - t0) & 1) * kBoth;
+    const KeyTile tile = tile_of(range, t, KT);
+    // The scores need the keys as they are: those without what is not finite lie where the
+    // next tile will, which is fetched after them.
+    const bool apart = !whole_tile(a, tile, KT, b_lo, b_hi) &&
+        __syncthreads_or(odd_values<T, S::kTile>(k_tile));
+    if (apart) {
+      odd = true;
+      copy_finite<T, S::kTile>(k_tile, next);
       __syncthreads();
-      const T* k_tile = lds + (t & 1) * kBoth;
-      const T* v_tile = k_tile + kBoth / 2;
-      const KeyTile tile = tile_of(range, t, KT);
-      if (t + 1 < range.tiles) {
-        T* next = lds + ((t + 1) & 1) * kBoth;
-        keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
-      }
-      const int begin = tile.begin;
-      if (!works || none_seen(begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
-        continue;
-      }
+    } else if (t + 1 < t1) {
+      keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
+    }
+    const T* cols = apart ? next : k_tile;
+    if (works && !none_seen(tile.begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
       const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
-      const int last = min(p, tile.end - 1);
-      const bool apart = careful != 0 && !whole;
+      const Seen sees(a, tile, p, 4 * h);
 #pragma unroll
       for (int g = 0; g < KT / 32; ++g) {
         floatx16 s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < DT / 16; ++c) {
-          s = mma32<T>(L::load_rows(k_tile, 32 * g + (lane & 31), 2 * c + h), q[c], s);
-          dp = mma32<T>(L::load_rows(v_tile, 32 * g + (lane & 31), 2 * c + h), dout[c], dp);
-        }
+        read_ahead<T, DT / 8>(
+            [&](int n) { return L::load_rows(n % 2 == 0 ? k_tile : v_tile, 32 * g, n / 2, lane); },
+            [&](int n, const Frag<T>& f) {
+              if (n % 2 == 0) {
+                s = mma32<T>(f, q[n / 2], s);
+              } else {
+                dp = mma32<T>(f, dout[n / 2], dp);
+              }
+            });
         float ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -137,72 +170,63 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int j = begin + 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            const bool sees = j >= tile.low && j <= last && (j >= seen_from || j < a.keep);
-            ds[i] = sees ? ds[i] : 0.0f;
+            ds[i] = sees(32 * g + 8 * (i / 4) + i % 4) ? ds[i] : 0.0f;
           }
         }
         const Frag<T> w[2] = {frag_of<T>(ds), frag_of<T>(ds + 8)};
-#pragma unroll
-        for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            Frag<T> f = L::load_cols(k_tile, 32 * g + 16 * n, 32 * d, lane);
-            if (apart) {
-              drop_not_finite<T>(f);
-            }
-            dq[d] = mma32<T>(f, w[n], dq[d]);
-          }
-        }
-      }
-      if (apart) {
-        for (int n = max(tile.low - begin, 0); n < tile.end - begin; ++n) {
-          const int j = begin + n;
-          const bool sees = j <= p && (j >= seen_from || j < a.keep);
-#pragma unroll
-          for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = L::value(k_tile, n, 32 * d + 8 * (i / 4) + 4 * h + i % 4);
-              dq[d][i] += sees && not_finite(x) ? x : 0.0f;
-            }
-          }
-        }
+        read_ahead<T, DT / 16>(
+            [&](int n) { return L::load_cols(cols, 32 * g + 16 * (n % 2), 32 * (n / 2), lane); },
+            [&](int n, const Frag<T>& f) { dq[n / 2] = mma32<T>(f, w[n % 2], dq[n / 2]); });
       }
     }
-    bool odd = false;
+    if (apart && t + 1 < t1) {
+      __syncthreads();
+      keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
+    }
+  }
+  const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
+  if (stored && splits > 1) {
+    store_part<DT>(ga.part_dq + (part + row) * a.D, dq, seeing, a.D, h);
+  } else if (stored) {
+    T* to = static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.G, row);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        odd = odd || not_finite(dq[d][i]);
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * d + 8 * i + 4 * h;
+        if (c < a.D) {
+          store4<T>(to + c, seeing ? floatx4{dq[d][4 * i], dq[d][4 * i + 1], dq[d][4 * i + 2],
+                                             dq[d][4 * i + 3]} *
+                                  ga.scale
+                                   : floatx4{});
+        }
       }
     }
-    if (!__syncthreads_or(odd && careful == 0)) {
-      break;
-    }
   }
-  if (!stored) {
-    return;
-  }
-  T* to = static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.G, row);
-#pragma unroll
-  for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 32 * d + 8 * i + 4 * h;
-      if (c < a.D) {
-        store4<T>(to + c, seeing ? floatx4{dq[d][4 * i], dq[d][4 * i + 1], dq[d][4 * i + 2],
-                                           dq[d][4 * i + 3]} *
-                               ga.scale
-                                 : floatx4{});
+  if (odd) { // the same for all
+    after_stores();
+    const int d = threadIdx.x;
+    for (int t = t0; t < t1 && d < a.D; ++t) {
+      const KeyTile tile = tile_of(range, t, KT);
+      for (int j = max(tile.begin, tile.low); j < tile.end; ++j) {
+        const float x = to_f32(static_cast<const T*>(a.k)[key_row<false>(a, b, hk, j).k + d]);
+        for (int r = lo; not_finite(x) && r <= hi; ++r) {
+          if (!sees_key(a, p0 + r / a.G, j)) {
+            continue;
+          }
+          if (splits > 1) {
+            add_to(ga.part_dq + (part + r) * a.D + d, x);
+          } else {
+            add_to(static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.G, r) + d, x);
+          }
+        }
       }
     }
   }
 }
 
 // ---- dk, dv: workgroups of 128 keys ------------------------------------------------------
-constexpr int kKeysBlock = 128;
+constexpr int kKeysBlock = kGradBlock;
 
 // What a row's probabilities need beside q: its sum, its delta and its position.
 struct RowStats {
@@ -217,9 +241,8 @@ struct StatsTile {
 
 // Fetches tiles of rows of q and dout to LDS (see KeyStream).  Where a power of two of heads
 // share a key head, a lane's rows lie at the same offsets from the first of each load.
-template <typename T, int DT>
+template <typename T, int DT, int ROWS>
 struct RowStream {
-  using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   const AttentionGradArgs& ga;
   int b, hk, end, wave;
@@ -243,14 +266,17 @@ struct RowStream {
     const AttentionArgs& a = ga.a;
     const T* q = static_cast<const T*>(a.q);
     const T* dout = static_cast<const T*>(ga.dout);
-    const bool inside = begin + S::kKeys <= end && (a.near & 2) != 0;
+    const bool inside = begin + ROWS <= end && (a.near & 2) != 0;
 #pragma unroll
-    for (int n = 0; n < S::kPasses; ++n) {
+    for (int n = 0; n < ROWS / L::kRowsOfPass; ++n) {
       const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
       const uint32_t to = row * L::kPitch * sizeof(T);
       if (inside) {
-        const T* qp = q + row_offset(a.q_strides, b, hk, a.G, begin + row);
-        const T* dp = dout + row_offset(ga.dout_strides, b, hk, a.G, begin + row);
+        const int i = (begin + row) >> a.g_log2;
+        const int head = hk * a.G + ((begin + row) & (a.G - 1));
+        const T* qp = q + b * a.q_strides[0] + head * a.q_strides[1] + i * a.q_strides[2];
+        const T* dp =
+            dout + b * ga.dout_strides[0] + head * ga.dout_strides[1] + i * ga.dout_strides[2];
         if (d < a.D) {
           dma16(lds_address(q_tile) + to, q_off, qp);
           dma16(lds_address(d_tile) + to, d_off, dp);
@@ -269,24 +295,48 @@ struct RowStream {
   }
 };
 
+// Two waves a SIMD leave 256 registers.  Both results of 128 columns take 128 of them, and keys
+// and values 64: the values stay in LDS then (read again for each tile, a quarter more
+// than is read anyway), and a tile is 32 rows, so that two workgroups fit.  With all in registers
+// and one wave a SIMD the compiler moves results between its two files around each product: 8192
+// tokens, 32 heads of 128 2.13 ms, spilling at two waves 5.2 ms.
 template <typename T, int DT>
-__global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_dkv_kernel(const AttentionGradArgs ga, int blocks) {
-  using S = RowsShape<T, DT>;
+struct DkvShape {
+  static constexpr bool kTwo = DT * sizeof(T) <= 256; // waves a SIMD
+  static constexpr bool kValuesInLds = sizeof(T) == 2 && (DT == 96 || DT == 128);
+  static constexpr int kRows = kValuesInLds ? 32 : RowsShape<T, DT>::kKeys; // of a tile
+  static constexpr int kTile = kRows * Tile<T, DT>::kPitch;
+  static constexpr int kAhead = DT == 128 && kValuesInLds ? 2 : 4; // (one more register is too many)
+};
+
+template <typename T, int DT>
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(DkvShape<T, DT>::kTwo ? 2 : 1, DkvShape<T, DT>::kTwo ? 2 : 1)))
+void attention_dkv_kernel(const AttentionGradArgs ga) {
+  using S = DkvShape<T, DT>;
   using L = Tile<T, DT>;
-  constexpr int RT = S::kKeys; // rows of a tile
+  constexpr int RT = S::kRows;
   constexpr int kBoth = 2 * S::kTile;
   // this lane's key and value: in registers, but for 256 floats, which are read again for
   // each tile (with both results they would need all 512 registers)
-  constexpr bool kHeld = DT * sizeof(T) <= 512;
+  constexpr bool kKeyHeld = DT * sizeof(T) <= 512;
+  constexpr bool kValueHeld = kKeyHeld && !S::kValuesInLds;
   __shared__ __align__(16) T lds[2 * kBoth];
+  __shared__ __align__(16) T values[S::kValuesInLds ? kKeysBlock * L::kPitch : 16];
   __shared__ __align__(16) StatsTile<RT> stats[2];
   const AttentionArgs& a = ga.a;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5;
-  int head, block;
-  piece_of(a.B * a.Hkv, blocks, &head, &block);
+  const GradPlan& plan = ga.plan;
+  int head, piece;
+  piece_of(a.B * a.Hkv, plan.pieces(), &head, &piece);
+  // the first keys are seen by most rows: they come first
+  const int wide = plan.wide_blocks * plan.wide_splits;
+  const int splits = piece < wide ? plan.wide_splits : plan.splits;
+  const int block = piece < wide ? piece / splits : plan.wide_blocks + (piece - wide) / splits;
+  const int split = (piece < wide ? piece : piece - wide) % splits;
   const int b = head / a.Hkv;
   const int hk = head - b * a.Hkv;
   const int length = length_of(a, b);
@@ -296,10 +346,13 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_
   // the tokens that see one of them
   const int i0 = max(max(0, -p0), k0 - p0);
   const int i1 = k0 < a.keep ? a.Lq : min(a.Lq, k1 - 1 + a.window - p0);
-  const bool any = k0 < k1 && i0 < i1;
-  const int begin_row = i0 * a.G;
-  const int end_row = i1 * a.G;
-  const int tiles = any ? (end_row - begin_row + RT - 1) / RT : 0;
+  const int all = k0 < k1 && i0 < i1 ? ((i1 - i0) * a.G + RT - 1) / RT : 0; // tiles of rows
+  const int s0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+  const int s1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits);
+  const int tiles = s1 - s0; // of this run
+  const bool any = tiles > 0;
+  const int begin_row = i0 * a.G + s0 * RT;
+  const int end_row = min(i1 * a.G, i0 * a.G + s1 * RT);
 
   const int w0 = k0 + 32 * wave;
   const int w1 = min(w0 + 32, k1); // the wave's keys [w0, w1)
@@ -318,13 +371,37 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_
     const int d = 16 * c + 8 * h;
     return d < a.D ? load_frag<T>(v_src + d) : zero_frag<T>();
   };
-  Frag<T> k[kHeld ? DT / 16 : 1], v[kHeld ? DT / 16 : 1];
-  if constexpr (kHeld) {
-    if (any) {
+  Frag<T> k[kKeyHeld ? DT / 16 : 1], v[kValueHeld ? DT / 16 : 1];
+  if (any) {
 #pragma unroll
-      for (int c = 0; c < DT / 16; ++c) {
+    for (int c = 0; c < DT / 16; ++c) {
+      if constexpr (kKeyHeld) {
         k[c] = key_frag(c);
+      }
+      if constexpr (kValueHeld) {
         v[c] = value_frag(c);
+      }
+    }
+  }
+  if (a.D < L::kPitch) {
+    clear_lds<T>(lds, 2 * kBoth);
+    if constexpr (S::kValuesInLds) {
+      clear_lds<T>(values, kKeysBlock * L::kPitch);
+    }
+  }
+  if constexpr (S::kValuesInLds) {
+    if (any) { // keys past the end repeat the last one
+#pragma unroll
+      for (int n = 0; n < kKeysBlock / L::kRowsOfPass; ++n) {
+        const int first = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+        const int r = first + lane / L::kPlaces;
+        const int d = ((lane % L::kPlaces) ^ L::swizzle(r)) * L::kUnit;
+        if (d < a.D) {
+          dma16_from(
+              lds_address(values) + first * L::kPitch * sizeof(T),
+              static_cast<const T*>(a.v) +
+                  key_row<false>(a, b, hk, min(k0 + r, length - 1)).v + d);
+        }
       }
     }
   }
@@ -335,151 +412,257 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_
     return RowStats{a.lse[n], ga.delta[n], p0 + i};
   };
 
-  if (a.D < L::kPitch) {
-    clear_lds<T>(lds, 2 * kBoth);
-  }
-  const RowStream<T, DT> rows(ga, b, hk, end_row, wave, lane);
+  const RowStream<T, DT, RT> rows(ga, b, hk, end_row, wave, lane);
   floatx16 dk[DT / 32], dv[DT / 32];
-  // (a masked row that is not finite: see attention_rows_kernel)
-  for (int careful = 0;; careful = 1) {
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d) {
-      dk[d] = floatx16{};
-      dv[d] = floatx16{};
+  for (int d = 0; d < DT / 32; ++d) {
+    dk[d] = floatx16{};
+    dv[d] = floatx16{};
+  }
+  RowStats mine = {};
+  if (tiles > 0) {
+    if (threadIdx.x < RT) {
+      mine = stats_of(0);
     }
-    RowStats mine = {};
-    if (tiles > 0) {
-      if (threadIdx.x < RT) {
-        mine = stats_of(0);
-      }
-      rows.fetch(begin_row, lds, lds + kBoth / 2);
+    rows.fetch(begin_row, lds, lds + kBoth / 2);
+  }
+  bool odd = false; // some row was left out of the products
+  for (int t = 0; t < tiles; ++t) {
+    StatsTile<RT>& st = stats[t & 1];
+    wait_loads();
+    if (threadIdx.x < RT) {
+      st.lse[threadIdx.x] = mine.lse;
+      st.delta[threadIdx.x] = mine.delta;
+      st.p[threadIdx.x] = mine.p;
     }
-    for (int t = 0; t < tiles; ++t) {
-      StatsTile<RT>& st = stats[t & 1];
-      wait_loads();
-      if (threadIdx.x < RT) {
-        st.lse[threadIdx.x] = mine.lse;
-        st.delta[threadIdx.x] = mine.delta;
-        st.p[threadIdx.x] = mine.p;
-      }
+    __syncthreads();
+    const T* q_tile = lds + (t & 1) * kBoth;
+    const T* d_tile = q_tile + kBoth / 2;
+    T* next = lds + ((t + 1) & 1) * kBoth;
+    const int begin = begin_row + t * RT;
+    const int count = min(RT, end_row - begin);
+    if (t + 1 < tiles && threadIdx.x < RT) {
+      mine = stats_of(t + 1);
+    }
+    const int p_lo = __builtin_amdgcn_readfirstlane(st.p[0]);
+    const int p_hi = __builtin_amdgcn_readfirstlane(st.p[count - 1]);
+    // (as in attention_dq_kernel)
+    const bool apart =
+        !(count == RT && all_seen(k0, k1, p_lo, p_hi, a.window, a.keep)) &&
+        __syncthreads_or(odd_values<T, 2 * S::kTile>(q_tile));
+    if (apart) {
+      odd = true;
+      copy_finite<T, 2 * S::kTile>(q_tile, next);
       __syncthreads();
-      const T* q_tile = lds + (t & 1) * kBoth;
-      const T* d_tile = q_tile + kBoth / 2;
-      const int begin = begin_row + t * RT;
-      const int count = min(RT, end_row - begin);
-      if (t + 1 < tiles) {
-        if (threadIdx.x < RT) {
-          mine = stats_of(t + 1);
-        }
-        T* next = lds + ((t + 1) & 1) * kBoth;
-        rows.fetch(begin + RT, next, next + kBoth / 2);
-      }
-      const int p_lo = st.p[0];
-      const int p_hi = st.p[count - 1];
-      if (!works || none_seen(w0, w1, p_lo, p_hi, a.window, a.keep)) {
-        continue;
-      }
+    } else if (t + 1 < tiles) {
+      rows.fetch(begin + RT, next, next + kBoth / 2);
+    }
+    const T* q_cols = apart ? next : q_tile;
+    const T* d_cols = q_cols + kBoth / 2;
+    if (works && !none_seen(w0, w1, p_lo, p_hi, a.window, a.keep)) {
       const bool whole = count == RT && w1 - w0 == 32 &&
           all_seen(w0, w1, p_lo, p_hi, a.window, a.keep);
-      const bool apart = careful != 0 && !whole;
-#pragma unroll
-      for (int g = 0; g < RT / 32; ++g) {
-        floatx16 s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < DT / 16; ++c) {
-          const Frag<T> kc = kHeld ? k[kHeld ? c : 0] : key_frag(c);
-          const Frag<T> vc = kHeld ? v[kHeld ? c : 0] : value_frag(c);
-          s = mma32<T>(L::load_rows(q_tile, 32 * g + (lane & 31), 2 * c + h), kc, s);
-          dp = mma32<T>(L::load_rows(d_tile, 32 * g + (lane & 31), 2 * c + h), vc, dp);
+      // Products of the two halves of the tile in turn, the exponentials of one half beside
+      // the products of the other.
+      constexpr int kHalves = RT / 32;
+      constexpr int kSteps = DT / 16; // matrix instructions of a product
+      floatx16 e[kHalves], dp[kHalves]; // scores, probabilities, and their gradients at last
+      uint32_t sees[kHalves];           // of 16 rows
+      const auto product = [&](const auto& read, const auto& use, const auto& beside) {
+        read_ahead<T, kSteps, S::kAhead>(read, [&](int n, const Frag<T>& f) {
+          use(n, f);
+          beside(n);
+        });
+      };
+      const auto nothing = [](int) {};
+      const auto scores = [&](int g, const auto& beside) {
+        e[g] = floatx16{};
+        product(
+            [&](int n) { return L::load_rows(q_tile, 32 * g, n, lane); },
+            [&](int n, const Frag<T>& f) {
+              e[g] = mma32<T>(f, kKeyHeld ? k[kKeyHeld ? n : 0] : key_frag(n), e[g]);
+            },
+            beside);
+      };
+      const auto d_weights = [&](int g, const auto& beside) {
+        dp[g] = floatx16{};
+        if constexpr (S::kValuesInLds) {
+          Frag<T> d_rows;
+          read_ahead<T, 2 * kSteps, S::kAhead>(
+              [&](int n) {
+                return n % 2 == 0 ? L::load_rows(d_tile, 32 * g, n / 2, lane)
+                                  : L::load_rows(values, 32 * wave, n / 2, lane);
+              },
+              [&](int n, const Frag<T>& f) {
+                if (n % 2 == 0) {
+                  d_rows = f;
+                } else {
+                  dp[g] = mma32<T>(d_rows, f, dp[g]);
+                  beside(n / 2);
+                }
+              });
+        } else {
+          product(
+              [&](int n) { return L::load_rows(d_tile, 32 * g, n, lane); },
+              [&](int n, const Frag<T>& f) {
+                dp[g] = mma32<T>(f, kValueHeld ? v[kValueHeld ? n : 0] : value_frag(n), dp[g]);
+              },
+              beside);
         }
-        float e[16], ds[16];
+      };
+      struct Weights {
+        Frag<T> of[2]; // 16 rows each
+      };
+      const auto packed = [&](int g) {
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int n = 32 * g + 2 * i + 4 * h;
-          const float4 lse = *reinterpret_cast<const float4*>(st.lse + n);
-          const float4 delta = *reinterpret_cast<const float4*>(st.delta + n);
-          const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
-          const float de[4] = {delta.x, delta.y, delta.z, delta.w};
+        for (int i = 0; i < 16; ++i) {
+          x[i] = e[g][i];
+        }
+        return Weights{{frag_of<T>(x), frag_of<T>(x + 8)}};
+      };
+      const auto add_packed = [&](const T* cols, int g, const Weights& w, floatx16(&to)[DT / 32],
+                                  const auto& beside) {
+        product(
+            [&](int n) { return L::load_cols(cols, 32 * g + 16 * (n % 2), 32 * (n / 2), lane); },
+            [&](int n, const Frag<T>& f) { to[n / 2] = mma32<T>(f, w.of[n % 2], to[n / 2]); },
+            beside);
+      };
+      const auto add = [&](const T* cols, int g, floatx16(&to)[DT / 32], const auto& beside) {
+        add_packed(cols, g, packed(g), to, beside);
+      };
+      // the n-th of kSteps parts of a half's exponentials, and of what becomes of them
+      const auto exponentials = [&](int g) {
+        return [&, g](int n) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            e[i + x] = __builtin_amdgcn_exp2f(fmaf(s[i + x], a.scale_log2, -ls[x]));
-            ds[i + x] = e[i + x] * (dp[i + x] - de[x]);
+          for (int i = 0; i < 16; ++i) {
+            if (i * kSteps / 16 == n) {
+              e[g][i] = __builtin_amdgcn_exp2f(fmaf(
+                  e[g][i], a.scale_log2, -st.lse[32 * g + 8 * (i / 4) + 4 * h + i % 4]));
+            }
           }
-        }
+        };
+      };
+      const auto d_scores = [&](int g) {
+        return [&, g](int n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (i * kSteps / 16 == n) {
+              e[g][i] *= dp[g][i] - st.delta[32 * g + 8 * (i / 4) + 4 * h + i % 4];
+            }
+          }
+        };
+      };
+      const auto hide = [&](int g) {
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int n = 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            const int p = st.p[n];
-            const bool sees = n < count && key < k1 && key <= p &&
-                (p - key < a.window || key < a.keep);
-            e[i] = sees ? e[i] : 0.0f;
-            ds[i] = sees ? ds[i] : 0.0f;
+            e[g][i] = (sees[g] >> i & 1) != 0 ? e[g][i] : 0.0f;
           }
         }
-        const Frag<T> we[2] = {frag_of<T>(e), frag_of<T>(e + 8)};
-        const Frag<T> ws[2] = {frag_of<T>(ds), frag_of<T>(ds + 8)};
+      };
+      if (!whole) {
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d) {
+        for (int g = 0; g < kHalves; ++g) {
+          sees[g] = 0;
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            Frag<T> fd = L::load_cols(d_tile, 32 * g + 16 * n, 32 * d, lane);
-            Frag<T> fq = L::load_cols(q_tile, 32 * g + 16 * n, 32 * d, lane);
-            if (apart) {
-              drop_not_finite<T>(fd);
-              drop_not_finite<T>(fq);
-            }
-            dv[d] = mma32<T>(fd, we[n], dv[d]);
-            dk[d] = mma32<T>(fq, ws[n], dk[d]);
+          for (int i = 0; i < 16; ++i) {
+            const int n = 32 * g + 8 * (i / 4) + 4 * h + i % 4;
+            sees[g] |= (n < count && key < k1 && sees_key(a, st.p[n], key) ? 1u : 0u) << i;
           }
         }
       }
-      if (apart) {
-        for (int n = 0; n < count; ++n) {
-          const int p = st.p[n];
-          const bool sees = key < k1 && key <= p && (p - key < a.window || key < a.keep);
+      if constexpr (kHalves == 2) {
+        scores(0, nothing);
+        scores(1, exponentials(0));
+        hide(0);
+        d_weights(0, exponentials(1));
+        hide(1);
+        add(d_cols, 0, dv, d_scores(0));
+        hide(0); // (again: what is not finite in a row that is not seen)
+        d_weights(1, nothing);
+        add(q_cols, 0, dk, nothing);
+        add(d_cols, 1, dv, d_scores(1));
+        hide(1);
+        add(q_cols, 1, dk, nothing);
+      } else { // (in the order that holds the fewest registers)
+        d_weights(0, nothing);
+        scores(0, nothing);
 #pragma unroll
-          for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int c = 32 * d + 8 * (i / 4) + 4 * h + i % 4;
-              const float x = L::value(q_tile, n, c);
-              const float y = L::value(d_tile, n, c);
-              dk[d][i] += sees && not_finite(x) ? x : 0.0f;
-              dv[d][i] += sees && not_finite(y) ? y : 0.0f;
-            }
-          }
+        for (int n = 0; n < kSteps; ++n) {
+          exponentials(0)(n);
         }
+        hide(0);
+        const auto probabilities = packed(0);
+#pragma unroll
+        for (int n = 0; n < kSteps; ++n) {
+          d_scores(0)(n);
+        }
+        hide(0);
+        const auto d_probabilities = packed(0);
+        add_packed(d_cols, 0, probabilities, dv, nothing);
+        add_packed(q_cols, 0, d_probabilities, dk, nothing);
       }
     }
-    bool odd = false;
+    if (apart && t + 1 < tiles) {
+      __syncthreads();
+      rows.fetch(begin + RT, next, next + kBoth / 2);
+    }
+  }
+  const bool parts = plan.dkv_split();
+  float* part = ga.part_dkv +
+      (static_cast<int64_t>(head) * plan.pieces() + piece) * (kKeysBlock * 2 * a.D);
+  if (parts) {
+    float* to = part + (key - k0) * 2 * a.D;
+    store_part<DT>(to, dk, key < k1, a.D, h);
+    store_part<DT>(to + a.D, dv, key < k1, a.D, h);
+  } else if (key < a.keys) {
+    const bool seen = key < k1;
+    const int64_t k_to = b * ga.dk_strides[0] + hk * ga.dk_strides[1] + key * ga.dk_strides[2];
+    const int64_t v_to = b * ga.dv_strides[0] + hk * ga.dv_strides[1] + key * ga.dv_strides[2];
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        odd = odd || not_finite(dk[d][i]) || not_finite(dv[d][i]);
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * d + 8 * i + 4 * h;
+        if (c < a.D) {
+          const floatx4 x = {dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+          const floatx4 y = {dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+          store4<T>(static_cast<T*>(ga.dk) + k_to + c, seen ? x * ga.scale : floatx4{});
+          store4<T>(static_cast<T*>(ga.dv) + v_to + c, seen ? y : floatx4{});
+        }
       }
     }
-    if (!__syncthreads_or(odd && careful == 0)) {
-      break;
-    }
   }
-  if (key >= a.keys || key >= k0 + kKeysBlock) {
-    return;
-  }
-  const bool seen = key < k1;
-  const int64_t k_to = b * ga.dk_strides[0] + hk * ga.dk_strides[1] + key * ga.dk_strides[2];
-  const int64_t v_to = b * ga.dv_strides[0] + hk * ga.dv_strides[1] + key * ga.dv_strides[2];
-#pragma unroll
-  for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 32 * d + 8 * i + 4 * h;
-      if (c < a.D) {
-        const floatx4 x = {dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
-        const floatx4 y = {dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
-        store4<T>(static_cast<T*>(ga.dk) + k_to + c, seen ? x * ga.scale : floatx4{});
-        store4<T>(static_cast<T*>(ga.dv) + v_to + c, seen ? y : floatx4{});
+  if (odd) { // the same for all
+    after_stores();
+    const int d = threadIdx.x;
+    for (int r = begin_row; r < end_row && d < a.D; ++r) {
+      const float x = to_f32(
+          static_cast<const T*>(a.q)[row_offset(a.q_strides, b, hk, a.G, r) + d]);
+      const float y = to_f32(
+          static_cast<const T*>(ga.dout)[row_offset(ga.dout_strides, b, hk, a.G, r) + d]);
+      for (int j = k0; (not_finite(x) || not_finite(y)) && j < k1; ++j) {
+        if (!sees_key(a, p0 + r / a.G, j)) {
+          continue;
+        }
+        if (parts) {
+          add_to(part + (j - k0) * 2 * a.D + d, not_finite(x) ? x : 0.0f);
+          add_to(part + (j - k0) * 2 * a.D + a.D + d, not_finite(y) ? y : 0.0f);
+          continue;
+        }
+        if (not_finite(x)) {
+          add_to(
+              static_cast<T*>(ga.dk) + b * ga.dk_strides[0] + hk * ga.dk_strides[1] +
+                  j * ga.dk_strides[2] + d,
+              x);
+        }
+        if (not_finite(y)) {
+          add_to(
+              static_cast<T*>(ga.dv) + b * ga.dv_strides[0] + hk * ga.dv_strides[1] +
+                  j * ga.dv_strides[2] + d,
+              y);
+        }
       }
     }
   }
@@ -488,15 +671,18 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 128 ? 2 : 1) void attention_
 template <typename T, int DT>
 int launch_grad_of(const AttentionGradArgs& g, hipStream_t s) {
   const AttentionArgs& a = g.a;
+  MLXROCM_REHEARSE(
+      "attention_dq(dim=%d,splits=%d)+attention_dkv(dim=%d,splits=%d,kept=%dx%d)", DT,
+      g.plan.dq_splits, DT, g.plan.splits, g.plan.wide_blocks, g.plan.wide_splits);
   const int rows = static_cast<int>(
       (static_cast<int64_t>(a.G) * a.Lq + kRowsBlock - 1) / kRowsBlock);
-  const int keys = (a.keys + kKeysBlock - 1) / kKeysBlock;
   if (rows > 0) {
-    attention_dq_kernel<T, DT><<<rows * a.B * a.Hkv, 256, 0, s>>>(g, rows);
+    attention_dq_kernel<T, DT>
+        <<<rows * g.plan.dq_splits * a.B * a.Hkv, 256, 0, s>>>(g, rows);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
-  if (keys > 0) {
-    attention_dkv_kernel<T, DT><<<keys * a.B * a.Hkv, 256, 0, s>>>(g, keys);
+  if (g.plan.blocks > 0) {
+    attention_dkv_kernel<T, DT><<<g.plan.pieces() * a.B * a.Hkv, 256, 0, s>>>(g);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
   return static_cast<int>(MLXROCM_OK);

@@ -70,7 +70,88 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   }
 }
 
+// Sums of partial gradients: a thread has four columns of a row of dq, or of a key's dk or dv.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_sum_dq_kernel(const AttentionGradArgs g) {
+  const AttentionArgs& a = g.a;
+  const int R = a.G * a.Lq;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * R;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n = at / (a.D / 4);
+  const int d = static_cast<int>(at - n * (a.D / 4)) * 4;
+  if (n >= rows) {
+    return;
+  }
+  floatx4 sum = {};
+#pragma unroll 4
+  for (int s = 0; s < g.plan.dq_splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(g.part_dq + (s * rows + n) * a.D + d);
+    sum += floatx4{v.x, v.y, v.z, v.w};
+  }
+  const int head = static_cast<int>(n / R);
+  const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
+  const int b = head / a.Hkv;
+  T* to = static_cast<T*>(g.dq) + row_offset(g.dq_strides, b, head - b * a.Hkv, a.G, row) + d;
+  store4<T>(to, sum * g.scale);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void attention_sum_dkv_kernel(const AttentionGradArgs g) {
+  const AttentionArgs& a = g.a;
+  const GradPlan& plan = g.plan;
+  const int each = 2 * a.D / 4; // of a key
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n = at / each;
+  if (n >= static_cast<int64_t>(a.B) * a.Hkv * a.keys) {
+    return;
+  }
+  const int c = static_cast<int>(at - n * each) * 4; // column of dk, then of dv
+  const int head = static_cast<int>(n / a.keys);
+  const int key = static_cast<int>(n - static_cast<int64_t>(head) * a.keys);
+  const int block = key / kGradBlock;
+  const bool wide = block < plan.wide_blocks;
+  const int splits = wide ? plan.wide_splits : plan.splits;
+  const int piece = wide ? block * plan.wide_splits
+                         : plan.wide_blocks * plan.wide_splits + (block - plan.wide_blocks) * splits;
+  const float* part = g.part_dkv +
+      (static_cast<int64_t>(head) * plan.pieces() + piece) * (kGradBlock * 2 * a.D) +
+      (key - block * kGradBlock) * 2 * a.D + c;
+  floatx4 sum = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(
+        part + static_cast<int64_t>(s) * (kGradBlock * 2 * a.D));
+    sum += floatx4{v.x, v.y, v.z, v.w};
+  }
+  const int b = head / a.Hkv;
+  const int hk = head - b * a.Hkv;
+  const bool of_k = c < a.D;
+  const int64_t* strides = of_k ? g.dk_strides : g.dv_strides;
+  T* to = static_cast<T*>(of_k ? g.dk : g.dv) + b * strides[0] + hk * strides[1] +
+      key * strides[2] + (of_k ? c : c - a.D);
+  store4<T>(to, of_k ? sum * g.scale : sum);
+}
+
 } // namespace
+
+int launch_attention_grad_join(const AttentionGradArgs& g, int dtype, hipStream_t s) {
+  const AttentionArgs& a = g.a;
+  MLXROCM_REHEARSE("attention_sum");
+  return dispatch_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (g.plan.dq_splits > 1) {
+      const int64_t n = static_cast<int64_t>(a.B) * a.Hq * a.Lq * (a.D / 4);
+      attention_sum_dq_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g);
+      MLXROCM_HIP_TRY(hipGetLastError());
+    }
+    if (g.plan.dkv_split()) {
+      const int64_t n = static_cast<int64_t>(a.B) * a.Hkv * a.keys * (a.D / 2);
+      attention_sum_dkv_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g);
+      MLXROCM_HIP_TRY(hipGetLastError());
+    }
+    return static_cast<int>(MLXROCM_OK);
+  });
+}
 
 int launch_attention_join(const AttentionArgs& a, int dtype, hipStream_t s) {
   MLXROCM_REHEARSE("attention_join");

@@ -73,21 +73,30 @@ struct KeyStream {
     const T* v = static_cast<const T*>(a.v) + hk * a.v_strides[1];
     const bool inside = begin + S::kKeys <= length && (a.near & 1) != 0;
     if (inside) {
+      int at = begin + wave * L::kRowsOfLoad;
+      const T* kp = k;
+      const T* vp = v;
+      if constexpr (!PAGED) {
+        kp += b * a.k_strides[0] + at * a.k_strides[2];
+        vp += b * a.v_strides[0] + at * a.v_strides[2];
+      }
 #pragma unroll
       for (int n = 0; n < S::kPasses; ++n) {
         const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
-        int64_t first = b;
-        int at = begin + row;
         if constexpr (PAGED) {
-          first = __builtin_amdgcn_readlane(ids, row / 16);
-          page_of(a, at, &at);
+          const int64_t id = __builtin_amdgcn_readlane(ids, row / 16);
+          page_of(a, begin + row, &at);
+          kp = k + id * a.k_strides[0] + at * a.k_strides[2];
+          vp = v + id * a.v_strides[0] + at * a.v_strides[2];
         }
-        const T* kp = k + first * a.k_strides[0] + at * a.k_strides[2];
-        const T* vp = v + first * a.v_strides[0] + at * a.v_strides[2];
         const uint32_t to = row * L::kPitch * sizeof(T);
         if (d < a.D) {
           dma16(lds_address(k_tile) + to, k_off, kp);
           dma16(lds_address(v_tile) + to, v_off, vp);
+        }
+        if constexpr (!PAGED) {
+          kp += L::kRowsOfPass * a.k_strides[2];
+          vp += L::kRowsOfPass * a.v_strides[2];
         }
       }
     } else { // keys past the end repeat the last one
@@ -107,7 +116,9 @@ struct KeyStream {
 };
 
 template <typename T, int DT, bool PAGED>
-__global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_rows_kernel(const AttentionArgs a, int blocks) {
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(DT * sizeof(T) <= 256 ? 2 : 1, DT * sizeof(T) <= 256 ? 2 : 1)))
+void attention_rows_kernel(const AttentionArgs a, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
@@ -146,11 +157,12 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
   const int w_hi = min(r0 + 31, R - 1);
   const bool works = w_lo <= w_hi && length > 0;
   const int p0 = length - a.Lq;
+  const int b_lo = p0 + lo / a.G; // the workgroup's, and the wave's
+  const int b_hi = p0 + hi / a.G;
   const int p_lo = p0 + w_lo / a.G;
   const int p_hi = p0 + w_hi / a.G;
   const int from = min(max(row, lo), hi); // a row that sees something, in any lane
   const int p = p0 + from / a.G;
-  const int seen_from = p - a.window + 1;
 
   Frag<T> q[DT / 16];
   if (t0 < t1) {
@@ -169,172 +181,171 @@ __global__ __launch_bounds__(256, DT * sizeof(T) <= 256 ? 2 : 1) void attention_
     clear_lds<T>(lds, 2 * kBoth);
   }
   KeyStream<T, DT, PAGED> keys(a, b, hk, length, wave, lane);
-  // A masked value that is not finite would reach rows that do not see it, as 0 * inf: where a
-  // result is not finite the rows are done again, those values apart from the products.
-  for (int careful = 0;; careful = 1) {
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d) {
-      o[d] = floatx16{};
+  for (int d = 0; d < DT / 32; ++d) {
+    o[d] = floatx16{};
+  }
+  m = -INFINITY;
+  l = 0.0f;
+  bool odd = false; // some value was left out of the products
+  if (t0 < t1) {
+    const int begin = tile_of(range, t0, KT).begin;
+    keys.look_up(begin);
+    keys.fetch(begin, lds, lds + kBoth / 2);
+    keys.look_up(tile_of(range, t0 + 1, KT).begin);
+  }
+  for (int t = t0; t < t1; ++t) {
+    wait_loads();
+    __syncthreads();
+    T* k_tile = lds + ((t - t0) & 1) * kBoth;
+    T* v_tile = k_tile + kBoth / 2;
+    const KeyTile tile = tile_of(range, t, KT);
+    if (t + 1 < t1) {
+      T* next = lds + ((t + 1 - t0) & 1) * kBoth;
+      keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
+      keys.look_up(tile_of(range, t + 2, KT).begin);
     }
-    m = -INFINITY;
-    l = 0.0f;
-    if (t0 < t1) {
-      const int begin = tile_of(range, t0, KT).begin;
-      keys.look_up(begin);
-      keys.fetch(begin, lds, lds + kBoth / 2);
-      keys.look_up(tile_of(range, t0 + 1, KT).begin);
-    }
-    for (int t = t0; t < t1; ++t) {
-      wait_loads();
+    const int begin = tile.begin;
+    if (!whole_tile(a, tile, KT, b_lo, b_hi) &&
+        __syncthreads_or(odd_values<T, S::kTile>(v_tile))) {
+      odd = true;
+      copy_finite<T, S::kTile>(v_tile, v_tile);
       __syncthreads();
-      const T* k_tile = lds + ((t - t0) & 1) * kBoth;
-      const T* v_tile = k_tile + kBoth / 2;
-      const KeyTile tile = tile_of(range, t, KT);
-      if (t + 1 < t1) {
-        T* next = lds + ((t + 1 - t0) & 1) * kBoth;
-        keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
-        keys.look_up(tile_of(range, t + 2, KT).begin);
-      }
-      const int begin = tile.begin;
-      if (!works || none_seen(begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
-        continue;
-      }
-      floatx16 s[KT / 32];
+    }
+    if (!works || none_seen(begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
+      continue;
+    }
+    floatx16 s[KT / 32];
 #pragma unroll
-      for (int g = 0; g < KT / 32; ++g) {
-        s[g] = floatx16{};
-#pragma unroll
-        for (int c = 0; c < DT / 16; ++c) {
-          s[g] = mma32<T>(L::load_rows(k_tile, 32 * g + (lane & 31), 2 * c + h), q[c], s[g]);
-        }
-      }
-      const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
-      if (!whole) {
-        const int last = min(p, tile.end - 1);
-#pragma unroll
-        for (int g = 0; g < KT / 32; ++g) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = begin + 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            const bool sees = j >= tile.low && j <= last && (j >= seen_from || j < a.keep);
-            s[g][i] = sees ? s[g][i] : -INFINITY;
-          }
-        }
-      }
-      float top = s[0][0];
+    for (int g = 0; g < KT / 32; ++g) {
+      s[g] = floatx16{};
+    }
+    read_ahead<T, (KT / 32) * (DT / 16)>(
+        [&](int n) { return L::load_rows(k_tile, 32 * (n % (KT / 32)), n / (KT / 32), lane); },
+        [&](int n, const Frag<T>& f) {
+          s[n % (KT / 32)] = mma32<T>(f, q[n / (KT / 32)], s[n % (KT / 32)]);
+        });
+    const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
+    if (!whole) {
+      const Seen sees(a, tile, p, 4 * h);
 #pragma unroll
       for (int g = 0; g < KT / 32; ++g) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          top = fmaxf(top, s[g][i]);
-        }
-      }
-      top = max_halves(top) * a.scale_log2;
-      if (__any(top > m + kSlack)) {
-        const float now = fmaxf(m, top);
-        const float by = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-        m = now;
-        l *= by;
-#pragma unroll
-        for (int d = 0; d < DT / 32; ++d) {
-          o[d] *= by;
-        }
-      }
-      const float less = m == -INFINITY ? 0.0f : m;
-      float sum = 0.0f;
-      Frag<T> w[KT / 16];
-#pragma unroll
-      for (int g = 0; g < KT / 32; ++g) {
-        float e[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], a.scale_log2, -less));
-          sum += e[i];
-        }
-        w[2 * g] = frag_of<T>(e);
-        w[2 * g + 1] = frag_of<T>(e + 8);
-      }
-      l += sum;
-      const bool apart = careful != 0 && !whole;
-#pragma unroll
-      for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-        for (int g = 0; g < KT / 16; ++g) {
-          Frag<T> f = L::load_cols(v_tile, 16 * g, 32 * d, lane);
-          if (apart) {
-            drop_not_finite<T>(f);
-          }
-          o[d] = mma32<T>(f, w[g], o[d]);
-        }
-      }
-      if (apart) {
-        for (int n = max(tile.low - begin, 0); n < tile.end - begin; ++n) {
-          const int j = begin + n;
-          const bool sees = j <= p && (j >= seen_from || j < a.keep);
-#pragma unroll
-          for (int d = 0; d < DT / 32; ++d) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = L::value(v_tile, n, 32 * d + 8 * (i / 4) + 4 * h + i % 4);
-              o[d][i] += sees && not_finite(x) ? x : 0.0f;
-            }
-          }
+          s[g][i] = sees(32 * g + 8 * (i / 4) + i % 4) ? s[g][i] : -INFINITY;
         }
       }
     }
-    bool odd = false;
+    float top = s[0][0];
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d) {
+    for (int g = 0; g < KT / 32; ++g) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        odd = odd || not_finite(o[d][i]);
+        top = fmaxf(top, s[g][i]);
       }
     }
-    if (!__syncthreads_or(odd && careful == 0)) {
-      break;
+    top = max_halves(top) * a.scale_log2;
+    if (__any(top > m + kSlack)) {
+      const float now = fmaxf(m, top);
+      const float by = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < DT / 32; ++d) {
+        o[d] *= by;
+      }
     }
+    const float less = m == -INFINITY ? 0.0f : m;
+    // 16 keys at a time: their products run beside the exponentials of the next 16
+    constexpr int kSteps = DT / 32; // products of 16 keys
+    float sum = 0.0f;
+    float e[8];
+    const auto weigh = [&](int g, int i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + i], a.scale_log2, -less));
+      sum += e[i];
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      weigh(0, i);
+    }
+    Frag<T> w = frag_of<T>(e);
+    read_ahead<T, (KT / 16) * kSteps>(
+        [&](int n) { return L::load_cols(v_tile, 16 * (n / kSteps), 32 * (n % kSteps), lane); },
+        [&](int n, const Frag<T>& f) {
+          o[n % kSteps] = mma32<T>(f, w, o[n % kSteps]);
+          const int g = n / kSteps + 1;
+          if (g < KT / 16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (i * kSteps / 8 == n % kSteps) {
+                weigh(g, i);
+              }
+            }
+            if (n % kSteps == kSteps - 1) {
+              w = frag_of<T>(e);
+            }
+          }
+        });
+    l += sum;
   }
-
   l = sum_halves(l);
-  if (!stored) {
-    return;
-  }
-  if (a.splits > 1) {
-    const int64_t at = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R + row;
+  const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
+  if (stored && a.splits > 1) {
+    float* to = a.part_out + (part + row) * a.D;
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = 32 * d + 8 * i + 4 * h;
         if (c < a.D) {
-          *reinterpret_cast<float4*>(a.part_out + at * a.D + c) =
+          *reinterpret_cast<float4*>(to + c) =
               make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
         }
       }
     }
     if (h == 0) {
-      a.part_ml[at] = make_float2(m, seeing ? l : 0.0f);
+      a.part_ml[part + row] = make_float2(m, seeing ? l : 0.0f);
     }
-    return;
-  }
-  const float by = l == 0.0f ? 0.0f : 1.0f / l; // nothing but scores of -inf
-  T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row);
+  } else if (stored) {
+    const float by = l == 0.0f ? 0.0f : 1.0f / l; // nothing but scores of -inf
+    T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row);
 #pragma unroll
-  for (int d = 0; d < DT / 32; ++d) {
+    for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 32 * d + 8 * i + 4 * h;
-      if (c < a.D) {
-        store4<T>(out + c, seeing ? floatx4{o[d][4 * i] * by, o[d][4 * i + 1] * by,
-                                            o[d][4 * i + 2] * by, o[d][4 * i + 3] * by}
-                                  : floatx4{});
+      for (int i = 0; i < 4; ++i) {
+        const int c = 32 * d + 8 * i + 4 * h;
+        if (c < a.D) {
+          store4<T>(out + c, seeing ? floatx4{o[d][4 * i] * by, o[d][4 * i + 1] * by,
+                                              o[d][4 * i + 2] * by, o[d][4 * i + 3] * by}
+                                    : floatx4{});
+        }
       }
     }
+    if (a.lse != nullptr && h == 0) {
+      const int i = row / a.G;
+      a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
+          seeing ? m + log2f(l) : 0.0f;
+    }
   }
-  if (a.lse != nullptr && h == 0) {
-    const int i = row / a.G;
-    a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
-        seeing ? m + log2f(l) : 0.0f;
+  if (odd) { // the same for all
+    after_stores();
+    const int d = threadIdx.x;
+    for (int t = t0; t < t1 && d < a.D; ++t) {
+      const KeyTile tile = tile_of(range, t, KT);
+      for (int j = max(tile.begin, tile.low); j < tile.end; ++j) {
+        const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
+        for (int r = lo; not_finite(x) && r <= hi; ++r) {
+          if (!sees_key(a, p0 + r / a.G, j)) {
+            continue;
+          }
+          if (a.splits > 1) {
+            add_to(a.part_out + (part + r) * a.D + d, x);
+          } else {
+            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, r) + d, x);
+          }
+        }
+      }
+    }
   }
 }
 
