@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._copy import astype as _astype, contiguous as _contiguous, copy as _copy
 from .ops import _DTYPE_CODE, _FLOATING, _require_gpu, _stream_ptr
 
@@ -158,6 +158,9 @@ def window_attention(
     ``q`` ``[B, Hq, Lq, D]``, ``k`` and ``v`` ``[B, Hkv, Lk, D]``; ``lengths`` ``[B]``: how many of
     the ``Lk`` keys each sequence has, all without it.  The result has ``q``'s shape and, where
     that is dense, its memory order.  Differentiable with respect to q, k and v."""
+    out = ops._fast.window_attention(q, k, v, scale, window, keep, lengths)
+    if out is not None:
+        return out
     tag = "window_attention"
     scale, window, keep = _check_visible(tag, scale, window, keep)
     _check_heads(tag, q, k, v, "")
@@ -217,6 +220,8 @@ def paged_cache_update(
     size a multiple of 16; token ``j`` of sequence ``b`` has row ``j % page size`` of page
     ``block_table[b, j // page size]``.  ``lengths`` ``[B]`` counts the tokens of each sequence with
     the new ones; where it is below ``L``, those in front are padding and not written."""
+    if ops._fast.paged_cache_update(k, v, k_pages, v_pages, block_table, lengths):
+        return k_pages, v_pages
     tag = "paged_cache_update"
     for name, t in (("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages)):
         if t.dim() != 4:
@@ -265,6 +270,10 @@ def paged_attention(
     1 for decoding, a few for drafted tokens, any number for a chunk of a prompt.  The work is laid
     out for the keys that ``block_table`` has room for: a table much wider than the
     sequences is better passed as its first columns.  No gradients."""
+    out = ops._fast.paged_attention(
+        q, k_pages, v_pages, block_table, lengths, scale, window, keep)
+    if out is not None:
+        return out
     tag = "paged_attention"
     scale, window, keep = _check_visible(tag, scale, window, keep)
     _check_heads(tag, q, k_pages, v_pages, "_pages")
@@ -317,6 +326,10 @@ def verify_draft(
     from the target.  Returns ``(tokens [B, K + 1], accepted [B])`` as int32: the kept drafts, the
     token drawn (-1 if no token has any probability), then -1.  Weights are summed as whole
     multiples of 2**-40, so the same inputs give the same tokens whatever the order of sums."""
+    out = ops._fast.verify_draft(
+        draft, target_probs, draft_probs, accept_uniform, sample_uniform, lengths)
+    if out is not None:
+        return out
     tag = "verify_draft"
     if draft.dim() != 2:
         raise ValueError(f"[{tag}] draft must have 2 dimensions but has shape {tuple(draft.shape)}.")

@@ -26,6 +26,7 @@ struct FewShape {
   static constexpr int kE = DT == 64 ? 4 : DT == 96 ? 6 : 8; // columns of a lane
   static constexpr int kGroups = DT == 256 ? 2 : 1;          // of 16 kE columns
   static constexpr int kDwords = kE * sizeof(T) / 4;
+  static constexpr bool kNext = DT * sizeof(T) <= 256;
 };
 
 // The keys of one tile as this lane's operands need them.
@@ -139,7 +140,9 @@ __device__ __forceinline__ float sum_quarters(float v) {
 
 // NT: tiles of 16 rows
 template <typename T, int DT, int NT, bool PAGED>
-__global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(DT * NT * sizeof(T) <= 256 ? 2 : 1)))
+void attention_few_kernel(const AttentionArgs a) {
   using S = FewShape<T, DT>;
   constexpr int KT = kFewKeys;
   __shared__ struct { // the waves' results of 16 rows, while they are joined
@@ -200,13 +203,25 @@ __global__ __launch_bounds__(256) void attention_few_kernel(const AttentionArgs 
     }
   }
   bool odd = false; // some value was left out of the products
+  // the next tile is on its way while one is worked on, where registers are left for it
+  FewTile<T, DT> tile, next;
+  const auto load = [&](int t, FewTile<T, DT>& to) {
+    const KeyTile at = tile_of(range, t, KT);
+    load_tile<T, DT, PAGED>(a, b, hk, at.begin, at.low, at.end, lane, to);
+  };
+  if (S::kNext && t0 + wave < t1) {
+    load(t0 + wave, next);
+  }
   for (int t = t0 + wave; t < t1; t += 4) {
     const KeyTile at = tile_of(range, t, KT);
-    const int begin = at.begin;
-    const int low = at.low;
-    const int end = at.end;
-    FewTile<T, DT> tile;
-    load_tile<T, DT, PAGED>(a, b, hk, begin, low, end, lane, tile);
+    if constexpr (S::kNext) {
+      tile = next;
+      if (t + 4 < t1) {
+        load(t + 4, next);
+      }
+    } else {
+      load(t, tile);
+    }
     const bool whole = whole_tile(a, at, KT, p_lo, p_hi);
     Frag<T> w[NT];
 #pragma unroll

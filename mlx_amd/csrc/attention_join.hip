@@ -1,10 +1,11 @@
 // attention_join.hip -- joins what several workgroups have of the same rows, each over a run of
 // the keys: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, m = max_s m_s.
 //
-// A wave has a row, a lane the maximum and sum of one run (there are at most 64), so the
-// weights of all runs are there after one load; then its lanes add up the runs, four columns each
-// and 64 / width runs at a time, with nothing to wait for between their loads.  (With the
-// runs in turn, each behind the one before, 28 rows of 64 runs took 45 us.)
+// A row is joined by WAVES waves.  A lane has the maximum and sum of one run (there are at most
+// 64), so the weights of all runs are there after one load; then lanes add up the runs, four
+// columns each and 64 WAVES / WIDTH runs at a time, with nothing to wait for between their
+// loads.  Few rows of many runs take a workgroup each, many rows a wave each.  (28 rows of 64 runs:
+// one run behind the other 45 us, a wave for a row 13.7, a workgroup for a row 4.)
 #include "attention.h"
 
 namespace mlxrocm {
@@ -12,14 +13,16 @@ namespace mlxrocm {
 namespace {
 
 // WIDTH lanes have the columns of a run
-template <typename T, int WIDTH>
+template <typename T, int WIDTH, int WAVES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
-  constexpr int kAtOnce = 64 / WIDTH;
+  constexpr int kAtOnce = 64 / WIDTH * WAVES;
+  __shared__ floatx4 sums[WAVES > 1 ? WAVES : 1][WIDTH];
   const int R = a.G * a.Lq;
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * R;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6;
+  const int64_t n = WAVES > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave;
   if (n >= rows) {
-    return;
+    return; // (whole waves; with WAVES > 1 none)
   }
   const int lane = threadIdx.x & 63;
   const float2 ml =
@@ -37,9 +40,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const int d = 4 * (lane % WIDTH);
   const float* part = a.part_out + n * a.D + (d < a.D ? d : 0);
   floatx4 sum = {};
-#pragma unroll 4
+#pragma unroll 8
   for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
-    const int s = s0 + lane / WIDTH;
+    const int s = s0 + (WAVES > 1 ? wave * (64 / WIDTH) : 0) + lane / WIDTH;
     const float w = __shfl(by, s & 63, 64);
     const float4 v = *reinterpret_cast<const float4*>(part + min(s, a.splits - 1) * rows * a.D);
     if (s < a.splits && w != 0.0f) {
@@ -51,6 +54,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum[i] += __shfl_xor(sum[i], off, 64);
+    }
+  }
+  if constexpr (WAVES > 1) {
+    if (lane < WIDTH) {
+      sums[wave][lane] = sum;
+    }
+    __syncthreads();
+    if (wave != 0) {
+      return;
+    }
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      sum += sums[w][lane % WIDTH];
     }
   }
   const int head = static_cast<int>(n / R);
@@ -65,6 +81,54 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
     store4<T>(out, seeing ? sum * over : floatx4{});
   }
   if (a.lse != nullptr && lane == 0) {
+    a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
+        seeing ? top + log2f(total) : 0.0f;
+  }
+}
+
+// The same for two to four runs of many rows: a thread has four columns.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_few_kernel(const AttentionArgs a) {
+  const int R = a.G * a.Lq;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * R;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n = at / (a.D / 4);
+  const int d = static_cast<int>(at - n * (a.D / 4)) * 4;
+  if (n >= rows) {
+    return;
+  }
+  float2 ml[4];
+  floatx4 x[4];
+  float top = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int64_t from = min(s, a.splits - 1) * rows + n;
+    const float4 v = *reinterpret_cast<const float4*>(a.part_out + from * a.D + d);
+    x[s] = floatx4{v.x, v.y, v.z, v.w};
+    ml[s] = s < a.splits ? a.part_ml[from] : make_float2(-INFINITY, 0.0f);
+    top = fmaxf(top, ml[s].x);
+  }
+  const float less = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;
+  floatx4 sum = {};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    if (!(ml[s].y == 0.0f)) {
+      const float by = ml[s].x == less ? 1.0f : __builtin_amdgcn_exp2f(ml[s].x - less);
+      total = fmaf(by, ml[s].y, total);
+      sum += by * x[s];
+    }
+  }
+  const int head = static_cast<int>(n / R);
+  const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
+  const int b = head / a.Hkv;
+  const int hk = head - b * a.Hkv;
+  const int i = row / a.G;
+  const bool seeing = length_of(a, b) - a.Lq + i >= 0;
+  const float over = total == 0.0f ? 0.0f : 1.0f / total;
+  T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row) + d;
+  store4<T>(out, seeing ? sum * over : floatx4{});
+  if (a.lse != nullptr && d == 0) {
     a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
         seeing ? top + log2f(total) : 0.0f;
   }
@@ -153,18 +217,33 @@ int launch_attention_grad_join(const AttentionGradArgs& g, int dtype, hipStream_
   });
 }
 
+namespace {
+
+template <typename T, int WIDTH>
+void launch_join_of(const AttentionArgs& a, int64_t rows, hipStream_t s) {
+  if (rows <= 2048) {
+    attention_join_kernel<T, WIDTH, 4><<<static_cast<unsigned>(rows), 256, 0, s>>>(a);
+  } else {
+    attention_join_kernel<T, WIDTH, 1><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, s>>>(a);
+  }
+}
+
+} // namespace
+
 int launch_attention_join(const AttentionArgs& a, int dtype, hipStream_t s) {
   MLXROCM_REHEARSE("attention_join");
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Lq;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.D <= 64) {
-      attention_join_kernel<T, 16><<<grid, 256, 0, s>>>(a);
+    if (a.splits <= 4) {
+      const int64_t n = rows * (a.D / 4);
+      attention_join_few_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(a);
+    } else if (a.D <= 64) {
+      launch_join_of<T, 16>(a, rows, s);
     } else if (a.D <= 128) {
-      attention_join_kernel<T, 32><<<grid, 256, 0, s>>>(a);
+      launch_join_of<T, 32>(a, rows, s);
     } else {
-      attention_join_kernel<T, 64><<<grid, 256, 0, s>>>(a);
+      launch_join_of<T, 64>(a, rows, s);
     }
     MLXROCM_HIP_TRY(hipGetLastError());
     return static_cast<int>(MLXROCM_OK);

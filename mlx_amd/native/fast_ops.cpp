@@ -25,6 +25,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 
@@ -56,6 +57,13 @@ struct Abi {
   decltype(&mlxrocm_affine_dequantize) affine_dequantize;
   decltype(&mlxrocm_fp_quantize) fp_quantize;
   decltype(&mlxrocm_fp_dequantize) fp_dequantize;
+  decltype(&mlxrocm_window_attention_workspace_size) window_workspace_size;
+  decltype(&mlxrocm_window_attention) window_attention;
+  decltype(&mlxrocm_paged_attention_workspace_size) paged_workspace_size;
+  decltype(&mlxrocm_paged_attention) paged_attention;
+  decltype(&mlxrocm_paged_cache_update) paged_cache_update;
+  decltype(&mlxrocm_verify_draft_workspace_size) verify_workspace_size;
+  decltype(&mlxrocm_verify_draft) verify_draft;
 };
 Abi abi{};
 bool bound = false;
@@ -644,6 +652,341 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FAST_CATCH
 }
 
+// ---- attention (attention.py) ------------------------------------------------------
+
+// A tensor of four dimensions on `device` whose rows along the last are dense and aligned to 16
+// bytes, with no gradient to be recorded.
+const at::Tensor* heads_of(PyObject* o, c10::DeviceIndex device) {
+  if (!THPVariable_CheckExact(o)) {
+    return nullptr;
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !t.is_cuda() || t.device().index() != device || t.dim() != 4 ||
+      t.numel() == 0 || t.is_conj() || t.is_neg() || records_grad(t) ||
+      dtype_code(t.scalar_type()) < 0 || t.stride(3) != 1 ||
+      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) {
+    return nullptr;
+  }
+  const int64_t unit = 16 / static_cast<int64_t>(t.element_size());
+  for (int i = 0; i < 3; ++i) {
+    if (t.size(i) != 1 && t.stride(i) % unit != 0) {
+      return nullptr;
+    }
+  }
+  return &t;
+}
+
+// int32, dense rows
+const at::Tensor* indices_of(PyObject* o, c10::DeviceIndex device, int64_t dims, int64_t rows) {
+  if (!THPVariable_CheckExact(o)) {
+    return nullptr;
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.defined() && t.is_cuda() && t.device().index() == device && t.dim() == dims &&
+          t.scalar_type() == at::kInt && t.numel() > 0 && t.size(0) == rows &&
+          (dims == 1 ? t.is_contiguous() : t.stride(1) == 1)
+      ? &t
+      : nullptr;
+}
+
+// What a query sees: scale, a float, window, a positive int or None, keep, an int
+struct Sight {
+  double scale;
+  int window, keep;
+};
+bool sight_of(PyObject* scale, PyObject* window, PyObject* keep, Sight* s) {
+  constexpr int kMost = 1 << 30;
+  const auto whole = [](PyObject* o, int least, int* v) {
+    if (!PyLong_CheckExact(o)) {
+      return false;
+    }
+    int overflow = 0;
+    const long x = PyLong_AsLongAndOverflow(o, &overflow);
+    if (overflow != 0 || x < least) {
+      return false;
+    }
+    *v = x < kMost ? static_cast<int>(x) : kMost;
+    return true;
+  };
+  if (!PyFloat_CheckExact(scale)) {
+    return false;
+  }
+  s->scale = PyFloat_AS_DOUBLE(scale);
+  s->window = kMost;
+  return std::isfinite(static_cast<float>(s->scale)) &&
+      (window == Py_None || whole(window, 1, &s->window)) && whole(keep, 0, &s->keep);
+}
+
+// Of the first three dimensions, in elements; 0 where there is one element
+void strides_of(const at::Tensor& t, int64_t* to) {
+  for (int i = 0; i < 3; ++i) {
+    to[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
+}
+
+// A new tensor with q's sizes and memory order, if q is dense
+bool like(const at::Tensor& q, c10::DeviceIndex device, at::Tensor* out) {
+  if (!q.is_non_overlapping_and_dense()) {
+    return false;
+  }
+  *out = at::Tensor(at::detail::empty_strided_cuda(
+      q.sizes(), q.strides(), q.scalar_type(), c10::Device(c10::DeviceType::CUDA, device)));
+  return true;
+}
+
+bool attends(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+  const int64_t D = q.size(3);
+  return k.sizes() == v.sizes() && k.scalar_type() == q.scalar_type() &&
+      v.scalar_type() == q.scalar_type() && k.size(3) == D && D % 8 == 0 && D <= 256 &&
+      q.size(1) % k.size(1) == 0;
+}
+
+// window_attention(q, k, v, scale, window, keep, lengths), lengths a tensor or None
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!bound || n != 7) {
+    NOT_PLAIN;
+  }
+  FAST_TRY
+  const c10::DeviceIndex device = device_of(args[0]);
+  Sight sight;
+  if (device < 0 || !sight_of(args[3], args[4], args[5], &sight)) {
+    NOT_PLAIN;
+  }
+  const at::Tensor* q = heads_of(args[0], device);
+  const at::Tensor* k = heads_of(args[1], device);
+  const at::Tensor* v = heads_of(args[2], device);
+  if (q == nullptr || k == nullptr || v == nullptr || !attends(*q, *k, *v) ||
+      k->size(0) != q->size(0)) {
+    NOT_PLAIN;
+  }
+  const at::Tensor* lengths = nullptr;
+  if (args[6] != Py_None) {
+    lengths = indices_of(args[6], device, 1, q->size(0));
+    if (lengths == nullptr) {
+      NOT_PLAIN;
+    }
+  }
+  const int64_t sizes[] = {q->size(0), q->size(1), k->size(1), q->size(2), k->size(2), q->size(3)};
+  for (const int64_t s : sizes) {
+    if (!fits_int(s)) {
+      NOT_PLAIN;
+    }
+  }
+  at::Tensor out;
+  if (!like(*q, device, &out)) {
+    NOT_PLAIN;
+  }
+  const int code = dtype_code(q->scalar_type());
+  int64_t strides[12];
+  strides_of(*q, strides);
+  strides_of(*k, strides + 3);
+  strides_of(*v, strides + 6);
+  strides_of(out, strides + 9);
+  const Workspace ws(
+      abi.window_workspace_size(
+          sizes[0], sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], sight.window, sight.keep,
+          code),
+      device);
+  void* stream = stream_of(device);
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = abi.window_attention(
+      q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), nullptr,
+      lengths == nullptr ? nullptr : static_cast<const int32_t*>(lengths->data_ptr()), sizes[0],
+      sizes[1], sizes[2], sizes[3], sizes[4], sizes[5], strides, static_cast<float>(sight.scale),
+      sight.window, sight.keep, code, ws.ptr(), ws.bytes, stream);
+  Py_END_ALLOW_THREADS;
+  if (rc != MLXROCM_OK) {
+    NOT_PLAIN;
+  }
+  return wrap(std::move(out));
+  FAST_CATCH
+}
+
+// The pages of a cache and where a batch's sequences lie in them
+struct Cache {
+  const at::Tensor *k, *v, *table, *lengths;
+};
+bool cache_of(
+    PyObject* const* args, c10::DeviceIndex device, int64_t batch, at::ScalarType type, Cache* c) {
+  c->k = heads_of(args[0], device);
+  c->v = heads_of(args[1], device);
+  c->table = indices_of(args[2], device, 2, batch);
+  c->lengths = indices_of(args[3], device, 1, batch);
+  return c->k != nullptr && c->v != nullptr && c->table != nullptr && c->lengths != nullptr &&
+      c->k->sizes() == c->v->sizes() && c->k->scalar_type() == type &&
+      c->v->scalar_type() == type && c->k->size(2) % 16 == 0 && fits_int(c->k->size(0)) &&
+      fits_int(c->k->size(2)) && fits_int(c->table->size(1)) &&
+      fits_int(c->table->size(1) * c->k->size(2));
+}
+
+// paged_attention(q, k_pages, v_pages, block_table, lengths, scale, window, keep)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!bound || n != 8) {
+    NOT_PLAIN;
+  }
+  FAST_TRY
+  const c10::DeviceIndex device = device_of(args[0]);
+  Sight sight;
+  if (device < 0 || !sight_of(args[5], args[6], args[7], &sight)) {
+    NOT_PLAIN;
+  }
+  const at::Tensor* q = heads_of(args[0], device);
+  Cache c;
+  if (q == nullptr || !cache_of(args + 1, device, q->size(0), q->scalar_type(), &c) ||
+      !attends(*q, *c.k, *c.v)) {
+    NOT_PLAIN;
+  }
+  const int64_t B = q->size(0), Hq = q->size(1), Hkv = c.k->size(1), Lq = q->size(2);
+  const int64_t D = q->size(3), page = c.k->size(2), width = c.table->size(1);
+  if (!fits_int(B) || !fits_int(Hq) || !fits_int(Lq)) {
+    NOT_PLAIN;
+  }
+  at::Tensor out;
+  if (!like(*q, device, &out)) {
+    NOT_PLAIN;
+  }
+  const int code = dtype_code(q->scalar_type());
+  int64_t strides[13];
+  strides_of(*q, strides);
+  strides_of(*c.k, strides + 3);
+  strides_of(*c.v, strides + 6);
+  strides_of(out, strides + 9);
+  strides[12] = c.table->stride(0);
+  const Workspace ws(
+      abi.paged_workspace_size(
+          B, Hq, Hkv, Lq, D, width * page, sight.window, sight.keep, code),
+      device);
+  void* stream = stream_of(device);
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = abi.paged_attention(
+      q->data_ptr(), c.k->data_ptr(), c.v->data_ptr(),
+      static_cast<const int32_t*>(c.table->data_ptr()),
+      static_cast<const int32_t*>(c.lengths->data_ptr()), out.data_ptr(), B, Hq, Hkv, Lq, D,
+      c.k->size(0), page, width, strides, static_cast<float>(sight.scale), sight.window,
+      sight.keep, code, ws.ptr(), ws.bytes, stream);
+  Py_END_ALLOW_THREADS;
+  if (rc != MLXROCM_OK) {
+    NOT_PLAIN;
+  }
+  return wrap(std::move(out));
+  FAST_CATCH
+}
+
+// paged_cache_update(k, v, k_pages, v_pages, block_table, lengths): True where it was done
+PyObject* paged_cache_update(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!bound || n != 6) {
+    NOT_PLAIN;
+  }
+  FAST_TRY
+  const c10::DeviceIndex device = device_of(args[0]);
+  if (device < 0) {
+    NOT_PLAIN;
+  }
+  const at::Tensor* k = heads_of(args[0], device);
+  const at::Tensor* v = heads_of(args[1], device);
+  Cache c;
+  if (k == nullptr || v == nullptr || k->sizes() != v->sizes() ||
+      k->scalar_type() != v->scalar_type() ||
+      !cache_of(args + 2, device, k->size(0), k->scalar_type(), &c) ||
+      k->size(1) != c.k->size(1) || k->size(3) != c.k->size(3) || !fits_int(k->size(0)) ||
+      !fits_int(k->size(2)) || !fits_int(k->size(3))) {
+    NOT_PLAIN;
+  }
+  int64_t strides[13];
+  strides_of(*k, strides);
+  strides_of(*v, strides + 3);
+  strides_of(*c.k, strides + 6);
+  strides_of(*c.v, strides + 9);
+  strides[12] = c.table->stride(0);
+  void* stream = stream_of(device);
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = abi.paged_cache_update(
+      k->data_ptr(), v->data_ptr(), c.k->data_ptr(), c.v->data_ptr(),
+      static_cast<const int32_t*>(c.table->data_ptr()),
+      static_cast<const int32_t*>(c.lengths->data_ptr()), k->size(0), k->size(1), k->size(2),
+      k->size(3), c.k->size(0), c.k->size(2), c.table->size(1), strides,
+      dtype_code(k->scalar_type()), stream);
+  Py_END_ALLOW_THREADS;
+  if (rc != MLXROCM_OK) {
+    NOT_PLAIN;
+  }
+  Py_RETURN_TRUE;
+  FAST_CATCH
+}
+
+// verify_draft(draft, target_probs, draft_probs, accept, sample, lengths); draft_probs and lengths
+// may be None
+PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!bound || n != 6) {
+    NOT_PLAIN;
+  }
+  FAST_TRY
+  const c10::DeviceIndex device = device_of(args[0]);
+  if (device < 0) {
+    NOT_PLAIN;
+  }
+  const at::Tensor* draft = matrix_of(args[0], device, at::kInt);
+  const at::Tensor* target = tensor_of(args[1], device);
+  const at::Tensor* accept = matrix_of(args[3], device, at::kFloat);
+  const at::Tensor* sample = tensor_of(args[4], device);
+  if (draft == nullptr || target == nullptr || accept == nullptr || sample == nullptr ||
+      target->dim() != 3 || accept->sizes() != draft->sizes() || sample->dim() != 1 ||
+      sample->scalar_type() != at::kFloat) {
+    NOT_PLAIN;
+  }
+  const int64_t B = draft->size(0), K = draft->size(1), V = target->size(2);
+  const int code = dtype_code(target->scalar_type());
+  const at::Tensor* probs = nullptr;
+  const at::Tensor* lengths = nullptr;
+  if (args[2] != Py_None) {
+    probs = tensor_of(args[2], device);
+    if (probs == nullptr || probs->dim() != 3 || probs->scalar_type() != target->scalar_type() ||
+        probs->size(0) != B || probs->size(1) != K || probs->size(2) != V) {
+      NOT_PLAIN;
+    }
+  }
+  if (args[5] != Py_None) {
+    lengths = indices_of(args[5], device, 1, B);
+    if (lengths == nullptr) {
+      NOT_PLAIN;
+    }
+  }
+  if (code < 0 || target->size(0) != B || target->size(1) != K + 1 || sample->size(0) != B ||
+      !fits_int(B) || !fits_int(K + 1) || !fits_int(V)) {
+    NOT_PLAIN;
+  }
+  at::Tensor tokens = new_tensor({B, K + 1}, at::kInt, device);
+  at::Tensor accepted = new_tensor({B}, at::kInt, device);
+  const int64_t strides[4] = {(K + 1) * V, V, K * V, V};
+  const Workspace ws(abi.verify_workspace_size(B, V), device);
+  void* stream = stream_of(device);
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = abi.verify_draft(
+      static_cast<const int32_t*>(draft->data_ptr()), target->data_ptr(),
+      probs == nullptr ? nullptr : probs->data_ptr(),
+      static_cast<const float*>(accept->data_ptr()),
+      static_cast<const float*>(sample->data_ptr()),
+      lengths == nullptr ? nullptr : static_cast<const int32_t*>(lengths->data_ptr()),
+      static_cast<int32_t*>(tokens.data_ptr()), static_cast<int32_t*>(accepted.data_ptr()), B, K,
+      V, strides, code, ws.ptr(), ws.bytes, stream);
+  Py_END_ALLOW_THREADS;
+  if (rc != MLXROCM_OK) {
+    NOT_PLAIN;
+  }
+  PyObject* out = PyTuple_New(2);
+  if (out == nullptr) {
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(out, 0, wrap(std::move(tokens)));
+  PyTuple_SET_ITEM(out, 1, wrap(std::move(accepted)));
+  return out;
+  FAST_CATCH
+}
+
 // bind({entry point: address}): the library whose entry points are to be called
 PyObject* bind(PyObject*, PyObject* table) {
   if (!PyDict_Check(table)) {
@@ -686,7 +1029,14 @@ PyObject* bind(PyObject*, PyObject* table) {
       take("mlxrocm_affine_quantize", abi.affine_quantize) &&
       take("mlxrocm_affine_dequantize", abi.affine_dequantize) &&
       take("mlxrocm_fp_quantize", abi.fp_quantize) &&
-      take("mlxrocm_fp_dequantize", abi.fp_dequantize);
+      take("mlxrocm_fp_dequantize", abi.fp_dequantize) &&
+      take("mlxrocm_window_attention_workspace_size", abi.window_workspace_size) &&
+      take("mlxrocm_window_attention", abi.window_attention) &&
+      take("mlxrocm_paged_attention_workspace_size", abi.paged_workspace_size) &&
+      take("mlxrocm_paged_attention", abi.paged_attention) &&
+      take("mlxrocm_paged_cache_update", abi.paged_cache_update) &&
+      take("mlxrocm_verify_draft_workspace_size", abi.verify_workspace_size) &&
+      take("mlxrocm_verify_draft", abi.verify_draft);
   if (!bound) {
     return nullptr;
   }
@@ -702,6 +1052,10 @@ PyMethodDef methods[] = {
     FASTCALL(qqmm),
     FASTCALL(quantize),
     FASTCALL(dequantize),
+    FASTCALL(window_attention),
+    FASTCALL(paged_attention),
+    FASTCALL(paged_cache_update),
+    FASTCALL(verify_draft),
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
