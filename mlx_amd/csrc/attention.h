@@ -26,6 +26,34 @@
 
 namespace mlxrocm {
 
+// n / d for n below 2^31 in a multiplication: with m = 2^32 / d the quotient is short by one at
+// most.  (The compiler's own division takes some forty instructions, and a workgroup has several
+// before its first load.)
+struct Divisor {
+  int d = 1;
+  uint32_t m = 0xffffffffu;
+  Divisor() = default;
+  explicit Divisor(int64_t by)
+      : d(by < 1 ? 1 : static_cast<int>(by)),
+        m(by <= 1 ? 0xffffffffu : static_cast<uint32_t>((uint64_t{1} << 32) / by)) {}
+#ifdef __HIPCC__
+  __device__ __forceinline__ int divide(int n, int* rest) const {
+    int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), m));
+    int r = n - q * d;
+    if (r >= d) {
+      ++q;
+      r -= d;
+    }
+    *rest = r;
+    return q;
+  }
+  __device__ __forceinline__ int divide(int n) const {
+    int rest;
+    return divide(n, &rest);
+  }
+#endif
+};
+
 struct AttentionArgs {
   const void* q;
   const void* k;
@@ -37,9 +65,9 @@ struct AttentionArgs {
   int64_t table_stride;
   int B, Hq, Hkv, G, Lq, D;
   int keys;      // most keys a sequence can have
-  int page;      // rows of a page (table), and what divides by it
-  uint32_t page_magic;
+  Divisor page;  // rows of a page (table)
   int pages;
+  Divisor of_G, of_Hkv, of_splits;
   // strides in elements; of k and v: [sequence or page, head, row]
   int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3]; // [sequence, head, token]
   float scale_log2; // |scale| log2(e)
@@ -56,14 +84,14 @@ struct AttentionArgs {
 // dv over rows.  The blocks of the keys that every later row sees (under a window) have many more
 // rows than the others.
 struct GradPlan {
-  int dq_splits;
+  Divisor dq_splits;
   int wide_blocks; // blocks of kept keys, with wide_splits runs each; the others have splits
-  int wide_splits, splits;
+  Divisor wide_splits, splits;
   int blocks; // of keys
   __host__ __device__ int pieces() const {
-    return wide_blocks * wide_splits + (blocks - wide_blocks) * splits;
+    return wide_blocks * wide_splits.d + (blocks - wide_blocks) * splits.d;
   }
-  __host__ __device__ bool dkv_split() const { return wide_splits > 1 || splits > 1; }
+  __host__ __device__ bool dkv_split() const { return wide_splits.d > 1 || splits.d > 1; }
 };
 
 // The gradients' further operands.
@@ -82,9 +110,6 @@ struct AttentionGradArgs {
 };
 
 constexpr int kGradBlock = 128; // rows or keys of a workgroup
-
-// Whether the few-rows kernel takes a call (else the tiles of 128 rows).
-constexpr int kFewRows = 64;
 
 // One unit for each type: by the dtype of a call
 int launch_attention_few_f32(const AttentionArgs& a, hipStream_t s);
@@ -292,8 +317,8 @@ struct KeyRange {
 
 __device__ __forceinline__ KeyRange
 keys_of(const AttentionArgs& a, int length, int first_row, int last_row, int kt) {
-  const int p_lo = length - a.Lq + first_row / a.G;
-  const int p_hi = length - a.Lq + last_row / a.G;
+  const int p_lo = length - a.Lq + a.of_G.divide(first_row);
+  const int p_hi = length - a.Lq + a.of_G.divide(last_row);
   KeyRange r;
   r.w_end = p_hi + 1;
   r.w_low = max(0, p_lo - a.window + 1);
@@ -319,6 +344,15 @@ __device__ __forceinline__ KeyTile tile_of(const KeyRange& r, int t, int kt) {
   k.end = min(k.begin + kt, a ? r.a_end : r.w_end);
   return k;
 }
+// Tiles [*first, *last) of run `split`: as equal as they come
+__device__ __forceinline__ void
+run_of(int tiles, int split, const Divisor& splits, int* first, int* last) {
+  int rest;
+  const int each = splits.divide(tiles, &rest);
+  *first = split * each + min(split, rest);
+  *last = *first + each + (split < rest ? 1 : 0);
+}
+
 // Whether positions lo .. hi see all of a tile
 __device__ __forceinline__ bool
 whole_tile(const AttentionArgs& a, const KeyTile& k, int kt, int lo, int hi) {
@@ -350,18 +384,6 @@ struct Seen {
   }
 };
 
-// Divides by the page size: page_magic = 2^32 / page + 1 overshoots by one at most.
-__device__ __forceinline__ int page_of(const AttentionArgs& a, int j, int* in_page) {
-  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(j), a.page_magic));
-  int r = j - q * a.page;
-  if (r < 0) {
-    --q;
-    r += a.page;
-  }
-  *in_page = r;
-  return q;
-}
-
 // Offsets of key j's row in k and in v: through the page table, whose entries are clamped to
 // pages that exist, or along contiguous keys.
 struct KeyRow {
@@ -373,7 +395,7 @@ __device__ __forceinline__ KeyRow key_row(const AttentionArgs& a, int b, int hk,
   int at = j;
   if constexpr (PAGED) {
     int in_page;
-    const int page = page_of(a, j, &in_page);
+    const int page = a.page.divide(j, &in_page);
     const int id = a.table[b * a.table_stride + page];
     first = min(max(id, 0), a.pages - 1);
     at = in_page;
@@ -391,27 +413,43 @@ __device__ __forceinline__ int length_of(const AttentionArgs& a, int b) {
 
 // Offset of row r's token in a [sequence, head, token] tensor
 __device__ __forceinline__ int64_t row_offset(
-    const int64_t (&strides)[3], int b, int hk, int G, int r) {
-  const int i = r / G;
-  return b * strides[0] + (hk * G + (r - i * G)) * strides[1] + i * strides[2];
+    const int64_t (&strides)[3], int b, int hk, const Divisor& G, int r) {
+  int g;
+  const int i = G.divide(r, &g);
+  return b * strides[0] + (hk * G.d + g) * strides[1] + i * strides[2];
 }
 
-// Which (sequence, key head) and which of its `per` pieces a workgroup has.  Workgroups go
-// to the 8 dies in turn, and each die has an L2 of its own: eight heads side by side, one
-// on each die, so that all that read a head's keys find them in one L2.
-__device__ __forceinline__ void piece_of(int heads, int per, int* head, int* piece) {
-  const int block = blockIdx.x;
-  const int group = block / (8 * per);
-  const int rest = block - group * 8 * per;
-  const int width = min(8, heads - group * 8);
-  *head = group * 8 + rest % width;
-  *piece = rest / width;
-}
+// Which (sequence, key head) and which of its pieces a workgroup has.  Workgroups go to the 8 dies
+// in turn, and each die has an L2 of its own: eight heads side by side, one on each die, so that
+// all that read a head's keys find them in one L2.
+struct Grid {
+  int heads, pieces;
+  Divisor of_eight, of_last; // 8 pieces, the heads of the last, smaller group
+  Grid(int64_t heads_, int64_t pieces_)
+      : heads(static_cast<int>(heads_)),
+        pieces(static_cast<int>(pieces_)),
+        of_eight(8 * pieces_),
+        of_last(heads_ % 8) {}
+  unsigned blocks() const { return static_cast<unsigned>(heads) * pieces; }
+  __device__ __forceinline__ void find(int* head, int* piece) const {
+    int rest, at;
+    const int group = of_eight.divide(blockIdx.x, &rest);
+    if (group * 8 + 8 <= heads) {
+      at = rest & 7;
+      *piece = rest >> 3;
+    } else {
+      *piece = of_last.divide(rest, &at);
+    }
+    *head = group * 8 + at;
+  }
+};
 
 // ---- tiles in LDS -----------------------------------------------------------------
+typedef __attribute__((address_space(3))) const char* LdsBytes;
+
 // Rows of DT elements in 16-byte units, a power of two of places for them, unit u of row r at
-// place u ^ swizzle(r): eight rows read at one column (load_rows) fall into eight different
-// places, and four rows read 32 bytes wide (load_cols) too.
+// place u ^ swizzle(r).  LDS has 64 banks: sixteen rows read at one unit (load_rows) and four rows
+// read 64 bytes wide (load_cols) lie in all of them once.
 template <typename T, int DT>
 struct Tile {
   static constexpr int kUnit = 16 / sizeof(T);
@@ -419,40 +457,46 @@ struct Tile {
   static constexpr int kPlaces = kPitch / kUnit;
   static constexpr int kRowsOfLoad = 64 / kPlaces; // that the 64 lanes of one load cover
   static constexpr int kRowsOfPass = 4 * kRowsOfLoad; // ... and those of a workgroup's four waves
+  // Loads after which a lane's columns repeat (the swizzle has the low bits of a row's number)
+  static constexpr int kTurns = kRowsOfPass >= 16 ? 1 : 16 / kRowsOfPass;
 
   static __device__ __forceinline__ int swizzle(int row) {
-    // (with 64 places a pass is four rows: a lane then loads the same column in each)
-    return kPlaces == 64 ? (row & 3) << 1 : (row & 3) << 1 | (row >> 2 & 1);
+    if constexpr (kPlaces == 8) { // two rows to the banks' width
+      return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    } else {
+      return (row & 3) << 2 | (row >> 2 & 3);
+    }
   }
   static __device__ __forceinline__ int at(int row, int unit) {
     return row * kPitch + (unit ^ swizzle(row)) * kUnit;
   }
   // Elements 16 c + 8 h .. 16 c + 8 h + 7 of row `row` + lane % 32, h = lane / 32; row: a multiple of
-  // 32.  Written so that few addresses differ by more than an offset in the instruction: a
-  // unit's three low bits are exclusive ored with what depends on the lane alone.
+  // 32.  Tiles are aligned to 1024 bytes, the longest row: the unit's number is exclusive ored into
+  // the address.
   static __device__ __forceinline__ Frag<T> load_rows(const T* tile, int row, int c, int lane) {
-    const int r = lane & 31;
-    const int h = lane >> 5;
     constexpr int kOf8 = 8 / kUnit; // units of 8 elements
-    const int t = (kOf8 * h) ^ swizzle(r);
-    const int unit = 2 * kOf8 * c;
-    const T* p = tile + row * kPitch + (unit & ~7) * kUnit + r * kPitch;
+    const int r = lane & 31;
+    const uint32_t own =
+        (r * kPlaces + ((kOf8 * (lane >> 5)) ^ swizzle(r))) * 16 + lds_address(tile);
+    const uint32_t p = own ^ (2 * kOf8 * c * 16);
+    Frag<T> f;
+    const auto a = *(__attribute__((address_space(3))) const raw_u32x4*)(
+        (LdsBytes)(uintptr_t)p + row * kPitch * sizeof(T));
     if constexpr (sizeof(T) == 4) {
-      Frag<T> f;
-      const float4 a = *reinterpret_cast<const float4*>(p + ((unit & 7) ^ t) * kUnit);
-      const float4 b = *reinterpret_cast<const float4*>(p + ((unit & 7) ^ t ^ 1) * kUnit);
-      f.w[0] = a.x;
-      f.w[1] = a.y;
-      f.w[2] = a.z;
-      f.w[3] = a.w;
-      f.w[4] = b.x;
-      f.w[5] = b.y;
-      f.w[6] = b.z;
-      f.w[7] = b.w;
-      return f;
+      const auto b = *(__attribute__((address_space(3))) const raw_u32x4*)(
+          (LdsBytes)(uintptr_t)(p ^ 16) + row * kPitch * sizeof(T));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f.w[i] = __uint_as_float(a[i]);
+        f.w[4 + i] = __uint_as_float(b[i]);
+      }
     } else {
-      return load_frag<T>(p + ((unit & 7) ^ t) * kUnit);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f.w[i] = a[i];
+      }
     }
+    return f;
   }
   // element d + lane % 32 of rows row + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}; row: a multiple of
   // 16, d of 32.  The transposing read takes four rows of 16 columns from 16 lanes' addresses and
@@ -468,24 +512,22 @@ struct Tile {
         f.w[j] = tile[at(r, c / 4) + c % 4];
       }
     } else {
-      const int y = lane >> 2 & 3;
-      const int t = ((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ swizzle(4 * h + y);
-      const int unit = d / 8;
-      const T* p = tile + row * kPitch + (unit & ~7) * kUnit + (4 * h + y) * kPitch +
-          ((unit & 7) ^ t) * kUnit + 4 * (lane & 1);
+      const int y = 4 * h + (lane >> 2 & 3); // row of the first four
+      const int u = (lane >> 4 & 1) << 1 | (lane >> 1 & 1);
+      const uint32_t own =
+          (y * kPlaces + (u ^ swizzle(y))) * 16 + 8 * (lane & 1) + lds_address(tile);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        const uint32_t p = own ^ ((d / 8) ^ (swizzle(8 * half))) * 16;
         const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) shortx4*)(p + half * 8 * kPitch));
-        const uint2 u = __builtin_bit_cast(uint2, x);
-        f.w[2 * half] = u.x;
-        f.w[2 * half + 1] = u.y;
+            (__attribute__((address_space(3))) shortx4*)(
+                (LdsBytes)(uintptr_t)p + (row + 8 * half) * kPitch * sizeof(T)));
+        const uint2 w = __builtin_bit_cast(uint2, x);
+        f.w[2 * half] = w.x;
+        f.w[2 * half + 1] = w.y;
       }
     }
     return f;
-  }
-  static __device__ __forceinline__ float value(const T* tile, int row, int d) {
-    return to_f32(tile[at(row, d / kUnit) + d % kUnit]);
   }
 };
 
@@ -496,6 +538,13 @@ __device__ __forceinline__ void dma16_from(uint32_t at, const void* p) {
                :
                : "v"(p), "s"(at)
                : "memory");
+}
+// dma16 from an address that is the same in all lanes, wherever the compiler keeps it
+__device__ __forceinline__ void dma16_at(uint32_t at, uint32_t voff, const void* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+  dma16(at, voff, reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo));
 }
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -531,6 +580,11 @@ __device__ __forceinline__ bool odd_values(const T* tile) {
     bits |= odd_bits<T>(w.x) | odd_bits<T>(w.y) | odd_bits<T>(w.z) | odd_bits<T>(w.w);
   }
   return is_odd<T>(bits);
+}
+
+// Whether any thread of the workgroup says so, as a scalar: what follows from it does too
+__device__ __forceinline__ bool any_of_block(bool v) {
+  return __builtin_amdgcn_readfirstlane(__syncthreads_or(v)) != 0;
 }
 
 // This thread's 256th of a tile, with zeros for what is not finite

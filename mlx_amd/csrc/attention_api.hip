@@ -12,25 +12,43 @@ namespace {
 constexpr int kMostKeys = 1 << 30; // positions and their differences stay in 32 bits
 constexpr int kMostSplits = 64;
 
-bool few(const AttentionArgs& a) {
-  return static_cast<int64_t>(a.G) * a.Lq <= kFewRows;
+// Whether the kernel for few rows takes a call, else the one of 128-row tiles.  us, few / tiles, each
+// with its best number of runs, 4096 keys: 8 sequences of 32 rows of 128 39.2 / 31.4, of 64 columns
+// 22.0 / 24.5; 4 of 16 rows of 256 17.6 / 20.1, of 32 rows 24.1 / 20.4; in float32 8 of 32 rows of
+// 128 85 / 176, 4 of 32 rows of 256 44 / 38.
+bool few(const AttentionArgs& a, int dtype) {
+  const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
+  const int wide = dtype == MLXROCM_FLOAT32 ? 128 : 64; // columns of which 32 rows are few
+  return rows <= (a.D <= wide ? 32 : 16);
 }
 
 int64_t heads_of(const AttentionArgs& a) {
   return static_cast<int64_t>(a.B) * a.Hkv;
 }
 
-// Runs that the keys of a row are cut into: as many as give the chip work, with some tiles left
-// to each.
+// Runs that the keys of a row are cut into.  Few rows, by runs, us (16-bit, 8 or 64 key heads of
+// 128, 256 workgroups marked): one sequence of 515 tokens 4 9.3, 8 8.4, 16 8.7; of 2048 8 10.1,
+// 16 9.1, 32* 9.7; of 8192 16 15.1, 32* 12.9, 64 14.4; 8 of 1024 2 14.2, 4* 11.5, 8 11.8; 8 of 20011
+// under a window of 4096 4* 23.4, 8 21.8, 16 26.7; 32 of 8192 1* 190, 2 187, 4 188.  Tiles: 64 rows over
+// 4096 8 22.6, 16 17.4, 32* 17.5, 64 22.9; 8 times 64 rows over 500 2 17.3, 4* 16.7, 8 22.2; 512 rows
+// over 32768 2* 480, 4 306, 8 317.
 int splits_of(const AttentionArgs& a, int dtype) {
   const int64_t span =
       std::min<int64_t>(a.keys, static_cast<int64_t>(a.window) + a.keep + a.Lq);
+  const int64_t heads = heads_of(a);
   int64_t splits;
-  if (few(a)) {
-    splits = std::min<int64_t>((1024 + heads_of(a) - 1) / heads_of(a), span / 256);
+  if (few(a, dtype)) {
+    const int64_t once = (256 + heads - 1) / heads; // a workgroup for each CU
+    splits = std::min<int64_t>(
+        std::max<int64_t>(once, std::min<int64_t>(2 * once, span / 512)), span / 72);
   } else {
-    const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads_of(a);
-    splits = std::min<int64_t>(512 / blocks, span / (dtype == MLXROCM_FLOAT32 ? 64 : 512));
+    const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads;
+    // (float32's matrix instruction takes 16 times as long: fewer keys are a run's worth)
+    splits = std::min<int64_t>(
+        512 / blocks,
+        dtype == MLXROCM_FLOAT32
+            ? span / 64
+            : std::max<int64_t>(span / 256, std::min<int64_t>(span / 128, 256 / blocks)));
   }
   return static_cast<int>(std::min<int64_t>(std::max<int64_t>(splits, 1), kMostSplits));
 }
@@ -64,18 +82,20 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
     return static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>({wanted, length / least, int64_t{kMostSplits}})));
   };
-  p.dq_splits = row_blocks > 0 ? parts(row_blocks, span) : 1;
+  p.dq_splits = Divisor(row_blocks > 0 ? parts(row_blocks, span) : 1);
   const int64_t seen_by = std::min<int64_t>(a.Lq, reach) * a.G;
   if (a.window < a.keys && seen_by < rows) {
     p.wide_blocks = static_cast<int>(std::min<int64_t>(
         p.blocks, (static_cast<int64_t>(a.keep) + kGradBlock - 1) / kGradBlock));
   }
-  p.splits = p.blocks > 0 ? parts(p.blocks, seen_by) : 1;
+  const int splits = p.blocks > 0 ? parts(p.blocks, seen_by) : 1;
+  p.splits = Divisor(splits);
   // runs no longer than the others'
-  p.wide_splits = p.wide_blocks == 0
-      ? p.splits
-      : static_cast<int>(std::min<int64_t>(
-            kMostSplits, std::max<int64_t>(1, rows * p.splits / std::max<int64_t>(seen_by, 1))));
+  p.wide_splits = Divisor(
+      p.wide_blocks == 0 ? splits
+                         : std::min<int64_t>(
+                               kMostSplits,
+                               std::max<int64_t>(1, rows * splits / std::max<int64_t>(seen_by, 1))));
   return p;
 }
 
@@ -86,7 +106,7 @@ struct GradWorkspace {
     const size_t rows = static_cast<size_t>(a.B) * a.Hq * a.Lq;
     part_dq = round256(rows * sizeof(float));
     part_dkv = part_dq +
-        (p.dq_splits > 1 ? round256(rows * a.D * p.dq_splits * sizeof(float)) : 0);
+        (p.dq_splits.d > 1 ? round256(rows * a.D * p.dq_splits.d * sizeof(float)) : 0);
     total = part_dkv +
         (p.dkv_split() ? static_cast<size_t>(heads_of(a)) * p.pieces() * kGradBlock * 2 * a.D *
                  sizeof(float)
@@ -120,7 +140,7 @@ int check_shape(const char* name, const AttentionArgs& a, int dtype) {
   // what indexes the launch and the rows in 32 bits
   const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
   if (a.keys > kMostKeys || rows > kMostKeys ||
-      ((rows + 15) / 16 * kMostSplits + a.keys / 128 + 1) * a.B * a.Hkv > INT32_MAX) {
+      ((rows + 15) / 16 * kMostSplits + a.keys / 128 + 1) * a.B * a.Hkv > INT32_MAX / 8) {
     return fail(MLXROCM_UNSUPPORTED, "[%s] the problem exceeds the grid", name);
   }
   return MLXROCM_OK;
@@ -181,6 +201,8 @@ AttentionArgs shape_of(
   a.Lq = Lq;
   a.keys = keys;
   a.D = D;
+  a.of_G = Divisor(a.G);
+  a.of_Hkv = Divisor(Hkv);
   a.window = std::min(window, kMostKeys);
   a.keep = std::min(keep, kMostKeys);
   return a;
@@ -193,6 +215,7 @@ bool empty(const AttentionArgs& a) {
 int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t bytes,
         hipStream_t s) {
   a.splits = splits_of(a, dtype);
+  a.of_splits = Divisor(a.splits);
   set_near(a, dtype);
   if (a.splits > 1 && !rehearsing()) {
     const size_t need = workspace_of(a, dtype);
@@ -208,7 +231,7 @@ int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t b
     a.part_ml = reinterpret_cast<float2*>(
         static_cast<char*>(workspace) + round256(rows * a.D * sizeof(float)));
   }
-  if (few(a)) {
+  if (few(a, dtype)) {
     TRY(dtype == MLXROCM_FLOAT32       ? launch_attention_few_f32(a, s)
             : dtype == MLXROCM_FLOAT16 ? launch_attention_few_f16(a, s)
                                        : launch_attention_few_bf16(a, s));
@@ -224,7 +247,7 @@ int run_grad(const AttentionGradArgs& g, int dtype, hipStream_t s) {
   TRY(dtype == MLXROCM_FLOAT32       ? launch_attention_grad_f32(g, s)
           : dtype == MLXROCM_FLOAT16 ? launch_attention_grad_f16(g, s)
                                      : launch_attention_grad_bf16(g, s));
-  return g.plan.dq_splits > 1 || g.plan.dkv_split() ? launch_attention_grad_join(g, dtype, s)
+  return g.plan.dq_splits.d > 1 || g.plan.dkv_split() ? launch_attention_grad_join(g, dtype, s)
                                                     : static_cast<int>(MLXROCM_OK);
 }
 
@@ -392,7 +415,7 @@ extern "C" int mlxrocm_window_attention_vjp(
   }
   set_scale(a, scale, dtype);
   set_near(a, dtype);
-  if ((a.G & (a.G - 1)) == 0 && near(a.q_strides, dtype, a.G) &&
+  if ((a.G & (a.G - 1)) == 0 && a.G <= 32 && near(a.q_strides, dtype, a.G) &&
       near(g.dout_strides, dtype, a.G)) {
     a.near |= 2;
     a.g_log2 = __builtin_ctz(a.G);
@@ -461,8 +484,7 @@ extern "C" int mlxrocm_paged_attention(
   a.out = out;
   a.lengths = lengths;
   a.table = table;
-  a.page = page_size;
-  a.page_magic = static_cast<uint32_t>((uint64_t{1} << 32) / page_size + 1);
+  a.page = Divisor(page_size);
   a.pages = pages;
   take(a.q_strides, strides);
   take(a.k_strides, strides + 3);

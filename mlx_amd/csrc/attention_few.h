@@ -1,4 +1,4 @@
-// attention_few.h -- attention of up to 64 rows (a token, or a few, for all heads that
+// attention_few.h -- attention of up to 32 rows (a token, or a few, for all heads that
 // share a key head): bound by reading the keys and values once.
 //
 // The keys of a (sequence, key head) are cut into `splits` runs of tiles of 32, a workgroup
@@ -142,7 +142,7 @@ __device__ __forceinline__ float sum_quarters(float v) {
 template <typename T, int DT, int NT, bool PAGED>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(DT * NT * sizeof(T) <= 256 ? 2 : 1)))
-void attention_few_kernel(const AttentionArgs a) {
+void attention_few_kernel(const AttentionArgs a, const Grid grid) {
   using S = FewShape<T, DT>;
   constexpr int KT = kFewKeys;
   __shared__ struct { // the waves' results of 16 rows, while they are joined
@@ -154,9 +154,9 @@ void attention_few_kernel(const AttentionArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4;
   int head, split;
-  piece_of(a.B * a.Hkv, a.splits, &head, &split);
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
+  grid.find(&head, &split);
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
   const int R = a.G * a.Lq;
   const int length = length_of(a, b);
   const int first_row = max(0, a.Lq - length) * a.G;
@@ -166,11 +166,10 @@ void attention_few_kernel(const AttentionArgs a) {
   int t0 = 0, t1 = 0;
   if (any) {
     range = keys_of(a, length, first_row, R - 1, KT);
-    t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / a.splits);
-    t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / a.splits);
+    run_of(range.tiles, split, a.of_splits, &t0, &t1);
   }
   const int p0 = length - a.Lq;
-  const int p_lo = p0 + first_row / a.G;
+  const int p_lo = p0 + a.of_G.divide(first_row);
   const int p_hi = p0 + a.Lq - 1;
 
   Frag<T> q[NT][DT / 32];
@@ -178,8 +177,8 @@ void attention_few_kernel(const AttentionArgs a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = min(max(16 * n + (lane & 15), first_row), R - 1);
-    p[n] = p0 + row / a.G;
-    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.G, row);
+    p[n] = p0 + a.of_G.divide(row);
+    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, row);
 #pragma unroll
     for (int c = 0; c < DT / 32; ++c) {
       const int d = 32 * c + 8 * g;
@@ -342,7 +341,7 @@ void attention_few_kernel(const AttentionArgs a) {
       const bool seeing = any && row >= first_row;
       const float over = total == 0.0f ? 0.0f : 1.0f / total;
       const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R + row;
-      T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row);
+      T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row);
       for (int d = 4 * (threadIdx.x & 15); d < a.D; d += 64) {
         floatx4 sum4 = {};
 #pragma unroll
@@ -361,14 +360,14 @@ void attention_few_kernel(const AttentionArgs a) {
         if (a.splits > 1) {
           a.part_ml[part] = make_float2(top, seeing ? total : 0.0f);
         } else if (a.lse != nullptr) {
-          const int i = row / a.G;
+          const int i = a.of_G.divide(row);
           a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
               seeing ? top + log2f(total) : 0.0f;
         }
       }
     }
   }
-  if (a.Lq > 1 && __syncthreads_or(odd)) {
+  if (a.Lq > 1 && any_of_block(odd)) {
     after_stores();
     const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
     const int d = threadIdx.x;
@@ -377,13 +376,13 @@ void attention_few_kernel(const AttentionArgs a) {
       for (int j = max(at.begin, at.low); j < at.end; ++j) {
         const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
         for (int r = first_row; not_finite(x) && r < R; ++r) {
-          if (!sees_key(a, p0 + r / a.G, j)) {
+          if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
             continue;
           }
           if (a.splits > 1) {
             add_to(a.part_out + (part + r) * a.D + d, x);
           } else {
-            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, r) + d, x);
+            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d, x);
           }
         }
       }
@@ -394,11 +393,11 @@ void attention_few_kernel(const AttentionArgs a) {
 template <typename T, int DT, int NT>
 int launch_few_rows(const AttentionArgs& a, hipStream_t s) {
   MLXROCM_REHEARSE("attention_few(dim=%d,rows=%d,splits=%d)", DT, 16 * NT, a.splits);
-  const dim3 grid(static_cast<unsigned>(a.B * a.Hkv * a.splits));
+  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, a.splits);
   if (a.table != nullptr) {
-    attention_few_kernel<T, DT, NT, true><<<grid, 256, 0, s>>>(a);
+    attention_few_kernel<T, DT, NT, true><<<grid.blocks(), 256, 0, s>>>(a, grid);
   } else {
-    attention_few_kernel<T, DT, NT, false><<<grid, 256, 0, s>>>(a);
+    attention_few_kernel<T, DT, NT, false><<<grid.blocks(), 256, 0, s>>>(a, grid);
   }
   MLXROCM_HIP_TRY(hipGetLastError());
   return static_cast<int>(MLXROCM_OK);
@@ -406,10 +405,12 @@ int launch_few_rows(const AttentionArgs& a, hipStream_t s) {
 
 template <typename T, int DT>
 int launch_few_of(const AttentionArgs& a, hipStream_t s) {
-  const int rows = a.G * a.Lq;
-  return rows <= 16 ? launch_few_rows<T, DT, 1>(a, s)
-      : rows <= 32  ? launch_few_rows<T, DT, 2>(a, s)
-                    : launch_few_rows<T, DT, 4>(a, s);
+  if constexpr (DT <= 64 || (sizeof(T) == 4 && DT <= 128)) {
+    if (a.G * a.Lq > 16) {
+      return launch_few_rows<T, DT, 2>(a, s);
+    }
+  }
+  return launch_few_rows<T, DT, 1>(a, s);
 }
 
 template <typename T>

@@ -39,24 +39,23 @@ __device__ __forceinline__ void store_part(
 template <typename T, int DT>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(DT * sizeof(T) <= 256 ? 2 : 1, DT * sizeof(T) <= 256 ? 2 : 1)))
-void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
+void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
   constexpr int kBoth = 2 * S::kTile;
-  __shared__ __align__(16) T lds[2 * kBoth];
+  __shared__ __align__(1024) T lds[2 * kBoth];
   const AttentionArgs& a = ga.a;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5;
-  const int splits = ga.plan.dq_splits;
-  int head, piece;
-  piece_of(a.B * a.Hkv, blocks * splits, &head, &piece);
-  const int block = blocks - 1 - piece / splits;
-  const int split = piece % splits;
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
+  const Divisor& splits = ga.plan.dq_splits;
+  int head, piece, split;
+  grid.find(&head, &piece);
+  const int block = blocks - 1 - splits.divide(piece, &split);
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
   const int R = a.G * a.Lq;
   const int length = length_of(a, b);
   const int first_row = max(0, a.Lq - length) * a.G;
@@ -69,26 +68,26 @@ void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
 
   const bool any = lo <= hi && length > 0;
   const KeyRange range = any ? keys_of(a, length, lo, hi, KT) : KeyRange{};
-  const int t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / splits);
+  int t0, t1;
+  run_of(range.tiles, split, splits, &t0, &t1);
   const int w_lo = max(r0, first_row);
   const int w_hi = min(r0 + 31, R - 1);
   const bool works = w_lo <= w_hi && length > 0;
   const int p0 = length - a.Lq;
-  const int b_lo = p0 + lo / a.G; // the workgroup's, and the wave's
-  const int b_hi = p0 + hi / a.G;
-  const int p_lo = p0 + w_lo / a.G;
-  const int p_hi = p0 + w_hi / a.G;
+  const int b_lo = p0 + a.of_G.divide(lo); // the workgroup's, and the wave's
+  const int b_hi = p0 + a.of_G.divide(hi);
+  const int p_lo = p0 + a.of_G.divide(w_lo);
+  const int p_hi = p0 + a.of_G.divide(w_hi);
   const int from = min(max(row, lo), hi);
-  const int i_from = from / a.G;
+  const int i_from = a.of_G.divide(from);
   const int p = p0 + i_from;
 
   Frag<T> q[DT / 16], dout[DT / 16];
   float lse = 0.0f, delta = 0.0f;
   if (any) {
-    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.G, from);
-    const T* dsrc = static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.G, from);
-    const T* osrc = static_cast<const T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, from);
+    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, from);
+    const T* dsrc = static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.of_G, from);
+    const T* osrc = static_cast<const T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, from);
 #pragma unroll
     for (int c = 0; c < DT / 16; ++c) {
       const int d = 16 * c + 8 * h;
@@ -137,7 +136,7 @@ void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
     // The scores need the keys as they are: those without what is not finite lie where the
     // next tile will, which is fetched after them.
     const bool apart = !whole_tile(a, tile, KT, b_lo, b_hi) &&
-        __syncthreads_or(odd_values<T, S::kTile>(k_tile));
+        any_of_block(odd_values<T, S::kTile>(k_tile));
     if (apart) {
       odd = true;
       copy_finite<T, S::kTile>(k_tile, next);
@@ -185,10 +184,10 @@ void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
     }
   }
   const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
-  if (stored && splits > 1) {
+  if (stored && splits.d > 1) {
     store_part<DT>(ga.part_dq + (part + row) * a.D, dq, seeing, a.D, h);
   } else if (stored) {
-    T* to = static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.G, row);
+    T* to = static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.of_G, row);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
@@ -211,13 +210,13 @@ void attention_dq_kernel(const AttentionGradArgs ga, int blocks) {
       for (int j = max(tile.begin, tile.low); j < tile.end; ++j) {
         const float x = to_f32(static_cast<const T*>(a.k)[key_row<false>(a, b, hk, j).k + d]);
         for (int r = lo; not_finite(x) && r <= hi; ++r) {
-          if (!sees_key(a, p0 + r / a.G, j)) {
+          if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
             continue;
           }
-          if (splits > 1) {
+          if (splits.d > 1) {
             add_to(ga.part_dq + (part + r) * a.D + d, x);
           } else {
-            add_to(static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.G, r) + d, x);
+            add_to(static_cast<T*>(ga.dq) + row_offset(ga.dq_strides, b, hk, a.of_G, r) + d, x);
           }
         }
       }
@@ -244,51 +243,76 @@ struct StatsTile {
 template <typename T, int DT, int ROWS>
 struct RowStream {
   using L = Tile<T, DT>;
+  static constexpr int kPasses = ROWS / L::kRowsOfPass;
   const AttentionGradArgs& ga;
   int b, hk, end, wave;
-  int d;
-  uint32_t q_off, d_off;
+  int d[L::kTurns];
+  uint32_t q_off[L::kTurns], d_off[L::kTurns];
+  bool near;
+  const T *q, *dout;                       // the first row of the next tile
+  int64_t q_pass[kPasses], d_pass[kPasses]; // from there, of each load
 
   __device__ __forceinline__ RowStream(
-      const AttentionGradArgs& args, int b_, int hk_, int end_, int wave_, int lane)
-      : ga(args), b(b_), hk(hk_), end(end_), wave(wave_) {
-    const int row = lane / L::kPlaces;
-    const int i = row / ga.a.G;
-    const int g = row - i * ga.a.G;
-    d = ((lane % L::kPlaces) ^ L::swizzle(wave * L::kRowsOfLoad + row)) * L::kUnit;
-    q_off = static_cast<uint32_t>(
-        (g * ga.a.q_strides[1] + i * ga.a.q_strides[2] + d) * sizeof(T));
-    d_off = static_cast<uint32_t>(
-        (g * ga.dout_strides[1] + i * ga.dout_strides[2] + d) * sizeof(T));
-  }
-  // Rows from `begin` on (a multiple of G); rows past the end repeat the last one
-  __device__ __forceinline__ void fetch(int begin, T* q_tile, T* d_tile) const {
+      const AttentionGradArgs& args, int b_, int hk_, int begin, int end_, int wave_, int lane)
+      : ga(args), b(b_), hk(hk_), end(end_), wave(wave_), near((args.a.near & 2) != 0) {
     const AttentionArgs& a = ga.a;
-    const T* q = static_cast<const T*>(a.q);
-    const T* dout = static_cast<const T*>(ga.dout);
-    const bool inside = begin + ROWS <= end && (a.near & 2) != 0;
+    const int row = lane / L::kPlaces;
+    const int i = row >> a.g_log2;
+    const int g = row & (a.G - 1);
 #pragma unroll
-    for (int n = 0; n < ROWS / L::kRowsOfPass; ++n) {
-      const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
-      const uint32_t to = row * L::kPitch * sizeof(T);
-      if (inside) {
-        const int i = (begin + row) >> a.g_log2;
-        const int head = hk * a.G + ((begin + row) & (a.G - 1));
-        const T* qp = q + b * a.q_strides[0] + head * a.q_strides[1] + i * a.q_strides[2];
-        const T* dp =
-            dout + b * ga.dout_strides[0] + head * ga.dout_strides[1] + i * ga.dout_strides[2];
-        if (d < a.D) {
-          dma16(lds_address(q_tile) + to, q_off, qp);
-          dma16(lds_address(d_tile) + to, d_off, dp);
+    for (int x = 0; x < L::kTurns; ++x) {
+      d[x] = ((lane % L::kPlaces) ^
+              L::swizzle(x * L::kRowsOfPass + wave * L::kRowsOfLoad + row)) *
+          L::kUnit;
+      q_off[x] = static_cast<uint32_t>(
+          (g * a.q_strides[1] + i * a.q_strides[2] + d[x]) * sizeof(T));
+      d_off[x] = static_cast<uint32_t>(
+          (g * ga.dout_strides[1] + i * ga.dout_strides[2] + d[x]) * sizeof(T));
+    }
+    q = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, begin);
+    dout = static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.of_G, begin);
+#pragma unroll
+    for (int n = 0; n < kPasses; ++n) {
+      const int first = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+      const int fi = first >> a.g_log2;
+      const int fg = first & (a.G - 1);
+      q_pass[n] = fg * a.q_strides[1] + fi * a.q_strides[2];
+      d_pass[n] = fg * ga.dout_strides[1] + fi * ga.dout_strides[2];
+    }
+  }
+  // Rows from `begin` on, one tile after the other; rows past the end repeat the last one
+  __device__ __forceinline__ void fetch(int begin, T* q_tile, T* d_tile) {
+    const AttentionArgs& a = ga.a;
+    const bool inside = near && begin + ROWS <= end;
+    if (inside) {
+#pragma unroll
+      for (int n = 0; n < kPasses; ++n) {
+        const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+        const uint32_t to = row * L::kPitch * sizeof(T);
+        if (d[n % L::kTurns] < a.D) {
+          dma16_at(lds_address(q_tile) + to, q_off[n % L::kTurns], q + q_pass[n]);
+          dma16_at(lds_address(d_tile) + to, d_off[n % L::kTurns], dout + d_pass[n]);
         }
-      } else {
+      }
+      // (a tile is whole tokens: a power of two of heads up to its rows share a key head)
+      q += (ROWS >> a.g_log2) * a.q_strides[2];
+      dout += (ROWS >> a.g_log2) * ga.dout_strides[2];
+    } else {
+#pragma unroll
+      for (int n = 0; n < kPasses; ++n) {
+        const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
+        const uint32_t to = row * L::kPitch * sizeof(T);
         const int r =
             min(begin + row + static_cast<int>(threadIdx.x & 63) / L::kPlaces, end - 1);
-        if (d < a.D) {
+        if (d[n % L::kTurns] < a.D) {
           dma16_from(
-              lds_address(q_tile) + to, q + row_offset(a.q_strides, b, hk, a.G, r) + d);
+              lds_address(q_tile) + to,
+              static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, r) +
+                  d[n % L::kTurns]);
           dma16_from(
-              lds_address(d_tile) + to, dout + row_offset(ga.dout_strides, b, hk, a.G, r) + d);
+              lds_address(d_tile) + to,
+              static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.of_G, r) +
+                  d[n % L::kTurns]);
         }
       }
     }
@@ -312,7 +336,7 @@ struct DkvShape {
 template <typename T, int DT>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(DkvShape<T, DT>::kTwo ? 2 : 1, DkvShape<T, DT>::kTwo ? 2 : 1)))
-void attention_dkv_kernel(const AttentionGradArgs ga) {
+void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
   using S = DkvShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int RT = S::kRows;
@@ -321,8 +345,8 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
   // each tile (with both results they would need all 512 registers)
   constexpr bool kKeyHeld = DT * sizeof(T) <= 512;
   constexpr bool kValueHeld = kKeyHeld && !S::kValuesInLds;
-  __shared__ __align__(16) T lds[2 * kBoth];
-  __shared__ __align__(16) T values[S::kValuesInLds ? kKeysBlock * L::kPitch : 16];
+  __shared__ __align__(1024) T lds[2 * kBoth];
+  __shared__ __align__(1024) T values[S::kValuesInLds ? kKeysBlock * L::kPitch : 16];
   __shared__ __align__(16) StatsTile<RT> stats[2];
   const AttentionArgs& a = ga.a;
 
@@ -331,14 +355,15 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
   const int h = lane >> 5;
   const GradPlan& plan = ga.plan;
   int head, piece;
-  piece_of(a.B * a.Hkv, plan.pieces(), &head, &piece);
+  grid.find(&head, &piece);
   // the first keys are seen by most rows: they come first
-  const int wide = plan.wide_blocks * plan.wide_splits;
-  const int splits = piece < wide ? plan.wide_splits : plan.splits;
-  const int block = piece < wide ? piece / splits : plan.wide_blocks + (piece - wide) / splits;
-  const int split = (piece < wide ? piece : piece - wide) % splits;
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
+  const int wide = plan.wide_blocks * plan.wide_splits.d;
+  const Divisor& splits = piece < wide ? plan.wide_splits : plan.splits;
+  int split;
+  const int block = piece < wide ? splits.divide(piece, &split)
+                                 : plan.wide_blocks + splits.divide(piece - wide, &split);
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
   const int length = length_of(a, b);
   const int k0 = block * kKeysBlock;
   const int k1 = min(k0 + kKeysBlock, length); // keys of this workgroup that are seen
@@ -347,8 +372,8 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
   const int i0 = max(max(0, -p0), k0 - p0);
   const int i1 = k0 < a.keep ? a.Lq : min(a.Lq, k1 - 1 + a.window - p0);
   const int all = k0 < k1 && i0 < i1 ? ((i1 - i0) * a.G + RT - 1) / RT : 0; // tiles of rows
-  const int s0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
-  const int s1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits);
+  int s0, s1;
+  run_of(all, split, splits, &s0, &s1);
   const int tiles = s1 - s0; // of this run
   const bool any = tiles > 0;
   const int begin_row = i0 * a.G + s0 * RT;
@@ -407,12 +432,12 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
   }
   const auto stats_of = [&](int t) {
     const int r = min(begin_row + t * RT + static_cast<int>(threadIdx.x), end_row - 1);
-    const int i = r / a.G;
+    const int i = a.of_G.divide(r);
     const int64_t n = (static_cast<int64_t>(b) * a.Hq + hk * a.G + r - i * a.G) * a.Lq + i;
     return RowStats{a.lse[n], ga.delta[n], p0 + i};
   };
 
-  const RowStream<T, DT, RT> rows(ga, b, hk, end_row, wave, lane);
+  RowStream<T, DT, RT> rows(ga, b, hk, begin_row, end_row, wave, lane);
   floatx16 dk[DT / 32], dv[DT / 32];
 #pragma unroll
   for (int d = 0; d < DT / 32; ++d) {
@@ -449,7 +474,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
     // (as in attention_dq_kernel)
     const bool apart =
         !(count == RT && all_seen(k0, k1, p_lo, p_hi, a.window, a.keep)) &&
-        __syncthreads_or(odd_values<T, 2 * S::kTile>(q_tile));
+        any_of_block(odd_values<T, 2 * S::kTile>(q_tile));
     if (apart) {
       odd = true;
       copy_finite<T, 2 * S::kTile>(q_tile, next);
@@ -639,11 +664,11 @@ void attention_dkv_kernel(const AttentionGradArgs ga) {
     const int d = threadIdx.x;
     for (int r = begin_row; r < end_row && d < a.D; ++r) {
       const float x = to_f32(
-          static_cast<const T*>(a.q)[row_offset(a.q_strides, b, hk, a.G, r) + d]);
+          static_cast<const T*>(a.q)[row_offset(a.q_strides, b, hk, a.of_G, r) + d]);
       const float y = to_f32(
-          static_cast<const T*>(ga.dout)[row_offset(ga.dout_strides, b, hk, a.G, r) + d]);
+          static_cast<const T*>(ga.dout)[row_offset(ga.dout_strides, b, hk, a.of_G, r) + d]);
       for (int j = k0; (not_finite(x) || not_finite(y)) && j < k1; ++j) {
-        if (!sees_key(a, p0 + r / a.G, j)) {
+        if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
           continue;
         }
         if (parts) {
@@ -673,16 +698,18 @@ int launch_grad_of(const AttentionGradArgs& g, hipStream_t s) {
   const AttentionArgs& a = g.a;
   MLXROCM_REHEARSE(
       "attention_dq(dim=%d,splits=%d)+attention_dkv(dim=%d,splits=%d,kept=%dx%d)", DT,
-      g.plan.dq_splits, DT, g.plan.splits, g.plan.wide_blocks, g.plan.wide_splits);
+      g.plan.dq_splits.d, DT, g.plan.splits.d, g.plan.wide_blocks, g.plan.wide_splits.d);
   const int rows = static_cast<int>(
       (static_cast<int64_t>(a.G) * a.Lq + kRowsBlock - 1) / kRowsBlock);
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
   if (rows > 0) {
-    attention_dq_kernel<T, DT>
-        <<<rows * g.plan.dq_splits * a.B * a.Hkv, 256, 0, s>>>(g, rows);
+    const Grid grid(heads, static_cast<int64_t>(rows) * g.plan.dq_splits.d);
+    attention_dq_kernel<T, DT><<<grid.blocks(), 256, 0, s>>>(g, grid, rows);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
   if (g.plan.blocks > 0) {
-    attention_dkv_kernel<T, DT><<<g.plan.pieces() * a.B * a.Hkv, 256, 0, s>>>(g);
+    const Grid grid(heads, g.plan.pieces());
+    attention_dkv_kernel<T, DT><<<grid.blocks(), 256, 0, s>>>(g, grid);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
   return static_cast<int>(MLXROCM_OK);

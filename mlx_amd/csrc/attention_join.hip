@@ -71,13 +71,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   }
   const int head = static_cast<int>(n / R);
   const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
-  const int i = row / a.G;
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
+  const int i = a.of_G.divide(row);
   const bool seeing = length_of(a, b) - a.Lq + i >= 0;
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
   if (lane < WIDTH && d < a.D) {
-    T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row) + d;
+    T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row) + d;
     store4<T>(out, seeing ? sum * over : floatx4{});
   }
   if (a.lse != nullptr && lane == 0) {
@@ -121,12 +121,12 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Attention
   }
   const int head = static_cast<int>(n / R);
   const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
-  const int i = row / a.G;
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
+  const int i = a.of_G.divide(row);
   const bool seeing = length_of(a, b) - a.Lq + i >= 0;
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
-  T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row) + d;
+  T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row) + d;
   store4<T>(out, seeing ? sum * over : floatx4{});
   if (a.lse != nullptr && d == 0) {
     a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
@@ -148,14 +148,14 @@ __global__ __launch_bounds__(256) void attention_sum_dq_kernel(const AttentionGr
   }
   floatx4 sum = {};
 #pragma unroll 4
-  for (int s = 0; s < g.plan.dq_splits; ++s) {
+  for (int s = 0; s < g.plan.dq_splits.d; ++s) {
     const float4 v = *reinterpret_cast<const float4*>(g.part_dq + (s * rows + n) * a.D + d);
     sum += floatx4{v.x, v.y, v.z, v.w};
   }
   const int head = static_cast<int>(n / R);
   const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
   const int b = head / a.Hkv;
-  T* to = static_cast<T*>(g.dq) + row_offset(g.dq_strides, b, head - b * a.Hkv, a.G, row) + d;
+  T* to = static_cast<T*>(g.dq) + row_offset(g.dq_strides, b, head - b * a.Hkv, a.of_G, row) + d;
   store4<T>(to, sum * g.scale);
 }
 
@@ -174,9 +174,9 @@ __global__ __launch_bounds__(256) void attention_sum_dkv_kernel(const AttentionG
   const int key = static_cast<int>(n - static_cast<int64_t>(head) * a.keys);
   const int block = key / kGradBlock;
   const bool wide = block < plan.wide_blocks;
-  const int splits = wide ? plan.wide_splits : plan.splits;
-  const int piece = wide ? block * plan.wide_splits
-                         : plan.wide_blocks * plan.wide_splits + (block - plan.wide_blocks) * splits;
+  const int splits = wide ? plan.wide_splits.d : plan.splits.d;
+  const int piece = wide ? block * splits
+                         : plan.wide_blocks * plan.wide_splits.d + (block - plan.wide_blocks) * splits;
   const float* part = g.part_dkv +
       (static_cast<int64_t>(head) * plan.pieces() + piece) * (kGradBlock * 2 * a.D) +
       (key - block * kGradBlock) * 2 * a.D + c;
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256) void attention_sum_dkv_kernel(const AttentionG
         part + static_cast<int64_t>(s) * (kGradBlock * 2 * a.D));
     sum += floatx4{v.x, v.y, v.z, v.w};
   }
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
   const bool of_k = c < a.D;
   const int64_t* strides = of_k ? g.dk_strides : g.dv_strides;
   T* to = static_cast<T*>(of_k ? g.dk : g.dv) + b * strides[0] + hk * strides[1] +
@@ -203,7 +203,7 @@ int launch_attention_grad_join(const AttentionGradArgs& g, int dtype, hipStream_
   MLXROCM_REHEARSE("attention_sum");
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (g.plan.dq_splits > 1) {
+    if (g.plan.dq_splits.d > 1) {
       const int64_t n = static_cast<int64_t>(a.B) * a.Hq * a.Lq * (a.D / 4);
       attention_sum_dq_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g);
       MLXROCM_HIP_TRY(hipGetLastError());

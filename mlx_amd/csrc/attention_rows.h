@@ -47,56 +47,76 @@ struct KeyStream {
   using L = Tile<T, DT>;
   const AttentionArgs& a;
   int b, hk, length, wave;
-  int d;                 // this lane's column
-  uint32_t k_off, v_off; // bytes from the first row of a load
-  int ids = 0;           // PAGED: lane i has the page of keys 16 i .. 16 i + 15 of a tile
+  int d[L::kTurns];                            // this lane's column
+  uint32_t k_off[L::kTurns], v_off[L::kTurns]; // bytes from the first row of a load
+  const T *k, *v;                              // of the head; contiguous: of the sequence's head
+  // PAGED: lane i has where the rows of keys 16 i .. 16 i + 15 of a tile begin, or their pages
+  int ids = 0;
+  int in_page = 0;
 
   __device__ __forceinline__ KeyStream(
       const AttentionArgs& args, int b_, int hk_, int length_, int wave_, int lane)
-      : a(args), b(b_), hk(hk_), length(length_), wave(wave_) {
+      : a(args),
+        b(b_),
+        hk(hk_),
+        length(length_),
+        wave(wave_),
+        k(static_cast<const T*>(args.k) + hk_ * args.k_strides[1] +
+          (PAGED ? 0 : b_ * args.k_strides[0])),
+        v(static_cast<const T*>(args.v) + hk_ * args.v_strides[1] +
+          (PAGED ? 0 : b_ * args.v_strides[0])) {
     const int row = lane / L::kPlaces;
-    d = ((lane % L::kPlaces) ^ L::swizzle(wave * L::kRowsOfLoad + row)) * L::kUnit;
-    k_off = static_cast<uint32_t>((row * a.k_strides[2] + d) * sizeof(T));
-    v_off = static_cast<uint32_t>((row * a.v_strides[2] + d) * sizeof(T));
+#pragma unroll
+    for (int x = 0; x < L::kTurns; ++x) {
+      d[x] = ((lane % L::kPlaces) ^
+              L::swizzle(x * L::kRowsOfPass + wave * L::kRowsOfLoad + row)) *
+          L::kUnit;
+      k_off[x] = static_cast<uint32_t>((row * a.k_strides[2] + d[x]) * sizeof(T));
+      v_off[x] = static_cast<uint32_t>((row * a.v_strides[2] + d[x]) * sizeof(T));
+    }
   }
   // The pages of the tile from `begin` on, before the loads of the one before it
   __device__ __forceinline__ void look_up(int begin) {
     if constexpr (PAGED) {
-      int in_page;
       const int lane = threadIdx.x & 63;
       const int j = min(begin + 16 * (lane & (S::kKeys / 16 - 1)), a.keys - 1);
-      ids = min(max(a.table[b * a.table_stride + page_of(a, j, &in_page)], 0), a.pages - 1);
+      ids = a.table[b * a.table_stride + a.page.divide(j, &in_page)];
     }
   }
   __device__ __forceinline__ void fetch(int begin, T* k_tile, T* v_tile) const {
-    const T* k = static_cast<const T*>(a.k) + hk * a.k_strides[1];
-    const T* v = static_cast<const T*>(a.v) + hk * a.v_strides[1];
     const bool inside = begin + S::kKeys <= length && (a.near & 1) != 0;
     if (inside) {
-      int at = begin + wave * L::kRowsOfLoad;
-      const T* kp = k;
-      const T* vp = v;
-      if constexpr (!PAGED) {
-        kp += b * a.k_strides[0] + at * a.k_strides[2];
-        vp += b * a.v_strides[0] + at * a.v_strides[2];
+      // (a multiplication for all lanes, where the scalar unit would take one for each load)
+      int64_t k_at, v_at;
+      if constexpr (PAGED) {
+        const int64_t id = min(max(ids, 0), a.pages - 1);
+        k_at = id * a.k_strides[0] + in_page * a.k_strides[2];
+        v_at = id * a.v_strides[0] + in_page * a.v_strides[2];
+      } else {
+        k_at = begin * a.k_strides[2];
+        v_at = begin * a.v_strides[2];
       }
+      const auto from = [](const T* p, int64_t at, int lane) {
+        if constexpr (PAGED) {
+          at = static_cast<int64_t>(
+              static_cast<uint64_t>(static_cast<uint32_t>(
+                  __builtin_amdgcn_readlane(static_cast<int>(at >> 32), lane)))
+                  << 32 |
+              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at), lane)));
+        }
+        return p + at;
+      };
 #pragma unroll
       for (int n = 0; n < S::kPasses; ++n) {
         const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
-        if constexpr (PAGED) {
-          const int64_t id = __builtin_amdgcn_readlane(ids, row / 16);
-          page_of(a, begin + row, &at);
-          kp = k + id * a.k_strides[0] + at * a.k_strides[2];
-          vp = v + id * a.v_strides[0] + at * a.v_strides[2];
-        }
+        // rows from the first of the tile, or of the 16 in one page
+        const int64_t rest = PAGED ? row % 16 : row;
+        const T* kp = from(k, k_at, row / 16) + rest * a.k_strides[2];
+        const T* vp = from(v, v_at, row / 16) + rest * a.v_strides[2];
         const uint32_t to = row * L::kPitch * sizeof(T);
-        if (d < a.D) {
-          dma16(lds_address(k_tile) + to, k_off, kp);
-          dma16(lds_address(v_tile) + to, v_off, vp);
-        }
-        if constexpr (!PAGED) {
-          kp += L::kRowsOfPass * a.k_strides[2];
-          vp += L::kRowsOfPass * a.v_strides[2];
+        if (d[n % L::kTurns] < a.D) {
+          dma16_at(lds_address(k_tile) + to, k_off[n % L::kTurns], kp);
+          dma16_at(lds_address(v_tile) + to, v_off[n % L::kTurns], vp);
         }
       }
     } else { // keys past the end repeat the last one
@@ -104,11 +124,11 @@ struct KeyStream {
       for (int n = 0; n < S::kPasses; ++n) {
         const int row = n * L::kRowsOfPass + wave * L::kRowsOfLoad;
         const int j = begin + row + static_cast<int>(threadIdx.x & 63) / L::kPlaces;
-        const KeyRow r = key_row<PAGED>(a, b, 0, min(j, length - 1));
+        const KeyRow r = key_row<PAGED>(a, PAGED ? b : 0, 0, min(j, length - 1));
         const uint32_t to = row * L::kPitch * sizeof(T);
-        if (d < a.D) {
-          dma16_from(lds_address(k_tile) + to, k + r.k + d);
-          dma16_from(lds_address(v_tile) + to, v + r.v + d);
+        if (d[n % L::kTurns] < a.D) {
+          dma16_from(lds_address(k_tile) + to, k + r.k + d[n % L::kTurns]);
+          dma16_from(lds_address(v_tile) + to, v + r.v + d[n % L::kTurns]);
         }
       }
     }
@@ -118,23 +138,23 @@ struct KeyStream {
 template <typename T, int DT, bool PAGED>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(DT * sizeof(T) <= 256 ? 2 : 1, DT * sizeof(T) <= 256 ? 2 : 1)))
-void attention_rows_kernel(const AttentionArgs a, int blocks) {
+void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
   using S = RowsShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int KT = S::kKeys;
   constexpr int kBoth = 2 * S::kTile; // K and V
-  __shared__ __align__(16) T lds[2 * kBoth];
+  __shared__ __align__(1024) T lds[2 * kBoth];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5;
   int head, piece;
-  piece_of(a.B * a.Hkv, blocks * a.splits, &head, &piece);
+  grid.find(&head, &piece);
   // the last rows see most keys: they come first
-  const int block = blocks - 1 - piece / a.splits;
-  const int split = piece % a.splits;
-  const int b = head / a.Hkv;
-  const int hk = head - b * a.Hkv;
+  int split;
+  const int block = blocks - 1 - a.of_splits.divide(piece, &split);
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
   const int R = a.G * a.Lq;
   const int length = length_of(a, b);
   const int first_row = max(0, a.Lq - length) * a.G; // rows before it see nothing
@@ -149,24 +169,23 @@ void attention_rows_kernel(const AttentionArgs a, int blocks) {
   KeyRange range = {};
   if (lo <= hi && length > 0) {
     range = keys_of(a, length, lo, hi, KT);
-    t0 = static_cast<int>(static_cast<int64_t>(range.tiles) * split / a.splits);
-    t1 = static_cast<int>(static_cast<int64_t>(range.tiles) * (split + 1) / a.splits);
+    run_of(range.tiles, split, a.of_splits, &t0, &t1);
   }
   // what this wave's own rows see
   const int w_lo = max(r0, first_row);
   const int w_hi = min(r0 + 31, R - 1);
   const bool works = w_lo <= w_hi && length > 0;
   const int p0 = length - a.Lq;
-  const int b_lo = p0 + lo / a.G; // the workgroup's, and the wave's
-  const int b_hi = p0 + hi / a.G;
-  const int p_lo = p0 + w_lo / a.G;
-  const int p_hi = p0 + w_hi / a.G;
+  const int b_lo = p0 + a.of_G.divide(lo); // the workgroup's, and the wave's
+  const int b_hi = p0 + a.of_G.divide(hi);
+  const int p_lo = p0 + a.of_G.divide(w_lo);
+  const int p_hi = p0 + a.of_G.divide(w_hi);
   const int from = min(max(row, lo), hi); // a row that sees something, in any lane
-  const int p = p0 + from / a.G;
+  const int p = p0 + a.of_G.divide(from);
 
   Frag<T> q[DT / 16];
   if (t0 < t1) {
-    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.G, from);
+    const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, from);
 #pragma unroll
     for (int c = 0; c < DT / 16; ++c) {
       const int d = 16 * c + 8 * h;
@@ -207,7 +226,7 @@ void attention_rows_kernel(const AttentionArgs a, int blocks) {
     }
     const int begin = tile.begin;
     if (!whole_tile(a, tile, KT, b_lo, b_hi) &&
-        __syncthreads_or(odd_values<T, S::kTile>(v_tile))) {
+        any_of_block(odd_values<T, S::kTile>(v_tile))) {
       odd = true;
       copy_finite<T, S::kTile>(v_tile, v_tile);
       __syncthreads();
@@ -308,7 +327,7 @@ void attention_rows_kernel(const AttentionArgs a, int blocks) {
     }
   } else if (stored) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l; // nothing but scores of -inf
-    T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, row);
+    T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
@@ -322,7 +341,7 @@ void attention_rows_kernel(const AttentionArgs a, int blocks) {
       }
     }
     if (a.lse != nullptr && h == 0) {
-      const int i = row / a.G;
+      const int i = a.of_G.divide(row);
       a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
           seeing ? m + log2f(l) : 0.0f;
     }
@@ -335,13 +354,13 @@ void attention_rows_kernel(const AttentionArgs a, int blocks) {
       for (int j = max(tile.begin, tile.low); j < tile.end; ++j) {
         const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
         for (int r = lo; not_finite(x) && r <= hi; ++r) {
-          if (!sees_key(a, p0 + r / a.G, j)) {
+          if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
             continue;
           }
           if (a.splits > 1) {
             add_to(a.part_out + (part + r) * a.D + d, x);
           } else {
-            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.G, r) + d, x);
+            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d, x);
           }
         }
       }
@@ -353,11 +372,13 @@ template <typename T, int DT>
 int launch_rows_of(const AttentionArgs& a, hipStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + kRowsBlock - 1) / kRowsBlock;
   MLXROCM_REHEARSE("attention_rows(dim=%d,splits=%d)", DT, a.splits);
-  const dim3 grid(static_cast<unsigned>(blocks * a.B * a.Hkv * a.splits));
+  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits);
   if (a.table != nullptr) {
-    attention_rows_kernel<T, DT, true><<<grid, 256, 0, s>>>(a, static_cast<int>(blocks));
+    attention_rows_kernel<T, DT, true>
+        <<<grid.blocks(), 256, 0, s>>>(a, grid, static_cast<int>(blocks));
   } else {
-    attention_rows_kernel<T, DT, false><<<grid, 256, 0, s>>>(a, static_cast<int>(blocks));
+    attention_rows_kernel<T, DT, false>
+        <<<grid.blocks(), 256, 0, s>>>(a, grid, static_cast<int>(blocks));
   }
   MLXROCM_HIP_TRY(hipGetLastError());
   return static_cast<int>(MLXROCM_OK);
