@@ -539,12 +539,18 @@ __device__ __forceinline__ void dma16_from(uint32_t at, const void* p) {
                : "v"(p), "s"(at)
                : "memory");
 }
-// dma16 from an address that is the same in all lanes, wherever the compiler keeps it
+// dma16 from an address that is the same in all lanes, wherever the compiler keeps it: if a vector
+// instruction writes the scalar registers right before, the load has to keep five wait states
+// behind it, which the compiler does not do for inline assembly.
 __device__ __forceinline__ void dma16_at(uint32_t at, uint32_t voff, const void* p) {
   const uint64_t u = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u)); // (an int)
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
-  dma16(at, voff, reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo));
+  const uint64_t base = static_cast<uint64_t>(hi) << 32 | lo;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(voff), "s"(base), "s"(at)
+               : "memory");
 }
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -321,16 +321,16 @@ struct RowStream {
 
 // Two waves a SIMD leave 256 registers.  Both results of 128 columns take 128 of them, and keys
 // and values 64: the values stay in LDS then (read again for each tile, a quarter more
-// than is read anyway), and a tile is 32 rows, so that two workgroups fit.  With all in registers
-// and one wave a SIMD the compiler moves results between its two files around each product: 8192
-// tokens, 32 heads of 128 2.13 ms, spilling at two waves 5.2 ms.
+// than is read anyway), and a tile is 32 rows, so that two workgroups fit, of whose sums and deltas
+// four are in registers at a time.  8192 tokens, 32 heads of 128, both gradients 2.06 ms; with two
+// fragments read ahead instead of four 2.08 ms; with all in registers and one wave a SIMD the compiler
+// moves results between its two files around each product.
 template <typename T, int DT>
 struct DkvShape {
   static constexpr bool kTwo = DT * sizeof(T) <= 256; // waves a SIMD
   static constexpr bool kValuesInLds = sizeof(T) == 2 && (DT == 96 || DT == 128);
   static constexpr int kRows = kValuesInLds ? 32 : RowsShape<T, DT>::kKeys; // of a tile
   static constexpr int kTile = kRows * Tile<T, DT>::kPitch;
-  static constexpr int kAhead = DT == 128 && kValuesInLds ? 2 : 4; // (one more register is too many)
 };
 
 template <typename T, int DT>
@@ -494,7 +494,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       floatx16 e[kHalves], dp[kHalves]; // scores, probabilities, and their gradients at last
       uint32_t sees[kHalves];           // of 16 rows
       const auto product = [&](const auto& read, const auto& use, const auto& beside) {
-        read_ahead<T, kSteps, S::kAhead>(read, [&](int n, const Frag<T>& f) {
+        read_ahead<T, kSteps>(read, [&](int n, const Frag<T>& f) {
           use(n, f);
           beside(n);
         });
@@ -513,7 +513,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         dp[g] = floatx16{};
         if constexpr (S::kValuesInLds) {
           Frag<T> d_rows;
-          read_ahead<T, 2 * kSteps, S::kAhead>(
+          read_ahead<T, 2 * kSteps>(
               [&](int n) {
                 return n % 2 == 0 ? L::load_rows(d_tile, 32 * g, n / 2, lane)
                                   : L::load_rows(values, 32 * wave, n / 2, lane);
@@ -580,6 +580,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       };
       const auto hide = [&](int g) {
         if (!whole) {
+          asm volatile(""); // a branch, not 16 selections for every tile
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             e[g][i] = (sees[g] >> i & 1) != 0 ? e[g][i] : 0.0f;
@@ -613,16 +614,28 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       } else { // (in the order that holds the fewest registers)
         d_weights(0, nothing);
         scores(0, nothing);
+        // (four rows' numbers in registers at a time, not all sixteen)
+        const auto by_fours = [&](const float* of, const auto& use) {
+          float4 next = *reinterpret_cast<const float4*>(of + 4 * h);
 #pragma unroll
-        for (int n = 0; n < kSteps; ++n) {
-          exponentials(0)(n);
-        }
+          for (int x = 0; x < 4; ++x) {
+            const float4 now = next;
+            if (x < 3) {
+              next = *reinterpret_cast<const float4*>(of + 8 * (x + 1) + 4 * h);
+            }
+            use(4 * x, now.x);
+            use(4 * x + 1, now.y);
+            use(4 * x + 2, now.z);
+            use(4 * x + 3, now.w);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        };
+        by_fours(st.lse, [&](int i, float lse) {
+          e[0][i] = __builtin_amdgcn_exp2f(fmaf(e[0][i], a.scale_log2, -lse));
+        });
         hide(0);
         const auto probabilities = packed(0);
-#pragma unroll
-        for (int n = 0; n < kSteps; ++n) {
-          d_scores(0)(n);
-        }
+        by_fours(st.delta, [&](int i, float delta) { e[0][i] *= dp[0][i] - delta; });
         hide(0);
         const auto d_probabilities = packed(0);
         add_packed(d_cols, 0, probabilities, dv, nothing);
