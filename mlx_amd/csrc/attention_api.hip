@@ -43,12 +43,14 @@ int splits_of(const AttentionArgs& a, int dtype) {
         std::max<int64_t>(once, std::min<int64_t>(2 * once, span / 512)), span / 72);
   } else {
     const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads;
-    // (float32's matrix instruction takes 16 times as long: fewer keys are a run's worth)
-    splits = std::min<int64_t>(
-        512 / blocks,
-        dtype == MLXROCM_FLOAT32
-            ? span / 64
-            : std::max<int64_t>(span / 256, std::min<int64_t>(span / 128, 256 / blocks)));
+    // float32's matrix instruction takes 16 times as long: fewer keys are a run's worth, and it is
+    // busy with the one workgroup that a CU holds of more than 64 columns.  (3 times 16 heads of 80,
+    // 509 tokens, window 128: 1 52, 2 63; 16 heads of 256, 512 tokens: 1 230, 4* 90, 8 95.)
+    splits = dtype == MLXROCM_FLOAT32
+        ? std::min<int64_t>((a.D <= 64 ? 512 : 256) / blocks, span / 64)
+        : std::min<int64_t>(
+              512 / blocks,
+              std::max<int64_t>(span / 256, std::min<int64_t>(span / 128, 256 / blocks)));
   }
   return static_cast<int>(std::min<int64_t>(std::max<int64_t>(splits, 1), kMostSplits));
 }
@@ -74,7 +76,7 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   const int64_t row_blocks = (rows + kGradBlock - 1) / kGradBlock;
   p.blocks = (a.keys + kGradBlock - 1) / kGradBlock;
   // float32's matrix instruction takes 16 times as long: less is enough for a part
-  const int64_t least = dtype == MLXROCM_FLOAT32 ? 64 : 1024;
+  const int64_t least = dtype == MLXROCM_FLOAT32 ? 128 : 1024;
   const int64_t reach = static_cast<int64_t>(a.window) + kGradBlock; // tokens
   const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
   const auto parts = [&](int64_t blocks, int64_t length) {
