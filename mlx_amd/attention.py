@@ -219,7 +219,7 @@ def paged_cache_update(
     returns the pages.  ``k_pages`` and ``v_pages`` are ``[pages, Hkv, page size, D]``, the page
     size a multiple of 16; token ``j`` of sequence ``b`` has row ``j % page size`` of page
     ``block_table[b, j // page size]``.  ``lengths`` ``[B]`` counts the tokens of each sequence with
-    the new ones; where it is below ``L``, those in front are padding and not written."""
+    the new ones; where it is below ``L``, those in front are padding and not written.  No gradients."""
     if ops._fast.paged_cache_update(k, v, k_pages, v_pages, block_table, lengths):
         return k_pages, v_pages
     tag = "paged_cache_update"
@@ -241,6 +241,10 @@ def paged_cache_update(
                          "16 bytes.")
     _check_table(tag, block_table, lengths, k.shape[0])
     _check_pages(tag, k_pages, v_pages)
+    if any(n > 1 and s == 0 for t in (k_pages, v_pages) for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"[{tag}] Pages that share memory (expanded ones) cannot be written to.")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_pages, v_pages)):
+        raise NotImplementedError(f"[{tag}] no gradients through a paged cache.")
     _require_gpu(tag, k, v, k_pages, v_pages, block_table, lengths)
     lib = _lib.load()
     table, lengths = _table(block_table), _int32(lengths)

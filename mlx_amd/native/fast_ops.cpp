@@ -894,6 +894,11 @@ PyObject* paged_cache_update(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !fits_int(k->size(2)) || !fits_int(k->size(3))) {
     NOT_PLAIN;
   }
+  for (int i = 0; i < 3; ++i) { // (what shares memory is refused there)
+    if (c.k->size(i) > 1 && (c.k->stride(i) == 0 || c.v->stride(i) == 0)) {
+      NOT_PLAIN;
+    }
+  }
   int64_t strides[13];
   strides_of(*k, strides);
   strides_of(*v, strides + 3);
