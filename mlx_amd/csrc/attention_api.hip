@@ -12,18 +12,39 @@ namespace {
 constexpr int kMostKeys = 1 << 30; // positions and their differences stay in 32 bits
 constexpr int kMostSplits = 64;
 
-// Whether the kernel for few rows takes a call, else the one of 128-row tiles.  us, few / tiles, each
-// with its best number of runs, 4096 keys: 8 sequences of 32 rows of 128 39.2 / 31.4, of 64 columns
-// 22.0 / 24.5; 4 of 16 rows of 256 17.6 / 20.1, of 32 rows 24.1 / 20.4; in float32 8 of 32 rows of
-// 128 85 / 176, 4 of 32 rows of 256 44 / 38.
-bool few(const AttentionArgs& a, int dtype) {
-  const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
-  const int wide = dtype == MLXROCM_FLOAT32 ? 128 : 64; // columns of which 32 rows are few
-  return rows <= (a.D <= wide ? 32 : 16);
-}
-
 int64_t heads_of(const AttentionArgs& a) {
   return static_cast<int64_t>(a.B) * a.Hkv;
+}
+
+// Rows of a workgroup of the kernel for few rows
+int64_t few_block(const AttentionArgs& a, int dtype) {
+  const int wide = dtype == MLXROCM_FLOAT32 ? 128 : 64; // columns of which 32 rows are few
+  return static_cast<int64_t>(a.G) * a.Lq > 16 && a.D <= wide ? 32 : 16;
+}
+
+// Workgroups of the kernel for few rows, and the keys that one of them is over
+struct FewWork {
+  int64_t rows, each, blocks, keys;
+  FewWork(const AttentionArgs& a, int dtype)
+      : rows(static_cast<int64_t>(a.G) * a.Lq),
+        each(few_block(a, dtype)),
+        blocks((rows + each - 1) / each * heads_of(a)),
+        keys(std::min<int64_t>(
+            a.keys - std::min(a.Lq, a.keys) / 2,
+            static_cast<int64_t>(a.window) + a.keep + (each + a.G - 1) / a.G)) {}
+};
+
+// Whether the kernel for few rows takes a call, else the one of 128-row tiles, which reads keys and
+// values less often but has its waves wait for each other.  us, few / tiles, each with its best
+// number of runs.  One workgroup for all rows, 4096 keys: 8 sequences of 32 rows of 64 columns
+// 22.0 / 24.5; 4 of 16 rows of 256 17.6 / 20.1.  More, bfloat16 (workgroups x keys): 16 heads of 128,
+// 512 tokens (512 x 256) 15.5 / 21.5; 8 key heads of 128 for 32, 128 tokens (256 x 64) 6.9 / 10.0;
+// 64 rows each over 4096 keys (32 x 4096) 15.7 / 16.9; 36 rows for 32 key heads over 8192
+// (96 x 8192) 51 / 32; 16 heads of 64, 2048 tokens (1024 x 1024) 54 / 37; 16 heads of 64, 8 times
+// 512 tokens under a window of 64 (2048 x 96) 26 / 14.
+bool few(const AttentionArgs& a, int dtype) {
+  const FewWork w(a, dtype);
+  return w.rows <= w.each || (w.blocks <= 512 && w.blocks * w.keys <= 1 << 17);
 }
 
 // Runs that the keys of a row are cut into.  Few rows, by runs, us (16-bit, 8 or 64 key heads of
@@ -38,9 +59,11 @@ int splits_of(const AttentionArgs& a, int dtype) {
   const int64_t heads = heads_of(a);
   int64_t splits;
   if (few(a, dtype)) {
-    const int64_t once = (256 + heads - 1) / heads; // a workgroup for each CU
+    const FewWork w(a, dtype);
+    const int64_t once = (256 + w.blocks - 1) / w.blocks; // a workgroup for each CU
+    const int64_t reach = w.rows <= w.each ? span : w.keys;
     splits = std::min<int64_t>(
-        std::max<int64_t>(once, std::min<int64_t>(2 * once, span / 512)), span / 72);
+        std::max<int64_t>(once, std::min<int64_t>(2 * once, reach / 512)), reach / 72);
   } else {
     const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + 127) / 128 * heads;
     // float32's matrix instruction takes 16 times as long: fewer keys are a run's worth, and it is

@@ -1,5 +1,6 @@
-// attention_few.h -- attention of up to 32 rows (a token, or a few, for all heads that
-// share a key head): bound by reading the keys and values once.
+// attention_few.h -- attention of few rows, up to 32 for a workgroup (a token, or a few, for all
+// heads that share a key head; small problems in several workgroups): bound by reading the keys and
+// values once, or where those are few by the latency of some dependent reads.
 //
 // The keys of a (sequence, key head) are cut into `splits` runs of tiles of 32, a workgroup
 // each, and within a workgroup its four waves take tiles in turn, each with a running maximum
@@ -142,7 +143,7 @@ __device__ __forceinline__ float sum_quarters(float v) {
 template <typename T, int DT, int NT, bool PAGED>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(DT * NT * sizeof(T) <= 256 ? 2 : 1)))
-void attention_few_kernel(const AttentionArgs a, const Grid grid) {
+void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
   using S = FewShape<T, DT>;
   constexpr int KT = kFewKeys;
   __shared__ struct { // the waves' results of 16 rows, while they are joined
@@ -153,30 +154,35 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4;
-  int head, split;
-  grid.find(&head, &split);
+  int head, piece;
+  grid.find(&head, &piece);
+  int split;
+  const int block = blocks - 1 - a.of_splits.divide(piece, &split); // (the last see most keys)
   int hk;
   const int b = a.of_Hkv.divide(head, &hk);
   const int R = a.G * a.Lq;
   const int length = length_of(a, b);
   const int first_row = max(0, a.Lq - length) * a.G;
-  const bool any = length > 0; // then first_row < R
+  const int r0 = block * 16 * NT;
+  const int lo = max(r0, first_row);
+  const int hi = min(r0 + 16 * NT, R) - 1;
+  const bool any = length > 0 && lo <= hi;
 
   KeyRange range = {};
   int t0 = 0, t1 = 0;
   if (any) {
-    range = keys_of(a, length, first_row, R - 1, KT);
+    range = keys_of(a, length, lo, hi, KT);
     run_of(range.tiles, split, a.of_splits, &t0, &t1);
   }
   const int p0 = length - a.Lq;
-  const int p_lo = p0 + a.of_G.divide(first_row);
-  const int p_hi = p0 + a.Lq - 1;
+  const int p_lo = p0 + a.of_G.divide(lo);
+  const int p_hi = p0 + a.of_G.divide(hi);
 
   Frag<T> q[NT][DT / 32];
   int p[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int row = min(max(16 * n + (lane & 15), first_row), R - 1);
+    const int row = min(max(r0 + 16 * n + (lane & 15), lo), hi);
     p[n] = p0 + a.of_G.divide(row);
     const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, row);
 #pragma unroll
@@ -324,7 +330,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid) {
     __syncthreads();
     // 16 threads for a row
     const int at = threadIdx.x >> 4;
-    const int row = 16 * n + at;
+    const int row = r0 + 16 * n + at;
     if (row < R) {
       float top = join.m[0][at];
 #pragma unroll
@@ -375,7 +381,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid) {
       const KeyTile at = tile_of(range, t, KT);
       for (int j = max(at.begin, at.low); j < at.end; ++j) {
         const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
-        for (int r = first_row; not_finite(x) && r < R; ++r) {
+        for (int r = lo; not_finite(x) && r <= hi; ++r) {
           if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
             continue;
           }
@@ -393,11 +399,12 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid) {
 template <typename T, int DT, int NT>
 int launch_few_rows(const AttentionArgs& a, hipStream_t s) {
   MLXROCM_REHEARSE("attention_few(dim=%d,rows=%d,splits=%d)", DT, 16 * NT, a.splits);
-  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, a.splits);
+  const int blocks = (a.G * a.Lq + 16 * NT - 1) / (16 * NT);
+  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits);
   if (a.table != nullptr) {
-    attention_few_kernel<T, DT, NT, true><<<grid.blocks(), 256, 0, s>>>(a, grid);
+    attention_few_kernel<T, DT, NT, true><<<grid.blocks(), 256, 0, s>>>(a, grid, blocks);
   } else {
-    attention_few_kernel<T, DT, NT, false><<<grid.blocks(), 256, 0, s>>>(a, grid);
+    attention_few_kernel<T, DT, NT, false><<<grid.blocks(), 256, 0, s>>>(a, grid, blocks);
   }
   MLXROCM_HIP_TRY(hipGetLastError());
   return static_cast<int>(MLXROCM_OK);
