@@ -282,6 +282,37 @@ __device__ __forceinline__ float sum_halves(float v) {
   const float2 r = both_halves(v);
   return r.x + r.y;
 }
+// ... over the lanes l % 16 + 0, 16, 32, 48
+__device__ __forceinline__ float max_quarters(float v) {
+  const uint32_t u = __float_as_uint(max_halves(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+  const uint32_t u = __float_as_uint(sum_halves(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// ... and over all 64
+template <int N>
+__device__ __forceinline__ float rotated(float v) { // by N within 16 lanes
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max_lanes(float v) {
+  v = fmaxf(v, rotated<8>(v));
+  v = fmaxf(v, rotated<4>(v));
+  v = fmaxf(v, rotated<2>(v));
+  v = fmaxf(v, rotated<1>(v));
+  return max_quarters(v);
+}
+__device__ __forceinline__ float sum_lanes(float v) {
+  v += rotated<8>(v);
+  v += rotated<4>(v);
+  v += rotated<2>(v);
+  v += rotated<1>(v);
+  return sum_quarters(v);
+}
 
 // N products whose LDS operands are read AHEAD products ahead: use(i, operand) and what it does
 // beside the product stay in their order.  Left alone, the compiler reads an operand, waits for

@@ -127,18 +127,6 @@ __device__ __forceinline__ Frag<T> column(
   return f;
 }
 
-// max or sum over the four lanes that hold a column's keys
-__device__ __forceinline__ float max_quarters(float v) {
-  const uint32_t u = __float_as_uint(max_halves(v));
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_quarters(float v) {
-  const uint32_t u = __float_as_uint(sum_halves(v));
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // NT: tiles of 16 rows
 template <typename T, int DT, int NT, bool PAGED>
 __global__ __launch_bounds__(256)

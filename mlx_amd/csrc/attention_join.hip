@@ -2,10 +2,11 @@
 // the keys: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, m = max_s m_s.
 //
 // A row is joined by WAVES waves.  A lane has the maximum and sum of one run (there are at most
-// 64), so the weights of all runs are there after one load; then lanes add up the runs, four
-// columns each and 64 WAVES / WIDTH runs at a time, with nothing to wait for between their
-// loads.  Few rows of many runs take a workgroup each, many rows a wave each.  (28 rows of 64 runs:
-// one run behind the other 45 us, a wave for a row 13.7, a workgroup for a row 4.)
+// 64), so the weights of all runs are there after one load; lanes add up the runs, four
+// columns each and 64 WAVES / WIDTH runs at a time, whose loads do not wait for the weights.
+// Few rows of many runs take a workgroup each, many rows a wave each.  (28 rows of 64 runs:
+// one run behind the other 45 us, a wave for a row 13.7, a workgroup for a row 5.8, its loads
+// ahead of the weights 3.8.)
 #include "attention.h"
 
 namespace mlxrocm {
@@ -18,42 +19,61 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   constexpr int kAtOnce = 64 / WIDTH * WAVES;
   __shared__ floatx4 sums[WAVES > 1 ? WAVES : 1][WIDTH];
   const int R = a.G * a.Lq;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * R;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * R; // (less than 2^26)
   const int wave = threadIdx.x >> 6;
-  const int64_t n = WAVES > 1 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  const int n = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
   if (n >= rows) {
     return; // (whole waves; with WAVES > 1 none)
   }
   const int lane = threadIdx.x & 63;
   const float2 ml =
       lane < a.splits ? a.part_ml[lane * rows + n] : make_float2(-INFINITY, 0.0f);
-  float top = ml.x;
+  // the columns of 64 runs, or as many as eight loads have, are on their way with the weights
+  constexpr int kFirst = 64 / kAtOnce < 8 ? 64 / kAtOnce : 8;
+  const int d = 4 * (lane % WIDTH);
+  const float* part = a.part_out + static_cast<int64_t>(n) * a.D + (d < a.D ? d : 0);
+  const int own = (WAVES > 1 ? wave * (64 / WIDTH) : 0) + lane / WIDTH;
+  const auto load = [&](int s) {
+    return *reinterpret_cast<const float4*>(part + min(s, a.splits - 1) * rows * a.D);
+  };
+  float4 first[kFirst] = {};
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    top = fmaxf(top, __shfl_xor(top, off, 64));
+  for (int x = 0; x < kFirst; ++x) {
+    if (x * kAtOnce < a.splits) {
+      first[x] = load(x * kAtOnce + own);
+    }
   }
+  const int head = n / R;
+  const int row = n - head * R;
+  int hk;
+  const int b = a.of_Hkv.divide(head, &hk);
+  const int i = a.of_G.divide(row);
+  const bool seeing = length_of(a, b) - a.Lq + i >= 0;
+  const float top = max_lanes(ml.x);
   const float less = top == -INFINITY ? 0.0f : top;
   // a run that saw nothing has nothing
   const bool has = !(ml.y == 0.0f);
   const float by = !has ? 0.0f : ml.x == less ? 1.0f : __builtin_amdgcn_exp2f(ml.x - less);
-  const float total = wave_sum(by * ml.y);
-  const int d = 4 * (lane % WIDTH);
-  const float* part = a.part_out + n * a.D + (d < a.D ? d : 0);
+  const float total = sum_lanes(by * ml.y);
   floatx4 sum = {};
-#pragma unroll 8
-  for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
-    const int s = s0 + (WAVES > 1 ? wave * (64 / WIDTH) : 0) + lane / WIDTH;
+  const auto add = [&](int s, const float4& v) {
     const float w = __shfl(by, s & 63, 64);
-    const float4 v = *reinterpret_cast<const float4*>(part + min(s, a.splits - 1) * rows * a.D);
     if (s < a.splits && w != 0.0f) {
       sum += w * floatx4{v.x, v.y, v.z, v.w};
     }
+  };
+#pragma unroll
+  for (int x = 0; x < kFirst; ++x) {
+    add(x * kAtOnce + own, first[x]);
   }
+#pragma unroll 8
+  for (int s0 = kFirst * kAtOnce; s0 < a.splits; s0 += kAtOnce) {
+    add(s0 + own, load(s0 + own));
+  }
+  if constexpr (WIDTH <= 32) {
 #pragma unroll
-  for (int off = WIDTH; off < 64; off <<= 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[i] += __shfl_xor(sum[i], off, 64);
+    for (int x = 0; x < 4; ++x) {
+      sum[x] = WIDTH == 16 ? sum_quarters(sum[x]) : sum_halves(sum[x]);
     }
   }
   if constexpr (WAVES > 1) {
@@ -69,12 +89,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
       sum += sums[w][lane % WIDTH];
     }
   }
-  const int head = static_cast<int>(n / R);
-  const int row = static_cast<int>(n - static_cast<int64_t>(head) * R);
-  int hk;
-  const int b = a.of_Hkv.divide(head, &hk);
-  const int i = a.of_G.divide(row);
-  const bool seeing = length_of(a, b) - a.Lq + i >= 0;
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
   if (lane < WIDTH && d < a.D) {
     T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row) + d;

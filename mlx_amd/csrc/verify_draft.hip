@@ -13,7 +13,7 @@
 // Two kernels: sums of parts of the one row that is drawn from (bound by reading it), then one
 // workgroup for each sequence finds the part and the token in it (bound by the latency of a few
 // dependent reads, for which the first kernel leaves n behind).  32 sequences, 128256 tokens, f32:
-// 7.2 us and 3.9 us; one sequence, 32000 tokens: 4.2 us and 2.9 us.
+// 6.9 us and 3.9 us; one sequence, 32000 tokens: 3.8 us and 2.4 us.
 #include "common.h"
 
 namespace mlxrocm {
@@ -126,11 +126,23 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    v += __shfl_xor(static_cast<unsigned long long>(v), off, 64);
-  }
+// v of another lane of the wave, 0 where there is none or ROWS (of 16 lanes) leaves this one out
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(
+      0, static_cast<int>(static_cast<uint32_t>(v)), CONTROL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(
+      0, static_cast<int>(static_cast<uint32_t>(v >> 32)), CONTROL, ROWS, 0xf, false);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// Sums of lanes 0 .. this one
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v += moved<0x111, 0xf>(v); // from 1, 2, 4 and 8 lanes below
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v); // the last lane of a row for the next row, of rows 0 and 2
+  v += moved<0x143, 0xc>(v); // lane 31 for the upper half
   return v;
 }
 
@@ -162,7 +174,10 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(const VerifyArgs a) {
         s += whole(of[i][j]);
       }
     }
-    return wave_sum64(s);
+    const uint64_t all = wave_scan(s); // of the wave in lane 63
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(all), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(all >> 32), 63);
+    return static_cast<uint64_t>(hi) << 32 | lo;
   };
   const uint64_t of_w = sum(w);
   // where a weight is not zero anywhere, nothing is drawn from p itself
@@ -187,11 +202,7 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(const VerifyArgs a) {
 // Sums of the values of threads 0 .. this one
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* wave_totals) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t below = __shfl_up(static_cast<unsigned long long>(v), off, 64);
-    v += lane >= off ? below : 0;
-  }
+  v = wave_scan(v);
   __syncthreads();
   if (lane == 63) {
     wave_totals[threadIdx.x >> 6] = v;
