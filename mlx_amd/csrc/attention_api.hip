@@ -92,14 +92,17 @@ size_t workspace_of(const AttentionArgs& a, int dtype) {
 }
 
 // The cuts of the gradients' sums: parts of some tiles each, and a thousand workgroups if there
-// are as many.
+// are as many.  us of both gradients, bfloat16, parts of at least 256, 512, 768 and 1024 keys or rows:
+// 64 heads of 128 on 8, 500 tokens 104 (512), 126, 163; 28 on 4, 2 times 1000 tokens 182, 144, 166,
+// 188; 32 on 8, 4096 tokens under a window of 256 with 4 kept 282, 257, 270, 289, with none 217, 230,
+// 189, 225; 12 heads of 96 on 4, 1500 tokens under a window of 128 85 (rows cut in two), 122 (not).
 GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   GradPlan p{};
   const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
   const int64_t row_blocks = (rows + kGradBlock - 1) / kGradBlock;
   p.blocks = (a.keys + kGradBlock - 1) / kGradBlock;
   // float32's matrix instruction takes 16 times as long: less is enough for a part
-  const int64_t least = dtype == MLXROCM_FLOAT32 ? 128 : 1024;
+  const int64_t least = dtype == MLXROCM_FLOAT32 ? 128 : 512;
   const int64_t reach = static_cast<int64_t>(a.window) + kGradBlock; // tokens
   const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
   const auto parts = [&](int64_t blocks, int64_t length) {
@@ -113,7 +116,7 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
     p.wide_blocks = static_cast<int>(std::min<int64_t>(
         p.blocks, (static_cast<int64_t>(a.keep) + kGradBlock - 1) / kGradBlock));
   }
-  const int splits = p.blocks > 0 ? parts(p.blocks, seen_by) : 1;
+  const int splits = p.blocks > 0 ? parts(p.blocks, seen_by + least / 2) : 1;
   p.splits = Divisor(splits);
   // runs no longer than the others'
   p.wide_splits = Divisor(
