@@ -142,23 +142,23 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4;
-  int head, piece;
-  grid.find(&head, &piece);
-  int split;
-  const int block = blocks - 1 - a.of_splits.divide(piece, &split); // (the last see most keys)
+  int head, split;
+  grid.find(&head, &split);
+  int r0 = 0;
+  if (blocks > 1) { // (the last see most keys)
+    r0 = (blocks - 1 - a.of_splits.divide(split, &split)) * 16 * NT;
+  }
   int hk;
   const int b = a.of_Hkv.divide(head, &hk);
   const int R = a.G * a.Lq;
   const int length = length_of(a, b);
-  const int first_row = max(0, a.Lq - length) * a.G;
-  const int r0 = block * 16 * NT;
-  const int lo = max(r0, first_row);
+  // rows that see something: lo .. hi, or none (an empty sequence: lo >= R)
+  const int lo = max(r0, max(0, a.Lq - length) * a.G);
   const int hi = min(r0 + 16 * NT, R) - 1;
-  const bool any = length > 0 && lo <= hi;
 
   KeyRange range = {};
   int t0 = 0, t1 = 0;
-  if (any) {
+  if (lo <= hi) {
     range = keys_of(a, length, lo, hi, KT);
     run_of(range.tiles, split, a.of_splits, &t0, &t1);
   }
@@ -176,7 +176,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
 #pragma unroll
     for (int c = 0; c < DT / 32; ++c) {
       const int d = 32 * c + 8 * g;
-      q[n][c] = d < a.D && any ? load_frag<T>(src + d) : zero_frag<T>();
+      q[n][c] = d < a.D && lo <= hi ? load_frag<T>(src + d) : zero_frag<T>();
       flip<T>(q[n][c], a.q_sign);
     }
   }
@@ -319,7 +319,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     // 16 threads for a row
     const int at = threadIdx.x >> 4;
     const int row = r0 + 16 * n + at;
-    if (row < R) {
+    if (row <= hi) {
       float top = join.m[0][at];
 #pragma unroll
       for (int x = 1; x < 4; ++x) {
@@ -332,7 +332,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         by[x] = join.m[x][at] == less ? 1.0f : __builtin_amdgcn_exp2f(join.m[x][at] - less);
         total += by[x] * join.l[x][at];
       }
-      const bool seeing = any && row >= first_row;
+      const bool seeing = row >= lo;
       const float over = total == 0.0f ? 0.0f : 1.0f / total;
       const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R + row;
       T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row);
