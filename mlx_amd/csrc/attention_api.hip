@@ -92,7 +92,8 @@ size_t workspace_of(const AttentionArgs& a, int dtype) {
 }
 
 // The cuts of the gradients' sums: parts of some tiles each, and a thousand workgroups if there
-// are as many.  us of both gradients, bfloat16, parts of at least 256, 512, 768 and 1024 keys or rows:
+// are as many, half as many where a CU holds one (8 heads of 256 on 2, 4096 tokens 614 instead of
+// 743 us).  us of both gradients, bfloat16, parts of at least 256, 512, 768 and 1024 keys or rows:
 // 64 heads of 128 on 8, 500 tokens 104 (512), 126, 163; 28 on 4, 2 times 1000 tokens 182, 144, 166,
 // 188; 32 on 8, 4096 tokens under a window of 256 with 4 kept 282, 257, 270, 289, with none 217, 230,
 // 189, 225; 12 heads of 96 on 4, 1500 tokens under a window of 128 85 (rows cut in two), 122 (not).
@@ -103,10 +104,12 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   p.blocks = (a.keys + kGradBlock - 1) / kGradBlock;
   // float32's matrix instruction takes 16 times as long: less is enough for a part
   const int64_t least = dtype == MLXROCM_FLOAT32 ? 128 : 512;
+  const int64_t fill = a.D * dtype_size(dtype) <= 256 ? 1024 : 512;
   const int64_t reach = static_cast<int64_t>(a.window) + kGradBlock; // tokens
   const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
   const auto parts = [&](int64_t blocks, int64_t length) {
-    const int64_t wanted = (1024 + blocks * heads_of(a) - 1) / std::max<int64_t>(blocks * heads_of(a), 1);
+    const int64_t whole = std::max<int64_t>(blocks * heads_of(a), 1);
+    const int64_t wanted = (fill + whole - 1) / whole;
     return static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>({wanted, length / least, int64_t{kMostSplits}})));
   };
