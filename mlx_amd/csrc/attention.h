@@ -144,6 +144,15 @@ __device__ __forceinline__ uint4 frag_bits(const Frag<T>& f) {
   return make_uint4(f.w[0], f.w[1], f.w[2], f.w[3]);
 }
 
+// A sum that starts at zero, as the compiler is not to know: it splits vectors that it sees begin
+// with constants into scalars where paths meet, and then moves all of them between the two files
+// of registers around the products (16 times 16 of them in a tile of 256 columns).
+__device__ __forceinline__ floatx16 zero_sum() {
+  floatx16 x = {};
+  asm("" : "+v"(x));
+  return x;
+}
+
 // c + a b over 16 values of the contraction (8 in each half of the wave): one
 // instruction for the 16-bit types; float32 takes eight of two values each.
 template <typename T>

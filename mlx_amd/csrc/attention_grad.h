@@ -120,7 +120,7 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
   floatx16 dq[DT / 32];
 #pragma unroll
   for (int d = 0; d < DT / 32; ++d) {
-    dq[d] = floatx16{};
+    dq[d] = zero_sum();
   }
   if (t0 < t1) {
     keys.fetch(tile_of(range, t0, KT).begin, lds, lds + kBoth / 2);
@@ -323,33 +323,29 @@ struct RowStream {
 // and values 64: the values stay in LDS then (read again for each tile, a quarter more
 // than is read anyway), and a tile is 32 rows, so that two workgroups fit, of whose sums and deltas
 // four are in registers at a time.  8192 tokens, 32 heads of 128, both gradients 2.06 ms; with two
-// fragments read ahead instead of four 2.08 ms; with all in registers and one wave a SIMD the compiler
-// moves results between its two files around each product.
-//
-// Of 256 columns a kernel has one result, dv or dk: the scores are made twice, and in 16 bits
-// nothing is spilled.  4096 tokens, 8 heads of 256 on 2, both gradients 0.61 ms, with both
-// results 1.56.
-constexpr int kDv = 1;
-constexpr int kDk = 2;
-template <typename T, int DT, int RESULTS>
+// fragments read ahead instead of four 2.08 ms.  Of 256 columns one wave a SIMD has 512 registers:
+// 4096 tokens, 8 heads of 256 on 2 0.45 ms; a kernel for dk and one for dv, which make the scores
+// twice, 0.55 ms.
+template <typename T, int DT>
 struct DkvShape {
-  static constexpr bool kTwo = // waves a SIMD
-      DT * sizeof(T) <= (RESULTS == kDv ? 512 : 256);
-  static constexpr bool kValuesInLds = sizeof(T) == 2 && (DT == 96 || DT == 128);
-  static constexpr bool kValueHeld = !kValuesInLds && RESULTS != kDv;
-  static constexpr int kRows = kValuesInLds ? 32 : RowsShape<T, DT>::kKeys; // of a tile
+  static constexpr bool kTwo = DT * sizeof(T) <= 256; // waves a SIMD
+  static constexpr bool kValuesInLds = sizeof(T) == 2 && DT >= 96;
+  static constexpr int kRows = kValuesInLds || sizeof(T) == 4 ? 32 : 64; // of a tile
   static constexpr int kTile = kRows * Tile<T, DT>::kPitch;
 };
 
-template <typename T, int DT, int RESULTS>
+template <typename T, int DT>
 __global__ __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(
-    DkvShape<T, DT, RESULTS>::kTwo ? 2 : 1, DkvShape<T, DT, RESULTS>::kTwo ? 2 : 1)))
+__attribute__((amdgpu_waves_per_eu(DkvShape<T, DT>::kTwo ? 2 : 1, DkvShape<T, DT>::kTwo ? 2 : 1)))
 void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
-  using S = DkvShape<T, DT, RESULTS>;
+  using S = DkvShape<T, DT>;
   using L = Tile<T, DT>;
   constexpr int RT = S::kRows;
   constexpr int kBoth = 2 * S::kTile;
+  // this lane's key and value: in registers, but for 256 floats, which are read again for
+  // each tile (with both results they would need all 512 registers)
+  constexpr bool kKeyHeld = DT * sizeof(T) <= 512;
+  constexpr bool kValueHeld = kKeyHeld && !S::kValuesInLds;
   __shared__ __align__(1024) T lds[2 * kBoth];
   __shared__ __align__(1024) T values[S::kValuesInLds ? kKeysBlock * L::kPitch : 16];
   __shared__ __align__(16) StatsTile<RT> stats[2];
@@ -401,12 +397,14 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     const int d = 16 * c + 8 * h;
     return d < a.D ? load_frag<T>(v_src + d) : zero_frag<T>();
   };
-  Frag<T> k[DT / 16], v[S::kValueHeld ? DT / 16 : 1]; // this lane's key and value
+  Frag<T> k[kKeyHeld ? DT / 16 : 1], v[kValueHeld ? DT / 16 : 1];
   if (any) {
 #pragma unroll
     for (int c = 0; c < DT / 16; ++c) {
-      k[c] = key_frag(c);
-      if constexpr (S::kValueHeld) {
+      if constexpr (kKeyHeld) {
+        k[c] = key_frag(c);
+      }
+      if constexpr (kValueHeld) {
         v[c] = value_frag(c);
       }
     }
@@ -441,12 +439,11 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
   };
 
   RowStream<T, DT, RT> rows(ga, b, hk, begin_row, end_row, wave, lane);
-  floatx16 dk[(RESULTS & kDk) != 0 ? DT / 32 : 1], dv[(RESULTS & kDv) != 0 ? DT / 32 : 1];
-  for (floatx16& x : dk) {
-    x = floatx16{};
-  }
-  for (floatx16& x : dv) {
-    x = floatx16{};
+  floatx16 dk[DT / 32], dv[DT / 32];
+#pragma unroll
+  for (int d = 0; d < DT / 32; ++d) {
+    dk[d] = zero_sum();
+    dv[d] = zero_sum();
   }
   RowStats mine = {};
   if (tiles > 0) {
@@ -509,7 +506,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         product(
             [&](int n) { return L::load_rows(q_tile, 32 * g, n, lane); },
             [&](int n, const Frag<T>& f) {
-              e[g] = mma32<T>(f, k[n], e[g]);
+              e[g] = mma32<T>(f, kKeyHeld ? k[kKeyHeld ? n : 0] : key_frag(n), e[g]);
             },
             beside);
       };
@@ -534,7 +531,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
           product(
               [&](int n) { return L::load_rows(d_tile, 32 * g, n, lane); },
               [&](int n, const Frag<T>& f) {
-                dp[g] = mma32<T>(f, v[n], dp[g]);
+                dp[g] = mma32<T>(f, kValueHeld ? v[kValueHeld ? n : 0] : value_frag(n), dp[g]);
               },
               beside);
         }
@@ -603,7 +600,6 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         }
       }
       if constexpr (kHalves == 2) {
-        static_assert(RESULTS == (kDk | kDv), "");
         scores(0, nothing);
         scores(1, exponentials(0));
         hide(0);
@@ -617,9 +613,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         hide(1);
         add(q_cols, 1, dk, nothing);
       } else { // (in the order that holds the fewest registers)
-        if constexpr ((RESULTS & kDk) != 0) {
-          d_weights(0, nothing);
-        }
+        d_weights(0, nothing);
         scores(0, nothing);
         // (four rows' numbers in registers at a time, not all sixteen)
         const auto by_fours = [&](const float* of, const auto& use) {
@@ -642,17 +636,11 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         });
         hide(0);
         const auto probabilities = packed(0);
-        if constexpr ((RESULTS & kDk) != 0) {
-          by_fours(st.delta, [&](int i, float delta) { e[0][i] *= dp[0][i] - delta; });
-          hide(0);
-        }
+        by_fours(st.delta, [&](int i, float delta) { e[0][i] *= dp[0][i] - delta; });
+        hide(0);
         const auto d_probabilities = packed(0);
-        if constexpr ((RESULTS & kDv) != 0) {
-          add_packed(d_cols, 0, probabilities, dv, nothing);
-        }
-        if constexpr ((RESULTS & kDk) != 0) {
-          add_packed(q_cols, 0, d_probabilities, dk, nothing);
-        }
+        add_packed(d_cols, 0, probabilities, dv, nothing);
+        add_packed(q_cols, 0, d_probabilities, dk, nothing);
       }
     }
     if (apart && t + 1 < tiles) {
@@ -665,12 +653,8 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       (static_cast<int64_t>(head) * plan.pieces() + piece) * (kKeysBlock * 2 * a.D);
   if (parts) {
     float* to = part + (key - k0) * 2 * a.D;
-    if constexpr ((RESULTS & kDk) != 0) {
-      store_part<DT>(to, dk, key < k1, a.D, h);
-    }
-    if constexpr ((RESULTS & kDv) != 0) {
-      store_part<DT>(to + a.D, dv, key < k1, a.D, h);
-    }
+    store_part<DT>(to, dk, key < k1, a.D, h);
+    store_part<DT>(to + a.D, dv, key < k1, a.D, h);
   } else if (key < a.keys) {
     const bool seen = key < k1;
     const int64_t k_to = b * ga.dk_strides[0] + hk * ga.dk_strides[1] + key * ga.dk_strides[2];
@@ -681,16 +665,10 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       for (int i = 0; i < 4; ++i) {
         const int c = 32 * d + 8 * i + 4 * h;
         if (c < a.D) {
-          const auto four = [&](const floatx16& of) {
-            return floatx4{of[4 * i], of[4 * i + 1], of[4 * i + 2], of[4 * i + 3]};
-          };
-          if constexpr ((RESULTS & kDk) != 0) {
-            store4<T>(
-                static_cast<T*>(ga.dk) + k_to + c, seen ? four(dk[d]) * ga.scale : floatx4{});
-          }
-          if constexpr ((RESULTS & kDv) != 0) {
-            store4<T>(static_cast<T*>(ga.dv) + v_to + c, seen ? four(dv[d]) : floatx4{});
-          }
+          const floatx4 x = {dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+          const floatx4 y = {dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+          store4<T>(static_cast<T*>(ga.dk) + k_to + c, seen ? x * ga.scale : floatx4{});
+          store4<T>(static_cast<T*>(ga.dv) + v_to + c, seen ? y : floatx4{});
         }
       }
     }
@@ -699,25 +677,17 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     after_stores();
     const int d = threadIdx.x;
     for (int r = begin_row; r < end_row && d < a.D; ++r) {
-      // (what this kernel has no result of: as if it were zero)
-      const float x = (RESULTS & kDk) == 0
-          ? 0.0f
-          : to_f32(static_cast<const T*>(a.q)[row_offset(a.q_strides, b, hk, a.of_G, r) + d]);
-      const float y = (RESULTS & kDv) == 0
-          ? 0.0f
-          : to_f32(
-                static_cast<const T*>(ga.dout)[row_offset(ga.dout_strides, b, hk, a.of_G, r) + d]);
+      const float x = to_f32(
+          static_cast<const T*>(a.q)[row_offset(a.q_strides, b, hk, a.of_G, r) + d]);
+      const float y = to_f32(
+          static_cast<const T*>(ga.dout)[row_offset(ga.dout_strides, b, hk, a.of_G, r) + d]);
       for (int j = k0; (not_finite(x) || not_finite(y)) && j < k1; ++j) {
         if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
           continue;
         }
         if (parts) {
-          if (not_finite(x)) {
-            add_to(part + (j - k0) * 2 * a.D + d, x);
-          }
-          if (not_finite(y)) {
-            add_to(part + (j - k0) * 2 * a.D + a.D + d, y);
-          }
+          add_to(part + (j - k0) * 2 * a.D + d, not_finite(x) ? x : 0.0f);
+          add_to(part + (j - k0) * 2 * a.D + a.D + d, not_finite(y) ? y : 0.0f);
           continue;
         }
         if (not_finite(x)) {
@@ -753,13 +723,7 @@ int launch_grad_of(const AttentionGradArgs& g, hipStream_t s) {
   }
   if (g.plan.blocks > 0) {
     const Grid grid(heads, g.plan.pieces());
-    if constexpr (DT == 256) {
-      attention_dkv_kernel<T, DT, kDv><<<grid.blocks(), 256, 0, s>>>(g, grid);
-      MLXROCM_HIP_TRY(hipGetLastError());
-      attention_dkv_kernel<T, DT, kDk><<<grid.blocks(), 256, 0, s>>>(g, grid);
-    } else {
-      attention_dkv_kernel<T, DT, kDk | kDv><<<grid.blocks(), 256, 0, s>>>(g, grid);
-    }
+    attention_dkv_kernel<T, DT><<<grid.blocks(), 256, 0, s>>>(g, grid);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
   return static_cast<int>(MLXROCM_OK);
