@@ -757,12 +757,15 @@ int mlxrocm_switch_glu(
  * only during the call, 16-byte aligned, of _workspace_size bytes (0: it may be NULL).
  *
  * mlxrocm_window_attention: q [B, Hq, Lq, D], k and v [B, Hkv, Lk, D], out as q.  lengths may be
- * NULL (Lk each).  strides: of q, k, v, out.  lse: NULL, or [B, Hq, Lq] floats that the gradients
- * need.
+ * NULL (Lk each).  strides: of q, k, v, out.  lse: NULL, or _lse_size bytes, aligned to 16, for what
+ * the gradients need: log2 of each row's sum, and in 16-bit types, where a token sees at most 2048,
+ * what rounding took from out.
  * mlxrocm_window_attention_vjp: the gradients dq, dk, dv of q, k, v from dout, that of out.
  * strides: of q, k, v, out, dout, dq, dk, dv.  Sums are taken in a fixed order.
  */
 size_t mlxrocm_window_attention_workspace_size(
+    int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype);
+size_t mlxrocm_window_attention_lse_size(
     int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype);
 int mlxrocm_window_attention(
     const void* q,

@@ -55,6 +55,7 @@ SIGNATURES = {
         [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i64, _i64, _i, _i, _i, _i, _p],
     ),
     "mlxrocm_window_attention_workspace_size": (_sz, [_i] * 9),
+    "mlxrocm_window_attention_lse_size": (_sz, [_i] * 9),
     "mlxrocm_window_attention": (_i, [_p] * 6 + [_i] * 6 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
     "mlxrocm_window_attention_vjp_workspace_size": (_sz, [_i] * 9),
     "mlxrocm_window_attention_vjp": (

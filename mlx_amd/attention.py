@@ -102,8 +102,11 @@ def _window_forward(q, k, v, lengths, scale, window, keep, wants_lse):
     out = _empty_like(q)
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1:3]
-    lse = (torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if wants_lse else None)
     code = _DTYPE_CODE[q.dtype]
+    lse = None
+    if wants_lse:
+        size = lib.mlxrocm_window_attention_lse_size(B, Hq, Hkv, Lq, Lk, D, window, keep, code)
+        lse = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
     size = lib.mlxrocm_window_attention_workspace_size(B, Hq, Hkv, Lq, Lk, D, window, keep, code)
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _lib.check(lib.mlxrocm_window_attention(

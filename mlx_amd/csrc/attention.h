@@ -60,6 +60,7 @@ struct AttentionArgs {
   const void* v;
   void* out;
   float* lse; // [B, Hq, Lq]: log2 of the sum of exp(score), for the gradients; may be null
+  void* low;  // [B, Hq, Lq, D]: what rounding took from out, for the gradients; may be null
   const int* lengths; // [B], or null: every sequence has `keys`
   const int* table;   // [B, table_stride], or null: contiguous keys
   int64_t table_stride;
@@ -92,6 +93,10 @@ struct GradPlan {
     return wide_blocks * wide_splits.d + (blocks - wide_blocks) * splits.d;
   }
   __host__ __device__ bool dkv_split() const { return wide_splits.d > 1 || splits.d > 1; }
+  // Those of which partial sums are kept: the first ones, the wide blocks'
+  __host__ __device__ int part_pieces() const {
+    return splits.d > 1 ? pieces() : wide_blocks * wide_splits.d;
+  }
 };
 
 // The gradients' further operands.
@@ -648,6 +653,34 @@ __device__ __forceinline__ void copy_finite(const T* from, T* to) {
 template <typename T>
 __device__ __forceinline__ void add_to(T* p, float x) {
   *p = from_f32<T>(to_f32(*p) + x);
+}
+
+// Row r among the sums that the gradients need
+__device__ __forceinline__ int64_t lse_at(const AttentionArgs& a, int b, int hk, int r) {
+  int g;
+  const int i = a.of_G.divide(r, &g);
+  return (static_cast<int64_t>(b) * a.Hq + hk * a.G + g) * a.Lq + i;
+}
+
+// Four columns of a result, and what rounding takes from them: delta would be as far off as the
+// gradients' own rounding (of tokens that see few), were it formed from the rounded result alone
+template <typename T>
+__device__ __forceinline__ T* low_of(const AttentionArgs& a, int64_t row) { // (row: lse_at)
+  return a.low == nullptr ? nullptr : static_cast<T*>(a.low) + row * a.D;
+}
+template <typename T>
+__device__ __forceinline__ void store_result(T* out, T* low, floatx4 x) {
+  store4<T>(out, x);
+  if constexpr (sizeof(T) == 2) {
+    if (low != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float rounded = to_f32(from_f32<T>(x[i]));
+        x[i] = not_finite(rounded) ? 0.0f : x[i] - rounded;
+      }
+      store4<T>(low, x);
+    }
+  }
 }
 
 // Stores of this workgroup are behind, its threads may add to them

@@ -336,6 +336,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       const float over = total == 0.0f ? 0.0f : 1.0f / total;
       const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R + row;
       T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row);
+      T* low = low_of<T>(a, lse_at(a, b, hk, row));
       for (int d = 4 * (threadIdx.x & 15); d < a.D; d += 64) {
         floatx4 sum4 = {};
 #pragma unroll
@@ -347,16 +348,15 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
           *reinterpret_cast<float4*>(a.part_out + part * a.D + d) =
               make_float4(sum4[0], sum4[1], sum4[2], sum4[3]);
         } else {
-          store4<T>(out + d, seeing ? sum4 * over : floatx4{});
+          store_result<T>(
+              out + d, low == nullptr ? nullptr : low + d, seeing ? sum4 * over : floatx4{});
         }
       }
       if ((threadIdx.x & 15) == 0) {
         if (a.splits > 1) {
           a.part_ml[part] = make_float2(top, seeing ? total : 0.0f);
         } else if (a.lse != nullptr) {
-          const int i = a.of_G.divide(row);
-          a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
-              seeing ? top + log2f(total) : 0.0f;
+          a.lse[lse_at(a, b, hk, row)] = seeing ? top + log2f(total) : 0.0f;
         }
       }
     }

@@ -88,6 +88,8 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
     const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, from);
     const T* dsrc = static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.of_G, from);
     const T* osrc = static_cast<const T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, from);
+    const int64_t at = lse_at(a, b, hk, from);
+    const T* low = low_of<T>(a, at);
 #pragma unroll
     for (int c = 0; c < DT / 16; ++c) {
       const int d = 16 * c + 8 * h;
@@ -102,11 +104,16 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
         for (int e = 0; e < 8; ++e) {
           delta = fmaf(x[e], y[e], delta);
         }
+        if (sizeof(T) == 2 && low != nullptr) {
+          load8<T>(low + d, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            delta = fmaf(x[e], y[e], delta);
+          }
+        }
       }
     }
     delta = sum_halves(delta);
-    const int64_t at =
-        (static_cast<int64_t>(b) * a.Hq + hk * a.G + from - i_from * a.G) * a.Lq + i_from;
     lse = a.lse[at];
     if (seeing && h == 0 && split == 0) {
       ga.delta[at] = delta;
@@ -648,9 +655,9 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       rows.fetch(begin + RT, next, next + kBoth / 2);
     }
   }
-  const bool parts = plan.dkv_split();
+  const bool parts = splits.d > 1;
   float* part = ga.part_dkv +
-      (static_cast<int64_t>(head) * plan.pieces() + piece) * (kKeysBlock * 2 * a.D);
+      (static_cast<int64_t>(head) * plan.part_pieces() + piece) * (kKeysBlock * 2 * a.D);
   if (parts) {
     float* to = part + (key - k0) * 2 * a.D;
     store_part<DT>(to, dk, key < k1, a.D, h);

@@ -9,6 +9,8 @@
 // ahead of the weights 3.8.)
 #include "attention.h"
 
+#include <algorithm>
+
 namespace mlxrocm {
 
 namespace {
@@ -92,11 +94,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
   if (lane < WIDTH && d < a.D) {
     T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row) + d;
-    store4<T>(out, seeing ? sum * over : floatx4{});
+    T* low = low_of<T>(a, lse_at(a, b, hk, row));
+    store_result<T>(out, low == nullptr ? nullptr : low + d, seeing ? sum * over : floatx4{});
   }
   if (a.lse != nullptr && lane == 0) {
-    a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
-        seeing ? top + log2f(total) : 0.0f;
+    a.lse[lse_at(a, b, hk, row)] = seeing ? top + log2f(total) : 0.0f;
   }
 }
 
@@ -141,10 +143,10 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Attention
   const bool seeing = length_of(a, b) - a.Lq + i >= 0;
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
   T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row) + d;
-  store4<T>(out, seeing ? sum * over : floatx4{});
+  T* low = low_of<T>(a, lse_at(a, b, hk, row));
+  store_result<T>(out, low == nullptr ? nullptr : low + d, seeing ? sum * over : floatx4{});
   if (a.lse != nullptr && d == 0) {
-    a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
-        seeing ? top + log2f(total) : 0.0f;
+    a.lse[lse_at(a, b, hk, row)] = seeing ? top + log2f(total) : 0.0f;
   }
 }
 
@@ -174,25 +176,28 @@ __global__ __launch_bounds__(256) void attention_sum_dq_kernel(const AttentionGr
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void attention_sum_dkv_kernel(const AttentionGradArgs g) {
+__global__ __launch_bounds__(256) void attention_sum_dkv_kernel(const AttentionGradArgs g, int keys) {
   const AttentionArgs& a = g.a;
   const GradPlan& plan = g.plan;
   const int each = 2 * a.D / 4; // of a key
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t n = at / each;
-  if (n >= static_cast<int64_t>(a.B) * a.Hkv * a.keys) {
+  if (n >= static_cast<int64_t>(a.B) * a.Hkv * keys) {
     return;
   }
   const int c = static_cast<int>(at - n * each) * 4; // column of dk, then of dv
-  const int head = static_cast<int>(n / a.keys);
-  const int key = static_cast<int>(n - static_cast<int64_t>(head) * a.keys);
+  const int head = static_cast<int>(n / keys);
+  const int key = static_cast<int>(n - static_cast<int64_t>(head) * keys);
   const int block = key / kGradBlock;
   const bool wide = block < plan.wide_blocks;
   const int splits = wide ? plan.wide_splits.d : plan.splits.d;
+  if (splits == 1) {
+    return; // (whole already)
+  }
   const int piece = wide ? block * splits
                          : plan.wide_blocks * plan.wide_splits.d + (block - plan.wide_blocks) * splits;
   const float* part = g.part_dkv +
-      (static_cast<int64_t>(head) * plan.pieces() + piece) * (kGradBlock * 2 * a.D) +
+      (static_cast<int64_t>(head) * plan.part_pieces() + piece) * (kGradBlock * 2 * a.D) +
       (key - block * kGradBlock) * 2 * a.D + c;
   floatx4 sum = {};
 #pragma unroll 4
@@ -223,8 +228,11 @@ int launch_attention_grad_join(const AttentionGradArgs& g, int dtype, hipStream_
       MLXROCM_HIP_TRY(hipGetLastError());
     }
     if (g.plan.dkv_split()) {
-      const int64_t n = static_cast<int64_t>(a.B) * a.Hkv * a.keys * (a.D / 2);
-      attention_sum_dkv_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g);
+      // (only the blocks of kept keys, if the others are not cut)
+      const int keys =
+          g.plan.splits.d > 1 ? a.keys : std::min(a.keys, g.plan.wide_blocks * kGradBlock);
+      const int64_t n = static_cast<int64_t>(a.B) * a.Hkv * keys * (a.D / 2);
+      attention_sum_dkv_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(g, keys);
       MLXROCM_HIP_TRY(hipGetLastError());
     }
     return static_cast<int>(MLXROCM_OK);

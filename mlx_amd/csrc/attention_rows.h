@@ -327,23 +327,23 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     }
   } else if (stored) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l; // nothing but scores of -inf
+    const int64_t n = lse_at(a, b, hk, row);
     T* out = static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, row);
+    T* low = low_of<T>(a, n);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = 32 * d + 8 * i + 4 * h;
         if (c < a.D) {
-          store4<T>(out + c, seeing ? floatx4{o[d][4 * i] * by, o[d][4 * i + 1] * by,
-                                              o[d][4 * i + 2] * by, o[d][4 * i + 3] * by}
-                                    : floatx4{});
+          const floatx4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+          store_result<T>(
+              out + c, low == nullptr ? nullptr : low + c, seeing ? x * by : floatx4{});
         }
       }
     }
     if (a.lse != nullptr && h == 0) {
-      const int i = a.of_G.divide(row);
-      a.lse[(static_cast<int64_t>(b) * a.Hq + hk * a.G + row - i * a.G) * a.Lq + i] =
-          seeing ? m + log2f(l) : 0.0f;
+      a.lse[n] = seeing ? m + log2f(l) : 0.0f;
     }
   }
   if (odd) { // the same for all
