@@ -162,6 +162,8 @@ def window_attention(
     the ``Lk`` keys each sequence has, all without it.  The result has ``q``'s shape and, where
     that is dense, its memory order.  Differentiable with respect to q, k and v."""
     out = ops._fast.window_attention(q, k, v, scale, window, keep, lengths)
+    if out is None and torch.is_grad_enabled():
+        out = ops._fast.window_attention_recorded(q, k, v, scale, window, keep, lengths)
     if out is not None:
         return out
     tag = "window_attention"

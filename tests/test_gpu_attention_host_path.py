@@ -112,3 +112,70 @@ def test_on_another_stream():
         got = [mlx_amd.paged_attention(q, *pages, table, lengths, scale=0.125) for _ in range(20)]
     stream.synchronize()
     assert all(torch.equal(t, want) for t in got)
+
+
+def _leaves(dtype=torch.bfloat16, length=40):
+    fused = _x(2, length, 8, 64, dtype=dtype)  # four heads of q, two of k, two of v, side by side
+    return [t.transpose(1, 2).detach().requires_grad_() for t in fused.split((4, 2, 2), 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [None, [40, 13]])
+def test_gradients(both, lengths, dtype):  # noqa: F811
+    n = None if lengths is None else _int(lengths)
+    cotangent = _x(2, 40, 4, 64, dtype=dtype).transpose(1, 2)
+
+    def run(cotangent):
+        leaves = _leaves(dtype)
+        out = mlx_amd.window_attention(*leaves, scale=0.125, window=9, keep=2, lengths=n)
+        grads = torch.autograd.grad(out, leaves, cotangent)
+        assert [g.stride() for g in grads] == [torch.empty_like(t).stride() for t in leaves]
+        return (out.detach(), *grads)
+
+    both(lambda: run(cotangent))
+    both(lambda: run(cotangent[:, :, :1].expand(2, 4, 40, 64)))
+    both(lambda: run(cotangent[..., :1].expand(2, 4, 40, 64)))  # not dense
+    assert _lib.load_fast().window_attention_recorded(*_leaves(dtype), 0.125, 9, 2, n) is not None
+
+
+def test_what_is_recorded():
+    fast = _lib.load_fast()
+    q, k, v = _leaves()
+    rest = (0.125, None, 0, None)
+    plain = [t.detach() for t in (q, k, v)]
+    assert fast.window_attention_recorded(*plain, *rest) is None
+    assert fast.window_attention_recorded(q.float(), k, v, *rest) is None
+    with torch.no_grad():
+        assert fast.window_attention_recorded(q, k, v, *rest) is None
+    # a gradient of one operand, twice from one graph, and added up
+    out = fast.window_attention_recorded(*plain[:2], v, *rest)
+    assert out.requires_grad and out.grad_fn is not None
+    (dv,) = torch.autograd.grad(out.sum(), v, retain_graph=True)
+    out.sum().backward()
+    assert torch.equal(v.grad, dv) and q.grad is None
+    with pytest.raises(RuntimeError, match="second time"):
+        out.sum().backward()
+    # once differentiable
+    out = fast.window_attention_recorded(q, k, v, *rest)
+    (dq,) = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dq.float().sum().backward()
+    # what it needs was written to
+    x = q * 1
+    out = fast.window_attention_recorded(x, k, v, *rest)
+    x.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+
+
+def test_gradients_on_another_stream():
+    want = None
+    for stream in (None, torch.cuda.Stream()):
+        leaves = _leaves(length=300)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            out = mlx_amd.window_attention(*leaves, scale=0.125)
+            grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+        torch.cuda.synchronize()
+        want = grads if want is None else want
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
