@@ -748,7 +748,7 @@ int mlxrocm_switch_glu(
  * negative positions -- a sequence with fewer than Lq tokens, padded in front -- see nothing and
  * give zeros.  Hq query heads share Hkv key heads, Hq / Hkv in a row each.  D: a multiple of 8 up
  * to 256.  Scores, sums and results are formed in 32 bits; with 16-bit types the probabilities are
- * rounded to the type for their product with v.  What a row does not see does not reach it,
+ * rounded to the type for their product with v (to the sum of two such numbers where rows are few).  What a row does not see does not reach it,
  * whatever it holds (infinities and NaN too).
  *
  * lengths: [B] on the device, clamped to 0 .. most keys.  strides: host array, in elements, three

@@ -256,6 +256,18 @@ __device__ __forceinline__ Frag<T> frag_of(const float* p) {
   return f;
 }
 
+// What rounding to frag_of's 16-bit operand took from 8 values
+template <typename T>
+__device__ __forceinline__ Frag<T> rest_of(const float* p, const Frag<T>& rounded) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t bits = static_cast<uint16_t>(rounded.w[i / 2] >> 16 * (i % 2));
+    rest[i] = p[i] - to_f32(__builtin_bit_cast(T, bits));
+  }
+  return frag_of<T>(rest);
+}
+
 // 4 values to consecutive elements (aligned to all of them)
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const floatx4& v) {

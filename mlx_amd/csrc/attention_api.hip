@@ -241,7 +241,7 @@ AttentionArgs shape_of(
 
 // Whether the gradients get what rounding took from a 16-bit result: its share in delta is that of a
 // mean over the keys that a token sees, and matters where those are few.  Errors of dq in their own
-// rounding's, with / without it (1.42 with delta exact): 23 tokens 1.49 / 1.58, 235 1.44 / 1.51, 1500
+// rounding's, with / without it (1.42 with delta exact): 23 tokens 1.43 / 1.58, 235 1.42 / 1.51, 1500
 // without it 1.46.  8192 tokens, 32 heads of 128, forward and gradients 2.62 / 2.60 ms.
 bool keeps_low(const AttentionArgs& a, int dtype) {
   return dtype != MLXROCM_FLOAT32 &&
