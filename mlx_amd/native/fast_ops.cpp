@@ -13,7 +13,7 @@
 // A function returns None -- and ops.py goes on with its own body -- for
 // everything that is not the plain case: another device than the current one,
 // operands to be converted, expanded or made contiguous, a gradient to be
-// recorded, a shape or an option that ops.py refuses, and any status other than
+// recorded (but for attention), a shape or an option that ops.py refuses, and any status other than
 // MLXROCM_OK (ops.py then makes the same call and turns it into an exception).
 // So the rules and messages stay in one place; here are only the conditions
 // under which nothing of them applies.
