@@ -399,7 +399,7 @@ template <typename T, int DT, int NT>
 int launch_few_rows(const AttentionArgs& a, hipStream_t s) {
   MLXROCM_REHEARSE("attention_few(dim=%d,rows=%d,splits=%d)", DT, 16 * NT, a.splits);
   const int blocks = (a.G * a.Lq + 16 * NT - 1) / (16 * NT);
-  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits);
+  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits, false);
   if (a.table != nullptr) {
     attention_few_kernel<T, DT, NT, true><<<grid.blocks(), 256, 0, s>>>(a, grid, blocks);
   } else {

@@ -726,12 +726,13 @@ int launch_grad_of(const AttentionGradArgs& g, hipStream_t s) {
       (static_cast<int64_t>(a.G) * a.Lq + kRowsBlock - 1) / kRowsBlock);
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
   if (rows > 0) {
-    const Grid grid(heads, static_cast<int64_t>(rows) * g.plan.dq_splits.d);
+    const Grid grid(
+        heads, static_cast<int64_t>(rows) * g.plan.dq_splits.d, DT * sizeof(T) <= kPairBytes);
     attention_dq_kernel<T, DT><<<grid.blocks(), 256, 0, s>>>(g, grid, rows);
     MLXROCM_HIP_TRY(hipGetLastError());
   }
   if (g.plan.blocks > 0) {
-    const Grid grid(heads, g.plan.pieces());
+    const Grid grid(heads, g.plan.pieces(), DT * sizeof(T) <= kPairBytes);
     attention_dkv_kernel<T, DT><<<grid.blocks(), 256, 0, s>>>(g, grid);
     MLXROCM_HIP_TRY(hipGetLastError());
   }

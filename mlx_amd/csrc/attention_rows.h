@@ -376,7 +376,8 @@ template <typename T, int DT>
 int launch_rows_of(const AttentionArgs& a, hipStream_t s) {
   const int64_t blocks = (static_cast<int64_t>(a.G) * a.Lq + kRowsBlock - 1) / kRowsBlock;
   MLXROCM_REHEARSE("attention_rows(dim=%d,splits=%d)", DT, a.splits);
-  const Grid grid(static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits);
+  const Grid grid(
+      static_cast<int64_t>(a.B) * a.Hkv, blocks * a.splits, DT * sizeof(T) <= kPairBytes);
   if (a.table != nullptr) {
     attention_rows_kernel<T, DT, true>
         <<<grid.blocks(), 256, 0, s>>>(a, grid, static_cast<int>(blocks));
