@@ -41,10 +41,14 @@ struct FewWork {
 // 512 tokens (512 x 256) 15.5 / 21.5; 8 key heads of 128 for 32, 128 tokens (256 x 64) 6.9 / 10.0;
 // 64 rows each over 4096 keys (32 x 4096) 15.7 / 16.9; 36 rows for 32 key heads over 8192
 // (96 x 8192) 51 / 32; 16 heads of 64, 2048 tokens (1024 x 1024) 54 / 37; 16 heads of 64, 8 times
-// 512 tokens under a window of 64 (2048 x 96) 26 / 14.
+// 512 tokens under a window of 64 (2048 x 96) 26 / 14.  Of 96 columns, whose lines the tiles pad to
+// 128, more: 12 heads on 4, twice 400 tokens (608 x 200) 11.8 / 18.6, 16 heads, twice 330 (672 x 165)
+// 12.9 / 18.1; but 16 heads of 64, 4 times 330 (704 x 165) 15.9 / 12.8, of 128, 4 times 160 (640 x 80)
+// 14.5 / 10.7.
 bool few(const AttentionArgs& a, int dtype) {
   const FewWork w(a, dtype);
-  return w.rows <= w.each || (w.blocks <= 512 && w.blocks * w.keys <= 1 << 17);
+  const int64_t most = a.D == 96 && dtype != MLXROCM_FLOAT32 ? 768 : 512;
+  return w.rows <= w.each || (w.blocks <= most && w.blocks * w.keys <= 1 << 17);
 }
 
 // Runs that the keys of a row are cut into.  Few rows, by runs, us (16-bit, 8 or 64 key heads of
