@@ -101,6 +101,8 @@ size_t workspace_of(const AttentionArgs& a, int dtype) {
 // 64 heads of 128 on 8, 500 tokens 104 (512), 126, 163; 28 on 4, 2 times 1000 tokens 182, 144, 166,
 // 188; 32 on 8, 4096 tokens under a window of 256 with 4 kept 282, 257, 270, 289, with none 217, 230,
 // 189, 225; 12 heads of 96 on 4, 1500 tokens under a window of 128 85 (rows cut in two), 122 (not).
+// Up to a workgroup for each CU parts of 64 are enough: 16 heads of 128 on 4, 300 tokens 55 (128: 58,
+// 256: 61, 512: 91), 8 of 256 on one, 500 73 (75, 97, 128), float32, 32 of 128 on 8, 150 77 (104).
 GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   GradPlan p{};
   const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;
@@ -113,9 +115,10 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
   const auto parts = [&](int64_t blocks, int64_t length) {
     const int64_t whole = std::max<int64_t>(blocks * heads_of(a), 1);
-    const int64_t wanted = (fill + whole - 1) / whole;
-    return static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({wanted, length / least, int64_t{kMostSplits}})));
+    const int64_t wanted = std::max<int64_t>(
+        std::min<int64_t>((fill + whole - 1) / whole, length / least),
+        std::min<int64_t>((256 + whole - 1) / whole, length / 64));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, kMostSplits)));
   };
   p.dq_splits = Divisor(row_blocks > 0 ? parts(row_blocks, span) : 1);
   const int64_t seen_by = std::min<int64_t>(a.Lq, reach) * a.G;

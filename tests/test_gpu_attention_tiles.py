@@ -84,10 +84,10 @@ def test_what_is_not_seen_does_not_reach_a_row(gpu, Lq, D, value, dtype):
 @pytest.mark.parametrize("keep", (5, 130))
 def test_gradients_of_kept_keys(gpu, keep, dtype):
     """Keys that all rows see, whose sums are cut, beside keys whose are not."""
-    B, Hq, Hkv, D, L, window = 2, 2, 1, 72, 1500, 64
+    B, Hq, Hkv, D, L, window = 2, 22, 11, 72, 1500, 64
     if dtype == F32:
         window = 40  # (168 rows of two heads: not cut either)
-        Hq = 1
+        Hq = 11
     rc, plan = _lib.attention_vjp_plan(B, Hq, Hkv, L, L, D, window, keep, ops._DTYPE_CODE[dtype])
     assert rc == 0 and "attention_dkv(dim=96,splits=1,kept=" in plan and plan.endswith("+attention_sum")
     q, k, v, do = tensors(B, Hq, Hkv, D, L, L, dtype, gpu, seed=6, grad=True)
