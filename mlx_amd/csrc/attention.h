@@ -441,6 +441,11 @@ struct Seen {
   }
 };
 
+// The bits below x
+__device__ __forceinline__ uint32_t bits_below(int x) {
+  return x >= 32 ? ~0u : (1u << max(x, 0)) - 1;
+}
+
 // Offsets of key j's row in k and in v: through the page table, whose entries are clamped to
 // pages that exist, or along contiguous keys.
 struct KeyRow {

@@ -239,12 +239,10 @@ constexpr int kKeysBlock = kGradBlock;
 // What a row's probabilities need beside q: its sum, its delta and its position.
 struct RowStats {
   float lse, delta;
-  int p;
 };
 template <int N>
 struct StatsTile {
   float lse[N], delta[N];
-  int p[N];
 };
 
 // Fetches tiles of rows of q and dout to LDS (see KeyStream).  Where a power of two of heads
@@ -393,6 +391,13 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
   const int w1 = min(w0 + 32, k1); // the wave's keys [w0, w1)
   const bool works = w0 < w1;
   const int key = w0 + (lane & 31);
+  // The rows that see this lane's key are [see_from, see_to): the tokens from its own on, as long as
+  // it is in their windows
+  const int64_t left = static_cast<int64_t>(key) + a.window - p0;
+  const int see_from = min(max(key - p0, 0), a.Lq) * a.G;
+  const int see_to = key >= k1      ? 0
+      : key < a.keep || left > a.Lq ? a.Lq * a.G
+                                    : max(static_cast<int>(left), 0) * a.G;
   const KeyRow at = key_row<false>(a, b, hk, min(key, max(length, 1) - 1));
   const T* k_src = static_cast<const T*>(a.k) + at.k;
   const T* v_src = static_cast<const T*>(a.v) + at.v;
@@ -444,7 +449,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     const int r = min(begin_row + t * RT + static_cast<int>(threadIdx.x), end_row - 1);
     const int i = a.of_G.divide(r);
     const int64_t n = (static_cast<int64_t>(b) * a.Hq + hk * a.G + r - i * a.G) * a.Lq + i;
-    return RowStats{a.lse[n], ga.delta[n], p0 + i};
+    return RowStats{a.lse[n], ga.delta[n]};
   };
 
   RowStream<T, DT, RT> rows(ga, b, hk, begin_row, end_row, wave, lane);
@@ -468,7 +473,6 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     if (threadIdx.x < RT) {
       st.lse[threadIdx.x] = mine.lse;
       st.delta[threadIdx.x] = mine.delta;
-      st.p[threadIdx.x] = mine.p;
     }
     __syncthreads();
     const T* q_tile = lds + (t & 1) * kBoth;
@@ -479,8 +483,8 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     if (t + 1 < tiles && threadIdx.x < RT) {
       mine = stats_of(t + 1);
     }
-    const int p_lo = __builtin_amdgcn_readfirstlane(st.p[0]);
-    const int p_hi = __builtin_amdgcn_readfirstlane(st.p[count - 1]);
+    const int p_lo = p0 + a.of_G.divide(begin);
+    const int p_hi = p0 + a.of_G.divide(begin + count - 1);
     // (as in attention_dq_kernel)
     const bool apart =
         !(count == RT && all_seen(k0, k1, p_lo, p_hi, a.window, a.keep)) &&
@@ -502,7 +506,7 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       constexpr int kHalves = RT / 32;
       constexpr int kSteps = DT / 16; // matrix instructions of a product
       floatx16 e[kHalves], dp[kHalves]; // scores, probabilities, and their gradients at last
-      uint32_t sees[kHalves];           // of 16 rows
+      uint32_t sees[kHalves];           // of 32 rows, this lane's from 4 h on
       const auto product = [&](const auto& read, const auto& use, const auto& beside) {
         read_ahead<T, kSteps>(read, [&](int n, const Frag<T>& f) {
           use(n, f);
@@ -593,19 +597,16 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
           asm volatile(""); // a branch, not 16 selections for every tile
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            e[g][i] = (sees[g] >> i & 1) != 0 ? e[g][i] : 0.0f;
+            e[g][i] = (sees[g] >> (8 * (i / 4) + i % 4) & 1) != 0 ? e[g][i] : 0.0f;
           }
         }
       };
       if (!whole) {
 #pragma unroll
         for (int g = 0; g < kHalves; ++g) {
-          sees[g] = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int n = 32 * g + 8 * (i / 4) + 4 * h + i % 4;
-            sees[g] |= (n < count && key < k1 && sees_key(a, st.p[n], key) ? 1u : 0u) << i;
-          }
+          sees[g] = (bits_below(min(see_to, end_row) - begin - 32 * g) &
+                     ~bits_below(see_from - begin - 32 * g)) >>
+              4 * h;
         }
       }
       if constexpr (kHalves == 2) {
