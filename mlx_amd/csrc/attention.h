@@ -446,6 +446,15 @@ __device__ __forceinline__ uint32_t bits_below(int x) {
   return x >= 32 ? ~0u : (1u << max(x, 0)) - 1;
 }
 
+// The same of keys first .. first + 31 of a tile, a bit each
+__device__ __forceinline__ uint32_t seen_bits(
+    const AttentionArgs& a, const KeyTile& t, int p, int first) {
+  const int begin = t.begin + first;
+  const int low = t.low - begin, to = min(p + 1, t.end) - begin;
+  return (bits_below(to) & ~bits_below(max(low, p - a.window + 1 - begin))) |
+      (bits_below(min(a.keep - begin, to)) & ~bits_below(low));
+}
+
 // Offsets of key j's row in k and in v: through the page table, whose entries are clamped to
 // pages that exist, or along contiguous keys.
 struct KeyRow {

@@ -156,7 +156,6 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
     const T* cols = apart ? next : k_tile;
     if (works && !none_seen(tile.begin, tile.end, p_lo, p_hi, a.window, a.keep)) {
       const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
-      const Seen sees(a, tile, p, 4 * h);
 #pragma unroll
       for (int g = 0; g < KT / 32; ++g) {
         floatx16 s = {}, dp = {};
@@ -176,9 +175,11 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
           ds[i] = e * (dp[i] - delta);
         }
         if (!whole) {
+          asm volatile(""); // a branch, not 16 selections for every tile
+          const uint32_t sees = seen_bits(a, tile, p, 32 * g) >> 4 * h;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            ds[i] = sees(32 * g + 8 * (i / 4) + i % 4) ? ds[i] : 0.0f;
+            ds[i] = (sees >> (8 * (i / 4) + i % 4) & 1) != 0 ? ds[i] : 0.0f;
           }
         }
         const Frag<T> w[2] = {frag_of<T>(ds), frag_of<T>(ds + 8)};

@@ -250,12 +250,12 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         });
     const bool whole = whole_tile(a, tile, KT, p_lo, p_hi);
     if (!whole) {
-      const Seen sees(a, tile, p, 4 * h);
 #pragma unroll
       for (int g = 0; g < KT / 32; ++g) {
+        const uint32_t sees = seen_bits(a, tile, p, 32 * g) >> 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[g][i] = sees(32 * g + 8 * (i / 4) + i % 4) ? s[g][i] : -INFINITY;
+          s[g][i] = (sees >> (8 * (i / 4) + i % 4) & 1) != 0 ? s[g][i] : -INFINITY;
         }
       }
     }
