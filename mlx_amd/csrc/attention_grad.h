@@ -330,8 +330,8 @@ struct RowStream {
 // Two waves a SIMD leave 256 registers.  Both results of 128 columns take 128 of them, and keys
 // and values 64: the values stay in LDS then (read again for each tile, a quarter more
 // than is read anyway), and a tile is 32 rows, so that two workgroups fit, of whose sums and deltas
-// four are in registers at a time.  8192 tokens, 32 heads of 128, both gradients 2.06 ms; with two
-// fragments read ahead instead of four 2.08 ms.  Of 256 columns one wave a SIMD has 512 registers:
+// four are in registers at a time.  8192 tokens, 32 heads of 128, both gradients 2.05 ms; with two
+// fragments read ahead instead of four a hundredth more.  Of 256 columns one wave a SIMD has 512 registers:
 // 4096 tokens, 8 heads of 256 on 2 0.45 ms; a kernel for dk and one for dv, which make the scores
 // twice, 0.55 ms.
 template <typename T, int DT>
