@@ -650,7 +650,8 @@ __device__ __forceinline__ void wait_loads() {
 // A masked value that is not finite would reach rows that do not see it: 0 * inf.  Tiles that not
 // all rows see are looked through for such values (the exponent's bits, plus one, carry into the
 // sign's place).  Where there are any, the product takes zeros for them, and when the result
-// is stored they are added to it for the rows that do see them.  (Added twice they change nothing.)
+// is stored the rows that do see them get them (store_infinite; of keys and of the gradients' rows
+// they are added; added twice they change nothing).
 template <typename T>
 __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
   constexpr uint32_t kOne = sizeof(T) == 4           ? 0x00800000u
@@ -736,6 +737,32 @@ __device__ __forceinline__ void after_stores() {
 
 __device__ __forceinline__ bool sees_key(const AttentionArgs& a, int p, int j) {
   return j <= p && (p - j < a.window || j < a.keep);
+}
+
+// Column d of the rows lo .. hi that see a value of v which is not finite: the sum of all such values
+// that they see, whatever the products made of it (NaN, where a probability was rounded to zero).  A
+// row whose sum of probabilities is NaN stays NaN.  tile(t): a tile's keys, value(j): that of key j,
+// total(r): a row's sum, with(r, store): calls store with the place of row r's result.
+template <typename Tile, typename Value, typename Total, typename With>
+__device__ __forceinline__ void store_infinite(
+    const AttentionArgs& a, int d, int t0, int t1, const Tile& tile, const Value& value, int lo,
+    int hi, int p0, const Total& total, const With& with) {
+  for (int turn = 0; turn < 2; ++turn) { // zeros, then the sums
+    for (int t = t0; t < t1 && d < a.D; ++t) {
+      const KeyTile k = tile(t);
+      for (int j = max(k.begin, k.low); j < k.end; ++j) {
+        const float x = value(j);
+        for (int r = lo; not_finite(x) && r <= hi; ++r) {
+          if (sees_key(a, p0 + a.of_G.divide(r), j) && total(r) == total(r)) {
+            with(r, [&](auto* p) {
+              using T = std::remove_reference_t<decltype(*p)>;
+              *p = turn == 0 ? from_f32<T>(0.0f) : from_f32<T>(to_f32(*p) + x);
+            });
+          }
+        }
+      }
+    }
+  }
 }
 
 #endif // __HIPCC__

@@ -138,6 +138,8 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
   __shared__ struct { // the waves' results of 16 rows, while they are joined
     float o[4][16][DT + 4];
     float m[4][16], l[4][16];
+    float total[16 * NT];
+    int odd[4];
   } join;
 
   const int lane = threadIdx.x & 63;
@@ -196,7 +198,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       }
     }
   }
-  bool odd = false; // some value was left out of the products
+  bool odd = false; // some value is not finite
   // the next tile is on its way while one is worked on, where registers are left for it
   FewTile<T, DT> tile, next;
   const auto load = [&](int t, FewTile<T, DT>& to) {
@@ -271,7 +273,9 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         w[n][1] = rest_of<T>(e, w[n][0]);
       }
     }
-    // (rows of one position see the same keys, and those alone are loaded)
+    // (rows of one position see the same keys, and those alone are loaded, as are those of whole
+    // tiles: a value that is not finite reaches all rows, if as NaN where a probability or its second
+    // term is zero or of the other sign.  That is seen of the sums.)
     if (a.Lq > 1 && !whole) {
       uint32_t bits = 0;
 #pragma unroll
@@ -308,6 +312,19 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     }
   }
 
+  floatx4 probe = {}; // NaN if some sum is not finite
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int x = 0; x < S::kGroups * S::kE; ++x) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        probe[i] = fmaf(o[n][x / S::kE][x % S::kE][i], 0.0f, probe[i]);
+      }
+    }
+  }
+  odd = odd || !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
+
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float sum = sum_quarters(l[n]);
@@ -315,6 +332,9 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     if (g == 0) {
       join.m[wave][lane] = m[n];
       join.l[wave][lane] = sum;
+    }
+    if (n == 0) {
+      join.odd[wave] = __any(odd);
     }
 #pragma unroll
     for (int x = 0; x < S::kGroups; ++x) {
@@ -364,6 +384,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         }
       }
       if ((threadIdx.x & 15) == 0) {
+        join.total[16 * n + at] = total;
         if (a.splits > 1) {
           a.part_ml[part] = make_float2(top, seeing ? total : 0.0f);
         } else if (a.lse != nullptr) {
@@ -372,26 +393,23 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       }
     }
   }
-  if (a.Lq > 1 && any_of_block(odd)) {
+  if ((join.odd[0] | join.odd[1] | join.odd[2] | join.odd[3]) != 0) { // the same for all
     after_stores();
     const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
     const int d = threadIdx.x;
-    for (int t = t0; t < t1 && d < a.D; ++t) {
-      const KeyTile at = tile_of(range, t, KT);
-      for (int j = max(at.begin, at.low); j < at.end; ++j) {
-        const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
-        for (int r = lo; not_finite(x) && r <= hi; ++r) {
-          if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
-            continue;
-          }
+    store_infinite(
+        a, d, t0, t1, [&](int t) { return tile_of(range, t, KT); },
+        [&](int j) {
+          return to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
+        },
+        lo, hi, p0, [&](int r) { return join.total[r - r0]; },
+        [&](int r, auto store) {
           if (a.splits > 1) {
-            add_to(a.part_out + (part + r) * a.D + d, x);
+            store(a.part_out + (part + r) * a.D + d);
           } else {
-            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d, x);
+            store(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d);
           }
-        }
-      }
-    }
+        });
   }
 }
 

@@ -15,6 +15,11 @@ namespace mlxrocm {
 
 namespace {
 
+// 2^(m_s - m): not zero, so that an infinite o_s stays infinite
+__device__ __forceinline__ float weight_of(float part, float top) {
+  return part == top ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(part - top), 0x1p-126f);
+}
+
 // WIDTH lanes have the columns of a run
 template <typename T, int WIDTH, int WAVES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
@@ -55,7 +60,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const float less = top == -INFINITY ? 0.0f : top;
   // a run that saw nothing has nothing
   const bool has = !(ml.y == 0.0f);
-  const float by = !has ? 0.0f : ml.x == less ? 1.0f : __builtin_amdgcn_exp2f(ml.x - less);
+  const float by = has ? weight_of(ml.x, less) : 0.0f;
   const float total = sum_lanes(by * ml.y);
   floatx4 sum = {};
   const auto add = [&](int s, const float4& v) {
@@ -130,7 +135,7 @@ __global__ __launch_bounds__(256) void attention_join_few_kernel(const Attention
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     if (!(ml[s].y == 0.0f)) {
-      const float by = ml[s].x == less ? 1.0f : __builtin_amdgcn_exp2f(ml[s].x - less);
+      const float by = weight_of(ml[s].x, less);
       total = fmaf(by, ml[s].y, total);
       sum += by * x[s];
     }
