@@ -210,7 +210,7 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
   }
   m = -INFINITY;
   l = 0.0f;
-  bool odd = false; // some value was left out of the products
+  bool odd = false; // some value is not finite
   if (t0 < t1) {
     const int begin = tile_of(range, t0, KT).begin;
     keys.look_up(begin);
@@ -312,6 +312,20 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     l += sum;
   }
   l = sum_halves(l);
+  // In float16 a probability below 2^-25 is zero: what is not finite in a tile that all rows see may
+  // have made NaN of a sum
+  constexpr bool kProbe = std::is_same<T, f16_t>::value;
+  if constexpr (kProbe) {
+    floatx4 probe = {};
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        probe[i % 4] = fmaf(o[d][i], 0.0f, probe[i % 4]);
+      }
+    }
+    odd = odd || !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
+  }
   const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
   if (stored && a.splits > 1) {
     float* to = a.part_out + (part + row) * a.D;
@@ -350,25 +364,27 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       a.lse[n] = seeing ? m + log2f(l) : 0.0f;
     }
   }
-  if (odd) { // the same for all
+  if (kProbe ? any_of_block(odd) : odd) { // the same for all
+    float* totals = reinterpret_cast<float*>(lds); // of the rows
+    __syncthreads(); // (no tile is read any more)
+    if (h == 0) {
+      totals[32 * wave + lane] = l;
+    }
     after_stores();
     const int d = threadIdx.x;
-    for (int t = t0; t < t1 && d < a.D; ++t) {
-      const KeyTile tile = tile_of(range, t, KT);
-      for (int j = max(tile.begin, tile.low); j < tile.end; ++j) {
-        const float x = to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
-        for (int r = lo; not_finite(x) && r <= hi; ++r) {
-          if (!sees_key(a, p0 + a.of_G.divide(r), j)) {
-            continue;
-          }
+    store_infinite(
+        a, d, t0, t1, [&](int t) { return tile_of(range, t, KT); },
+        [&](int j) {
+          return to_f32(static_cast<const T*>(a.v)[key_row<PAGED>(a, b, hk, j).v + d]);
+        },
+        lo, hi, p0, [&](int r) { return totals[r - block * kRowsBlock]; },
+        [&](int r, auto store) {
           if (a.splits > 1) {
-            add_to(a.part_out + (part + r) * a.D + d, x);
+            store(a.part_out + (part + r) * a.D + d);
           } else {
-            add_to(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d, x);
+            store(static_cast<T*>(a.out) + row_offset(a.out_strides, b, hk, a.of_G, r) + d);
           }
-        }
-      }
-    }
+        });
   }
 }
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import mlx_amd
+from mlx_amd import _lib, ops
 from tests.attention_util import pages_of, tensors, visible
 from tests.test_gpu_attention import BF16, F16, F32
 
@@ -69,3 +70,23 @@ def test_a_row_without_a_sum_stays_so(gpu, Lq, dtype):
         assert torch.isnan(out[0, 1, -1]).all()
         assert (out[0, 2:, -1, 7] == math.inf).all()
         assert torch.isfinite(out[0, 2:, -1, :7].float()).all()
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16))
+@pytest.mark.parametrize("Lq, Lk, window, D", (
+    (200, 500, None, 128), (200, 333, 100, 64), (150, 400, 30, 96), (130, 300, 250, 256)))
+def test_many_rows(gpu, Lq, Lk, window, D, dtype):
+    """Enough key heads for the kernel of tiles; keys inside tiles that all rows see, at their ends
+    and before every window.  The keys before 100 are given scores some 20 to 30 below the others',
+    whose probabilities round to zero in float16."""
+    heads = next(n for n in (8, 64, 512) if _lib.attention_plan(
+        2, n, n, Lq, Lk, D, window or 1 << 30, 0, ops._DTYPE_CODE[dtype])[1].startswith("attention_rows"))
+    q, k, v = tensors(2, heads, heads, D, Lq, Lk, dtype, gpu, seed=D + Lk)
+    q[..., 0] = 5
+    k[..., 0] = 5
+    k[:, :, :100, 0] = -45
+    first, last = Lk - window if window else 0, Lk - 1
+    places = [(last, 1, math.inf), (first, 2, -math.inf), (last, D - 1, -math.inf),
+              (first, D - 1, math.inf), (20, 33, -math.inf), (Lk - Lq - 1, 34, math.inf),
+              (Lk - Lq // 2, 35, math.inf), (99, 36, -math.inf), (last - 64, 40, math.nan)]
+    check(q, k, v, [Lk, Lk - 7], window, places)
