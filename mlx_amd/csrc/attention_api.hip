@@ -274,6 +274,11 @@ bool empty(const AttentionArgs& a) {
   return a.B == 0 || a.Hq == 0 || a.Lq == 0;
 }
 
+// (keys and values that no query reads have gradients of zero)
+bool no_gradients(const AttentionArgs& a) {
+  return empty(a) && (a.B == 0 || a.Hkv == 0 || a.keys == 0);
+}
+
 int run(const char* name, AttentionArgs& a, int dtype, void* workspace, size_t bytes,
         hipStream_t s) {
   a.splits = splits_of(a, dtype);
@@ -428,7 +433,7 @@ extern "C" int mlxrocm_window_attention_vjp(
   AttentionArgs& a = g.a;
   a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
   TRY(check_shape(name, a, dtype));
-  if (B == 0 || Hq == 0 || (Lq == 0 && Lk == 0)) {
+  if (no_gradients(a)) {
     return MLXROCM_OK;
   }
   if (!std::isfinite(scale) || strides == nullptr) {
@@ -454,7 +459,7 @@ extern "C" int mlxrocm_window_attention_vjp(
   take(g.dq_strides, strides + 15);
   take(g.dk_strides, strides + 18);
   take(g.dv_strides, strides + 21);
-  if (Lq > 0) {
+  if (!empty(a)) {
     TRY(check_operand(name, "q", q, a.q_strides, dtype));
     TRY(check_operand(name, "out", out, a.out_strides, dtype));
     TRY(check_operand(name, "dout", dout, g.dout_strides, dtype));
@@ -487,7 +492,7 @@ extern "C" int mlxrocm_window_attention_vjp(
   }
   set_scale(a, scale, dtype);
   set_near(a, dtype);
-  if ((a.G & (a.G - 1)) == 0 && a.G <= 32 && near(a.q_strides, dtype, a.G) &&
+  if (a.G > 0 && (a.G & (a.G - 1)) == 0 && a.G <= 32 && near(a.q_strides, dtype, a.G) &&
       near(g.dout_strides, dtype, a.G)) {
     a.near |= 2;
     a.g_log2 = __builtin_ctz(a.G);
@@ -617,6 +622,5 @@ extern "C" int mlxrocm_window_attention_vjp_plan(
   g.a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
   TRY(check_shape("window_attention_vjp_plan", g.a, dtype));
   g.plan = grad_plan_of(g.a, dtype);
-  return B == 0 || Hq == 0 || (Lq == 0 && Lk == 0) ? static_cast<int>(MLXROCM_OK)
-                                                   : run_grad(g, dtype, nullptr);
+  return no_gradients(g.a) ? static_cast<int>(MLXROCM_OK) : run_grad(g, dtype, nullptr);
 }
