@@ -113,26 +113,27 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   const int64_t fill = a.D * dtype_size(dtype) <= 256 ? 1024 : 512;
   const int64_t reach = static_cast<int64_t>(a.window) + kGradBlock; // tokens
   const int64_t span = std::min<int64_t>(a.keys, reach + a.keep);
-  const auto parts = [&](int64_t blocks, int64_t length) {
+  const auto parts = [&](int64_t blocks, int64_t of_least, int64_t of_64) {
     const int64_t whole = std::max<int64_t>(blocks * heads_of(a), 1);
     const int64_t wanted = std::max<int64_t>(
-        std::min<int64_t>((fill + whole - 1) / whole, length / least),
-        std::min<int64_t>((256 + whole - 1) / whole, length / 64));
+        std::min<int64_t>((fill + whole - 1) / whole, of_least),
+        std::min<int64_t>((256 + whole - 1) / whole, of_64));
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(wanted, kMostSplits)));
   };
-  p.dq_splits = Divisor(row_blocks > 0 ? parts(row_blocks, span) : 1);
+  p.dq_splits = Divisor(row_blocks > 0 ? parts(row_blocks, span / least, span / 64) : 1);
   const int64_t seen_by = std::min<int64_t>(a.Lq, reach) * a.G;
   if (a.window < a.keys && seen_by < rows) {
     p.wide_blocks = static_cast<int>(std::min<int64_t>(
         p.blocks, (static_cast<int64_t>(a.keep) + kGradBlock - 1) / kGradBlock));
   }
-  const int splits = p.blocks > 0 ? parts(p.blocks, seen_by + least / 2) : 1;
+  const int splits =
+      p.blocks > 0 ? parts(p.blocks, (seen_by + least / 2) / least, (seen_by + 63) / 64) : 1;
   p.splits = Divisor(splits);
   // runs no longer than the others'
   p.wide_splits = Divisor(
       p.wide_blocks == 0 ? splits
                          : std::min<int64_t>(
-                               kMostSplits,
+                               std::min<int64_t>(kMostSplits, (rows + 63) / 64),
                                std::max<int64_t>(1, rows * splits / std::max<int64_t>(seen_by, 1))));
   return p;
 }

@@ -19,3 +19,27 @@ def test_gradients_without_query_heads_are_written(dtype):
     assert "attention_dkv" in vjp_plan(1, 0, 4, 100, 100, 64, dtype=dtype)
     assert vjp_plan(1, 0, 0, 100, 100, 64, dtype=dtype) == ""
     assert vjp_plan(0, 4, 4, 100, 100, 64, dtype=dtype) == ""
+
+
+def cuts(*args, **kw):
+    """(runs of dq, runs of dk and dv, blocks of kept keys, their runs)"""
+    plan = vjp_plan(*args, **kw)
+    return tuple(int(x) for x in re.search(
+        r"attention_dq\(dim=\d+,splits=(\d+)\)\+attention_dkv\(dim=\d+,splits=(\d+),kept=(\d+)x(\d+)\)",
+        plan).groups())
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16))
+def test_no_more_runs_than_there_are_tiles(dtype):
+    # one tile of rows and of keys: one run, and nothing to sum
+    for args in ((1, 4, 4, 1, 1, 64), (1, 32, 32, 16, 16, 128), (2, 8, 4, 7, 90, 256)):
+        assert vjp_plan(*args, dtype=dtype).endswith("splits=1,kept=0x1)"), args
+    # 64 rows or keys a run, the last one's excepted: a tile, or two of 32
+    for args in ((1, 16, 16, 128, 128, 64), (1, 4, 1, 100, 100, 128), (1, 1, 1, 1000, 1000, 96),
+                 (1, 8, 2, 3000, 3000, 64), (1, 2, 2, 200, 5000, 128)):
+        for window, keep in ((1 << 30, 0), (64, 0), (200, 40)):
+            dq, dkv, blocks, kept = cuts(*args, window=window, keep=keep, dtype=dtype)
+            rows = args[1] // args[2] * args[3]
+            assert dq == 1 or 64 * dq <= min(args[4], window + keep + 128)
+            assert dkv == 1 or 64 * (dkv - 1) < min(rows, (window + 128) * args[1] // args[2])
+            assert kept == 1 or 64 * (kept - 1) < rows
