@@ -129,12 +129,17 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   const int splits =
       p.blocks > 0 ? parts(p.blocks, (seen_by + least / 2) / least, (seen_by + 63) / 64) : 1;
   p.splits = Divisor(splits);
-  // runs no longer than the others'
-  p.wide_splits = Divisor(
-      p.wide_blocks == 0 ? splits
-                         : std::min<int64_t>(
-                               std::min<int64_t>(kMostSplits, (rows + 63) / 64),
-                               std::max<int64_t>(1, rows * splits / std::max<int64_t>(seen_by, 1))));
+  // Runs no longer than the others', but no more workgroups than fill the card: each keeps 128 keys' sums
+  // in float32.  us of both gradients, bfloat16, 8192 tokens, with as many as fill it / as would be no
+  // longer: 32 heads on 8 under a window of 64, all kept 2080 / 3530 (4.3 GB), 8 times that with 4096 kept
+  // 13350 / 16540 (11.3 GB); 8 heads of 256 on 2, 4096 tokens, 1000 kept 333 / 390.
+  int64_t wide = splits;
+  if (p.wide_blocks > 0) {
+    const int64_t whole = p.wide_blocks * heads_of(a);
+    wide = std::min<int64_t>(rows * splits / std::max<int64_t>(seen_by, 1), (fill + whole - 1) / whole);
+    wide = std::max<int64_t>(1, std::min<int64_t>({wide, (rows + 63) / 64, kMostSplits}));
+  }
+  p.wide_splits = Divisor(wide);
   return p;
 }
 

@@ -43,3 +43,19 @@ def test_no_more_runs_than_there_are_tiles(dtype):
             assert dq == 1 or 64 * dq <= min(args[4], window + keep + 128)
             assert dkv == 1 or 64 * (dkv - 1) < min(rows, (window + 128) * args[1] // args[2])
             assert kept == 1 or 64 * (kept - 1) < rows
+
+
+@pytest.mark.parametrize("B, Hq, Hkv, D, L, window, keep, dtype", (
+    (1, 32, 8, 128, 8192, 64, 8192, BF16), (8, 32, 8, 128, 8192, 64, 4096, BF16),
+    (8, 32, 32, 128, 8192, 128, 2048, BF16), (1, 32, 32, 128, 32768, 1024, 16384, F16),
+    (4, 16, 16, 256, 4096, 100, 1000, F32), (1, 8, 1, 64, 20000, 256, 9000, BF16),
+    (1, 64, 8, 128, 4096, 256, 4, BF16), (2, 28, 4, 128, 3000, 1 << 30, 0, F16)))
+def test_the_sums_parts_are_bounded(B, Hq, Hkv, D, L, window, keep, dtype):
+    """Parts are made for workgroups that fill the card, so there are at most as many as it takes
+    twice over (1024 workgroups, each with the sums of 128 keys or rows, where there are parts)."""
+    size = _lib.load().mlxrocm_window_attention_vjp_workspace_size(
+        B, Hq, Hkv, L, L, D, window, keep, dtype)
+    delta = 4 * B * Hq * L + 256
+    of_keys, of_rows = 2 * 1024 * 128 * 2 * D * 4, 2 * 1024 * 128 * D * 4
+    # (and the blocks of keys that are not kept have theirs)
+    assert size <= delta + 2 * of_keys + of_rows
