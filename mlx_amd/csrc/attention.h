@@ -107,6 +107,7 @@ struct AttentionGradArgs {
   void* dk;
   void* dv;
   float* delta; // [B, Hq, Lq]: sum over D of dout * out
+  float* largest; // float16: [B Hkv, splits of dq, 32 rows] of the probabilities' gradients
   int64_t dout_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
   float scale;
   GradPlan plan;

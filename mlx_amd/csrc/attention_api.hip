@@ -143,12 +143,18 @@ GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   return p;
 }
 
-// delta, then the partial sums of dq, then those of dk and dv
+// delta, in float16 the largest gradients of probabilities, then the partial sums of dq, then those of
+// dk and dv
 struct GradWorkspace {
-  size_t part_dq, part_dkv, total;
-  GradWorkspace(const AttentionArgs& a, const GradPlan& p) {
+  size_t largest, part_dq, part_dkv, total;
+  GradWorkspace(const AttentionArgs& a, const GradPlan& p, int dtype) {
     const size_t rows = static_cast<size_t>(a.B) * a.Hq * a.Lq;
-    part_dq = round256(rows * sizeof(float));
+    const size_t blocks = (static_cast<size_t>(a.G) * a.Lq + kGradBlock - 1) / kGradBlock;
+    largest = round256(rows * sizeof(float));
+    part_dq = largest +
+        (dtype == MLXROCM_FLOAT16
+             ? round256(heads_of(a) * p.dq_splits.d * blocks * (kGradBlock / 32) * sizeof(float))
+             : 0);
     part_dkv = part_dq +
         (p.dq_splits.d > 1 ? round256(rows * a.D * p.dq_splits.d * sizeof(float)) : 0);
     total = part_dkv +
@@ -404,7 +410,7 @@ extern "C" size_t mlxrocm_window_attention_vjp_workspace_size(
   const AttentionArgs a = shape_of(B, Hq, Hkv, Lq, Lk, D, window, keep);
   return check_shape("window_attention_vjp", a, dtype) != MLXROCM_OK
       ? 0
-      : GradWorkspace(a, grad_plan_of(a, dtype)).total;
+      : GradWorkspace(a, grad_plan_of(a, dtype), dtype).total;
 }
 
 extern "C" int mlxrocm_window_attention_vjp(
@@ -475,7 +481,7 @@ extern "C" int mlxrocm_window_attention_vjp(
     }
   }
   g.plan = grad_plan_of(a, dtype);
-  const GradWorkspace parts(a, g.plan);
+  const GradWorkspace parts(a, g.plan, dtype);
   if (parts.total > 0) {
     if (workspace == nullptr || workspace_bytes < parts.total) {
       return fail(
@@ -487,6 +493,7 @@ extern "C" int mlxrocm_window_attention_vjp(
     }
     char* at = static_cast<char*>(workspace);
     g.delta = static_cast<float*>(workspace);
+    g.largest = reinterpret_cast<float*>(at + parts.largest);
     g.part_dq = reinterpret_cast<float*>(at + parts.part_dq);
     g.part_dkv = reinterpret_cast<float*>(at + parts.part_dkv);
   }

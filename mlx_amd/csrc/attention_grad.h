@@ -37,6 +37,53 @@ __device__ __forceinline__ void store_part(
   }
 }
 
+// Float16 has five bits of exponent: as an operand the probabilities of many keys, and more so their
+// gradients beside a small dout, would lose bits or be zero, those beside a large one infinite (2048
+// tokens, 128 columns, dout of 1e-4: dq three times as far off as its own rounding, now as far).  So
+// probabilities count 2^kProbabilityUp times.  Their gradients, and so the sums, count 2^up times: of
+// dq for each row, a number that only falls, to where the largest is some 2^kRangeFirst once one is
+// above 2^kRangeMost; of dk for all of a workgroup, by the largest ones of its rows, which dq's kernel
+// leaves behind.  (The sums of dk and dv take all registers: to multiply them on the way, 256 columns,
+// took 530 us instead of 240.)
+template <typename T>
+constexpr bool kRanged = std::is_same<T, f16_t>::value;
+constexpr int kProbabilityUp = 14;
+constexpr int kRangeStart = 64; // (a gradient below 2^-49 is nothing in the results)
+constexpr int kRangeFirst = 9;
+constexpr int kRangeMost = 15;
+
+__device__ __forceinline__ int exponent_of(float x) { // of x > 0
+  return static_cast<int>(__float_as_uint(x) >> 23) - 127;
+}
+
+// A row's 16 gradients, which count 2^up times, as do the largest so far and the sums that have them
+template <int STEPS>
+__device__ __forceinline__ void
+fit_range(float (&ds)[16], int& up, float& largest, floatx16 (&sums)[STEPS]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    top = fmaxf(top, fabsf(ds[i]));
+  }
+  top = max_halves(top);
+  largest = fmaxf(largest, top);
+  constexpr float kMost = 1 << kRangeMost;
+  if (__any(top > kMost)) {
+    const int by = top > kMost ? kRangeFirst - exponent_of(top) : 0;
+    up += by;
+    const float times = ldexpf(1.0f, by);
+    largest *= times;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      ds[i] *= times;
+    }
+#pragma unroll
+    for (int d = 0; d < STEPS; ++d) {
+      sums[d] *= times;
+    }
+  }
+}
+
 // ---- dq: workgroups of 128 rows, as the forward -----------------------------------------
 template <typename T, int DT>
 __global__ __launch_bounds__(256)
@@ -86,6 +133,8 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
 
   Frag<T> q[DT / 16], dout[DT / 16];
   float lse = 0.0f, delta = 0.0f;
+  int up = kRanged<T> ? kRangeStart : 0;
+  float largest = 0.0f;
   if (any) {
     const T* src = static_cast<const T*>(a.q) + row_offset(a.q_strides, b, hk, a.of_G, from);
     const T* dsrc = static_cast<const T*>(ga.dout) + row_offset(ga.dout_strides, b, hk, a.of_G, from);
@@ -169,9 +218,10 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
               }
             });
         float ds[16];
+        const float less = kRanged<T> ? lse - up : lse;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -lse));
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -less));
           ds[i] = e * (dp[i] - delta);
         }
         if (!whole) {
@@ -182,6 +232,9 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
             ds[i] = (sees >> (8 * (i / 4) + i % 4) & 1) != 0 ? ds[i] : 0.0f;
           }
         }
+        if constexpr (kRanged<T>) {
+          fit_range(ds, up, largest, dq);
+        }
         const Frag<T> w[2] = {frag_of<T>(ds), frag_of<T>(ds + 8)};
         read_ahead<T, DT / 16>(
             [&](int n) { return L::load_cols(cols, 32 * g + 16 * (n % 2), 32 * (n / 2), lane); },
@@ -191,6 +244,19 @@ void attention_dq_kernel(const AttentionGradArgs ga, const Grid grid, int blocks
     if (apart && t + 1 < t1) {
       __syncthreads();
       keys.fetch(tile_of(range, t + 1, KT).begin, next, next + kBoth / 2);
+    }
+  }
+  if constexpr (kRanged<T>) {
+    const float down = ldexpf(1.0f, -up);
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d) {
+      dq[d] *= down;
+    }
+    // (a row that has an infinite one has no others)
+    largest = max_lanes(not_finite(largest) ? 0.0f : largest * down);
+    if (lane == 0) {
+      ga.largest[((static_cast<int64_t>(head) * splits.d + split) * blocks + block) * 4 + wave] =
+          largest;
     }
   }
   const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
@@ -446,11 +512,37 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
       }
     }
   }
+  // 2^(up - kProbabilityUp), for gradients of at most 2^kRangeMost
+  float times = 1.0f;
+  if constexpr (kRanged<T>) {
+    __shared__ float tops[4];
+    if (any) {
+      const int waves = (a.G * a.Lq + kRowsBlock - 1) / kRowsBlock * 4; // of dq's kernel, 32 rows each
+      const int first = begin_row / 32, count = (end_row + 31) / 32 - first;
+      float top = 0.0f;
+      for (int x = 0; x < plan.dq_splits.d; ++x) {
+        const float* of = ga.largest + (static_cast<int64_t>(head) * plan.dq_splits.d + x) * waves;
+        for (int i = threadIdx.x; i < count; i += 256) {
+          top = fmaxf(top, of[first + i]);
+        }
+      }
+      top = max_lanes(top);
+      if (lane == 0) {
+        tops[wave] = top;
+      }
+      __syncthreads();
+      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      const int up = min(kRangeStart, kRangeMost - 1 - exponent_of(top));
+      times = __int_as_float(__builtin_amdgcn_readfirstlane(
+          __float_as_int(ldexpf(1.0f, up - kProbabilityUp))));
+    }
+  }
   const auto stats_of = [&](int t) {
     const int r = min(begin_row + t * RT + static_cast<int>(threadIdx.x), end_row - 1);
     const int i = a.of_G.divide(r);
     const int64_t n = (static_cast<int64_t>(b) * a.Hq + hk * a.G + r - i * a.G) * a.Lq + i;
-    return RowStats{a.lse[n], ga.delta[n]};
+    return kRanged<T> ? RowStats{a.lse[n] - kProbabilityUp, ga.delta[n] * times}
+                      : RowStats{a.lse[n], ga.delta[n]};
   };
 
   RowStream<T, DT, RT> rows(ga, b, hk, begin_row, end_row, wave, lane);
@@ -588,7 +680,8 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             if (i * kSteps / 16 == n) {
-              e[g][i] *= dp[g][i] - st.delta[32 * g + 8 * (i / 4) + 4 * h + i % 4];
+              const float delta = st.delta[32 * g + 8 * (i / 4) + 4 * h + i % 4];
+              e[g][i] *= kRanged<T> ? fmaf(dp[g][i], times, -delta) : dp[g][i] - delta;
             }
           }
         };
@@ -647,7 +740,9 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
         });
         hide(0);
         const auto probabilities = packed(0);
-        by_fours(st.delta, [&](int i, float delta) { e[0][i] *= dp[0][i] - delta; });
+        by_fours(st.delta, [&](int i, float delta) {
+          e[0][i] *= kRanged<T> ? fmaf(dp[0][i], times, -delta) : dp[0][i] - delta;
+        });
         hide(0);
         const auto d_probabilities = packed(0);
         add_packed(d_cols, 0, probabilities, dv, nothing);
@@ -657,6 +752,15 @@ void attention_dkv_kernel(const AttentionGradArgs ga, const Grid grid) {
     if (apart && t + 1 < tiles) {
       __syncthreads();
       rows.fetch(begin + RT, next, next + kBoth / 2);
+    }
+  }
+  if constexpr (kRanged<T>) {
+    constexpr float kDown = 1.0f / (1 << kProbabilityUp);
+    const float down = kDown / times;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d) {
+      dk[d] *= down;
+      dv[d] *= kDown;
     }
   }
   const bool parts = splits.d > 1;

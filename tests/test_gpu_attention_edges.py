@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import mlx_amd
-from tests.attention_util import pages_of, tensors
+from tests.attention_util import pages_of, tensors, visible
 from tests.test_gpu_attention import BF16, F16, F32
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +25,40 @@ def test_gradients_without_query_heads(gpu, Lq, Lk, D, dtype):
         torch.full((2, 3, Lk, D), math.nan, dtype=dtype, device=gpu)
     dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.zeros_like(out))
     assert dq.shape == q.shape and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize("size", (2.0 ** 11, 1.0, 1e-3, 1e-4, 1e-5))
+@pytest.mark.parametrize("L, D, window", ((2048, 128, None), (300, 64, None), (1500, 96, 200),
+                                          (700, 256, None)))
+def test_gradients_of_any_size_in_float16(gpu, L, D, window, size):
+    """In the mean as far off as with probabilities and their gradients rounded to eleven bits, the
+    results to float16 (as in test_gpu_attention_tiles.py, with its tenth more): float16's few
+    exponents may cost nothing beside.  2^11: gradients of the probabilities are beyond its range."""
+    q, k, v, do = tensors(1, 4, 2, D, L, L, F16, gpu, seed=L, grad=True)
+    do = (do.float() * size).to(F16)
+    scale = D ** -0.5 if size <= 1 else D ** -1.5
+    if size > 1:
+        v = v * 16
+    x, y, z, dout = (t.double() for t in (q, k, v, do))
+    y, z = (t.repeat_interleave(2, 1) for t in (y, z))
+
+    def eleven(t):  # bits
+        m, e = torch.frexp(t)
+        return torch.ldexp((m * 2048).round(), e - 11)
+
+    seen = visible(L, L, [L], window, 0, gpu)
+    p = torch.softmax((scale * x @ y.transpose(2, 3)).masked_fill(~seen, -math.inf), -1)
+    exact_ds = p * (dout @ z.transpose(2, 3) - (dout * (p @ z)).sum(-1, keepdim=True))
+    ds = eleven(p * (dout @ z.transpose(2, 3) - (dout * (eleven(p) @ z)).sum(-1, keepdim=True)))
+    two = lambda t: t.unflatten(1, (2, 2)).sum(2)  # noqa: E731  (heads that share one)
+    want = dict(dq=scale * exact_ds @ y, dk=two(scale * exact_ds.transpose(2, 3) @ x),
+                dv=two(p.transpose(2, 3) @ dout))
+    model = dict(dq=scale * ds @ y, dk=two(scale * ds.transpose(2, 3) @ x),
+                 dv=two(eleven(p).transpose(2, 3) @ dout))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = mlx_amd.window_attention(*leaves, scale=scale, window=window)
+    for name, t in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)):
+        off = float((t.double() - want[name]).norm())
+        by_design = float((model[name].half().double() - want[name]).norm())
+        assert by_design < math.inf
+        assert off <= 1.1 * by_design, (name, off / by_design)
