@@ -56,6 +56,11 @@ def _empty_like(t: torch.Tensor) -> torch.Tensor:
         t.shape, dtype=t.dtype, device=t.device)
 
 
+def _tangents(*tensors: torch.Tensor) -> bool:
+    """Whether forward-mode gradients are wanted of any of them."""
+    return any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _check_visible(tag: str, scale, window, keep) -> Tuple[float, int, int]:
     scale = float(scale)
     if not math.isfinite(scale):
@@ -160,7 +165,8 @@ def window_attention(
     """``softmax(scale q k^T) v`` over the tokens that each one of ``q`` sees (see the module).
     ``q`` ``[B, Hq, Lq, D]``, ``k`` and ``v`` ``[B, Hkv, Lk, D]``; ``lengths`` ``[B]``: how many of
     the ``Lk`` keys each sequence has, all without it.  The result has ``q``'s shape and, where
-    that is dense, its memory order.  Differentiable with respect to q, k and v."""
+    that is dense, its memory order.  Differentiable with respect to q, k and v (once,
+    in reverse mode)."""
     out = ops._fast.window_attention(q, k, v, scale, window, keep, lengths)
     if out is None and torch.is_grad_enabled():
         out = ops._fast.window_attention_recorded(q, k, v, scale, window, keep, lengths)
@@ -175,6 +181,8 @@ def window_attention(
     dtype = torch.promote_types(torch.promote_types(q.dtype, k.dtype), v.dtype)
     if dtype not in _FLOATING:
         raise ValueError(f"[{tag}] Received unsupported type {dtype}.")
+    if _tangents(q, k, v):
+        raise NotImplementedError(f"[{tag}] no forward-mode gradients.")
     if lengths is not None:
         _check_ints(tag, "lengths", lengths, (q.shape[0],))
         _require_gpu(tag, lengths)
@@ -248,7 +256,8 @@ def paged_cache_update(
     _check_pages(tag, k_pages, v_pages)
     if any(n > 1 and s == 0 for t in (k_pages, v_pages) for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"[{tag}] Pages that share memory (expanded ones) cannot be written to.")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_pages, v_pages)):
+    if _tangents(k, v, k_pages, v_pages) or (torch.is_grad_enabled() and any(
+            t.requires_grad for t in (k, v, k_pages, v_pages))):
         raise NotImplementedError(f"[{tag}] no gradients through a paged cache.")
     _require_gpu(tag, k, v, k_pages, v_pages, block_table, lengths)
     lib = _lib.load()
@@ -291,8 +300,8 @@ def paged_attention(
                          f"{q.dtype}, {k_pages.dtype} and {v_pages.dtype}.")
     _check_table(tag, block_table, lengths, q.shape[0])
     _check_pages(tag, k_pages, v_pages)
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad
-                                    or v_pages.requires_grad):
+    if _tangents(q, k_pages, v_pages) or (torch.is_grad_enabled() and any(
+            t.requires_grad for t in (q, k_pages, v_pages))):
         raise NotImplementedError(f"[{tag}] no gradients through a paged cache.")
     _require_gpu(tag, q, k_pages, v_pages, block_table, lengths)
     lib = _lib.load()

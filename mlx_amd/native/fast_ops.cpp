@@ -673,7 +673,7 @@ bool dense_rows(const at::Tensor& t) {
   return t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
-// Such a tensor on `device`, with no gradient to be recorded (or `recorded`).
+// Such a tensor on `device`, with no gradient to be recorded (or `recorded`) and no tangent.
 const at::Tensor* heads_of(PyObject* o, c10::DeviceIndex device, bool recorded = false) {
   if (!THPVariable_CheckExact(o)) {
     return nullptr;
@@ -681,7 +681,7 @@ const at::Tensor* heads_of(PyObject* o, c10::DeviceIndex device, bool recorded =
   const at::Tensor& t = THPVariable_Unpack(o);
   return t.defined() && t.is_cuda() && t.device().index() == device && t.dim() == 4 &&
           t.numel() != 0 && !t.is_conj() && !t.is_neg() && (recorded || !records_grad(t)) &&
-          dtype_code(t.scalar_type()) >= 0 && dense_rows(t)
+          !t._fw_grad(0).defined() && dtype_code(t.scalar_type()) >= 0 && dense_rows(t)
       ? &t
       : nullptr;
 }

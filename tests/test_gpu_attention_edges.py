@@ -62,3 +62,21 @@ def test_gradients_of_any_size_in_float16(gpu, L, D, window, size):
         by_design = float((model[name].half().double() - want[name]).norm())
         assert by_design < math.inf
         assert off <= 1.1 * by_design, (name, off / by_design)
+
+
+def test_forward_mode_is_refused(gpu):
+    from torch.autograd import forward_ad
+
+    q, k, v = tensors(2, 4, 2, 64, 3, 40, BF16, gpu)
+    k_pages, v_pages, table = pages_of(k, v, 16)
+    n = torch.tensor([40, 7], dtype=torch.int32, device=gpu)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(q), k, v), (q, dual(k), v), (q.clone().requires_grad_(), k, dual(v))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                mlx_amd.window_attention(*args, scale=0.1)
+        with pytest.raises(NotImplementedError, match="no gradients"):
+            mlx_amd.paged_attention(dual(q), k_pages, v_pages, table, n, scale=0.1)
+        with pytest.raises(NotImplementedError, match="no gradients"):
+            mlx_amd.paged_cache_update(dual(k), v, k_pages, v_pages, table, n)
+        mlx_amd.window_attention(q, k, v, scale=0.1)  # (what has no tangent is computed)
