@@ -269,6 +269,9 @@ def paged_cache_update(
         lengths.data_ptr(), B, H, L, D, k_pages.shape[0], k_pages.shape[2], table.shape[1],
         _array(_strides(k, v, k_pages, v_pages) + [table.stride(0)]), _DTYPE_CODE[k.dtype],
         _stream_ptr(k)))
+    for pages in (k_pages, v_pages):  # written to: a graph that saved them is to know
+        if not pages.is_inference():
+            torch.autograd.graph.increment_version(pages)
     return k_pages, v_pages
 
 

@@ -1070,6 +1070,11 @@ PyObject* paged_cache_update(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (rc != MLXROCM_OK) {
     NOT_PLAIN;
   }
+  for (const at::Tensor* pages : {c.k, c.v}) { // written to: a graph that saved them is to know
+    if (!pages->is_inference()) {
+      pages->unsafeGetTensorImpl()->bump_version();
+    }
+  }
   Py_RETURN_TRUE;
   FAST_CATCH
 }

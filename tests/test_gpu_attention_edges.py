@@ -80,3 +80,24 @@ def test_forward_mode_is_refused(gpu):
         with pytest.raises(NotImplementedError, match="no gradients"):
             mlx_amd.paged_cache_update(dual(k), v, k_pages, v_pages, table, n)
         mlx_amd.window_attention(q, k, v, scale=0.1)  # (what has no tangent is computed)
+
+
+def test_an_update_is_seen_by_graphs(gpu):
+    """Pages that a graph has saved have been written to when its gradients are wanted."""
+    k, v = tensors(2, 4, 2, 64, 3, 40, BF16, gpu)[1:]
+    n = torch.tensor([40, 7], dtype=torch.int32, device=gpu)
+    for make in (lambda t: t, lambda t: t.long()):  # by the native host path, and not
+        k_pages, v_pages, table = pages_of(k, v, 16)
+        x = torch.ones((), dtype=BF16, device=gpu, requires_grad=True)
+        saved = [(x * pages).sum() for pages in (k_pages, v_pages)]
+        before = [pages._version for pages in (k_pages, v_pages)]
+        mlx_amd.paged_cache_update(k, v, k_pages, v_pages, table, make(n))
+        assert [pages._version for pages in (k_pages, v_pages)] == [b + 1 for b in before]
+        for s in saved:
+            with pytest.raises(RuntimeError, match="inplace"):
+                s.backward()
+    with torch.inference_mode():
+        pages = [p.clone() for p in (k_pages, v_pages)]
+        mlx_amd.paged_cache_update(k, v, *pages, table, n)
+    mlx_amd.paged_cache_update(k, v, *pages, table, n)  # (these have no version)
+    assert torch.equal(pages[0], k_pages) and torch.equal(pages[1], v_pages)
