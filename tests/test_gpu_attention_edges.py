@@ -101,3 +101,17 @@ def test_an_update_is_seen_by_graphs(gpu):
         mlx_amd.paged_cache_update(k, v, *pages, table, n)
     mlx_amd.paged_cache_update(k, v, *pages, table, n)  # (these have no version)
     assert torch.equal(pages[0], k_pages) and torch.equal(pages[1], v_pages)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16))
+@pytest.mark.parametrize("Lq, Lk, page, window, keep, lengths", (
+    (1, 512, 16, None, 0, [512, 77]), (5, 960, 48, 300, 7, [960, 400]), (40, 2048, 128, 64, 0, [2048, 9]),
+    (300, 768, 32, None, 0, [768, 300]), (500, 1024, 64, 200, 3, [1024, 1000])))
+@pytest.mark.parametrize("D", (64, 96, 256))
+def test_pages_give_the_bits_of_contiguous_keys(gpu, Lq, Lk, page, window, keep, lengths, D, dtype):
+    """Where the table has room for these keys alone, so that both are cut alike."""
+    q, k, v = tensors(2, 8, 2, D, Lq, Lk, dtype, gpu, seed=D + Lq)
+    n = torch.tensor(lengths, dtype=torch.int32, device=gpu)
+    args = dict(scale=D ** -0.5, window=window, keep=keep)
+    out = mlx_amd.paged_attention(q, *pages_of(k, v, page, fill=math.nan), n, **args)
+    assert torch.equal(out, mlx_amd.window_attention(q, k, v, lengths=n, **args))
