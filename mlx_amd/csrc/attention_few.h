@@ -312,9 +312,10 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     }
   }
 
-  floatx4 probe = {}; // NaN if some sum is not finite
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    l[n] = sum_quarters(l[n]);
+    floatx4 probe = {}; // NaN if some sum is not finite
 #pragma unroll
     for (int x = 0; x < S::kGroups * S::kE; ++x) {
 #pragma unroll
@@ -322,16 +323,16 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         probe[i] = fmaf(o[n][x / S::kE][x % S::kE][i], 0.0f, probe[i]);
       }
     }
+    // (a row without a sum of probabilities is NaN as it is)
+    odd = odd || (l[n] == l[n] && !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f));
   }
-  odd = odd || !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
 
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float sum = sum_quarters(l[n]);
     __syncthreads(); // the tile of rows before has been joined
     if (g == 0) {
       join.m[wave][lane] = m[n];
-      join.l[wave][lane] = sum;
+      join.l[wave][lane] = l[n];
     }
     if (n == 0) {
       join.odd[wave] = __any(odd);

@@ -324,7 +324,8 @@ void attention_rows_kernel(const AttentionArgs a, const Grid grid, int blocks) {
         probe[i % 4] = fmaf(o[d][i], 0.0f, probe[i % 4]);
       }
     }
-    odd = odd || !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
+    // (a row without a sum is NaN as it is)
+    odd = odd || (l == l && !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f));
   }
   const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
   if (stored && a.splits > 1) {
