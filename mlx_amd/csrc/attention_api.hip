@@ -44,11 +44,17 @@ struct FewWork {
 // 512 tokens under a window of 64 (2048 x 96) 26 / 14.  Of 96 columns, whose lines the tiles pad to
 // 128, more: 12 heads on 4, twice 400 tokens (608 x 200) 11.8 / 18.6, 16 heads, twice 330 (672 x 165)
 // 12.9 / 18.1; but 16 heads of 64, 4 times 330 (704 x 165) 15.9 / 12.8, of 128, 4 times 160 (640 x 80)
-// 14.5 / 10.7.
+// 14.5 / 10.7.  Of 96 above 768: 800 x 200 14.0 / 18.7, 832 x 100 12.6 / 11.8, 912 x 150 16.4 / 11.9,
+// 1088 x 90 15.5 / 10.1, 1200 x 200 18.6 / 14.4.
+// float32, 80 columns: 64 x 64 13.2 / 17.9, 32 x 1580 23.1 / 25.9, 26 x 2150 23.6 / 25.7, 512 x 96
+// 25.2 / 28.2, 512 x 128 29.5 / 30.7, 256 x 256 31.4 / 32.0, 304 x 132 30.3 / 27.3; above 2^16 512 x 160
+// 37.3 / 32.9, 256 x 500 53.7 / 46.5, 768 x 160 54.9 / 42.5, 1024 x 64 48 / 31.  256 columns, of which the
+// tiles hold a workgroup of 128 rows to a CU: 64 x 64 16.4 / 43.2, 304 x 80 29.2 / 62.0.
 bool few(const AttentionArgs& a, int dtype) {
   const FewWork w(a, dtype);
   const int64_t most = a.D == 96 && dtype != MLXROCM_FLOAT32 ? 768 : 512;
-  return w.rows <= w.each || (w.blocks <= most && w.blocks * w.keys <= 1 << 17);
+  const int64_t work = dtype == MLXROCM_FLOAT32 && a.D <= 128 ? 1 << 16 : 1 << 17;
+  return w.rows <= w.each || (w.blocks <= most && w.blocks * w.keys <= work);
 }
 
 // Runs that the keys of a row are cut into.  Few rows, by runs, us (16-bit, 8 or 64 key heads of
@@ -64,7 +70,10 @@ int splits_of(const AttentionArgs& a, int dtype) {
   int64_t splits;
   if (few(a, dtype)) {
     const FewWork w(a, dtype);
-    const int64_t once = (256 + w.blocks - 1) / w.blocks; // a workgroup for each CU
+    // a workgroup for each CU; not one more of float32, of which a CU holds one (26 workgroups of 80 columns
+    // over 2150 keys 9 runs 23.6, 10 37.2; one token, 3 sequences of 4600, 8 key heads of 128 32 / 42)
+    const int64_t once = dtype == MLXROCM_FLOAT32 ? std::max<int64_t>(256 / w.blocks, 1)
+                                                  : (256 + w.blocks - 1) / w.blocks;
     const int64_t reach = w.rows <= w.each ? span : w.keys;
     splits = std::min<int64_t>(
         std::max<int64_t>(once, std::min<int64_t>(2 * once, reach / 512)), reach / 72);
