@@ -139,7 +139,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     float o[4][16][DT + 4];
     float m[4][16], l[4][16];
     float total[16 * NT];
-    int odd[4];
+    int4 odd; // of each wave
   } join;
 
   const int lane = threadIdx.x & 63;
@@ -327,6 +327,8 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     odd = odd || (l[n] == l[n] && !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f));
   }
 
+  const int any_odd = __any(odd);
+  int4 all_odd = {};
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     __syncthreads(); // the tile of rows before has been joined
@@ -334,8 +336,8 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       join.m[wave][lane] = m[n];
       join.l[wave][lane] = l[n];
     }
-    if (n == 0) {
-      join.odd[wave] = __any(odd);
+    if (n == 0 && lane == 0) {
+      reinterpret_cast<int*>(&join.odd)[wave] = any_odd;
     }
 #pragma unroll
     for (int x = 0; x < S::kGroups; ++x) {
@@ -348,6 +350,9 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       }
     }
     __syncthreads();
+    if (n == 0) {
+      all_odd = join.odd;
+    }
     // 16 threads for a row
     const int at = threadIdx.x >> 4;
     const int row = r0 + 16 * n + at;
@@ -394,7 +399,7 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
       }
     }
   }
-  if ((join.odd[0] | join.odd[1] | join.odd[2] | join.odd[3]) != 0) { // the same for all
+  if ((all_odd.x | all_odd.y | all_odd.z | all_odd.w) != 0) { // the same for all
     after_stores();
     const int64_t part = (static_cast<int64_t>(split) * a.B * a.Hkv + head) * R;
     const int d = threadIdx.x;
