@@ -748,8 +748,9 @@ int mlxrocm_switch_glu(
  * negative positions -- a sequence with fewer than Lq tokens, padded in front -- see nothing and
  * give zeros.  Hq query heads share Hkv key heads, Hq / Hkv in a row each.  D: a multiple of 8 up
  * to 256.  Scores, sums and results are formed in 32 bits; with 16-bit types the probabilities are
- * rounded to the type for their product with v (to the sum of two such numbers where rows are few).  What a row does not see does not reach it,
- * whatever it holds (infinities and NaN too).
+ * rounded to the type for their product with v (to the sum of two such numbers where rows are few),
+ * and in the gradients so are theirs.  What a row does not see does not reach it, whatever it holds
+ * (infinities and NaN too); an infinite value that it sees makes its result infinite.
  *
  * lengths: [B] on the device, clamped to 0 .. most keys.  strides: host array, in elements, three
  * for each operand in the order [sequence, head, token] (the last dimension is dense); operands
@@ -761,7 +762,8 @@ int mlxrocm_switch_glu(
  * the gradients need: log2 of each row's sum, and in 16-bit types, where a token sees at most 2048,
  * what rounding took from out.
  * mlxrocm_window_attention_vjp: the gradients dq, dk, dv of q, k, v from dout, that of out.
- * strides: of q, k, v, out, dout, dq, dk, dv.  Sums are taken in a fixed order.
+ * strides: of q, k, v, out, dout, dq, dk, dv.  Sums are taken in a fixed order.  Keys and values that no
+ * query reads (no query heads, no queries, past a sequence's length) have gradients of zero.
  */
 size_t mlxrocm_window_attention_workspace_size(
     int B, int Hq, int Hkv, int Lq, int Lk, int D, int window, int keep, int dtype);

@@ -2,12 +2,18 @@
 between the quantized projections of a decoder when it is served or tuned.
 
 A sequence's token at position ``p`` sees the tokens ``j <= p`` with ``p - j < window`` or
-``j < keep``: the newest ``window`` ones, itself included, and the first ``keep`` (the ``keep``
-of mlx-lm's rotating cache); without a window, plain causal attention.  ``q`` holds the newest
+``j < keep``: the newest ``window`` ones, itself included, and the first ``keep`` beside them
+(mlx-lm's rotating cache counts the tokens that it keeps in its size; here ``window + keep`` are
+visible); without a window, plain causal attention.  ``q`` holds the newest
 tokens of each sequence (``mx.fast.scaled_dot_product_attention(..., mask="causal")`` aligns
 them so too); where a sequence has fewer tokens than ``q``, those in front are padding and
 give zeros.  Heads are laid out as there: ``[B, heads, L, D]``, with any strides (a transposed
 ``[B, L, heads, D]`` is read and answered in place), and several query heads may share a key head.
+
+Scores, sums and results are formed in 32 bits.  With 16-bit types probabilities are rounded to the
+type where they multiply values, and in the gradients so are theirs: results are up to 1.4 times as far
+off as their own rounding.  Where rows are few (decoding, drafted tokens) probabilities keep
+twice the bits there, and the results' own rounding is all.
 
 As in ``ops``, tensors are torch tensors on the GPU, and every computation is done by the
 HIP kernels behind the C ABI.

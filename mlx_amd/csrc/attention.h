@@ -239,7 +239,10 @@ __device__ __forceinline__ void flip(Frag<T>& f, uint32_t sign) {
 // Probabilities (or their gradients) as an operand.  For the 16-bit types this is where
 // they are rounded to the type of the values they multiply: the matrix instruction takes
 // both operands in one type, and a probability's relative error of 2^-9 (2^-12) is that of
-// the value beside it.  Sums of probabilities are taken before it, in 32 bits.
+// the value beside it.  Sums of probabilities are taken before it, in 32 bits.  Results are 1.4 times as
+// far off as their own rounding for it (2048 tokens over 32768, bfloat16, against 64 bits 0.0023 of the
+// norm instead of 0.0017).  A second term (rest_of) is taken where it costs nothing, of few rows; of many
+// it would cost a quarter to a third: 1.02 ms would be 1.35, 4096 tokens under a window of 1024 86 us 107.
 template <typename T>
 __device__ __forceinline__ Frag<T> frag_of(const float* p) {
   Frag<T> f;

@@ -106,12 +106,13 @@ size_t workspace_of(const AttentionArgs& a, int dtype) {
 
 // The cuts of the gradients' sums: parts of some tiles each, and a thousand workgroups if there
 // are as many, half as many where a CU holds one (8 heads of 256 on 2, 4096 tokens 614 instead of
-// 743 us).  us of both gradients, bfloat16, parts of at least 256, 512, 768 and 1024 keys or rows:
-// 64 heads of 128 on 8, 500 tokens 104 (512), 126, 163; 28 on 4, 2 times 1000 tokens 182, 144, 166,
-// 188; 32 on 8, 4096 tokens under a window of 256 with 4 kept 282, 257, 270, 289, with none 217, 230,
-// 189, 225; 12 heads of 96 on 4, 1500 tokens under a window of 128 85 (rows cut in two), 122 (not).
-// Up to a workgroup for each CU parts of 64 are enough: 16 heads of 128 on 4, 300 tokens 55 (128: 58,
-// 256: 61, 512: 91), 8 of 256 on one, 500 73 (75, 97, 128), float32, 32 of 128 on 8, 150 77 (104).
+// 743 us).  us of the gradients' kernels, bfloat16, parts of at least 256, 512, 768 and 1024 keys or
+// rows: 64 heads of 128 on 8, 500 tokens 73, 83, 100, 113; 28 on 4, 2 times 1000 tokens 188, 140, 141,
+// 149; 32 on 8, 4096 tokens under a window of 256 with 4 kept 266, 247, 255, 256, with none 217, 221,
+// 197, 198.
+// Up to a workgroup for each CU parts of 64 are enough: 16 heads of 128 on 4, 300 tokens 48 (128: 50,
+// 256: 53, 512: 73), 8 of 256 on one, 500 75 (75, 93, 116), 12 of 96 on 4, 1500 under a window of 128 56 (56,
+// 49, 58), float32, 32 of 128 on 8, 150 79 (103).
 GradPlan grad_plan_of(const AttentionArgs& a, int dtype) {
   GradPlan p{};
   const int64_t rows = static_cast<int64_t>(a.G) * a.Lq;

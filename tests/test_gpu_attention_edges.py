@@ -115,3 +115,27 @@ def test_pages_give_the_bits_of_contiguous_keys(gpu, Lq, Lk, page, window, keep,
     args = dict(scale=D ** -0.5, window=window, keep=keep)
     out = mlx_amd.paged_attention(q, *pages_of(k, v, page, fill=math.nan), n, **args)
     assert torch.equal(out, mlx_amd.window_attention(q, k, v, lengths=n, **args))
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16))
+@pytest.mark.parametrize("fill", (math.nan, math.inf, -math.inf))
+@pytest.mark.parametrize("D, keep", ((64, 0), (128, 3), (256, 0)))
+def test_rows_that_are_not_finite_reach_their_keys_alone(gpu, D, keep, fill, dtype):
+    """One row of q or of dout: the other rows' and the keys' that it does not see are what they are
+    with zeros there, bit for bit (and finite)."""
+    L, window = 300, 20
+    q, k, v, do = tensors(1, 4, 2, D, L, L, dtype, gpu, seed=D, grad=True)
+    j = torch.arange(L, device=gpu)
+    apart = ((j > 90) | (j <= 90 - window)) & (j >= keep)
+    for which in range(2):
+        results = []
+        for value in (fill, 0.0):
+            x = [q.clone(), do.clone()]
+            x[which][0, :, 90] = value
+            leaves = [t.clone().requires_grad_() for t in (x[0], k, v)]
+            out = mlx_amd.window_attention(*leaves, scale=D ** -0.5, window=window, keep=keep)
+            results.append((out.detach(), *torch.autograd.grad(out, leaves, x[1])))
+        for i, (a, b) in enumerate(zip(*results)):
+            rows = j != 90 if i < 2 else apart
+            assert torch.isfinite(a[:, :, rows].float()).all(), (which, i)
+            assert torch.equal(a[:, :, rows], b[:, :, rows]), (which, i)
