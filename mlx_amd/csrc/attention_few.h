@@ -220,8 +220,8 @@ void attention_few_kernel(const AttentionArgs a, const Grid grid, int blocks) {
     }
     const bool whole = whole_tile(a, at, KT, p_lo, p_hi);
     // In 16 bits a probability is the sum of two numbers: little here waits for the products (8
-    // sequences of 5 tokens over a window of 4096 22.6 us, 21.9 with one, a token over 65000 33.3 and
-    // 33.2), and the result is as near as its own rounding lets it be (with one, 1.4 times as far off)
+    // sequences of 5 tokens over a window of 4096 22.4 us, 21.6 with one, a token over 65000 27.8 and
+    // 27.7), and the result is as near as its own rounding lets it be (with one, 1.4 times as far off)
     constexpr int kTerms = sizeof(T) == 2 ? 2 : 1;
     Frag<T> w[NT][kTerms];
 #pragma unroll

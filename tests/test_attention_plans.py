@@ -63,8 +63,9 @@ def test_the_sums_parts_are_bounded(B, Hq, Hkv, D, L, window, keep, dtype):
 
 def test_float32_takes_the_cus_once():
     """A CU holds one workgroup of the kernel for few rows in float32."""
-    for B, Hq, Hkv, D, Lq, Lk in ((3, 32, 8, 128, 1, 4600), (7, 32, 4, 128, 1, 2600), (1, 8, 2, 80, 100, 2200),
-                                  (1, 4, 1, 128, 100, 1500), (100, 32, 8, 64, 1, 900)):
+    for B, Hq, Hkv, D, Lq, Lk in ((3, 32, 8, 128, 1, 4600), (7, 32, 4, 128, 1, 2600),
+                                  (1, 8, 2, 80, 100, 2200), (1, 4, 1, 128, 100, 1500),
+                                  (100, 32, 8, 64, 1, 900)):
         rc, plan = _lib.attention_plan(B, Hq, Hkv, Lq, Lk, D, dtype=F32)
         rows, splits = re.match(r"attention_few\(dim=\d+,rows=(\d+),splits=(\d+)\)", plan).groups()
         blocks = -(-(Hq // Hkv * Lq) // int(rows)) * B * Hkv
