@@ -873,6 +873,177 @@ int mlxrocm_paged_cache_update(
     mlxrocm_stream_t stream);
 
 /*
+ * Rotary positions: out = x [B, H, L, D] with the first `dims` columns turned, pair i by scale *
+ * position / freqs[i], freqs[i] = base^(2 i / dims) unless freqs (device, dims / 2 floats) is
+ * given.  Pairs are columns (i, i + dims / 2), or (2 i, 2 i + 1) if traditional.  positions: on the
+ * device, [axes, B, L] with three strides, int64 if wide_positions, else int32; with several axes
+ * (4 at most) sections[axes] (on the host) says how many pairs go by each.  inverse: turns back (the
+ * gradient).  strides: of x, then of out [sequence, head, token], in elements; rows are dense.
+ * dims: even, 256 at most.
+ * mlxrocm_rope_cache_update: q and k turned, to q_out [B, Hq, L, D] and to the pages, v to the pages,
+ * as mlxrocm_paged_cache_update puts them there; positions NULL: a token's place in its
+ * sequence.  Padding in front gives zeros in q_out.  strides: of q, k, v, q_out, k_pages,
+ * v_pages and of a row of table (19).
+ */
+int mlxrocm_rope(
+    const void* x,
+    void* out,
+    int B,
+    int H,
+    int L,
+    int D,
+    const int64_t* strides,
+    const void* positions,
+    const int64_t* position_strides,
+    int wide_positions,
+    int axes,
+    const int* sections,
+    int dims,
+    int traditional,
+    double base,
+    double scale,
+    const float* freqs,
+    int inverse,
+    int dtype,
+    mlxrocm_stream_t stream);
+int mlxrocm_rope_cache_update(
+    const void* q,
+    const void* k,
+    const void* v,
+    void* q_out,
+    void* k_pages,
+    void* v_pages,
+    const int32_t* table,
+    const int32_t* lengths,
+    int B,
+    int Hq,
+    int Hkv,
+    int L,
+    int D,
+    int pages,
+    int page_size,
+    int table_width,
+    const int64_t* strides,
+    const void* positions,
+    const int64_t* position_strides,
+    int wide_positions,
+    int axes,
+    const int* sections,
+    int dims,
+    int traditional,
+    double base,
+    double scale,
+    const float* freqs,
+    int dtype,
+    mlxrocm_stream_t stream);
+
+/*
+ * The experts of each row of logits [rows, experts] (row stride in elements): indices [rows, k], the
+ * largest choice first, the lowest index first of equal ones, and their weights [rows, k].  Scores
+ * are the softmax of a row or the sigmoid of its logits, choices the scores plus bias [experts]
+ * (or NULL); of `groups` runs of experts (16 at most, of one size) the top_groups with the largest sum
+ * of their group_best (1 or 2) largest choices count.  Weights are scores, divided by their sum if
+ * normalize, times scale.  An expert with a logit of -inf is chosen only where no other is left, as is
+ * one whose choice is NaN; where all chosen scores are 0 the weights are.  experts: 1024 at most, k 32.
+ * mlxrocm_route_experts_vjp: the gradient of logits, out [rows, experts], from that of the weights.
+ */
+int mlxrocm_route_experts(
+    const void* logits,
+    const float* bias,
+    int32_t* indices,
+    void* weights,
+    int64_t rows,
+    int64_t stride,
+    int experts,
+    int k,
+    int sigmoid,
+    int groups,
+    int top_groups,
+    int group_best,
+    int normalize,
+    float scale,
+    int dtype,
+    mlxrocm_stream_t stream);
+int mlxrocm_route_experts_vjp(
+    const void* logits,
+    const int32_t* indices,
+    const void* grad,
+    void* out,
+    int64_t rows,
+    int64_t stride,
+    int64_t grad_stride,
+    int experts,
+    int k,
+    int sigmoid,
+    int normalize,
+    float scale,
+    int dtype,
+    mlxrocm_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = y[t] + scale scales[i] (x[t] a[i]^T) b[i]^T,  i = indices[t / (rows / n_indices)]
+ * with x [rows, K], y (or NULL: zeros) and out [rows, N], a [adapters, rank, K], b [adapters, N,
+ * rank]; rows whose index is no adapter's keep y.  indices NULL: all rows have adapter 0
+ * (n_indices 1).  scales: on the device, or NULL.  adapters: 1024 at most, rank 256.  h: NULL, or
+ * where x a^T stays for the gradients (h_size bytes).
+ * mlxrocm_adapter_matmul_vjp: dx [rows, K] (zeros where there is no adapter), da and db as a and b
+ * (zeros for adapters without rows); each may be NULL.  y's gradient is dout.
+ */
+size_t mlxrocm_adapter_matmul_workspace_size(
+    int64_t rows, int n_indices, int adapters, int rank, int K, int N, int dtype);
+size_t mlxrocm_adapter_matmul_h_size(
+    int64_t rows, int n_indices, int adapters, int rank, int K, int N, int dtype);
+int mlxrocm_adapter_matmul(
+    const void* x,
+    const void* a,
+    const void* b,
+    const int32_t* indices,
+    const float* scales,
+    const void* y,
+    void* out,
+    float* h,
+    int64_t rows,
+    int n_indices,
+    int adapters,
+    int rank,
+    int K,
+    int N,
+    int64_t x_stride,
+    int64_t y_stride,
+    float scale,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+size_t mlxrocm_adapter_matmul_vjp_workspace_size(
+    int64_t rows, int n_indices, int adapters, int rank, int K, int N, int dtype);
+int mlxrocm_adapter_matmul_vjp(
+    const void* x,
+    const void* a,
+    const void* b,
+    const int32_t* indices,
+    const float* scales,
+    const float* h,
+    const void* dout,
+    void* dx,
+    void* da,
+    void* db,
+    int64_t rows,
+    int n_indices,
+    int adapters,
+    int rank,
+    int K,
+    int N,
+    int64_t x_stride,
+    int64_t dout_stride,
+    float scale,
+    int dtype,
+    void* workspace,
+    size_t workspace_bytes,
+    mlxrocm_stream_t stream);
+
+/*
  * The launches that either attention makes of a shape (keys: Lk, or table_width * page_size), and
  * those of the gradients, written to plan without touching a device, as mlxrocm_qmm_plan does.
  */

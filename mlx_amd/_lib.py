@@ -24,6 +24,7 @@ _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _p = ctypes.c_void_p
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (restype, argtypes); the list the symbol-export test walks.
 SIGNATURES = {
@@ -65,6 +66,25 @@ SIGNATURES = {
     "mlxrocm_paged_attention_workspace_size": (_sz, [_i] * 9),
     "mlxrocm_paged_attention": (_i, [_p] * 6 + [_i] * 8 + [_p, _f] + [_i] * 3 + [_p, _sz, _p]),
     "mlxrocm_paged_cache_update": (_i, [_p] * 6 + [_i] * 7 + [_p, _i, _p]),
+    "mlxrocm_rope": (_i, [_p] * 2 + [_i] * 4 + [_p] * 3 + [_i] * 2 + [_p] + [_i] * 2 + [_d] * 2
+                     + [_p] + [_i] * 2 + [_p]),
+    "mlxrocm_rope_cache_update": (
+        _i,
+        [_p] * 8 + [_i] * 8 + [_p] * 3 + [_i] * 2 + [_p] + [_i] * 2 + [_d] * 2 + [_p, _i, _p],
+    ),
+    "mlxrocm_route_experts": (_i, [_p] * 4 + [_i64] * 2 + [_i] * 7 + [_f, _i, _p]),
+    "mlxrocm_route_experts_vjp": (_i, [_p] * 4 + [_i64] * 3 + [_i] * 4 + [_f, _i, _p]),
+    "mlxrocm_adapter_matmul_workspace_size": (_sz, [_i64] + [_i] * 6),
+    "mlxrocm_adapter_matmul_h_size": (_sz, [_i64] + [_i] * 6),
+    "mlxrocm_adapter_matmul": (
+        _i,
+        [_p] * 8 + [_i64] + [_i] * 5 + [_i64] * 2 + [_f, _i, _p, _sz, _p],
+    ),
+    "mlxrocm_adapter_matmul_vjp_workspace_size": (_sz, [_i64] + [_i] * 6),
+    "mlxrocm_adapter_matmul_vjp": (
+        _i,
+        [_p] * 10 + [_i64] + [_i] * 5 + [_i64] * 2 + [_f, _i, _p, _sz, _p],
+    ),
     "mlxrocm_window_attention_vjp_plan": (_i, [_i] * 9 + [ctypes.c_char_p, _sz]),
     "mlxrocm_attention_plan": (_i, [_i] * 9 + [ctypes.c_char_p, _sz]),
     "mlxrocm_verify_draft_workspace_size": (_sz, [_i] * 2),

@@ -18,8 +18,9 @@ from typing import Callable, List, Optional, Tuple, Union
 import torch
 
 from . import ops
+from .adapters import adapter_matmul
 
-__all__ = ["QuantizedLinear", "QQLinear", "QuantizedEmbedding", "QuantizedSwitchLinear", "SwitchGLU",
+__all__ = ["QuantizedLinear", "LoRALinear", "QQLinear", "QuantizedEmbedding", "QuantizedSwitchLinear", "SwitchGLU",
            "quantize", "save_weights", "load_weights"]
 
 
@@ -118,6 +119,38 @@ class QuantizedLinear(torch.nn.Module):
         if getattr(linear_layer, "bias", None) is not None:
             ql._buffers["bias"] = linear_layer.bias.detach()
         return ql
+
+
+class LoRALinear(torch.nn.Module):
+    """A projection (:class:`QuantizedLinear`, or any module) and low-rank adapters beside it, one
+    of which each request uses: ``linear(x) + scale * (x @ lora_a[i].T) @ lora_b[i].T`` by
+    :func:`adapter_matmul`.  ``lora_a`` ``[adapters, rank, input_dims]`` is drawn, ``lora_b`` ``[adapters,
+    output_dims, rank]`` starts at zero; both are trained, a quantized projection is not."""
+
+    def __init__(self, linear: torch.nn.Module, rank: int = 8, adapters: int = 1, scale: float = 20.0,
+                 input_dims: Optional[int] = None, output_dims: Optional[int] = None, device=None,
+                 dtype=None):
+        super().__init__()
+        weight = linear.weight
+        if weight.dtype == torch.uint32:
+            input_dims = input_dims or weight.shape[-1] * 32 // linear.bits
+            like = linear.scales if linear.scales.is_floating_point() else None
+            dtype = dtype or (torch.bfloat16 if like is None else like.dtype)
+        output_dims, input_dims = output_dims or weight.shape[-2], input_dims or weight.shape[-1]
+        kw = dict(device=weight.device if device is None else device, dtype=dtype or weight.dtype)
+        self.linear, self.scale = linear, scale
+        a = (torch.rand((adapters, rank, input_dims), **kw) * 2 - 1) * math.sqrt(1.0 / input_dims)
+        self.lora_a = torch.nn.Parameter(a)
+        self.lora_b = torch.nn.Parameter(torch.zeros((adapters, output_dims, rank), **kw))
+
+    def forward(self, x: torch.Tensor, indices: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``indices``: the adapter of each request (:func:`adapter_matmul`), none with one adapter."""
+        return adapter_matmul(x, self.lora_a, self.lora_b, indices, scale=self.scale, y=self.linear(x))
+
+    def extra_repr(self) -> str:
+        adapters, rank, input_dims = self.lora_a.shape
+        return (f"input_dims={input_dims}, output_dims={self.lora_b.shape[1]}, rank={rank}, "
+                f"adapters={adapters}, scale={self.scale}")
 
 
 class QQLinear(torch.nn.Module):

@@ -65,6 +65,28 @@ def _require_gpu(tag: str, *tensors: torch.Tensor) -> None:
             )
 
 
+def _require_one_device(tag: str, *tensors: torch.Tensor) -> None:
+    devices = {t.device for t in tensors}
+    if len(devices) > 1:
+        raise ValueError(f"[{tag}] Tensors must be on one device but are on "
+                         f"{', '.join(sorted(map(str, devices)))}.")
+
+
+def _rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """t as rows of its last dimension that are dense and evenly spaced, in place where it can be,
+    and how many elements they are apart."""
+    n = t.shape[-1]
+    if t.numel() == 0:
+        return t, n
+    if t.stride(-1) != 1 and n != 1:
+        t = _contiguous(t)
+    try:
+        rows = t.view(-1, n)
+    except RuntimeError:  # no one distance between rows
+        rows = _contiguous(t).view(-1, n)
+    return rows, rows.stride(0) if rows.shape[0] > 1 else n
+
+
 def _mode(tag: str, mode: str) -> str:
     # string_to_quantization_mode, mlx/primitives.cpp
     if mode not in _MODES:

@@ -1,0 +1,272 @@
+"""route_experts against scores in 64 bits: indices are equal, weights and gradients as far off as
+their roundings."""
+import math
+
+import pytest
+import torch
+
+import mlx_amd
+from mlx_amd import nn
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+SMALLEST = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}
+TYPES = (torch.float32, torch.float16, torch.bfloat16)
+F = 2.0 ** -24
+
+
+def reference(logits, k, scoring="softmax", bias=None, groups=1, top_groups=None, group_best=1,
+              normalize=True, scale=1.0, grad=None):
+    """indices, weights and the gradient of the logits, one row after the other in 64 bits (CPU)."""
+    rows = logits.detach().double().cpu().reshape(-1, logits.shape[-1])
+    E = rows.shape[1]
+    top_groups = groups if top_groups is None else top_groups
+    indices, weights, grads = [], [], []
+    for n, l in enumerate(rows):
+        if scoring == "sigmoid":
+            s = torch.sigmoid(l)
+        else:
+            m = float(l.max())
+            s = torch.zeros_like(l) if m == -math.inf else torch.exp(l - m) / torch.exp(l - m).sum()
+        choice = (l if bias is None and not (group_best > 1 and top_groups < groups) else s).clone()
+        if bias is not None:
+            choice += bias.double().cpu()
+        choice[l == -math.inf] = -math.inf
+        order = choice.tolist()
+        size = E // groups
+        marks = [sum(sorted(order[g * size:(g + 1) * size], reverse=True)[:group_best])
+                 for g in range(groups)]
+        open_ = sorted(range(groups), key=lambda g: (-marks[g], g))[:top_groups]
+        left = [e for e in range(E) if e // size in open_]
+        chosen = sorted(left, key=lambda e: (-order[e], e))[:k]
+        c = s[chosen]
+        total = c.sum() if normalize else torch.ones(())
+        w = c / total if total > 0 else torch.zeros_like(c)
+        indices.append(chosen)
+        weights.append(w * scale)
+        if grad is not None:
+            g = torch.zeros_like(l)
+            up = grad.double().cpu().reshape(-1, k)[n] * scale
+            if normalize:
+                up = (up - (up * w).sum()) / total if total > 0 else torch.zeros_like(up)
+            g[chosen] = up
+            if scoring == "sigmoid":
+                grads.append(g * s * torch.sigmoid(-l))
+            else:
+                grads.append(s * (g - (g * s).sum()))
+    shape = (*logits.shape[:-1], k)
+    out = [torch.tensor(indices, dtype=torch.int32).reshape(shape), torch.stack(weights).reshape(shape)]
+    if grad is not None:
+        out.append(torch.stack(grads).reshape(logits.shape))
+    return out
+
+
+def relative(logits):
+    """How far a weight may be off before it is rounded: e^x by the rounding of x (differences up to the
+    spread of the logits) and two units, for itself and for the sum; the sum by an addition for each
+    of a lane's up to 64 values and the four steps over lanes, and four more operations."""
+    finite = logits.double()[logits.isfinite()]
+    spread = float(finite.max() - finite.min()) if finite.numel() else 0.0
+    return (2 * (spread + 4) + 64 + 4 + 4) * F
+
+
+def check(logits, k, seed=5, **options):
+    dtype = logits.dtype
+    g = torch.Generator().manual_seed(seed)
+    grad = torch.randn((*logits.shape[:-1], k), generator=g).to(dtype).cuda()
+    logits = logits.cuda().requires_grad_()
+    indices, weights = mlx_amd.route_experts(logits, k, **options)
+    assert indices.dtype == torch.int32 and weights.dtype == dtype and not indices.requires_grad
+    plain = mlx_amd.route_experts(logits.detach(), k, **options)
+    assert torch.equal(plain[0], indices) and torch.equal(plain[1], weights.detach())
+    dl, = torch.autograd.grad(weights, logits, grad)
+    want = reference(logits, k, grad=grad, **options)
+    assert torch.equal(indices.cpu(), want[0])
+    off = (weights.detach().cpu().double() - want[1]).abs()
+    bound = (relative(logits) + HALF_STEP[dtype]) * want[1].abs() + SMALLEST[dtype]
+    assert float((off - bound).max()) <= 0, float((off - bound).max())
+    # each term of the gradient is a product of at most three such numbers; a sum of k terms
+    scale = abs(options.get("scale", 1.0))
+    size = k * scale * float(grad.abs().max())
+    off = (dl.cpu().double() - want[2]).abs()
+    bound = (3 * relative(logits) + (k + 8) * F) * 2 * size + HALF_STEP[dtype] * want[2].abs() + SMALLEST[dtype]
+    assert float((off - bound).max()) <= 0, float((off - bound).max())
+    return indices, weights, dl
+
+
+def logits_of(*shape, dtype, std=2.0, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(dtype)
+
+
+SHAPES = ((1, 1, 1, 1, 1), (3, 2, 1, 1, 1), (5, 8, 2, 1, 1), (17, 60, 4, 1, 1), (33, 64, 6, 4, 2),
+          (9, 256, 8, 8, 4), (16, 160, 6, 8, 3), (2, 384, 8, 1, 1), (2, 1024, 32, 16, 5),
+          (4, 48, 17, 3, 2), (3, 45, 20, 5, 5), (2, 16, 1, 16, 1), (7, 33, 33 - 1, 1, 1),
+          (3, 130, 9, 13, 4), (2, 1000, 10, 1, 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, experts, k, groups, top", SHAPES)
+@pytest.mark.parametrize("scoring", ("softmax", "sigmoid"))
+def test_route_experts_and_its_gradient(gpu, dtype, rows, experts, k, groups, top, scoring):
+    logits = logits_of(rows, experts, dtype=dtype)
+    bias = torch.randn((experts,), generator=torch.Generator().manual_seed(1)).mul(50).round() * 0.001
+    best = 2 if experts // groups > 1 else 1
+    for options in (dict(), dict(normalize=False), dict(bias=bias.cuda(), scale=2.5),
+                    dict(group_best=best, scale=-0.5), dict(bias=bias.cuda(), group_best=best,
+                                                            normalize=False)):
+        check(logits, k, scoring=scoring, groups=groups, top_groups=top, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scoring", ("softmax", "sigmoid"))
+def test_equal_ones_go_by_index(gpu, dtype, scoring):
+    logits = torch.randint(-2, 3, (40, 96), generator=torch.Generator().manual_seed(2)).to(dtype)
+    logits[0] = 0
+    logits[1] = torch.tensor([0.0, -0.0] * 48)
+    bias = torch.randint(0, 2, (96,), generator=torch.Generator().manual_seed(3)).float().cuda()
+    for options in (dict(), dict(bias=bias), dict(groups=8, top_groups=3),
+                    dict(groups=8, top_groups=3, group_best=2, bias=bias)):
+        indices, *_ = check(logits, 12, scoring=scoring, **options)
+    assert mlx_amd.route_experts(logits[:2].cuda(), 5)[0].tolist() == [[0, 1, 2, 3, 4]] * 2
+
+
+def test_choices_that_differ_in_the_last_bits(gpu):
+    """Choices apart by less than 32 bits hold: their order is that of 64 bits."""
+    base = 0.25
+    logits = torch.zeros((1, 64))
+    bias = torch.full((64,), base)
+    order = torch.randperm(64, generator=torch.Generator().manual_seed(4))
+    # sigmoid(l) near 1/2 moves by l / 4: logits a few 2**-30 apart, scores 2**-32 apart
+    logits[0, order] = torch.arange(64, dtype=torch.float32) * 2.0 ** -30
+    indices, _ = mlx_amd.route_experts(logits.cuda(), 32, scoring="sigmoid", bias=bias.cuda())
+    assert indices[0].tolist() == order.flip(0)[:32].tolist()
+    logits = torch.tensor([[1.0, 1.0 - 2.0 ** -24, 1.0 - 2.0 ** -23, 0.0] * 4])
+    check(logits, 9, bias=torch.zeros(16, device="cuda"))
+
+
+def test_masked_and_empty_rows(gpu):
+    for dtype in TYPES:
+        logits = logits_of(6, 32, dtype=dtype)
+        logits[0] = -math.inf
+        logits[1, 3:] = -math.inf
+        logits[2, :30] = -math.inf
+        logits[3] = torch.finfo(dtype).min
+        bias = logits_of(32, dtype=torch.float32, std=0.1, seed=8).cuda()
+        for options in (dict(), dict(normalize=False), dict(scoring="sigmoid"), dict(bias=bias),
+                        dict(scoring="sigmoid", bias=bias, groups=4, top_groups=4, group_best=2)):
+            indices, weights = mlx_amd.route_experts(logits.cuda(), 5, **options)
+            want = reference(logits, 5, **options)
+            assert torch.equal(indices.cpu(), want[0])
+            assert (weights[0] == 0).all() and (weights[1, 3:] == 0).all()
+            if options.get("scoring") != "sigmoid":
+                off = (weights.cpu().double() - want[1]).abs()
+                assert float((off - (relative(logits[4:]) + HALF_STEP[dtype]) * want[1]).max()) <= 0
+            leaf = logits.cuda().requires_grad_()
+            weights = mlx_amd.route_experts(leaf, 5, **options)[1]
+            dl, = torch.autograd.grad(weights.float().square().sum(), leaf)
+            assert dl.isfinite().all() and (dl[0] == 0).all() and (dl[1, 3:] == 0).all()
+
+
+def test_tiny_sigmoids_keep_their_ratios(gpu):
+    logits = torch.tensor([[-200.0, -201.0, -200.5, -300.0], [-95.0, 3.0, -95.0, -95.0]])
+    _, weights = mlx_amd.route_experts(logits.cuda(), 2, scoring="sigmoid")
+    w = 1 / (1 + math.exp(-0.5))
+    assert weights[0].tolist() == pytest.approx([w, 1 - w], rel=1e-6)
+    assert weights[1].tolist() == pytest.approx([1.0, 0.0], abs=1e-30)
+
+
+def test_infinities_and_nan(gpu):
+    inf, nan = math.inf, math.nan
+    logits = torch.tensor([[0.0, inf, 1.0, inf, 2.0, 3.0], [0.0, nan, 1.0, 5.0, 2.0, 3.0],
+                           [nan] * 6, [0.0, 1.0, 2.0, 3.0, 4.0, 5.0]]).cuda()
+    indices, weights = mlx_amd.route_experts(logits, 3)
+    assert indices.tolist() == [[1, 3, 5], [3, 5, 4], [0, 1, 2], [5, 4, 3]]
+    assert weights[0].tolist() == [0.5, 0.5, 0.0] and weights[2].isnan().all()
+    assert weights[1].isfinite().all()  # depends on the chosen logits alone
+    clean = mlx_amd.route_experts(logits[3:], 3)[1]
+    assert torch.equal(weights[3:], clean)
+    whole = mlx_amd.route_experts(logits, 3, normalize=False)[1]
+    assert whole[1].isnan().all() and whole[3].isfinite().all()
+    indices, weights = mlx_amd.route_experts(logits, 6, scoring="sigmoid", normalize=False)
+    assert indices.tolist()[1] == [3, 5, 4, 2, 0, 1] and weights[1].isnan().tolist() == [False] * 5 + [True]
+    bias = torch.tensor([0.0, 0.0, nan, inf, -inf, 0.0], device="cuda")
+    for row in (1, 3):
+        indices, _ = mlx_amd.route_experts(logits[row:row + 1], 6, scoring="sigmoid", bias=bias)
+        assert indices.tolist() == [[3, 5, 0, 1, 2, 4] if row == 1 else [3, 5, 1, 0, 2, 4]]
+
+
+def test_shapes_strides_and_empties(gpu):
+    wide = logits_of(2, 3, 5, 70, dtype=torch.bfloat16).cuda()
+    want = reference(wide[..., 3:67], 4)
+    indices, weights = mlx_amd.route_experts(wide[..., 3:67], 4)
+    assert indices.shape == weights.shape == (2, 3, 5, 4) and torch.equal(indices.cpu(), want[0])
+    turned = wide.transpose(0, 2)[..., :64]
+    assert torch.equal(mlx_amd.route_experts(turned, 4)[0].cpu(), reference(turned, 4)[0])
+    columns = wide.transpose(2, 3)
+    assert torch.equal(mlx_amd.route_experts(columns, 2)[0].cpu(), reference(columns, 2)[0])
+    shared = wide[0, 0, :1].expand(9, 70)
+    assert torch.equal(mlx_amd.route_experts(shared, 4)[0].cpu(), reference(shared, 4)[0])
+    assert mlx_amd.route_experts(wide[0, 0, 0], 4)[0].shape == (4,)
+    leaf = wide[:, :0].detach().requires_grad_()
+    indices, weights = mlx_amd.route_experts(leaf, 4)
+    assert indices.shape == (2, 0, 5, 4)
+    assert torch.autograd.grad(weights.sum(), leaf)[0].shape == leaf.shape
+
+
+def test_gradient_against_differences(gpu):
+    logits = logits_of(6, 24, dtype=torch.float32).cuda().requires_grad_()
+    step = logits_of(6, 24, dtype=torch.float32, std=1.0, seed=9).cuda()
+    for options in (dict(), dict(normalize=False), dict(scoring="sigmoid"),
+                    dict(scoring="sigmoid", normalize=False, scale=3.0)):
+        _, weights = mlx_amd.route_experts(logits, 5, **options)
+        up = torch.cos(torch.arange(5, device="cuda") + 1.0)
+        dl, = torch.autograd.grad((weights * up).sum(), logits)
+        e = 1e-5
+        at = [(reference(logits.detach().double() + s * e * step.double(), 5, **options)[1]
+               * up.double().cpu()).sum() for s in (1, -1)]
+        want = float(at[0] - at[1]) / (2 * e)
+        # 32-bit gradients of 144 terms, and differences of third order in e
+        assert abs(float((dl.double() * step.double()).sum()) - want) <= 144 * 64 * F + 1e-8
+
+
+def test_rows_beyond_a_grid_of_blocks_and_the_gradient_of_expanded_ones(gpu):
+    logits = logits_of(70001, 8, dtype=torch.float16).cuda().requires_grad_()
+    indices, weights = mlx_amd.route_experts(logits, 2)
+    top = torch.sort(logits.detach().float(), dim=-1, descending=True, stable=True)
+    assert torch.equal(indices.long(), top[1][:, :2])
+    want = torch.softmax(top[0][:, :2].double(), -1)
+    assert float((weights.double() - want).abs().max()) <= 2.0 ** -11 + 100 * F
+    dl, = torch.autograd.grad(weights.sum(), logits)  # an expanded gradient: the weights sum to 1
+    assert float(dl.abs().max()) <= 2.0 ** -11
+
+
+def test_replays_and_experts(gpu):
+    """The router in front of the experts, captured and replayed on new hidden states."""
+    torch.manual_seed(0)
+    glu = nn.SwitchGLU(128, 192, 16, device="cuda", dtype=torch.bfloat16)
+    gate = torch.randn(16, 128, device="cuda", dtype=torch.bfloat16) * 0.1
+    x = torch.randn(12, 128, device="cuda", dtype=torch.bfloat16)
+
+    def block(x):
+        indices, weights = mlx_amd.route_experts(torch.nn.functional.linear(x, gate), 4)
+        return indices, weights, (glu(x, indices) * weights[..., None]).sum(-2)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        block(x)
+    torch.cuda.current_stream().wait_stream(stream)
+    held = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(held)
+    for _ in range(4):
+        x = torch.randn_like(x)
+        held.copy_(x)
+        graph.replay()
+        want = block(x)
+        torch.cuda.synchronize()
+        for got, ref in zip(out, want):
+            assert torch.equal(got, ref)
