@@ -105,6 +105,9 @@ def adapter_matmul(
     Sums are formed in 32 bits, ``x @ a.T`` is kept in 32 (float32) or twice the type's bits, and the
     result is rounded once.  Up to 1024 adapters of rank up to 256; adapters of a lower rank than others
     are filled up with zeros.  Differentiable with respect to x, a, b and y (once, in reverse mode)."""
+    out = ops._fast.adapter_matmul(x, a, b, indices, scale, y)
+    if out is not None:
+        return out
     tag = "adapter_matmul"
     if a.dim() == 2 and b.dim() == 2 and indices is None:
         a, b = a.unsqueeze(0), b.unsqueeze(0)

@@ -13,7 +13,7 @@
 // A function returns None -- and ops.py goes on with its own body -- for
 // everything that is not the plain case: another device than the current one,
 // operands to be converted, expanded or made contiguous, a gradient to be
-// recorded (but for attention), a shape or an option that ops.py refuses, and any status other than
+// recorded (but for attention and what decoder_ops.h has), a shape or an option that ops.py refuses, and any status other than
 // MLXROCM_OK (ops.py then makes the same call and turns it into an exception).
 // So the rules and messages stay in one place; here are only the conditions
 // under which nothing of them applies.
@@ -30,6 +30,8 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <stdexcept>
+#include <vector>
 
 #include "mlx_rocm_qmm.h"
 
@@ -71,6 +73,15 @@ struct Abi {
   decltype(&mlxrocm_paged_cache_update) paged_cache_update;
   decltype(&mlxrocm_verify_draft_workspace_size) verify_workspace_size;
   decltype(&mlxrocm_verify_draft) verify_draft;
+  decltype(&mlxrocm_rope) rope;
+  decltype(&mlxrocm_rope_cache_update) rope_cache_update;
+  decltype(&mlxrocm_route_experts) route_experts;
+  decltype(&mlxrocm_route_experts_vjp) route_experts_vjp;
+  decltype(&mlxrocm_adapter_matmul_workspace_size) adapter_workspace_size;
+  decltype(&mlxrocm_adapter_matmul_h_size) adapter_h_size;
+  decltype(&mlxrocm_adapter_matmul) adapter_matmul;
+  decltype(&mlxrocm_adapter_matmul_vjp_workspace_size) adapter_vjp_workspace_size;
+  decltype(&mlxrocm_adapter_matmul_vjp) adapter_vjp;
 };
 Abi abi{};
 bool bound = false;
@@ -1149,6 +1160,8 @@ PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FAST_CATCH
 }
 
+#include "decoder_ops.h"
+
 // bind({entry point: address}): the library whose entry points are to be called
 PyObject* bind(PyObject*, PyObject* table) {
   if (!PyDict_Check(table)) {
@@ -1203,7 +1216,16 @@ PyObject* bind(PyObject*, PyObject* table) {
       take("mlxrocm_paged_attention", abi.paged_attention) &&
       take("mlxrocm_paged_cache_update", abi.paged_cache_update) &&
       take("mlxrocm_verify_draft_workspace_size", abi.verify_workspace_size) &&
-      take("mlxrocm_verify_draft", abi.verify_draft);
+      take("mlxrocm_verify_draft", abi.verify_draft) &&
+      take("mlxrocm_rope", abi.rope) &&
+      take("mlxrocm_rope_cache_update", abi.rope_cache_update) &&
+      take("mlxrocm_route_experts", abi.route_experts) &&
+      take("mlxrocm_route_experts_vjp", abi.route_experts_vjp) &&
+      take("mlxrocm_adapter_matmul_workspace_size", abi.adapter_workspace_size) &&
+      take("mlxrocm_adapter_matmul_h_size", abi.adapter_h_size) &&
+      take("mlxrocm_adapter_matmul", abi.adapter_matmul) &&
+      take("mlxrocm_adapter_matmul_vjp_workspace_size", abi.adapter_vjp_workspace_size) &&
+      take("mlxrocm_adapter_matmul_vjp", abi.adapter_vjp);
   if (!bound) {
     return nullptr;
   }
@@ -1224,6 +1246,10 @@ PyMethodDef methods[] = {
     FASTCALL(paged_attention),
     FASTCALL(paged_cache_update),
     FASTCALL(verify_draft),
+    FASTCALL(rope),
+    FASTCALL(rope_cache_update),
+    FASTCALL(route_experts),
+    FASTCALL(adapter_matmul),
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

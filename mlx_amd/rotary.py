@@ -135,6 +135,9 @@ def rope(
     B, L]``.  ``dims`` (even, at most 256): the columns that turn, all without it; ``base``: 10000
     without it; ``freqs`` ``[dims / 2]`` in its place.  The result has ``x``'s shape and, where that is
     dense, its memory order.  Differentiable with respect to x (in reverse mode)."""
+    out = ops._fast.rope(x, positions, dims, traditional, base, scale, freqs, sections)
+    if out is not None:
+        return out
     tag = "rope"
     if x.dim() != 4:
         raise ValueError(f"[{tag}] x must have 4 dimensions but has shape {tuple(x.shape)}.")
@@ -178,6 +181,10 @@ def rope_cache_update(
     their places in their sequences, or by ``positions`` where those are given (the tokens go to the
     same places of the cache all the same).  Where ``lengths`` is below ``L`` the queries in front are
     padding and give zeros.  No gradients."""
+    out = ops._fast.rope_cache_update(q, k, v, k_pages, v_pages, block_table, lengths, positions, dims,
+                                      traditional, base, scale, freqs, sections)
+    if out is not None:
+        return out, k_pages, v_pages
     tag = "rope_cache_update"
     for name, t in (("q", q), ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages)):
         if t.dim() != 4:

@@ -84,6 +84,10 @@ def route_experts(
     one whose choice is NaN.  A token without any score has weights of zero.  A NaN makes NaN of the
     weights that depend on it.  Up to 1024 experts, 16 groups and 32 choices.
     Differentiable with respect to the logits (once, in reverse mode), not to the bias."""
+    out = ops._fast.route_experts(logits, k, scoring, bias, groups, top_groups, group_best, normalize,
+                                  scale)
+    if out is not None:
+        return out
     tag = "route_experts"
     if logits.dim() < 1 or not 1 <= logits.shape[-1] <= _MOST_EXPERTS:
         raise ValueError(f"[{tag}] logits must have 1 to {_MOST_EXPERTS} experts in the last dimension "
