@@ -15,9 +15,8 @@
 //            need none: the first token of an adapter finds the others by a vote.
 //   shrink   h or g, in 32 bits.  The four wavefronts of a workgroup and, for few tokens, several
 //            workgroups share a token's sum; the parts are added in one order by who reads them.
-//   expand   out or dx.  16-bit types: h as the sum of two numbers of the type, in one instruction
-//            of 32: sixteen ranks of the upper parts, then of the lower ones, against the same
-//            sixteen columns of B twice.  So h keeps 16 bits (bfloat16) or 22, and the result's own
+//   expand   out or dx.  16-bit types: h as the sum of two numbers of the type, against the same
+//            operand of B twice (up to 16 ranks: in one instruction of 32).  So h keeps 16 bits (bfloat16) or 22, and the result's own
 //            rounding is all that is seen.  float16: h counts a power of two that brings the
 //            token's largest to 2^13.
 //   turn     A and B with their two dimensions swapped, for the gradients: then g and dx are the
@@ -74,8 +73,8 @@ __device__ __forceinline__ int find_rows(const Rows& r, int block, int tile, int
     if (r.tiles != nullptr) {
       const bool is = block < *r.n_tiles;
       const Tile t = r.tiles[is ? block : 0];
-      if (is && lane < t.rows) {
-        to[lane] = r.row(t.first + lane);
+      for (int i = lane; is && i < t.rows; i += 64) {
+        to[i] = r.row(t.first + i);
       }
       if (lane == 0) {
         found[0] = is ? t.rows : 0;
@@ -84,8 +83,8 @@ __device__ __forceinline__ int find_rows(const Rows& r, int block, int tile, int
     } else if (r.n == 1) {
       const int first = block * tile;
       const int rows = min(tile, r.span.d - first);
-      if (lane < rows) {
-        to[lane] = first + lane;
+      for (int i = lane; i < rows; i += 64) {
+        to[i] = first + i;
       }
       if (lane == 0) {
         found[0] = rows;
@@ -129,10 +128,14 @@ __device__ __forceinline__ void multiply(const uint4& a, const uint4& b, floatx4
   }
 }
 
-// Elements k .. k + 15 / sizeof(T) of a row of n; what lies past its end is zero
-template <typename T, bool kAligned>
+// Elements k .. k + 15 / sizeof(T) of a row of n; what lies past its end is zero (kWhole: nothing
+// does)
+template <typename T, bool kAligned, bool kWhole = false>
 __device__ __forceinline__ uint4 operand(const T* row, int k, int n) {
   if constexpr (kAligned) { // (n is a multiple)
+    if constexpr (kWhole) {
+      return *reinterpret_cast<const uint4*>(row + k);
+    }
     return k < n ? *reinterpret_cast<const uint4*>(row + k) : uint4{0, 0, 0, 0};
   } else {
     union {
@@ -162,7 +165,9 @@ struct ShrinkArgs {
   int tile;
 };
 
-// kGroups groups of 16 tokens, kChunks of 16 ranks
+// kGroups groups of 16 tokens, kChunks of 16 ranks; the four wavefronts have parts of the sums.
+// (The same part for different tokens, so that A comes from memory once for 128 tokens: 86 us
+// instead of 66, 7813 tokens of 14336 values to rank 32, float16.)
 template <typename T, int kGroups, int kChunks, bool kAligned>
 __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
   __shared__ int rows[kDecode];
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15;
   const int quarter = lane >> 4;
   const int rank0 = blockIdx.z * kChunks * 16;
@@ -194,32 +199,67 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
           rows[min(base + 16 * i + column, count - 1)] * a.x_stride;
     }
     floatx4 sum[kGroups][kChunks] = {};
-    constexpr int kAhead = kChunks <= 2 ? 4 : 2; // steps whose operands are asked for at once
-    for (int k0 = begin + wave * kStep<T>; k0 < end; k0 += kAhead * 4 * kStep<T>) {
+    // A wavefront's steps are neighbours, so that it reads whole lines; while one turn's operands
+    // are multiplied the next one's are on their way
+    constexpr int kAhead = kGroups * kChunks <= 2 ? 4 : 2;
+    constexpr int kTurn = kAhead * kStep<T>;
+    struct Turn {
       uint4 x[kAhead][kGroups];
-      uint4 v[kAhead][kChunks];
+      uint4 w[kAhead][kChunks];
+    };
+    const auto ask = [&](Turn& t, int k0, auto whole) {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
-        const int k = k0 + s * 4 * kStep<T> + quarter * kPer<T>;
+        const int k = k0 + s * kStep<T> + quarter * kPer<T>;
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) {
-          x[s][i] = operand<T, kAligned>(x_row[i], k, end);
+          t.x[s][i] = operand<T, kAligned, whole.value>(x_row[i], k, end);
         }
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          v[s][c] = operand<T, kAligned>(w_row[c], k, end);
+          t.w[s][c] = operand<T, kAligned, whole.value>(w_row[c], k, end);
         }
       }
+    };
+    const auto add = [&](const Turn& t) {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
           for (int i = 0; i < kGroups; ++i) {
-            multiply<T>(v[s][c], x[s][i], sum[i][c]);
+            multiply<T>(t.w[s][c], t.x[s][i], sum[i][c]);
           }
         }
       }
+    };
+    const int k0 = begin + wave * kTurn;
+    const int whole = k0 + kTurn > end ? 0 : (end - kTurn - k0) / (4 * kTurn) + 1;
+    const auto at = [&](int n) { return k0 + n * 4 * kTurn; };
+    // (no conditions between a turn's loads and its products: a wait then leaves the next one's
+    // in flight)
+    Turn one;
+    Turn two;
+    if (whole > 0) {
+      ask(one, at(0), std::true_type{});
+      int n = 0;
+      for (; n + 2 < whole; n += 2) {
+        ask(two, at(n + 1), std::true_type{});
+        add(one);
+        ask(one, at(n + 2), std::true_type{});
+        add(two);
+      }
+      if (n + 1 < whole) {
+        ask(two, at(n + 1), std::true_type{});
+        add(one);
+        add(two);
+      } else {
+        add(one);
+      }
+    }
+    if (at(whole) < end) {
+      ask(one, at(whole), std::false_type{});
+      add(one);
     }
     if (wave > 0) {
 #pragma unroll
@@ -244,12 +284,12 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
           }
           const int rank = rank0 + 16 * c + 4 * quarter;
           if (slot < count && rank < a.padded) {
-            float4 v;
-            v.x = rank < a.r ? s[0] * scale : 0.0f;
-            v.y = rank + 1 < a.r ? s[1] * scale : 0.0f;
-            v.z = rank + 2 < a.r ? s[2] * scale : 0.0f;
-            v.w = rank + 3 < a.r ? s[3] * scale : 0.0f;
-            *reinterpret_cast<float4*>(
+            floatx4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[k] = rank + k < a.r ? s[k] * scale : 0.0f;
+            }
+            *reinterpret_cast<floatx4*>(
                 a.h + blockIdx.y * a.split_stride + static_cast<int64_t>(rows[slot]) * a.padded +
                 rank) = v;
           }
@@ -263,6 +303,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
 struct ExpandArgs {
   Rows rows;
   const float* h; // [splits, T, padded]
+  float* h_sum;   // null, or where its sum stays: [T, padded]
   int64_t split_stride;
   int splits, padded;
   const void* b; // [adapters, N, r]
@@ -275,9 +316,9 @@ struct ExpandArgs {
   int tile;
 };
 
-// Eight (float32: four) ranks of a token's h: the sum of its parts, times `by`
+// Eight ranks of a token's h times `by`, rounded, or what rounding took from them; float32: four
 template <typename T>
-__device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], int quarter, float by) {
+__device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], bool lower, float by) {
   if constexpr (sizeof(T) == 4) {
     return __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3]));
   } else {
@@ -290,7 +331,7 @@ __device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], int qua
         const float x = v[2 * i + j] * by;
         const float upper = round_to<T>(x);
         // (of what is not finite there is no lower part)
-        part[j] = quarter < 2 ? upper : fabsf(upper) < INFINITY ? x - upper : 0.0f;
+        part[j] = !lower ? upper : fabsf(upper) < INFINITY ? x - upper : 0.0f;
       }
       w[i] = pack2<T>(part[0], part[1]);
     }
@@ -298,63 +339,174 @@ __device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], int qua
   }
 }
 
-template <typename T, int kGroups, int kChunks, bool kAligned>
+template <typename T>
+union Part { // 16 bytes of a row
+  uint4 u;
+  T e[kPer<T>];
+};
+template <typename T, bool kAligned>
+__device__ __forceinline__ void store_part(T* row, int n, int end, const Part<T>& v) {
+  if constexpr (kAligned) {
+    if (n < end) {
+      *reinterpret_cast<uint4*>(row + n) = v.u;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) {
+      if (n + k < end) {
+        row[n + k] = v.e[k];
+      }
+    }
+  }
+}
+
+template <typename T, int kGroups, int kChunks, bool kAligned, bool kAdd>
 __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
+  constexpr int kPitch = 16 * kChunks + 4; // (rows of neighbouring tokens four banks apart)
+  constexpr int kParts = 16 / kPer<T>;     // of a lane's results
   __shared__ int rows[kDecode];
+  __shared__ alignas(16) float held[16 * kGroups][kPitch];
   int adapter;
   const int count = find_rows(a.rows, blockIdx.x, a.tile, rows, &adapter);
   if (count == 0) {
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15;
   const int quarter = lane >> 4;
-  // first of the ranks of a chunk that the lane has
-  const int rank_of = sizeof(T) == 4 ? 4 * quarter : 8 * (quarter & 1);
+  const T* y = static_cast<const T*>(a.y);
+  T* out = static_cast<T*>(a.out);
+  const int n_block = blockIdx.y * a.columns;
+  const int n_end = min(a.N, n_block + a.columns);
+  if (adapter < 0) { // y as it is
+    const int units = (n_end - n_block + kPer<T> - 1) / kPer<T>;
+    for (int n = threadIdx.x; n < count * units; n += 256) {
+      const int t = n / units;
+      const int at = n_block + (n - t * units) * kPer<T>;
+      const int64_t row = rows[t];
+      Part<T> v;
+      v.u = kAdd ? operand<T, kAligned>(y + row * a.y_stride, at, a.N) : uint4{0, 0, 0, 0};
+      store_part<T, kAligned>(out + row * a.N, at, n_end, v);
+    }
+    return;
+  }
+  // An instruction has 16 ranks (float32), 32, or 16 of the upper parts and the same of the lower
+  // ones; of those the lane has kPer from rank_of on
+  constexpr bool kPairs = sizeof(T) == 2 && kChunks > 1;
+  constexpr int kSteps = kPairs ? kChunks / 2 : kChunks;
+  constexpr int kRanks = kPairs ? 32 : 16;
+  const int rank_of = sizeof(T) == 4 ? 4 * quarter : kPairs ? 8 * quarter : 8 * (quarter & 1);
   const T* b = static_cast<const T*>(a.b) + adapter * a.b_stride;
-  const int n_end = min(a.N, static_cast<int>(blockIdx.y + 1) * a.columns);
+  const int n_begin = n_block + 64 * wave;
+  // Of 64 columns a lane's results are 16 bytes of neighbours, the four quarters' side by side: row
+  // 4 q + i of tile j is column 4 V (j / t) + V q + 4 (j % t) + i, V values in 16 bytes, t = V / 4
+  constexpr int kTiles = kPer<T> / 4;
+  uint4 weights[4][kSteps];
+  const auto ask_b = [&](int n0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 4 * kPer<T> * (j / kTiles) + kPer<T> * (column >> 2) + 4 * (j % kTiles) +
+          (column & 3);
+      const T* b_row = b + min(n, a.N - 1) * a.b_row;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        if constexpr (kAligned) { // (r is a multiple of what is read)
+          const int k = kRanks * c + rank_of;
+          const uint4 v = operand<T, true, true>(b_row, min(k, a.r - kPer<T>), a.r);
+          weights[j][c] = k < a.r ? v : uint4{0, 0, 0, 0};
+        } else {
+          weights[j][c] = operand<T, false>(b_row, kRanks * c + rank_of, a.r);
+        }
+      }
+    }
+  };
   for (int base = 0; base < count; base += 16 * kGroups) {
+    const int mine = min(16 * kGroups, count - base);
+    const bool works = n_begin < n_end;
+    if (works) {
+      ask_b(n_begin);
+    }
     int64_t row[kGroups];
-    uint4 h[kGroups][kChunks];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      row[i] = rows[base + min(16 * i + column, mine - 1)];
+    }
+    Part<T> next[kGroups][kParts];
+    const auto ask_y = [&](int n0) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          const int n = n0 + kPer<T> * (quarter + 4 * p);
+          if constexpr (kAligned) { // (what is past the end is not stored)
+            next[i][p].u =
+                operand<T, true, true>(y + row[i] * a.y_stride, min(n, a.N - kPer<T>), a.N);
+          } else {
+            next[i][p].u = operand<T, false>(y + row[i] * a.y_stride, n, a.N);
+          }
+        }
+      }
+    };
+    if (kAdd && works) {
+      ask_y(n_begin);
+    }
+    // the tokens' h, the sum of its parts, for all four wavefronts
+    const int quads = a.padded / 4;
+    for (int n = threadIdx.x; n < mine * quads; n += 256) {
+      const int t = n / quads;
+      const int k = 4 * (n - t * quads);
+      const int64_t at = static_cast<int64_t>(rows[base + t]) * a.padded + k;
+      const float* p = a.h + at;
+      floatx4 v = *reinterpret_cast<const floatx4*>(p);
+      for (int s = 1; s < a.splits; s += 5) { // (five asked for at once; 16 parts at most)
+        floatx4 part[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          part[i] = *reinterpret_cast<const floatx4*>(p + min(s + i, a.splits - 1) * a.split_stride);
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+          if (s + i < a.splits) {
+            v += part[i];
+          }
+        }
+      }
+      *reinterpret_cast<floatx4*>(&held[t][k]) = v;
+      if (a.h_sum != nullptr && blockIdx.y == 0) {
+        *reinterpret_cast<floatx4*>(a.h_sum + at) = v;
+      }
+    }
+    __syncthreads();
+    uint4 h[kGroups][kSteps];
+    uint4 lower[kGroups][kPairs ? kSteps : 1];
     float back[kGroups]; // float16: what h was divided by
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      row[i] = rows[min(base + 16 * i + column, count - 1)];
-      back[i] = 1.0f;
-      if (adapter < 0) {
-        continue;
-      }
-      float v[kChunks][kPer<T>];
+      const int t = min(16 * i + column, mine - 1);
+      float v[kSteps][kPer<T>];
       float most = 0.0f;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
+      for (int c = 0; c < kSteps; ++c) {
 #pragma unroll
-        for (int j = 0; j < kPer<T>; ++j) {
-          v[c][j] = 0.0f;
-        }
-        if (16 * c < a.padded) {
-          const float* p = a.h + row[i] * a.padded + 16 * c + rank_of;
-          for (int s = 0; s < a.splits; ++s, p += a.split_stride) {
-#pragma unroll
-            for (int j = 0; j < kPer<T>; j += 4) {
-              const float4 q = *reinterpret_cast<const float4*>(p + j);
-              v[c][j] += q.x;
-              v[c][j + 1] += q.y;
-              v[c][j + 2] += q.z;
-              v[c][j + 3] += q.w;
-            }
+        for (int j = 0; j < kPer<T>; j += 4) {
+          floatx4 q = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (kRanks * c + rank_of < a.padded) {
+            q = *reinterpret_cast<const floatx4*>(&held[t][kRanks * c + rank_of + j]);
           }
-        }
 #pragma unroll
-        for (int j = 0; j < kPer<T>; ++j) {
-          const float m = fabsf(v[c][j]);
-          most = m < INFINITY ? fmaxf(most, m) : most;
+          for (int k = 0; k < 4; ++k) {
+            v[c][j + k] = q[k];
+            const float m = fabsf(q[k]);
+            most = m < INFINITY ? fmaxf(most, m) : most;
+          }
         }
       }
       float by = 1.0f;
+      back[i] = 1.0f;
       if constexpr (std::is_same_v<T, f16_t>) {
         most = fmaxf(most, __shfl_xor(most, 16, 64)); // (the other ranks' lanes)
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
         // 2^13 over the power of two below the largest: exponents 13 - e and e - 13
         const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;
         const int up = min(max(13 - e, -100), 100);
@@ -362,69 +514,68 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
         back[i] = most > 0.0f ? __uint_as_float(static_cast<uint32_t>(127 - up) << 23) : 1.0f;
       }
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        h[i][c] = rank_operand<T>(v[c], quarter, by);
+      for (int c = 0; c < kSteps; ++c) {
+        if constexpr (kPairs) {
+          h[i][c] = rank_operand<T>(v[c], false, by);
+          lower[i][c] = rank_operand<T>(v[c], true, by);
+        } else {
+          h[i][c] = rank_operand<T>(v[c], quarter >= 2, by);
+        }
       }
     }
-    for (int n0 = blockIdx.y * a.columns + 64 * wave; n0 < n_end; n0 += 256) {
-      // Columns 16 q + 4 j + i of the 64 are row 4 q + i of the j-th tile, so that a lane's
-      // results are 16 neighbours
+    const auto columns = [&](int n0, auto more) {
       floatx4 sum[kGroups][4] = {};
-      if (adapter >= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = min(n0 + 16 * (column >> 2) + 4 * j + (column & 3), a.N - 1);
-          const T* b_row = b + n * a.b_row;
+      for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const uint4 v = operand<T, kAligned>(b_row, 16 * c + rank_of, a.r);
+        for (int c = 0; c < kSteps; ++c) {
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-              multiply<T>(v, h[i][c], sum[i][j]);
+          for (int i = 0; i < kGroups; ++i) {
+            multiply<T>(weights[j][c], h[i][c], sum[i][j]);
+            if constexpr (kPairs) {
+              multiply<T>(weights[j][c], lower[i][c], sum[i][j]);
             }
           }
         }
       }
-      const int n = n0 + 16 * quarter;
+      Part<T> v[kGroups][kParts];
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        if (base + 16 * i + column >= count) {
-          continue;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          v[i][p] = next[i][p];
         }
-        const T* y = a.y == nullptr ? nullptr : static_cast<const T*>(a.y) + row[i] * a.y_stride + n;
-        T* out = static_cast<T*>(a.out) + row[i] * a.N + n;
+      }
+      if constexpr (more.value) {
+        ask_b(n0 + 256);
+        if constexpr (kAdd) {
+          ask_y(n0 + 256);
+        }
+      }
 #pragma unroll
-        for (int part = 0; part < 16; part += kPer<T>) {
-          union {
-            uint4 u;
-            T e[kPer<T>];
-          } raw;
-          raw.u = uint4{0, 0, 0, 0};
-          if (y != nullptr) {
-            raw.u = operand<T, kAligned>(y + part, 0, a.N - n - part);
+      for (int i = 0; i < kGroups; ++i) {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+          for (int k = 0; k < kPer<T>; ++k) {
+            const float s = sum[i][kTiles * p + k / 4][k % 4] * back[i];
+            v[i][p].e[k] = from_f32<T>(kAdd ? to_f32(v[i][p].e[k]) + s : s);
           }
-          if (adapter >= 0) {
-#pragma unroll
-            for (int k = 0; k < kPer<T>; ++k) {
-              const float s = sum[i][(part + k) / 4][k % 4] * back[i];
-              raw.e[k] = from_f32<T>(y == nullptr ? s : to_f32(raw.e[k]) + s);
-            }
-          }
-          if constexpr (kAligned) {
-            if (n + part < a.N) {
-              *reinterpret_cast<uint4*>(out + part) = raw.u;
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < kPer<T>; ++k) {
-              if (n + part + k < a.N) {
-                out[part + k] = raw.e[k];
-              }
-            }
+          if (16 * i + column < mine) {
+            store_part<T, kAligned>(
+                out + row[i] * a.N, n0 + kPer<T> * (quarter + 4 * p), a.N, v[i][p]);
           }
         }
       }
+    };
+    if (works) {
+      int n0 = n_begin;
+      for (; n0 + 256 < n_end; n0 += 256) {
+        columns(n0, std::true_type{});
+      }
+      columns(n0, std::false_type{});
     }
+    __syncthreads(); // (the next tokens' h)
   }
 }
 
@@ -442,9 +593,13 @@ struct GroupArgs {
 
 constexpr int kGroupWaves = 8;
 
-// One workgroup; wavefront w has entries [w, w + 1) * run.  LDS: counts[wavefronts][adapters + 1].
+// One workgroup; wavefront w has entries [w, w + 1) * run.  LDS: (wavefronts + 5) (adapters + 1)
+// numbers.
 __global__ __launch_bounds__(64 * kGroupWaves) void group_kernel(const GroupArgs a) {
   extern __shared__ int32_t before[]; // [wave][adapter], the last "adapter" is none
+  // of each: first entry, tile, segment and partial sum; entries
+  int32_t* places = before + kGroupWaves * (a.adapters + 1);
+  int32_t* totals = places + 4 * (a.adapters + 1);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int buckets = a.adapters + 1;
@@ -515,16 +670,11 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_kernel(const GroupArgs
         for (int w = 0; w < kGroupWaves; ++w) {
           before[w * buckets + of] += at;
         }
-        const int adapter = of < a.adapters ? of : -1;
-        for (int i = 0; i < tiles; ++i) {
-          a.tiles[tile + up[1] - tiles + i] =
-              Tile{adapter, at * a.span + i * a.tile, min(a.tile, rows - i * a.tile), -1};
-        }
-        for (int i = 0; i < segments; ++i) {
-          a.segments[segment + up[2] - segments + i] =
-              Tile{adapter, at * a.span + i * a.segment, min(a.segment, rows - i * a.segment),
-                   slots > 0 ? slot + up[3] - slots + i : -1};
-        }
+        places[4 * of] = at;
+        places[4 * of + 1] = tile + up[1] - tiles;
+        places[4 * of + 2] = segment + up[2] - segments;
+        places[4 * of + 3] = slots > 0 ? slot + up[3] - slots : -1;
+        totals[of] = sum;
         if (a.segment != 0 && of < a.adapters) {
           a.slots[2 * of] = segments == 1 ? -1 : slot + up[3] - slots;
           a.slots[2 * of + 1] = slots;
@@ -541,6 +691,24 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_kernel(const GroupArgs
     }
   }
   __syncthreads();
+  // the tiles and segments of a bucket by a wavefront
+  for (int of = wave; of < buckets; of += kGroupWaves) {
+    const int rows = totals[of] * a.span;
+    const int from = places[4 * of] * a.span;
+    const int adapter = of < a.adapters ? of : -1;
+    for (int i = lane; i * a.tile < rows; i += 64) {
+      a.tiles[places[4 * of + 1] + i] =
+          Tile{adapter, from + i * a.tile, min(a.tile, rows - i * a.tile), -1};
+    }
+    if (a.segment != 0 && adapter >= 0) {
+      const int slot = places[4 * of + 3];
+      for (int i = lane; i * a.segment < rows; i += 64) {
+        a.segments[places[4 * of + 2] + i] =
+            Tile{adapter, from + i * a.segment, min(a.segment, rows - i * a.segment),
+                 slot < 0 ? -1 : slot + i};
+      }
+    }
+  }
   each([&](int i, int which, uint64_t same) {
     const int at = mine[which]; // (read by all before one writes: they are one wavefront)
     if (same >> lane & 1) {
@@ -554,32 +722,42 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_kernel(const GroupArgs
 
 // ---------------------------------------------------------------- turned weights
 struct TurnArgs {
-  const void* from; // [adapters, R, C]
-  void* to;         // [adapters, C, padded]: padded >= R, zeros behind
-  int R, C, padded;
+  struct {
+    const void* from; // [adapters, R, C]
+    void* to;         // [adapters, C, padded]: padded >= R, zeros behind
+    int R, C, padded, across; // blocks of 64 columns
+    int64_t blocks;
+  } of[2]; // B, and A (no blocks where it is not wanted)
   const int32_t* slots; // of adapters that are not in use: {0 or more, 0}
 };
 template <typename T>
 __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a) {
   __shared__ T tile[64][65 + (sizeof(T) == 2 ? 1 : 0)];
-  const int adapter = blockIdx.z;
+  const int adapter = blockIdx.y;
   if (a.slots[2 * adapter] >= 0 && a.slots[2 * adapter + 1] == 0) {
     return;
   }
-  const int c0 = blockIdx.x * 64;
-  const int r0 = blockIdx.y * 64;
-  const T* from = static_cast<const T*>(a.from) + static_cast<int64_t>(adapter) * a.R * a.C;
-  T* to = static_cast<T*>(a.to) + static_cast<int64_t>(adapter) * a.C * a.padded;
-  const int x = threadIdx.x & 63;
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-    const bool is = r0 + i < a.R && c0 + x < a.C;
-    tile[i][x] = is ? from[static_cast<int64_t>(r0 + i) * a.C + c0 + x] : static_cast<T>(0.0f);
+  const bool second = blockIdx.x >= a.of[0].blocks;
+  const auto& m = a.of[second];
+  const int block = blockIdx.x - (second ? static_cast<int>(a.of[0].blocks) : 0);
+  const int c0 = block % m.across * 64;
+  const int r0 = block / m.across * 64;
+  const T* from = static_cast<const T*>(m.from) + static_cast<int64_t>(adapter) * m.R * m.C;
+  T* to = static_cast<T*>(m.to) + static_cast<int64_t>(adapter) * m.C * m.padded;
+  // (a matrix of few columns or rows has few here, too)
+  const int columns = min(64, m.C - c0);
+  const int rows = min(64, m.padded - r0);
+  for (int n = threadIdx.x; n < rows * columns; n += 256) {
+    const int y = n / columns;
+    const int x = n - y * columns;
+    tile[y][x] =
+        r0 + y < m.R ? from[static_cast<int64_t>(r0 + y) * m.C + c0 + x] : static_cast<T>(0.0f);
   }
   __syncthreads();
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-    if (c0 + i < a.C && r0 + x < a.padded) {
-      to[static_cast<int64_t>(c0 + i) * a.padded + r0 + x] = tile[x][i];
-    }
+  for (int n = threadIdx.x; n < rows * columns; n += 256) {
+    const int y = n / rows;
+    const int x = n - y * rows;
+    to[static_cast<int64_t>(c0 + y) * m.padded + r0 + x] = tile[x][y];
   }
 }
 
@@ -599,72 +777,98 @@ struct TokenArgs {
 
 constexpr int kTokens = 32;  // of a tile in LDS
 constexpr int kColumns = 256;
+constexpr int kMostSegment = 2048;
 
 // The result's rows are columns of q, its columns are ranks: kChunks of 16.  A wavefront has 64
-// columns of q, in the order of expand_kernel.
+// columns of q, in the order of expand_kernel.  Two tiles of 32 tokens in LDS: one is read while
+// the other's loads are in flight.
 template <typename T, int kChunks, bool kAligned>
 __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
   // (rows a quarter of the banks apart, so that the four rows of a transposed read do not meet)
   constexpr int kPitch = kColumns + 32 / sizeof(T);
-  __shared__ alignas(16) T q_tile[kTokens][kPitch];
-  __shared__ float p_tile[kTokens][16 * kChunks + 4];
+  __shared__ alignas(16) T q_tile[2][kTokens][kPitch];
+  __shared__ alignas(16) float p_tile[2][kTokens][16 * kChunks + 4];
+  __shared__ int rows[kMostSegment];
   if (static_cast<int>(blockIdx.x) >= *a.rows.n_tiles) {
     return;
   }
   const Tile tile = a.rows.tiles[blockIdx.x];
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15;
   const int quarter = lane >> 4;
   const int c0 = blockIdx.y * kColumns;
   const int rank0 = blockIdx.z * kChunks * 16;
+  for (int n = threadIdx.x; n < tile.rows; n += 256) {
+    rows[n] = a.rows.row(tile.first + n);
+  }
+  __syncthreads();
   floatx4 sum[4][kChunks] = {};
-  for (int first = 0; first < tile.rows; first += kTokens) {
-    const int count = min(kTokens, tile.rows - first);
-    constexpr int kUnits = kColumns / kPer<T>;
-    uint4 got[kTokens * kUnits / 256];
+  constexpr int kUnits = kColumns / kPer<T>;
+  constexpr int kLoads = kTokens * kUnits / 256;
+  constexpr int kQuads = kTokens * 4 * kChunks; // of p
+  constexpr int kPLoads = (kQuads + 255) / 256;
+  uint4 got[kLoads];
+  floatx4 p_got[kPLoads];
+  const auto ask = [&](int first) {
 #pragma unroll
-    for (int i = 0; i < kTokens * kUnits / 256; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       const int n = i * 256 + threadIdx.x;
-      const int t = n / kUnits;
+      const int t = first + n / kUnits;
       const int c = c0 + (n % kUnits) * kPer<T>;
       got[i] = uint4{0, 0, 0, 0};
-      if (t < count && c < a.W) {
-        const int64_t row = a.rows.row(tile.first + first + t);
-        got[i] = operand<T, kAligned>(static_cast<const T*>(a.q) + row * a.q_stride, c, a.W);
+      if (t < tile.rows && c < a.W) {
+        got[i] = operand<T, kAligned>(
+            static_cast<const T*>(a.q) + rows[t] * a.q_stride, c, a.W);
       }
     }
-    __syncthreads(); // (the last tile has been read)
 #pragma unroll
-    for (int i = 0; i < kTokens * kUnits / 256; ++i) {
+    for (int i = 0; i < kPLoads; ++i) {
       const int n = i * 256 + threadIdx.x;
-      *reinterpret_cast<uint4*>(&q_tile[n / kUnits][(n % kUnits) * kPer<T>]) = got[i];
-    }
-    for (int n = threadIdx.x; n < kTokens * 16 * kChunks; n += 256) {
-      const int t = n / (16 * kChunks);
-      const int k = n % (16 * kChunks);
-      float v = 0.0f;
-      if (t < count && rank0 + k < a.r) {
-        const float* p =
-            a.p + static_cast<int64_t>(a.rows.row(tile.first + first + t)) * a.padded + rank0 + k;
-        for (int i = 0; i < a.splits; ++i) {
-          v += p[i * a.split_stride];
+      const int t = first + n / (4 * kChunks);
+      const int k = rank0 + n % (4 * kChunks) * 4;
+      p_got[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (n < kQuads && t < tile.rows && k < a.padded) {
+        const float* p = a.p + static_cast<int64_t>(rows[t]) * a.padded + k;
+        for (int s = 0; s < a.splits; ++s) {
+          p_got[i] += *reinterpret_cast<const floatx4*>(p + s * a.split_stride);
         }
       }
-      p_tile[t][k] = v;
+    }
+  };
+  ask(0);
+  int which = 0;
+  for (int first = 0; first < tile.rows; first += kTokens, which ^= 1) {
+    // (the other of the two tiles may still be read)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = i * 256 + threadIdx.x;
+      *reinterpret_cast<uint4*>(&q_tile[which][n / kUnits][(n % kUnits) * kPer<T>]) = got[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kPLoads; ++i) {
+      const int n = i * 256 + threadIdx.x;
+      if (n < kQuads) {
+        *reinterpret_cast<floatx4*>(
+            &p_tile[which][n / (4 * kChunks)][n % (4 * kChunks) * 4]) = p_got[i];
+      }
     }
     __syncthreads();
+    if (first + kTokens < tile.rows) {
+      ask(first + kTokens);
+    }
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int t0 = 0; t0 < kTokens; t0 += 4) {
         float q[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          q[j] = q_tile[t0 + quarter][64 * wave + 16 * (column >> 2) + 4 * j + (column & 3)];
+          q[j] = q_tile[which][t0 + quarter]
+                      [64 * wave + 16 * j + column];
         }
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          const float p = p_tile[t0 + quarter][16 * c + column];
+          const float p = p_tile[which][t0 + quarter][16 * c + column];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             sum[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j], p, sum[j][c], 0, 0, 0);
@@ -679,8 +883,8 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
         uint32_t w[2][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = p_tile[8 * quarter + 2 * i][16 * c + column];
-          const float y = p_tile[8 * quarter + 2 * i + 1][16 * c + column];
+          const float x = p_tile[which][8 * quarter + 2 * i][16 * c + column];
+          const float y = p_tile[which][8 * quarter + 2 * i + 1][16 * c + column];
           const float x_upper = round_to<bf16_t>(x);
           const float y_upper = round_to<bf16_t>(y);
           w[0][i] = pack2<bf16_t>(x_upper, y_upper);
@@ -699,7 +903,8 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
         for (int half = 0; half < 2; ++half) {
           const int t = 8 * quarter + 4 * half + (column >> 2);
           const uint32_t at =
-              lds_address(&q_tile[t][64 * wave + 16 * (column & 3) + 4 * j]);
+              lds_address(
+              &q_tile[which][t][64 * wave + 32 * (j / 2) + 8 * (column & 3) + 4 * (j % 2)]);
           const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) shortx4*)(LdsBytes)(uintptr_t)at);
           const uint2 u = __builtin_bit_cast(uint2, x);
@@ -739,8 +944,7 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
       }
     }
   }
-  // A lane has 16 neighbouring columns of q for rank 16 c + column
-  const int n = c0 + 64 * wave + 16 * quarter;
+  // A lane has 16 bytes of neighbouring columns of q (float32: 4, else 8) for rank 16 c + column
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
     const int rank = rank0 + 16 * c + column;
@@ -748,17 +952,31 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
       continue;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (n + i >= a.W) {
+    for (int j = 0; j < 4; ++j) {
+      constexpr int kTiles = kPer<T> / 4;
+      const int n = c0 + 64 * wave + 4 * kPer<T> * (j / kTiles) + kPer<T> * quarter + 4 * (j % kTiles);
+      const floatx4 v = sum[j][c];
+      if (tile.slot >= 0) {
+        float* to = a.parts + (static_cast<int64_t>(tile.slot) * a.r + rank) * a.W + n;
+        if (kAligned && n < a.W) { // (W is a multiple of 4 at least, the parts are aligned)
+          *reinterpret_cast<floatx4*>(to) = v;
+          continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (n + i < a.W) {
+            to[i] = v[i];
+          }
+        }
         continue;
       }
-      const float v = sum[i / 4][c][i % 4];
-      if (tile.slot >= 0) {
-        a.parts[(static_cast<int64_t>(tile.slot) * a.r + rank) * a.W + n + i] = v;
-      } else {
-        T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tile.adapter) * a.r * a.W;
-        out[a.turned ? static_cast<int64_t>(n + i) * a.r + rank
-                     : static_cast<int64_t>(rank) * a.W + n + i] = from_f32<T>(v);
+      T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tile.adapter) * a.r * a.W;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n + i < a.W) {
+          out[a.turned ? static_cast<int64_t>(n + i) * a.r + rank
+                       : static_cast<int64_t>(rank) * a.W + n + i] = from_f32<T>(v[i]);
+        }
       }
     }
   }
@@ -793,7 +1011,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
 // Sizes of a call and where things lie in its workspace, in bytes
 struct Plan {
   bool grouped;
-  int tile, groups;  // rows of a tile: 16 groups
+  int tile; // rows of a tile
   int chunks;        // of 16 ranks in a workgroup of shrink and of sums over tokens
   int rank_blocks;
   int padded;
@@ -801,7 +1019,7 @@ struct Plan {
   int splits, per_split; // of K (forward) or N (gradients)
   int columns;           // of a workgroup of expand
   int segment, most_segments, most_slots;
-  size_t order, tiles, counts, segments, slots, h, h_bytes, turned_a, turned_b, parts, bytes;
+  size_t order, tiles, counts, segments, slots, h, g_sum, turned_a, turned_b, parts, bytes;
   int padded_n;
 };
 
@@ -831,17 +1049,16 @@ Plan plan_of(const Sizes& s, bool gradients) {
   p.chunks = chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8;
   p.rank_blocks = (chunks + p.chunks - 1) / p.chunks;
   const bool few = s.T <= kDecode;
-  p.groups = few || p.chunks == 8 ? 1 : 2;
-  p.tile = 16 * p.groups;
+  p.tile = few || p.chunks == 8 ? 16 : 32;
   const int64_t kinds = s.n < s.adapters + 1 ? s.n : s.adapters + 1;
   const int64_t tiles = p.grouped ? s.T / p.tile + kinds
       : s.n == 1                  ? (s.T + p.tile - 1) / p.tile
                                   : s.n;
   p.most_tiles = static_cast<int>(tiles);
-  // parts of a sum until there are two workgroups a CU, each with two steps of its wavefronts
+  // parts of a sum until there is a workgroup for each CU
   const int sum_over = gradients ? s.N : s.K;
   int splits = 1;
-  while (splits < 16 && tiles * p.rank_blocks * splits < 512 &&
+  while (splits < 16 && tiles * p.rank_blocks * splits < 256 &&
          sum_over >= 2 * splits * 4 * step * 2) {
     splits *= 2;
   }
@@ -849,7 +1066,7 @@ Plan plan_of(const Sizes& s, bool gradients) {
   p.splits = (sum_over + p.per_split - 1) / p.per_split;
   const int out_columns = gradients ? s.K : s.N;
   p.columns = 256;
-  while (p.columns < 2048 && tiles * ((out_columns + 2 * p.columns - 1) / (2 * p.columns)) >= 2048) {
+  while (p.columns < 1024 && tiles * ((out_columns + 2 * p.columns - 1) / (2 * p.columns)) >= 512) {
     p.columns *= 2;
   }
   size_t at = 0;
@@ -858,13 +1075,15 @@ Plan plan_of(const Sizes& s, bool gradients) {
     p.tiles = claim(at, sizeof(Tile) * p.most_tiles);
     p.counts = claim(at, sizeof(int32_t) * 2);
   }
-  p.h_bytes = sizeof(float) * p.splits * s.T * p.padded;
-  p.h = claim(at, p.h_bytes); // (gradients: g)
+  p.h = claim(at, sizeof(float) * p.splits * s.T * p.padded); // (gradients: g)
+  if (gradients) {
+    p.g_sum = claim(at, sizeof(float) * s.T * p.padded);
+  }
   if (gradients) {
     const int wide = s.K > s.N ? s.K : s.N;
-    const int64_t blocks = (wide + kColumns - 1) / kColumns;
-    int64_t segment = s.T * blocks * p.rank_blocks / 1024 / kTokens * kTokens;
-    p.segment = static_cast<int>(segment < 64 ? 64 : segment > 4096 ? 4096 : segment);
+    const int64_t blocks = ((s.K + s.N - wide) + kColumns - 1) / kColumns; // of the narrower sums
+    int64_t segment = s.T * blocks * p.rank_blocks / 320 / kTokens * kTokens;
+    p.segment = static_cast<int>(segment < 64 ? 64 : segment > kMostSegment ? kMostSegment : segment);
     p.most_segments = static_cast<int>(s.T / p.segment + kinds);
     p.most_slots = static_cast<int>(2 * (s.T / p.segment) + 1);
     p.segments = claim(at, sizeof(Tile) * p.most_segments);
@@ -882,7 +1101,7 @@ int check_sizes(const char* tag, const Sizes& s) {
   if (!valid_dtype(s.dtype)) {
     return fail(MLXROCM_INVALID_ARGUMENT, "[%s] unknown dtype %d", tag, s.dtype);
   }
-  if (s.T < 0 || s.n < 0 || s.K < 0 || s.N < 0 || (s.n == 0 ? s.T != 0 : s.T % s.n != 0)) {
+  if (s.T < 0 || s.n < 0 || s.K < 1 || s.N < 1 || (s.n == 0 ? s.T != 0 : s.T % s.n != 0)) {
     return fail(
         MLXROCM_INVALID_ARGUMENT, "[%s] %d indices for %lld rows of %d and %d", tag, s.n,
         static_cast<long long>(s.T), s.K, s.N);
@@ -921,25 +1140,37 @@ int shrink(const ShrinkArgs& a, const Plan& p, bool aligned, hipStream_t stream)
   return by_chunks(p.chunks, aligned, [&](auto chunks, auto is) {
     constexpr int c = decltype(chunks)::value;
     constexpr bool al = decltype(is)::value;
-    if (p.groups == 1) {
-      shrink_kernel<T, 1, c, al><<<grid, 256, 0, stream>>>(a);
-    } else if constexpr (c < 8) {
-      shrink_kernel<T, 2, c, al><<<grid, 256, 0, stream>>>(a);
+    if constexpr (al && c <= 4) {
+      if (p.tile == 32) {
+        shrink_kernel<T, 2, c, al><<<grid, 256, 0, stream>>>(a);
+        return;
+      }
     }
+    shrink_kernel<T, 1, c, al><<<grid, 256, 0, stream>>>(a); // (in several turns)
   });
 }
 
 template <typename T>
 int expand(const ExpandArgs& a, const Plan& p, bool aligned, hipStream_t stream) {
   const dim3 grid(p.most_tiles, (a.N + p.columns - 1) / p.columns);
-  const auto go = [&](auto chunks, auto is) {
+  const auto launch = [&](auto groups, auto chunks, auto is) {
+    constexpr int g = decltype(groups)::value;
     constexpr int c = decltype(chunks)::value;
     constexpr bool al = decltype(is)::value;
-    if (p.groups == 1) {
-      expand_kernel<T, 1, c, al><<<grid, 256, 0, stream>>>(a);
-    } else if constexpr (c < 8) {
-      expand_kernel<T, 2, c, al><<<grid, 256, 0, stream>>>(a);
+    if (a.y != nullptr) {
+      expand_kernel<T, g, c, al, true><<<grid, 256, 0, stream>>>(a);
+    } else {
+      expand_kernel<T, g, c, al, false><<<grid, 256, 0, stream>>>(a);
     }
+  };
+  const auto go = [&](auto chunks, auto is) {
+    if constexpr (decltype(is)::value && decltype(chunks)::value <= 4) {
+      if (p.tile == 32) {
+        launch(IntC<2>{}, chunks, is);
+        return;
+      }
+    }
+    launch(IntC<1>{}, chunks, is);
   };
   if (p.padded > 128) {
     if (aligned) {
@@ -962,7 +1193,7 @@ int token_sums(const TokenArgs& a, const Plan& p, bool aligned, hipStream_t stre
 }
 
 int group(const GroupArgs& a, hipStream_t stream) {
-  const size_t lds = sizeof(int32_t) * kGroupWaves * (a.adapters + 1);
+  const size_t lds = sizeof(int32_t) * (kGroupWaves + 5) * (a.adapters + 1);
   group_kernel<<<1, 64 * kGroupWaves, lds, stream>>>(a);
   MLXROCM_HIP_TRY(hipGetLastError());
   return MLXROCM_OK;
@@ -1045,7 +1276,9 @@ extern "C" size_t mlxrocm_adapter_matmul_h_size(
     int64_t rows, int n_indices, int adapters, int rank, int K, int N, int dtype) {
   using namespace mlxrocm;
   const Sizes s{rows, n_indices, adapters, rank, K, N, dtype};
-  return check_sizes("adapter_matmul", s) != MLXROCM_OK || rows == 0 ? 0 : plan_of(s, false).h_bytes;
+  return check_sizes("adapter_matmul", s) != MLXROCM_OK
+      ? 0
+      : sizeof(float) * static_cast<size_t>(rows) * round_up(rank, 16);
 }
 
 extern "C" int mlxrocm_adapter_matmul(
@@ -1079,8 +1312,7 @@ extern "C" int mlxrocm_adapter_matmul(
     return rc;
   }
   const Plan p = plan_of(s, false);
-  if ((N > 0 && (out == nullptr || b == nullptr)) || (K > 0 && (x == nullptr || a == nullptr)) ||
-      (indices == nullptr && n_indices != 1) || (p.bytes > 0 && workspace == nullptr)) {
+  if (out == nullptr || b == nullptr || x == nullptr || a == nullptr || (indices == nullptr && n_indices != 1) || (p.bytes > 0 && workspace == nullptr)) {
     return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer", tag);
   }
   if (workspace_bytes < p.bytes) {
@@ -1098,10 +1330,8 @@ extern "C" int mlxrocm_adapter_matmul(
     }
   }
   const Rows r = rows_of(s, p, indices, ws);
-  if (h == nullptr) {
-    h = reinterpret_cast<float*>(ws + p.h);
-  }
-  ShrinkArgs sa = shrinking(s, p, r, h);
+  float* parts = reinterpret_cast<float*>(ws + p.h);
+  ShrinkArgs sa = shrinking(s, p, r, parts);
   sa.x = x;
   sa.x_stride = x_stride;
   sa.a = a;
@@ -1110,7 +1340,8 @@ extern "C" int mlxrocm_adapter_matmul(
   sa.scales = scales;
   sa.scale = scale;
   sa.K = K;
-  ExpandArgs ea = expanding(s, p, r, h);
+  ExpandArgs ea = expanding(s, p, r, parts);
+  ea.h_sum = h;
   ea.b = b;
   ea.b_stride = static_cast<int64_t>(N) * rank;
   ea.b_row = rank;
@@ -1121,15 +1352,9 @@ extern "C" int mlxrocm_adapter_matmul(
   ea.out = out;
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (p.splits > 0) {
-      const int status =
-          shrink<T>(sa, p, aligned16(x, x_stride, size) && aligned16(a, K, size), st);
-      if (status != MLXROCM_OK) {
-        return status;
-      }
-    }
-    if (N == 0) {
-      return static_cast<int>(MLXROCM_OK);
+    const int status = shrink<T>(sa, p, aligned16(x, x_stride, size) && aligned16(a, K, size), st);
+    if (status != MLXROCM_OK) {
+      return status;
     }
     return expand<T>(
         ea, p,
@@ -1180,9 +1405,7 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
     return rc;
   }
   const Plan p = plan_of(s, true);
-  const Plan forward = plan_of(s, false);
-  if ((K > 0 && (x == nullptr || a == nullptr)) || (N > 0 && (b == nullptr || dout == nullptr)) ||
-      (indices == nullptr && n_indices != 1) || (db != nullptr && h == nullptr) ||
+  if (x == nullptr || a == nullptr || b == nullptr || dout == nullptr || (indices == nullptr && n_indices != 1) || (db != nullptr && h == nullptr) ||
       workspace == nullptr) {
     return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer", tag);
   }
@@ -1204,12 +1427,21 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
   runs.tiles = grouped.segments;
   runs.n_tiles = grouped.counts + 1;
   float* g = reinterpret_cast<float*>(ws + p.h);
+  float* g_sum = reinterpret_cast<float*>(ws + p.g_sum);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const auto turn = [&](const void* from, size_t to, int R, int C, int padded) {
-      const TurnArgs ta{from, ws + to, R, C, padded, grouped.slots};
-      const dim3 grid((C + 63) / 64, (padded + 63) / 64, adapters);
+    const auto turn = [&](bool both) {
+      const auto tiles = [](int n) { return (n + 63) / 64; };
+      TurnArgs ta{};
+      ta.of[0] = {b, ws + p.turned_b, N, rank, p.padded_n, tiles(rank),
+                  static_cast<int64_t>(tiles(rank)) * tiles(p.padded_n)};
+      if (both) {
+        ta.of[1] = {a, ws + p.turned_a, rank, K, p.padded, tiles(K),
+                    static_cast<int64_t>(tiles(K)) * tiles(p.padded)};
+      }
+      ta.slots = grouped.slots;
+      const dim3 grid(static_cast<unsigned>(ta.of[0].blocks + ta.of[1].blocks), adapters);
       turn_kernel<T><<<grid, 256, 0, st>>>(ta);
       return hipGetLastError();
     };
@@ -1238,48 +1470,47 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
       MLXROCM_HIP_TRY(hipGetLastError());
       return static_cast<int>(MLXROCM_OK);
     };
-    if (K > 0 && (dx != nullptr || da != nullptr)) {
-      if (N > 0) {
-        MLXROCM_HIP_TRY(turn(b, p.turned_b, N, rank, p.padded_n));
-        ShrinkArgs sa = shrinking(s, p, r, g);
-        sa.x = dout;
-        sa.x_stride = dout_stride;
-        sa.a = ws + p.turned_b;
-        sa.a_stride = static_cast<int64_t>(rank) * p.padded_n;
-        sa.a_row = p.padded_n;
-        sa.scales = scales;
-        sa.scale = scale;
-        sa.K = N;
-        const int done = shrink<T>(
-            sa, p,
-            aligned16(dout, dout_stride, size) && static_cast<size_t>(N) * size % 16 == 0, st);
-        if (done != MLXROCM_OK) {
-          return done;
-        }
-      }
-      if (dx != nullptr) {
-        MLXROCM_HIP_TRY(turn(a, p.turned_a, rank, K, p.padded));
-        ExpandArgs ea = expanding(s, p, r, g);
-        ea.b = ws + p.turned_a;
-        ea.b_stride = static_cast<int64_t>(K) * p.padded;
-        ea.b_row = p.padded;
-        ea.N = K;
-        ea.r = p.padded;
-        ea.out = dx;
-        const int done = expand<T>(ea, p, aligned16(dx, K, size), st);
-        if (done != MLXROCM_OK) {
-          return done;
-        }
-      }
-      if (da != nullptr) {
-        const int done = sums(g, p.splits, x, x_stride, K, da, 0);
-        if (done != MLXROCM_OK) {
-          return done;
-        }
+    const bool needs_g = dx != nullptr || da != nullptr;
+    if (needs_g) {
+      MLXROCM_HIP_TRY(turn(dx != nullptr));
+      ShrinkArgs sa = shrinking(s, p, r, g);
+      sa.x = dout;
+      sa.x_stride = dout_stride;
+      sa.a = ws + p.turned_b;
+      sa.a_stride = static_cast<int64_t>(rank) * p.padded_n;
+      sa.a_row = p.padded_n;
+      sa.scales = scales;
+      sa.scale = scale;
+      sa.K = N;
+      const int done = shrink<T>(
+          sa, p, aligned16(dout, dout_stride, size) && static_cast<size_t>(N) * size % 16 == 0, st);
+      if (done != MLXROCM_OK) {
+        return done;
       }
     }
-    if (N > 0 && db != nullptr) {
-      return sums(h, forward.splits, dout, dout_stride, N, db, 1);
+    if (db != nullptr) { // (right behind what has read dout already)
+      const int done = sums(h, 1, dout, dout_stride, N, db, 1);
+      if (done != MLXROCM_OK) {
+        return done;
+      }
+    }
+    if (dx != nullptr) {
+      ExpandArgs ea = expanding(s, p, r, g);
+      ea.b = ws + p.turned_a;
+      ea.b_stride = static_cast<int64_t>(K) * p.padded;
+      ea.b_row = p.padded;
+      ea.N = K;
+      ea.r = p.padded;
+      ea.out = dx;
+      ea.h_sum = g_sum;
+      const int done = expand<T>(ea, p, aligned16(dx, K, size), st);
+      if (done != MLXROCM_OK) {
+        return done;
+      }
+    }
+    if (da != nullptr) {
+      return dx != nullptr ? sums(g_sum, 1, x, x_stride, K, da, 0)
+                           : sums(g, p.splits, x, x_stride, K, da, 0);
     }
     return static_cast<int>(MLXROCM_OK);
   });
