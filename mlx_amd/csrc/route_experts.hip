@@ -6,13 +6,17 @@
 // lowest index first where they are equal.  Weights w = scale s, or scale s / (sum of the chosen s).
 //
 // Choices decide what is computed, so their order is taken exactly: of the logits themselves where
-// they have the scores' order (no bias, no sums), else of choices formed in 64 bits.  Compared are
-// integers of the floats' order, with room below the lowest for what is taken already.
+// they have the scores' order (no bias, no sums), else of choices in 64 bits.  Those are formed in 32
+// bits first; where all that are chosen, and the first that is not, are further apart than 32 bits can be
+// off, the order is known, and only a wavefront with a row where they are not forms them in 64.  Compared
+// are integers of the floats' order, with room below the lowest for what is taken already.
 //
 // What bounds it: the instructions of k searches for the largest.  Sixteen lanes have a row, one of
 // the rows of lanes that DPP instructions rotate within: the largest of sixteen lanes is four
 // instructions, for four rows of a wavefront at once.  A lane holds neighbouring experts of one
 // group, so that the lowest lane that has the largest value has the lowest index.
+#include <type_traits>
+
 #include "common.h"
 
 namespace mlxrocm {
@@ -36,14 +40,16 @@ struct RouteArgs {
   int experts, k, groups, top_groups, group_best;
   int group_size;
   int group_lanes; // lanes of a group, a power of two
-  int sigmoid, normalize, vector;
+  int sigmoid, normalize;
+  int full; // whether every lane has V experts
+  int vector, wide_out, wide_bias; // whether rows of logits, their gradient, bias are aligned (kWide)
   float scale;
 };
 
 // ---- sixteen lanes ----
 template <int Rotate>
 __device__ __forceinline__ int rotated(int v) {
-  return __builtin_amdgcn_update_dpp(v, v, 0x120 + Rotate, 0xf, 0xf, false); // row_ror
+  return __builtin_amdgcn_mov_dpp(v, 0x120 + Rotate, 0xf, 0xf, true); // row_ror
 }
 template <int Rotate>
 __device__ __forceinline__ int64_t rotated(int64_t v) {
@@ -102,40 +108,47 @@ __device__ __forceinline__ double value_of(int64_t key) {
 }
 template <typename K>
 struct Lowest;
+// below every value's: what has been taken (in 32 steps), what does not exist
 template <>
 struct Lowest<int> {
-  using Value = float;
   static constexpr int taken = static_cast<int>(0x80000000u);
+  static constexpr int none = taken + 64;
+  static constexpr int least = static_cast<int>(0x807fffffu); // -inf
 };
 template <>
 struct Lowest<int64_t> {
-  using Value = double;
   static constexpr int64_t taken = static_cast<int64_t>(0x8000000000000000ULL);
+  static constexpr int64_t none = taken + 64;
 };
 
-// e^(l - m) of the largest logit m: 1 where they are equal (both may be infinite), and nothing
-// where there is no logit at all
+// e^(l - m) of the largest logit m: 1 where they are equal (both may be infinite).  Where there is no
+// logit at all (-inf) m is 0, so that nothing is above it.
+__device__ __forceinline__ float base_of(float most) {
+  return most == -INFINITY ? 0.0f : most;
+}
 __device__ __forceinline__ float above(float l, float m) {
-  return m == -INFINITY ? (l != l ? l : 0.0f) : l == m ? 1.0f : expf(l - m);
+  return expf(l == m ? 0.0f : l - m);
 }
 
-// Of the logits of a lane, V of a group's neighbours, those that exist: 0 .. n - 1
+// V of a group's neighbours in a lane are read and written W at a time where all rows allow it
+template <typename T, int V>
+constexpr int kWide = V * sizeof(T) <= 16 ? V : 16 / sizeof(T);
+template <typename T, int W>
+struct alignas(W * sizeof(T)) Wide {
+  T e[W];
+};
+
+// Those that exist: 0 .. n - 1
 template <typename T, int V>
 __device__ __forceinline__ void read_logits(const T* p, int n, int vector, float (&l)[V]) {
-  constexpr int kWide = 16 / sizeof(T);
-  if (V % kWide == 0 && vector && n == V) {
-    if constexpr (V % kWide == 0) {
+  constexpr int W = kWide<T, V>;
+  if (vector && n == V) {
 #pragma unroll
-      for (int j = 0; j < V; j += kWide) {
-        union {
-          uint4 u;
-          T e[kWide];
-        } raw;
-        raw.u = *reinterpret_cast<const uint4*>(p + j);
+    for (int j = 0; j < V; j += W) {
+      const Wide<T, W> raw = *reinterpret_cast<const Wide<T, W>*>(p + j);
 #pragma unroll
-        for (int i = 0; i < kWide; ++i) {
-          l[j + i] = to_f32(raw.e[i]);
-        }
+      for (int i = 0; i < W; ++i) {
+        l[j + i] = to_f32(raw.e[i]);
       }
     }
     return;
@@ -160,37 +173,86 @@ __device__ __forceinline__ Place place_of(const RouteArgs& a) {
   return p;
 }
 
-// Takes the largest of the row out of `keys` and says where it was: its key, and in the lane that
-// had it (the others -1) which of its values.
-template <int V, typename K>
-__device__ __forceinline__ K take(K (&keys)[V], int* which) {
-  K best = keys[0];
-#pragma unroll
-  for (int j = 1; j < V; ++j) {
-    best = max(best, keys[j]);
-  }
-  const K all = largest16(best);
-  const bool mine = first16(best == all) == (threadIdx.x & 15);
-  int at = -1;
-#pragma unroll
-  for (int j = V - 1; j >= 0; --j) {
-    at = mine && keys[j] == all ? j : at;
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    keys[j] = at == j ? Lowest<K>::taken : keys[j];
-  }
-  *which = at;
-  return all;
+// In which step it was taken, kMostChosen: in none
+template <typename K>
+__device__ __forceinline__ int step_of(K key) {
+  return key < Lowest<K>::none ? static_cast<int>(key - Lowest<K>::taken) : kMostChosen;
 }
 
-// Leaves the groups that count
+// Takes the k largest of a row out of `keys`, lowest index first of equal ones, and leaves
+// Lowest::taken + n in the place of the n-th
 template <int V, typename K>
-__device__ __forceinline__ void keep_groups(const RouteArgs& a, const Place& p, K (&keys)[V]) {
-  using F = typename Lowest<K>::Value;
+__device__ __forceinline__ void take_in_order(int k, K (&keys)[V]) {
+  for (int n = 0; n < k; ++n) {
+    K best = keys[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) {
+      best = max(best, keys[j]);
+    }
+    const K all = largest16(best);
+    bool mine = first16(best == all) == (threadIdx.x & 15);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool is = mine && keys[j] == all;
+      keys[j] = is ? Lowest<K>::taken + n : keys[j];
+      mine = mine && !is;
+    }
+  }
+}
+
+// The same where no two are equal or, if `margin` is not negative, nearer to each other than
+// margin (1 + the larger's size): false where two are, whose order this does not tell.  (Without
+// the search for the lowest index: 44 instructions a choice of 16 values a lane instead of 100.)
+template <int V>
+__device__ __forceinline__ bool take(int k, float margin, int (&keys)[V]) {
+  // (equal ones are taken in one step: they show in how many were)
+  const auto taken = [&] {
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      count += keys[j] < Lowest<int>::none;
+    }
+    count += rotated<8>(count);
+    count += rotated<4>(count);
+    count += rotated<2>(count);
+    return count + rotated<1>(count);
+  };
+  bool apart = true;
+  float last = 0.0f;
+  for (int n = 0;; ++n) {
+    int best = keys[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) {
+      best = max(best, keys[j]);
+    }
+    best = largest16(best);
+    if (margin >= 0.0f) {
+      const float v = value_of(best);
+      // (none left: as far as can be.  Infinities and NaN are not apart.)
+      apart = apart && (n == 0 || best < Lowest<int>::least || last - v > margin * (1.0f + fabsf(last)));
+      last = v;
+    }
+    if (n == k) {
+      return apart && taken() == k;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      keys[j] = keys[j] == best ? Lowest<int>::taken + n : keys[j];
+    }
+    if (margin < 0.0f && n + 1 == k) {
+      return true;
+    }
+  }
+}
+
+// Leaves the groups that count; says whether the last that does and the first that does not are
+// further than margin apart (if that is not negative)
+template <int V, typename K>
+__device__ __forceinline__ bool keep_groups(
+    const RouteArgs& a, const Place& p, float margin, K (&keys)[V]) {
   // the largest, and the second largest, of the lane's; then of the group's lanes
-  K one = Lowest<K>::taken;
-  K two = Lowest<K>::taken;
+  K one = Lowest<K>::none;
+  K two = Lowest<K>::none;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     two = max(two, min(one, keys[j]));
@@ -206,19 +268,24 @@ __device__ __forceinline__ void keep_groups(const RouteArgs& a, const Place& p, 
   if (a.group_best == 2) {
     mark = key_of(value_of(one) + value_of(two));
   }
-  mark = p.group < a.groups ? mark : Lowest<K>::taken;
+  mark = p.group < a.groups ? mark : Lowest<K>::none;
   bool stays = false;
+  K last = 0;
   for (int n = 0; n < a.top_groups; ++n) {
-    const K best = largest16(mark);
-    const int lane = first16(mark == best);
-    const bool mine = lane / a.group_lanes == p.group;
+    last = largest16(mark);
+    const bool mine = first16(mark == last) / a.group_lanes == p.group;
     stays |= mine;
-    mark = mine ? Lowest<K>::taken : mark;
+    mark = mine ? Lowest<K>::none : mark;
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    keys[j] = stays ? keys[j] : Lowest<K>::taken;
+    keys[j] = stays ? keys[j] : Lowest<K>::none;
   }
+  if (margin < 0.0f) {
+    return true;
+  }
+  const auto v = value_of(last);
+  return v - value_of(largest16(mark)) > margin * (1 + fabs(v));
 }
 
 struct Chosen {
@@ -228,7 +295,6 @@ struct Chosen {
 
 template <typename T, int V, bool kSums>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
-  using K = std::conditional_t<kSums, int64_t, int>;
   __shared__ Chosen chosen[kRows][kMostChosen];
   const int slot = threadIdx.x / kLanes;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
@@ -246,58 +312,141 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
     for (int j = 0; j < V; ++j) {
       most = fmaxf(most, l[j]);
     }
-    most = largest16(most);
+    most = base_of(largest16(most));
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      total += j < p.n ? above(l[j], most) : 0.0f;
+      total += above(l[j], most); // (what does not exist is -inf)
     }
     total = sum16(total);
   }
+  float b[V];
+  if (kSums && a.bias != nullptr) {
+    read_logits<float, V>(a.bias + p.first, p.n, a.wide_bias, b);
+  }
 
-  K keys[V];
-  if constexpr (kSums) {
-    double sum = 0.0;
-    double s[V];
-    if (!a.sigmoid) {
+  int place[V]; // which choice a value is
+  // Unique keys: a 16-bit logit leaves the lower 13 bits free, which tell the index, the lowest
+  // the largest.  Else margins: logits need not be apart by more than nothing; choices in 32 bits are
+  // off by 2^-21 and their rounding (sigmoid), by (V + 32) 2^-24 (softmax: sums of V values a lane,
+  // of e^x with x off by its rounding): what is further apart than twice that has the order of 64 bits.
+  constexpr bool kUnique = !kSums && sizeof(T) == 2;
+  const float margin = kUnique ? -1.0f : !kSums ? 0.0f : a.sigmoid ? 0x1p-19f : (V + 32) * 0x1p-22f;
+  const bool grouped = a.top_groups < a.groups;
+  bool known = true;
+  {
+    int keys[V];
+    if constexpr (kSums) {
+      float c[V];
+      if (a.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
+        }
+      } else {
+        const float by = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] = above(l[j], most) * by;
+        }
+      }
+      if (a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] += b[j];
+        }
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = l[j] == -INFINITY ? 0.0
-            : l[j] == most       ? 1.0
-                                 : exp(static_cast<double>(l[j]) - static_cast<double>(most));
-        sum += s[j];
+        // (neither masked nor NaN; -0 is no sum)
+        const int bits = __float_as_int(fmaxf(l[j] > -INFINITY ? c[j] : -INFINITY, -INFINITY));
+        keys[j] = bits ^ ((bits >> 31) & 0x7fffffff);
       }
-      for (int d = 1; d < kLanes; d *= 2) {
-        sum += __shfl_xor(sum, d, 64);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        keys[j] = key_of(l[j]);
+        if constexpr (kUnique) {
+          keys[j] = (keys[j] & ~0x1fff) + 0x1000 + (kMostExperts - 1 - p.first - j);
+        }
       }
     }
+    if (!a.full) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        keys[j] = j < p.n ? keys[j] : Lowest<int>::none;
+      }
+    }
+    if (grouped) {
+      // (a group's mark may be a sum of two)
+      known = keep_groups<V, int>(a, p, kSums ? 2.0f * margin : margin, keys);
+    }
+    known = take<V>(a.k, margin, keys) && known;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      double c = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l[j]))) : s[j] / sum;
-      if (a.bias != nullptr && j < p.n) {
-        c += static_cast<double>(a.bias[p.first + j]);
-      }
-      c = l[j] == -INFINITY ? -static_cast<double>(INFINITY) : c;
-      keys[j] = j < p.n ? key_of(c) : Lowest<K>::taken;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      keys[j] = j < p.n ? key_of(l[j]) : Lowest<K>::taken;
+      place[j] = step_of(keys[j]);
     }
   }
-  if (a.top_groups < a.groups) {
-    keep_groups<V, K>(a, p, keys);
-  }
-  for (int n = 0; n < a.k; ++n) {
-    int which;
-    take<V, K>(keys, &which);
-    if (which >= 0) {
-      float logit = l[0];
+  // (the sixteen lanes of a row agree)
+  if (!kUnique && __any(!known)) {
+    if constexpr (kSums) {
+      int64_t keys[V];
+      double c[V];
+      if (a.sigmoid) {
 #pragma unroll
-      for (int j = 1; j < V; ++j) {
-        logit = which == j ? l[j] : logit;
+        for (int j = 0; j < V; ++j) {
+          c[j] = 1.0 / (1.0 + exp(-static_cast<double>(l[j])));
+        }
+      } else {
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] = exp(l[j] == most ? 0.0 : static_cast<double>(l[j]) - static_cast<double>(most));
+          sum += c[j];
+        }
+        for (int d = 1; d < kLanes; d *= 2) {
+          sum += __shfl_xor(sum, d, 64);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] /= sum;
+        }
       }
-      chosen[slot][n] = {p.first + which, logit};
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (a.bias != nullptr) {
+          c[j] += static_cast<double>(b[j]);
+        }
+        keys[j] = key_of(l[j] == -INFINITY ? -static_cast<double>(INFINITY) : c[j]);
+        keys[j] = j < p.n ? keys[j] : Lowest<int64_t>::none;
+      }
+      if (grouped) {
+        keep_groups<V, int64_t>(a, p, -1.0f, keys);
+      }
+      take_in_order<V, int64_t>(a.k, keys);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        place[j] = step_of(keys[j]);
+      }
+    } else {
+      int keys[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        keys[j] = j < p.n ? key_of(l[j]) : Lowest<int>::none;
+      }
+      if (grouped) {
+        keep_groups<V, int>(a, p, -1.0f, keys);
+      }
+      take_in_order<V, int>(a.k, keys);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        place[j] = step_of(keys[j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (place[j] < a.k) {
+      chosen[slot][place[j]] = {p.first + j, l[j]};
     }
   }
   __syncthreads();
@@ -322,15 +471,14 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
       low = largest16(fmaxf(fminf(c[0].logit, 0.0f), fminf(c[1].logit, 0.0f)));
       low = low == -INFINITY ? 0.0f : low;
     } else {
-      most = largest16(fmaxf(c[0].logit, c[1].logit));
+      most = base_of(largest16(fmaxf(c[0].logit, c[1].logit)));
     }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    s[i] = a.sigmoid
-        ? expf(fminf(c[i].logit, 0.0f) - low) / (1.0f + expf(-fabsf(c[i].logit)))
-        : above(c[i].logit, most);
-    s[i] = c[i].logit != c[i].logit ? c[i].logit : s[i];
+    const float x = c[i].logit;
+    s[i] = a.sigmoid ? expf(fminf(x, 0.0f) - low) / (1.0f + expf(-fabsf(x))) : above(x, most);
+    s[i] = x != x ? x : s[i];
     s[i] = p.lane + 16 * i < a.k ? s[i] : 0.0f;
   }
   if (a.normalize) {
@@ -373,11 +521,11 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteArgs a) {
     for (int j = 0; j < V; ++j) {
       most = fmaxf(most, l[j]);
     }
-    most = largest16(most);
+    most = base_of(largest16(most));
     total = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      l[j] = j < p.n ? above(l[j], most) : 0.0f;
+      l[j] = above(l[j], most);
       total += l[j];
     }
     total = sum16(total);
@@ -406,7 +554,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteArgs a) {
       low = largest16(fmaxf(fminf(x[0], 0.0f), fminf(x[1], 0.0f)));
       low = low == -INFINITY ? 0.0f : low;
     } else {
-      most = largest16(fmaxf(x[0], x[1]));
+      most = base_of(largest16(fmaxf(x[0], x[1])));
     }
   }
   float s[2];
@@ -439,14 +587,25 @@ __global__ __launch_bounds__(256) void route_grad_kernel(const RouteArgs a) {
     return;
   }
   T* out = static_cast<T*>(a.out) + row * a.experts + p.first;
+  constexpr int W = kWide<T, V>;
+  const float by = total == 0.0f ? 0.0f : dot / total;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (j < p.n) {
-      float v = mine[p.first + j];
-      if (dense) {
-        v -= total == 0.0f ? 0.0f : l[j] / total * dot;
+  for (int j = 0; j < V; j += W) {
+    Wide<T, W> v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float g = j + i < p.n ? mine[p.first + j + i] : 0.0f;
+      v.e[i] = from_f32<T>(dense ? g - l[j + i] * by : g);
+    }
+    if (a.wide_out && p.n == V) {
+      *reinterpret_cast<Wide<T, W>*>(out + j) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if (j + i < p.n) {
+          out[j + i] = v.e[i];
+        }
       }
-      out[j] = from_f32<T>(v);
     }
   }
 }
@@ -504,9 +663,12 @@ int by_values(const RouteArgs& a, F&& go) {
   return MLXROCM_OK;
 }
 
-bool wide_rows(const void* p, int64_t stride, int group_size, size_t size) {
-  return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * size) |
-          static_cast<uintptr_t>(group_size * size)) % 16 == 0;
+// Whether every run of the values that a lane reads at once is aligned
+template <typename T, int V>
+bool wide_rows(const RouteArgs& a, const void* p, int64_t stride) {
+  constexpr uintptr_t bytes = kWide<T, V> * sizeof(T);
+  return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * sizeof(T)) |
+          (a.groups > 1 ? a.group_size * sizeof(T) : 0)) % bytes == 0;
 }
 
 } // namespace
@@ -549,12 +711,14 @@ extern "C" int mlxrocm_route_experts(
   a.sigmoid = sigmoid;
   a.normalize = normalize;
   a.scale = scale;
-  a.vector = wide_rows(logits, stride, a.group_size, dtype_size(dtype));
   const bool sums = bias != nullptr || (group_best > 1 && top_groups < groups);
   const unsigned grid = static_cast<unsigned>((rows + kRows - 1) / kRows);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return by_values(a, [&](auto v) {
+      a.full = a.group_size == decltype(v)::value * a.group_lanes && a.groups * a.group_lanes == kLanes;
+      a.vector = wide_rows<T, decltype(v)::value>(a, logits, stride);
+      a.wide_bias = wide_rows<float, decltype(v)::value>(a, bias, 0);
       if (sums) {
         route_kernel<T, decltype(v)::value, true>
             <<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(a);
@@ -600,12 +764,13 @@ extern "C" int mlxrocm_route_experts_vjp(
   a.sigmoid = sigmoid;
   a.normalize = normalize;
   a.scale = scale;
-  a.vector = wide_rows(logits, stride, a.group_size, dtype_size(dtype));
   const unsigned grid = static_cast<unsigned>((rows + kRows - 1) / kRows);
   const size_t lds = sizeof(float) * kRows * experts;
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return by_values(a, [&](auto v) {
+      a.vector = wide_rows<T, decltype(v)::value>(a, logits, stride);
+      a.wide_out = wide_rows<T, decltype(v)::value>(a, out, experts);
       route_grad_kernel<T, decltype(v)::value>
           <<<grid, 256, lds, static_cast<hipStream_t>(stream)>>>(a);
     });
