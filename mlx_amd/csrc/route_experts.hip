@@ -8,8 +8,7 @@
 // Choices decide what is computed, so their order is taken exactly: of the logits themselves where
 // they have the scores' order (no bias, no sums), else of choices in 64 bits.  Those are formed in 32
 // bits first; where all that are chosen, and the first that is not, are further apart than 32 bits can be
-// off, the order is known, and only a wavefront with a row where they are not forms them in 64.  Compared
-// are integers of the floats' order, with room below the lowest for what is taken already.
+// off, the order is known, and only a wavefront with a row where they are not forms them in 64.
 //
 // What bounds it: the instructions of k searches for the largest.  Sixteen lanes have a row, one of
 // the rows of lanes that DPP instructions rotate within: the largest of sixteen lanes is four
@@ -56,6 +55,10 @@ __device__ __forceinline__ int64_t rotated(int64_t v) {
   const uint32_t lo = rotated<Rotate>(static_cast<int>(v));
   const uint32_t hi = rotated<Rotate>(static_cast<int>(v >> 32));
   return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <int Rotate>
+__device__ __forceinline__ uint32_t rotated(uint32_t v) {
+  return static_cast<uint32_t>(rotated<Rotate>(static_cast<int>(v)));
 }
 template <int Rotate>
 __device__ __forceinline__ float rotated(float v) {
@@ -113,13 +116,43 @@ template <>
 struct Lowest<int> {
   static constexpr int taken = static_cast<int>(0x80000000u);
   static constexpr int none = taken + 64;
-  static constexpr int least = static_cast<int>(0x807fffffu); // -inf
+  static __device__ int sum(int one, int two) { return key_of(value_of(one) + value_of(two)); }
 };
 template <>
 struct Lowest<int64_t> {
   static constexpr int64_t taken = static_cast<int64_t>(0x8000000000000000ULL);
   static constexpr int64_t none = taken + 64;
+  static __device__ int64_t sum(int64_t one, int64_t two) {
+    return key_of(value_of(one) + value_of(two));
+  }
 };
+template <>
+struct Lowest<float> {
+  static constexpr float none = -INFINITY;
+  static __device__ float sum(float one, float two) { return one + two; }
+};
+template <>
+struct Lowest<uint32_t> {
+  static constexpr uint32_t none = 0;
+  static __device__ uint32_t sum(uint32_t one, uint32_t) { return one; } // (not called for)
+};
+
+template <typename K>
+__device__ __forceinline__ K larger(K a, K b) {
+  if constexpr (std::is_same_v<K, float>) {
+    return fmaxf(a, b);
+  } else {
+    return max(a, b);
+  }
+}
+template <typename K>
+__device__ __forceinline__ K smaller(K a, K b) {
+  if constexpr (std::is_same_v<K, float>) {
+    return fminf(a, b);
+  } else {
+    return min(a, b);
+  }
+}
 
 // e^(l - m) of the largest logit m: 1 where they are equal (both may be infinite).  Where there is no
 // logit at all (-inf) m is 0, so that nothing is above it.
@@ -200,102 +233,74 @@ __device__ __forceinline__ void take_in_order(int k, K (&keys)[V]) {
   }
 }
 
-// The same where no two are equal or, if `margin` is not negative, nearer to each other than
-// margin (1 + the larger's size): false where two are, whose order this does not tell.  (Without
-// the search for the lowest index: 44 instructions a choice of 16 values a lane instead of 100.)
-template <int V>
-__device__ __forceinline__ bool take(int k, float margin, int (&keys)[V]) {
-  // (equal ones are taken in one step: they show in how many were)
-  const auto taken = [&] {
-    int count = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      count += keys[j] < Lowest<int>::none;
-    }
-    count += rotated<8>(count);
-    count += rotated<4>(count);
-    count += rotated<2>(count);
-    return count + rotated<1>(count);
-  };
-  bool apart = true;
-  float last = 0.0f;
-  for (int n = 0;; ++n) {
-    int best = keys[0];
-#pragma unroll
-    for (int j = 1; j < V; ++j) {
-      best = max(best, keys[j]);
-    }
-    best = largest16(best);
-    if (margin >= 0.0f) {
-      const float v = value_of(best);
-      // (none left: as far as can be.  Infinities and NaN are not apart.)
-      apart = apart && (n == 0 || best < Lowest<int>::least || last - v > margin * (1.0f + fabsf(last)));
-      last = v;
-    }
-    if (n == k) {
-      return apart && taken() == k;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      keys[j] = keys[j] == best ? Lowest<int>::taken + n : keys[j];
-    }
-    if (margin < 0.0f && n + 1 == k) {
-      return true;
-    }
-  }
-}
-
-// Leaves the groups that count; says whether the last that does and the first that does not are
-// further than margin apart (if that is not negative)
+// The groups that count, by the sum of the group_best largest `keys` of each: whether the lane's does
 template <int V, typename K>
-__device__ __forceinline__ bool keep_groups(
-    const RouteArgs& a, const Place& p, float margin, K (&keys)[V]) {
+__device__ __forceinline__ bool group_counts(
+    const RouteArgs& a, const Place& p, const K (&keys)[V], float* gap) {
   // the largest, and the second largest, of the lane's; then of the group's lanes
-  K one = Lowest<K>::none;
+  K one = keys[0];
   K two = Lowest<K>::none;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    two = max(two, min(one, keys[j]));
-    one = max(one, keys[j]);
+  for (int j = 1; j < V; ++j) {
+    two = larger(two, smaller(one, keys[j]));
+    one = larger(one, keys[j]);
   }
   for (int d = 1; d < a.group_lanes; d *= 2) {
     const K other = __shfl_xor(one, d, 64);
     const K other_two = __shfl_xor(two, d, 64);
-    two = max(max(two, other_two), min(one, other));
-    one = max(one, other);
+    two = larger(larger(two, other_two), smaller(one, other));
+    one = larger(one, other);
   }
   K mark = one;
   if (a.group_best == 2) {
-    mark = key_of(value_of(one) + value_of(two));
+    mark = Lowest<K>::sum(one, two);
   }
   mark = p.group < a.groups ? mark : Lowest<K>::none;
   bool stays = false;
-  K last = 0;
+  K last = one;
   for (int n = 0; n < a.top_groups; ++n) {
     last = largest16(mark);
     const bool mine = first16(mark == last) / a.group_lanes == p.group;
     stays |= mine;
     mark = mine ? Lowest<K>::none : mark;
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    keys[j] = stays ? keys[j] : Lowest<K>::none;
+  if constexpr (std::is_same_v<K, float>) { // how far the first that does not is from the last that does
+    *gap = last - largest16(mark);
   }
-  if (margin < 0.0f) {
-    return true;
-  }
-  const auto v = value_of(last);
-  return v - value_of(largest16(mark)) > margin * (1 + fabs(v));
+  return stays;
 }
 
-struct Chosen {
-  int index;
-  float logit;
-};
+// The n-th largest of sixteen lanes' distinct unsigned `keys` is the largest u with u - (the one
+// before) nearest to 2^32: what is below the one before wraps round to the top, in order, what is
+// not stays at the bottom.  So a step is a subtraction and half a three-way maximum a value.  Lane n
+// gets the n-th in `mine`; false if two of them, or the last and the first that is not taken, are
+// nearer than `apart`.
+template <int V>
+__device__ __forceinline__ bool take(
+    int k, uint32_t apart, const uint32_t (&keys)[V], uint32_t (&mine)[2]) {
+  const int lane = threadIdx.x & 15;
+  bool known = true;
+  uint32_t last = 0;
+  for (int n = 0; n <= k; ++n) {
+    uint32_t best = keys[0] - last;
+#pragma unroll
+    for (int j = 1; j < V; ++j) {
+      best = max(best, keys[j] - last);
+    }
+    best = largest16(best);
+    known = known && (n == 0 || 0u - best > apart);
+    last += best;
+    mine[0] = lane == n ? last : mine[0];
+    if (k > 16) {
+      mine[1] = lane + 16 == n ? last : mine[1];
+    }
+  }
+  return known;
+}
 
 template <typename T, int V, bool kSums>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
-  __shared__ Chosen chosen[kRows][kMostChosen];
+  __shared__ int chosen[kRows][kMostChosen];
   const int slot = threadIdx.x / kLanes;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
   const int64_t at = min(row, a.rows - 1); // (sixteen lanes work or not together; all vote)
@@ -305,11 +310,12 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   read_logits<T, V>(logits + p.first, p.n, a.vector, l);
 
   // softmax: the largest logit and the sum above it
-  float most = -INFINITY;
+  float most = 0.0f;
   float total = 0.0f;
   if (!a.sigmoid && (kSums || !a.normalize)) {
+    most = l[0];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int j = 1; j < V; ++j) {
       most = fmaxf(most, l[j]);
     }
     most = base_of(largest16(most));
@@ -323,71 +329,136 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   if (kSums && a.bias != nullptr) {
     read_logits<float, V>(a.bias + p.first, p.n, a.wide_bias, b);
   }
-
-  int place[V]; // which choice a value is
-  // Unique keys: a 16-bit logit leaves the lower 13 bits free, which tell the index, the lowest
-  // the largest.  Else margins: logits need not be apart by more than nothing; choices in 32 bits are
-  // off by 2^-21 and their rounding (sigmoid), by (V + 32) 2^-24 (softmax: sums of V values a lane,
-  // of e^x with x off by its rounding): what is further apart than twice that has the order of 64 bits.
-  constexpr bool kUnique = !kSums && sizeof(T) == 2;
-  const float margin = kUnique ? -1.0f : !kSums ? 0.0f : a.sigmoid ? 0x1p-19f : (V + 32) * 0x1p-22f;
   const bool grouped = a.top_groups < a.groups;
+  int index[2];
+  float logit[2];
+
+  // 16-bit logits leave 13 bits of a float free: those tell the index, the lowest the largest, and
+  // every key is another.  Else a key is the distance from the row's largest choice in fixed point,
+  // and the place; two are told apart if they are further from each other than the choices can be off:
+  // logits by their rounding; sigmoids by 2^-21, softmaxes by (V + 32) 2^-24 (sums of V values a
+  // lane, of e^x with x off by its rounding), with their rounding 2^-23 of their size.
+  constexpr bool kUnique = !kSums && sizeof(T) == 2;
+  constexpr uint32_t kPlaces = 16 * V;
   bool known = true;
+  uint32_t mine[2] = {0, 0};
   {
-    int keys[V];
-    if constexpr (kSums) {
-      float c[V];
-      if (a.sigmoid) {
+    uint32_t keys[V];
+    if constexpr (kUnique) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const uint32_t key = static_cast<uint32_t>(key_of(l[j])) ^ 0x80000000u;
+        keys[j] = (key & ~0x1fffu) + 0x1000 + (kMostExperts - 1 - p.first - j);
+        keys[j] = j < p.n ? keys[j] : 0;
+      }
+      if (grouped) {
+        float gap;
+        const bool counts = group_counts<V, uint32_t>(a, p, keys, &gap);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
+          keys[j] = counts ? keys[j] : 0;
+        }
+      }
+      take<V>(a.k, 0, keys, mine);
+    } else {
+      float c[V];
+      float off; // of a choice
+      float scale = kSums ? 0x1p32f / kPlaces / 4 : 0x1p32f / kPlaces / 32;
+      if constexpr (kSums) {
+        if (a.sigmoid) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
+          }
+        } else {
+          const float by = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            c[j] = above(l[j], most) * by;
+          }
+        }
+        off = a.sigmoid ? 0x1p-20f : (V + 32) * 0x1p-23f;
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            c[j] += b[j];
+          }
         }
       } else {
-        const float by = total > 0.0f ? 1.0f / total : 0.0f;
+        off = 0x1p-20f; // (of a distance of 32 at most)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          c[j] = above(l[j], most) * by;
+          c[j] = l[j];
         }
       }
-      if (a.bias != nullptr) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          c[j] += b[j];
-        }
+      for (int j = 0; j < V; ++j) { // neither masked nor NaN
+        c[j] = fmaxf(l[j] > -INFINITY ? c[j] : -INFINITY, -INFINITY);
       }
+      float gap = INFINITY;
+      bool counts = p.n > 0;
+      if (grouped) {
+        counts = group_counts<V, float>(a, p, c, &gap) && counts;
+      }
+      float top = c[0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) {
+        top = fmaxf(top, c[j]);
+      }
+      top = largest16(counts ? top : -INFINITY);
+      off *= kSums ? 1.0f + fabsf(top) : 1.0f;
+      constexpr float kEnd = 0x1p32f / kPlaces - 256.0f; // (below the last in 24 bits)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        // (neither masked nor NaN; -0 is no sum)
-        const int bits = __float_as_int(fmaxf(l[j] > -INFINITY ? c[j] : -INFINITY, -INFINITY));
-        keys[j] = bits ^ ((bits >> 31) & 0x7fffffff);
+        const float far = fminf((top - c[j]) * scale, kEnd);
+        keys[j] = (0xffffffffu - static_cast<uint32_t>(far) * kPlaces) -
+            (static_cast<uint32_t>(p.lane) * V + j);
+        keys[j] = counts ? keys[j] : 0;
       }
+      if (!a.full) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          keys[j] = j < p.n ? keys[j] : 0;
+        }
+      }
+      // both of them off, and both cut to whole numbers
+      const uint32_t apart = (static_cast<uint32_t>(2.0f * off * scale) + 3) * kPlaces;
+      known = take<V>(a.k, apart, keys, mine);
+      known = known && fabsf(top) < INFINITY && gap > 4.0f * off;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (kUnique) {
+      index[i] = kMostExperts - 1 - static_cast<int>(mine[i] & 0xfff);
     } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        keys[j] = key_of(l[j]);
-        if constexpr (kUnique) {
-          keys[j] = (keys[j] & ~0x1fff) + 0x1000 + (kMostExperts - 1 - p.first - j);
-        }
-      }
-    }
-    if (!a.full) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        keys[j] = j < p.n ? keys[j] : Lowest<int>::none;
-      }
-    }
-    if (grouped) {
-      // (a group's mark may be a sum of two)
-      known = keep_groups<V, int>(a, p, kSums ? 2.0f * margin : margin, keys);
-    }
-    known = take<V>(a.k, margin, keys) && known;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      place[j] = step_of(keys[j]);
+      const int place = kPlaces - 1 - static_cast<int>(mine[i] & (kPlaces - 1));
+      const int lane = place / V;
+      index[i] = lane / a.group_lanes * a.group_size + (lane & (a.group_lanes - 1)) * V + place % V;
     }
   }
   // (the sixteen lanes of a row agree)
   if (!kUnique && __any(!known)) {
+    int place[V]; // which choice a value is
+    const auto order = [&](auto&& keys) {
+      using K = std::remove_reference_t<decltype(keys[0])>;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        keys[j] = j < p.n ? keys[j] : Lowest<K>::none;
+      }
+      if (grouped) {
+        const bool counts = group_counts<V, K>(a, p, keys, nullptr);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          keys[j] = counts ? keys[j] : Lowest<K>::none;
+        }
+      }
+      take_in_order<V, K>(a.k, keys);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        place[j] = step_of(keys[j]);
+      }
+    };
     if constexpr (kSums) {
       int64_t keys[V];
       double c[V];
@@ -417,39 +488,31 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
           c[j] += static_cast<double>(b[j]);
         }
         keys[j] = key_of(l[j] == -INFINITY ? -static_cast<double>(INFINITY) : c[j]);
-        keys[j] = j < p.n ? keys[j] : Lowest<int64_t>::none;
       }
-      if (grouped) {
-        keep_groups<V, int64_t>(a, p, -1.0f, keys);
-      }
-      take_in_order<V, int64_t>(a.k, keys);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        place[j] = step_of(keys[j]);
-      }
+      order(keys);
     } else {
       int keys[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        keys[j] = j < p.n ? key_of(l[j]) : Lowest<int>::none;
+        keys[j] = key_of(l[j]);
       }
-      if (grouped) {
-        keep_groups<V, int>(a, p, -1.0f, keys);
-      }
-      take_in_order<V, int>(a.k, keys);
+      order(keys);
+    }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        place[j] = step_of(keys[j]);
+    for (int j = 0; j < V; ++j) {
+      if (place[j] < a.k) {
+        chosen[slot][place[j]] = p.first + j;
       }
     }
-  }
+    // (the wavefront's own rows)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    if (place[j] < a.k) {
-      chosen[slot][place[j]] = {p.first + j, l[j]};
+    for (int i = 0; i < 2; ++i) {
+      index[i] = p.lane + 16 * i < a.k ? chosen[slot][p.lane + 16 * i] : 0;
     }
   }
-  __syncthreads();
   if (row >= a.rows) {
     return;
   }
@@ -457,26 +520,29 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   // each of the sixteen lanes has two of the chosen at most
   float s[2];
   float low = 0.0f; // sigmoid: all counted up, where all are tiny
-  Chosen c[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const bool is = p.lane + 16 * i < a.k;
-    c[i] = chosen[slot][is ? p.lane + 16 * i : 0];
-    if (!is) {
-      c[i].logit = -INFINITY;
+    logit[i] = -INFINITY;
+    if (p.lane + 16 * i < a.k) {
+      if constexpr (kUnique) { // (its lower 13 bits are none again)
+        const float v = value_of(static_cast<int>((mine[i] & ~0x1fffu) ^ 0x80000000u));
+        logit[i] = __int_as_float(__float_as_int(v) & ~0x1fff);
+      } else {
+        logit[i] = to_f32(logits[index[i]]);
+      }
     }
   }
   if (a.normalize) {
     if (a.sigmoid) {
-      low = largest16(fmaxf(fminf(c[0].logit, 0.0f), fminf(c[1].logit, 0.0f)));
+      low = largest16(fmaxf(fminf(logit[0], 0.0f), fminf(logit[1], 0.0f)));
       low = low == -INFINITY ? 0.0f : low;
     } else {
-      most = base_of(largest16(fmaxf(c[0].logit, c[1].logit)));
+      most = base_of(largest16(fmaxf(logit[0], logit[1])));
     }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float x = c[i].logit;
+    const float x = logit[i];
     s[i] = a.sigmoid ? expf(fminf(x, 0.0f) - low) / (1.0f + expf(-fabsf(x))) : above(x, most);
     s[i] = x != x ? x : s[i];
     s[i] = p.lane + 16 * i < a.k ? s[i] : 0.0f;
@@ -490,7 +556,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   for (int i = 0; i < 2; ++i) {
     if (p.lane + 16 * i < a.k) {
       const int64_t to = row * a.k + p.lane + 16 * i;
-      a.indices[to] = c[i].index;
+      a.indices[to] = index[i];
       const float w = total == 0.0f ? 0.0f : s[i] / total * a.scale;
       static_cast<T*>(a.weights)[to] = from_f32<T>(w);
     }
