@@ -11,8 +11,8 @@
 // adapter is read once for all of its tokens), as the columns of the matrix instruction's result; what
 // is read goes from memory into the instruction's operands without LDS, 16 bytes a lane.
 //
-//   group    the tokens by adapter, and the tiles of them (one workgroup).  Up to 64 single tokens
-//            need none: the first token of an adapter finds the others by a vote.
+//   group    the tokens by adapter, and the tiles of them (one workgroup).  Up to 64 indices need
+//            none: every workgroup finds its tile by itself, an index a lane (13 prompts: 6 us less).
 //   shrink   h or g, in 32 bits.  The four wavefronts of a workgroup and, for few tokens, several
 //            workgroups share a token's sum; the parts are added in one order by who reads them.
 //   expand   out or dx.  16-bit types: h as the sum of two numbers of the type, against the same
@@ -33,7 +33,7 @@ namespace mlxrocm {
 
 namespace {
 
-constexpr int kDecode = 64;        // single tokens that need no grouping
+constexpr int kFew = 64;           // indices, or rows of a tile, that a wavefront has in its lanes
 constexpr int kMostAdapters = 1024;
 constexpr int kMostRank = 256;
 
@@ -49,7 +49,7 @@ struct Rows {
   const int32_t* indices; // [n], each for `span` rows; null: all rows have adapter 0
   int n, adapters;
   Divisor span;
-  const int32_t* order; // [n] by adapter; null: no grouping (decode, or one index)
+  const int32_t* order; // [n] by adapter; null: no grouping (few indices)
   const Tile* tiles;
   const int32_t* n_tiles;
 
@@ -68,39 +68,80 @@ struct Rows {
 // if the workgroup has nothing to do.  All threads call it.
 __device__ __forceinline__ int find_rows(const Rows& r, int block, int tile, int* to, int* adapter) {
   __shared__ int found[2];
+  __shared__ int entries[kFew];
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
+    int rows = 0;
+    int of = -1;
     if (r.tiles != nullptr) {
-      const bool is = block < *r.n_tiles;
-      const Tile t = r.tiles[is ? block : 0];
-      for (int i = lane; is && i < t.rows; i += 64) {
-        to[i] = r.row(t.first + i);
-      }
-      if (lane == 0) {
-        found[0] = is ? t.rows : 0;
-        found[1] = t.adapter;
+      if (block < *r.n_tiles) {
+        const Tile t = r.tiles[block];
+        rows = t.rows;
+        of = t.adapter;
+        if (lane < rows) {
+          to[lane] = r.row(t.first + lane);
+        }
       }
     } else if (r.n == 1) {
       const int first = block * tile;
-      const int rows = min(tile, r.span.d - first);
-      for (int i = lane; i < rows; i += 64) {
-        to[i] = first + i;
+      rows = min(tile, r.span.d - first);
+      of = r.adapter_of(0);
+      if (lane < rows) {
+        to[lane] = first + lane;
       }
-      if (lane == 0) {
-        found[0] = rows;
-        found[1] = r.adapter_of(0);
+    } else if (r.span.d == 1) {
+      // Single tokens: the first of its kind has them all (a vote; by tiles: 34 us instead of 29, 48
+      // requests of rank 64)
+      const int mine = lane < r.n ? r.adapter_of(lane) : -2;
+      of = __shfl(mine, block, 64);
+      const uint64_t like = __ballot(mine == of);
+      if (__ffsll(static_cast<unsigned long long>(like)) - 1 == block) {
+        rows = __popcll(like);
+        if (mine == of) {
+          to[__popcll(like & ((uint64_t{1} << lane) - 1))] = lane;
+        }
       }
     } else {
-      const int of = lane < r.n ? r.adapter_of(lane) : -2;
-      const int mine = __shfl(of, block, 64);
-      const uint64_t same = __ballot(of == mine);
-      if (of == mine) {
-        to[__popcll(same & ((uint64_t{1} << lane) - 1))] = lane;
+      // Each lane an index: how many are like it, and how many of those before it.  The first of
+      // its kind has the kind's tiles.
+      of = lane < r.n ? r.adapter_of(lane) : -2;
+      int like = 0;
+      int before = 0;
+      for (int i = 0; i < r.n; ++i) {
+        const bool same = __builtin_amdgcn_readlane(of, i) == of;
+        like += same;
+        before += same && i < lane;
       }
-      if (lane == 0) {
-        found[0] = __ffsll(static_cast<unsigned long long>(same)) - 1 == block ? __popcll(same) : 0;
-        found[1] = mine;
+      const int all = like * r.span.d;
+      const int tiles = of != -2 && before == 0 ? (all + tile - 1) / tile : 0;
+      int up = tiles;
+      for (int d = 1; d < 64; d *= 2) {
+        const int other = __shfl_up(up, d, 64);
+        up += lane >= d ? other : 0;
       }
+      const uint64_t mine = __ballot(block >= up - tiles && block < up);
+      if (mine != 0) {
+        const int first = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+        const int from = (block - __shfl(up - tiles, first, 64)) * tile;
+        rows = min(tile, __shfl(all, first, 64) - from);
+        const int kind = __shfl(of, first, 64);
+        if (of == kind) {
+          entries[before] = lane;
+        }
+        of = kind;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (lane < rows) {
+          int rest;
+          const int entry = r.span.divide(from + lane, &rest);
+          to[lane] = entries[entry] * r.span.d + rest;
+        }
+      }
+    }
+    if (lane == 0) {
+      found[0] = rows;
+      found[1] = of;
     }
   }
   __syncthreads();
@@ -170,7 +211,7 @@ struct ShrinkArgs {
 // instead of 66, 7813 tokens of 14336 values to rank 32, float16.)
 template <typename T, int kGroups, int kChunks, bool kAligned>
 __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
-  __shared__ int rows[kDecode];
+  __shared__ int rows[kFew];
   __shared__ floatx4 parts[3][kGroups * kChunks][64];
   int adapter;
   const int count = find_rows(a.rows, blockIdx.x, a.tile, rows, &adapter);
@@ -364,7 +405,7 @@ template <typename T, int kGroups, int kChunks, bool kAligned, bool kAdd>
 __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
   constexpr int kPitch = 16 * kChunks + 4; // (rows of neighbouring tokens four banks apart)
   constexpr int kParts = 16 / kPer<T>;     // of a lane's results
-  __shared__ int rows[kDecode];
+  __shared__ int rows[kFew];
   __shared__ alignas(16) float held[16 * kGroups][kPitch];
   int adapter;
   const int count = find_rows(a.rows, blockIdx.x, a.tile, rows, &adapter);
@@ -1040,25 +1081,27 @@ int round_up(int v, int to) {
 
 Plan plan_of(const Sizes& s, bool gradients) {
   Plan p{};
-  const int64_t span = s.n == 0 ? 0 : s.T / s.n;
   const size_t size = dtype_size(s.dtype);
   const int step = s.dtype == MLXROCM_FLOAT32 ? 16 : 32;
-  p.grouped = gradients || !(s.n == 1 || (span == 1 && s.n <= kDecode));
+  p.grouped = gradients || s.n > kFew;
   p.padded = round_up(s.r, 16);
   const int chunks = p.padded / 16;
   p.chunks = chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8;
   p.rank_blocks = (chunks + p.chunks - 1) / p.chunks;
-  const bool few = s.T <= kDecode;
+  const bool few = s.T <= kFew;
   p.tile = few || p.chunks == 8 ? 16 : 32;
   const int64_t kinds = s.n < s.adapters + 1 ? s.n : s.adapters + 1;
-  const int64_t tiles = p.grouped ? s.T / p.tile + kinds
-      : s.n == 1                  ? (s.T + p.tile - 1) / p.tile
-                                  : s.n;
+  const int64_t tiles = p.grouped       ? s.T / p.tile + kinds
+      : s.n == 1    ? (s.T + p.tile - 1) / p.tile
+      : s.T == s.n ? s.n
+                    : s.T / p.tile + kinds;
   p.most_tiles = static_cast<int>(tiles);
-  // parts of a sum until there is a workgroup for each CU
+  // Parts of a sum until there are two workgroups a CU, if there is not one without.  us of 1, 2, 4, 8
+  // parts: 4 x 1024 tokens of 4096 values to rank 64 (132 tiles) 57, 57, 46, 50, 2000 tokens to rank 16
+  // (63 tiles) 24, 20, 18, 20, 7813 tokens of 14336 values (257 tiles) 114, 120, 122, 125.
   const int sum_over = gradients ? s.N : s.K;
   int splits = 1;
-  while (splits < 16 && tiles * p.rank_blocks * splits < 256 &&
+  while (splits < 16 && tiles * p.rank_blocks < 250 && tiles * p.rank_blocks * splits < 480 &&
          sum_over >= 2 * splits * 4 * step * 2) {
     splits *= 2;
   }

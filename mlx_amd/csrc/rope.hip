@@ -54,7 +54,8 @@ struct RopeArgs {
   const int32_t* table;
   const int32_t* lengths; // or null
   int64_t table_stride;
-  int pages, page, table_width;
+  int pages, table_width;
+  Divisor page; // rows of a page
   double turns[kMostPairs]; // per position, without freqs
 };
 
@@ -123,21 +124,33 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeArgs a) {
     if (!kCache || which == 0) {
       dst += b * ts[0] + head * ts[1] + token * ts[2];
     } else {
-      if (place < 0 || place >= static_cast<int64_t>(a.table_width) * a.page) {
+      if (place < 0 || place >= static_cast<int64_t>(a.table_width) * a.page.d) {
         continue;
       }
-      const int at = static_cast<int>(place) / a.page;
+      int row_of_page;
+      const int at = a.page.divide(static_cast<int>(place), &row_of_page);
       const int page = a.table[b * a.table_stride + at];
       if (page < 0 || page >= a.pages) {
         continue;
       }
-      dst += page * ts[0] + head * ts[1] + (static_cast<int>(place) - at * a.page) * ts[2];
+      dst += page * ts[0] + head * ts[1] + row_of_page * ts[2];
     }
     const bool turn = item < a.rotated && which < 2;
     const int one = !turn || a.step == 1 ? item * 2 * V : item * V;
     const int two = turn && a.step != 1 ? one + a.step : one + V;
-    Columns<T, V> x = *reinterpret_cast<const Columns<T, V>*>(src + one);
-    Columns<T, V> y = *reinterpret_cast<const Columns<T, V>*>(src + two);
+    Columns<T, V> x;
+    Columns<T, V> y;
+    if (kCache && place < 0) { // padding in front: zeros
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        x.v[i] = y.v[i] = from_f32<T>(0.0f);
+      }
+      *reinterpret_cast<Columns<T, V>*>(dst + one) = x;
+      *reinterpret_cast<Columns<T, V>*>(dst + two) = y;
+      continue;
+    }
+    x = *reinterpret_cast<const Columns<T, V>*>(src + one);
+    y = *reinterpret_cast<const Columns<T, V>*>(src + two);
     if (turn) {
       const float2* angles = table + t * a.pairs + item * V;
       if (a.step != 1) {
@@ -166,12 +179,6 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeArgs a) {
           z.v[j] = from_f32<T>(fmaf(p, r.x, -(q * r.y)));
           z.v[j + 1] = from_f32<T>(fmaf(q, r.x, p * r.y));
         }
-      }
-    }
-    if (kCache && which == 0 && place < 0) { // padding in front: zeros
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x.v[i] = y.v[i] = from_f32<T>(0.0f);
       }
     }
     *reinterpret_cast<Columns<T, V>*>(dst + one) = x;
@@ -272,11 +279,12 @@ int launch(const char* tag, RopeArgs& a, hipStream_t stream) {
   const int v = columns_of(a, kCache ? 3 : 1, sizeof(T));
   a.items = Divisor(a.D / (2 * v));
   a.rotated = a.pairs / v;
-  // Four tokens a workgroup share one table, as long as that makes two workgroups a CU; else one
-  // token, and its heads are cut until there are as many or a thread has one item.
+  // Two tokens a workgroup where there are four workgroups a CU of them (16 ragged prompts of up to
+  // 1531 tokens, 36 heads of 128: one 77 us, two 72, four 75, eight 83); else one token, and its
+  // heads are cut until there are two workgroups a CU or a thread has one item.
   const int heads = a.ends[2];
   const int64_t tokens = static_cast<int64_t>(a.B) * a.L;
-  a.tokens = tokens >= 4 * 512 ? 4 : 1;
+  a.tokens = tokens >= 4 * 512 ? 2 : 1;
   int slots = heads;
   if (a.tokens == 1) {
     while (slots > 1 && slots * a.items.d > kThreads &&
@@ -462,7 +470,7 @@ extern "C" int mlxrocm_rope_cache_update(
   a.table_stride = strides[18];
   a.lengths = lengths;
   a.pages = pages;
-  a.page = page_size;
+  a.page = Divisor(page_size);
   a.table_width = table_width;
   return dispatch_dtype(dtype, [&](auto t) {
     return launch<decltype(t), true>(tag, a, static_cast<hipStream_t>(stream));
