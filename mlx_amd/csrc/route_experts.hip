@@ -8,7 +8,8 @@
 // Choices decide what is computed, so their order is taken exactly: of the logits themselves where
 // they have the scores' order (no bias, no sums), else of choices in 64 bits.  Those are formed in 32
 // bits first; where all that are chosen, and the first that is not, are further apart than 32 bits can be
-// off, the order is known, and only a wavefront with a row where they are not forms them in 64.
+// off, the order is known.  Where they are not, the few that can be meant are formed in 64 (sigmoids: a
+// lane each), and only where that does not tell either, the whole row is.
 //
 // What bounds it: the instructions of k searches for the largest.  Sixteen lanes have a row, one of
 // the rows of lanes that DPP instructions rotate within: the largest of sixteen lanes is four
@@ -233,11 +234,10 @@ __device__ __forceinline__ void take_in_order(int k, K (&keys)[V]) {
   }
 }
 
-// The groups that count, by the sum of the group_best largest `keys` of each: whether the lane's does
+// The largest and the second largest of a group
 template <int V, typename K>
-__device__ __forceinline__ bool group_counts(
-    const RouteArgs& a, const Place& p, const K (&keys)[V], float* gap) {
-  // the largest, and the second largest, of the lane's; then of the group's lanes
+__device__ __forceinline__ void best_two(const RouteArgs& a, const K (&keys)[V], K* best, K* second) {
+  // of the lane's; then of the group's lanes
   K one = keys[0];
   K two = Lowest<K>::none;
 #pragma unroll
@@ -251,13 +251,16 @@ __device__ __forceinline__ bool group_counts(
     two = larger(larger(two, other_two), smaller(one, other));
     one = larger(one, other);
   }
-  K mark = one;
-  if (a.group_best == 2) {
-    mark = Lowest<K>::sum(one, two);
-  }
+  *best = one;
+  *second = two;
+}
+
+// The groups with the largest marks: whether the lane's is one of them
+template <typename K>
+__device__ __forceinline__ bool largest_groups(const RouteArgs& a, const Place& p, K mark, float* gap) {
   mark = p.group < a.groups ? mark : Lowest<K>::none;
   bool stays = false;
-  K last = one;
+  K last = mark;
   for (int n = 0; n < a.top_groups; ++n) {
     last = largest16(mark);
     const bool mine = first16(mark == last) / a.group_lanes == p.group;
@@ -268,6 +271,70 @@ __device__ __forceinline__ bool group_counts(
     *gap = last - largest16(mark);
   }
   return stays;
+}
+
+// By the sum of the group_best largest `keys` of each
+template <int V, typename K>
+__device__ __forceinline__ bool group_counts(
+    const RouteArgs& a, const Place& p, const K (&keys)[V], float* gap) {
+  K one, two;
+  best_two<V, K>(a, keys, &one, &two);
+  return largest_groups<K>(a, p, a.group_best == 2 ? Lowest<K>::sum(one, two) : one, gap);
+}
+
+// A choice of sigmoids (or a logit) in 64 bits
+__device__ __forceinline__ double exact_choice(bool sums, float l, float b) {
+  if (!sums) {
+    return static_cast<double>(l);
+  }
+  return l == -INFINITY ? -static_cast<double>(INFINITY)
+                        : 1.0 / (1.0 + exp(-static_cast<double>(l))) + static_cast<double>(b);
+}
+
+// The groups that count by the choices in 64 bits of those that are their best two (or one) of `c`,
+// which are off by less than a quarter of `apart`; *exact is false where it is not known which those are.
+template <int V>
+__device__ __forceinline__ bool exact_groups(
+    const RouteArgs& a, const Place& p, const float (&c)[V], const float (&l)[V], const float (&b)[V],
+    float apart, bool* exact) {
+  float one, two;
+  best_two<V, float>(a, c, &one, &two);
+  float third = -INFINITY;
+  float l_of[2] = {-INFINITY, -INFINITY};
+  float b_of[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    third = c[j] < two ? fmaxf(third, c[j]) : third;
+    if (c[j] == one) {
+      l_of[0] = l[j];
+      b_of[0] = a.bias == nullptr ? 0.0f : b[j];
+    } else if (c[j] == two) {
+      l_of[1] = l[j];
+      b_of[1] = a.bias == nullptr ? 0.0f : b[j];
+    }
+  }
+  for (int d = 1; d < a.group_lanes; d *= 2) {
+    third = fmaxf(third, __shfl_xor(third, d, 64));
+  }
+  // (equal ones cannot be told apart here)
+  bool known = one - two > apart;
+  // each lane the choices of those that it has; of a group's lanes one has the best, one the second
+  double sum = l_of[0] == -INFINITY ? 0.0 : exact_choice(true, l_of[0], b_of[0]);
+  int has = (l_of[0] != -INFINITY) + 256 * (l_of[1] != -INFINITY);
+  if (a.group_best == 2) {
+    known = known && two - third > apart;
+    sum += l_of[1] == -INFINITY ? 0.0 : exact_choice(true, l_of[1], b_of[1]);
+  }
+  for (int d = 1; d < a.group_lanes; d *= 2) {
+    sum += __shfl_xor(sum, d, 64);
+    has += __shfl_xor(has, d, 64);
+  }
+  known = known && (has & 255) == 1 && (a.group_best == 1 || has >> 8 == 1);
+  // (a group whose two are not known: nor are the row's)
+  const uint32_t not_known = static_cast<uint32_t>(
+      __ballot(!known && p.group < a.groups) >> (threadIdx.x & 48));
+  *exact = (not_known & 0xffff) == 0;
+  return largest_groups<int64_t>(a, p, key_of(sum), nullptr);
 }
 
 // The n-th largest of sixteen lanes' distinct unsigned `keys` is the largest u with u - (the one
@@ -296,6 +363,14 @@ __device__ __forceinline__ bool take(
     }
   }
   return known;
+}
+
+// The expert of a key that tells the distance from the largest, and the place
+template <int V>
+__device__ __forceinline__ int expert_of(const RouteArgs& a, uint32_t key) {
+  const int place = 16 * V - 1 - static_cast<int>(key & (16 * V - 1));
+  const int lane = place / V;
+  return lane / a.group_lanes * a.group_size + (lane & (a.group_lanes - 1)) * V + place % V;
 }
 
 template <typename T, int V, bool kSums>
@@ -341,6 +416,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   constexpr bool kUnique = !kSums && sizeof(T) == 2;
   constexpr uint32_t kPlaces = 16 * V;
   bool known = true;
+  int refined = -1; // the lane's choice, if it was found so
   uint32_t mine[2] = {0, 0};
   {
     uint32_t keys[V];
@@ -395,10 +471,28 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
       for (int j = 0; j < V; ++j) { // neither masked nor NaN
         c[j] = fmaxf(l[j] > -INFINITY ? c[j] : -INFINITY, -INFINITY);
       }
-      float gap = INFINITY;
       bool counts = p.n > 0;
       if (grouped) {
-        counts = group_counts<V, float>(a, p, c, &gap) && counts;
+        float gap;
+        const bool stays = group_counts<V, float>(a, p, c, &gap);
+        counts = stays && counts;
+        if constexpr (kSums) {
+          float size = fmaxf(fabsf(c[0]), 1.0f); // (of what the choices are off by)
+#pragma unroll
+          for (int j = 1; j < V; ++j) {
+            size = c[j] > -INFINITY ? fmaxf(size, fabsf(c[j])) : size;
+          }
+          const float apart = 4.0f * off * (1.0f + largest16(size));
+          known = gap > apart;
+          if (a.sigmoid && __any(!known)) {
+            bool exact;
+            const bool also = exact_groups<V>(a, p, c, l, b, apart, &exact);
+            counts = !known && exact ? also && p.n > 0 : counts;
+            known = known || exact;
+          }
+        } else {
+          known = gap >= 0.0f; // (logits are what they are; equal ones by index)
+        }
       }
       float top = c[0];
 #pragma unroll
@@ -423,8 +517,48 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
       }
       // both of them off, and both cut to whole numbers
       const uint32_t apart = (static_cast<uint32_t>(2.0f * off * scale) + 3) * kPlaces;
-      known = take<V>(a.k, apart, keys, mine);
-      known = known && fabsf(top) < INFINITY && gap > 4.0f * off;
+      known = known && fabsf(top) < INFINITY;
+      bool in_order = take<V>(a.k, apart, keys, mine);
+      // Where they are too near each other, but the first n >= k of sixteen are known to be the
+      // largest: a lane each, their choices in 64 bits, and a place for each.
+      if (__any(known && !in_order) && a.k < 16 && !(kSums && !a.sigmoid)) {
+        uint32_t one[2] = {0, 0};
+        take<V>(15, 0, keys, one);
+        const uint32_t next = __shfl_down(one[0], 1, kLanes);
+        const uint32_t ends = static_cast<uint32_t>(
+            __ballot(one[0] - next > apart && p.lane >= a.k - 1 && p.lane < 15) >>
+            (threadIdx.x & 48)) & 0xffffu;
+        const bool is = p.lane < __ffs(static_cast<int>(ends)); // (none: 0)
+        const int mine_of = expert_of<V>(a, one[0]);
+        const int e = is && mine_of < a.experts ? mine_of : 0;
+        const int64_t key = is ? key_of(exact_choice(
+                                     kSums, to_f32(logits[e]), a.bias == nullptr ? 0.0f : a.bias[e]))
+                               : Lowest<int64_t>::none;
+        int place = 0;
+        const auto behind = [&](auto r) {
+          const int64_t other = rotated<decltype(r)::value>(key);
+          const int index_of = rotated<decltype(r)::value>(e);
+          place += other > key || (other == key && index_of < e);
+        };
+        behind(IntC<1>{}); behind(IntC<2>{}); behind(IntC<3>{}); behind(IntC<4>{}); behind(IntC<5>{});
+        behind(IntC<6>{}); behind(IntC<7>{}); behind(IntC<8>{}); behind(IntC<9>{}); behind(IntC<10>{});
+        behind(IntC<11>{}); behind(IntC<12>{}); behind(IntC<13>{}); behind(IntC<14>{}); behind(IntC<15>{});
+        // (what is at the end of the range is only known to be there or beyond)
+        const uint32_t low = static_cast<uint32_t>(
+            __ballot(is && one[0] <= apart) >> (threadIdx.x & 48)) & 0xffffu;
+        const bool found = known && !in_order && ends != 0 && low == 0;
+        if (found && is && place < a.k) {
+          chosen[slot][place] = e;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (found) {
+          refined = p.lane < a.k ? chosen[slot][p.lane] : 0;
+          in_order = true;
+        }
+      }
+      known = known && in_order;
     }
   }
 #pragma unroll
@@ -432,11 +566,10 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
     if constexpr (kUnique) {
       index[i] = kMostExperts - 1 - static_cast<int>(mine[i] & 0xfff);
     } else {
-      const int place = kPlaces - 1 - static_cast<int>(mine[i] & (kPlaces - 1));
-      const int lane = place / V;
-      index[i] = lane / a.group_lanes * a.group_size + (lane & (a.group_lanes - 1)) * V + place % V;
+      index[i] = expert_of<V>(a, mine[i]);
     }
   }
+  index[0] = refined >= 0 ? refined : index[0];
   // (the sixteen lanes of a row agree)
   if (!kUnique && __any(!known)) {
     int place[V]; // which choice a value is

@@ -66,7 +66,7 @@ def relative(logits):
     """How far a weight may be off before it is rounded: e^x by the rounding of x (differences up to the
     spread of the logits) and two units, for itself and for the sum; the sum by an addition for each
     of a lane's up to 64 values and the four steps over lanes, and four more operations."""
-    finite = logits.double()[logits.isfinite()]
+    finite = logits.detach().double()[logits.isfinite()]
     spread = float(finite.max() - finite.min()) if finite.numel() else 0.0
     return (2 * (spread + 4) + 64 + 4 + 4) * F
 
@@ -144,6 +144,31 @@ def test_choices_that_differ_in_the_last_bits(gpu):
     assert indices[0].tolist() == order.flip(0)[:32].tolist()
     logits = torch.tensor([[1.0, 1.0 - 2.0 ** -24, 1.0 - 2.0 ** -23, 0.0] * 4])
     check(logits, 9, bias=torch.zeros(16, device="cuda"))
+
+
+@pytest.mark.parametrize("k", (1, 3, 8, 15, 16, 20))
+@pytest.mark.parametrize("near", (2.0 ** -21, 2.0 ** -24, 2.0 ** -27, 0.0))
+def test_choices_in_near_pairs(gpu, k, near):
+    """Two or three choices, or groups, nearer to each other than 32 bits can tell: in 64 they have an
+    order, whichever way that is found."""
+    g = torch.Generator().manual_seed(k)
+    E, rows = 64, 24
+    logits = (torch.randn((rows, E), generator=g) * 2).float()
+    logits[:, 1::2] = logits[:, ::2]  # pairs of one score
+    logits[4:8, 2::4] = logits[4:8, ::4]  # threes and fours
+    bias = (torch.randn((E,), generator=g) * 0.1).float()
+    bias[1::2] = (bias[::2].double() + near * torch.randn((E // 2,), generator=g).double()).float()
+    bias[2::4] = bias[::4]
+    logits[8:12, 32:] = logits[8:12, :32]  # groups that are alike but for that
+    bias[32:] = bias[:32] + near
+    for options in (dict(), dict(groups=4, top_groups=2), dict(groups=4, top_groups=2, group_best=2),
+                    dict(groups=16, top_groups=8, group_best=2), dict(groups=2, top_groups=1, group_best=2)):
+        for scoring in ("sigmoid", "softmax"):
+            for b in (bias, bias * 64):  # (choices far from 1 have fewer bits behind the point)
+                check(logits, k, scoring=scoring, bias=b.cuda(), **options)
+    check(logits, k)
+    check(logits * 2.0 ** -20, k, groups=4, top_groups=2)
+    check(logits * 2.0 ** 20, k)
 
 
 def test_masked_and_empty_rows(gpu):
