@@ -1,11 +1,11 @@
 """A small decoder of quantized projections, served and tuned with the framework's attention.
 
-Serving keeps keys and values in pages (``paged_cache_update``) and attends to them there
-(``paged_attention``), under a window with a few first tokens that stay visible.  The first layers
-of the decoder draft some tokens, the whole decoder reads them all at once, and ``verify_draft``
-keeps those that it would have sampled: what is generated is distributed as the whole decoder's own
-samples.  Tuning attends without a cache (``window_attention``) and differentiates through it and
-through the quantized products.
+Serving rotates queries and keys on their way into the pages of a cache (``rope_cache_update``) and
+attends to them there (``paged_attention``), under a window with a few first tokens that stay
+visible.  The first layers of the decoder draft some tokens, the whole decoder reads them all at
+once, and ``verify_draft`` keeps those that it would have sampled: what is generated is distributed as
+the whole decoder's own samples.  Tuning attends without a cache (``rope``, ``window_attention``) and differentiates through
+both and through the quantized products.
 
     python examples/speculative_decode.py [--batch 4] [--tokens 128] [--drafts 4] [--greedy]
 
@@ -41,16 +41,6 @@ class PagedCache:
             each, batch).t().contiguous()
 
 
-def rope(x, positions, base=10000.0):
-    """Rotates pairs of columns of ``x`` [B, heads, L, D] by ``positions`` [B, L]."""
-    half = x.shape[-1] // 2
-    rate = base ** (-torch.arange(half, device=x.device, dtype=torch.float32) / half)
-    angle = positions[:, None, :, None].float() * rate
-    cos, sin = angle.cos(), angle.sin()
-    a, b = x[..., :half].float(), x[..., half:].float()
-    return torch.cat((a * cos - b * sin, b * cos + a * sin), -1).to(x.dtype)
-
-
 class RMSNorm(torch.nn.Module):
     def __init__(self, dims, device):
         super().__init__()
@@ -80,15 +70,16 @@ class Layer(torch.nn.Module):
         def heads(y, n):
             return y.view(*y.shape[:2], n, self.dim).transpose(1, 2)
 
-        q = rope(heads(self.q_proj(x), self.heads), positions)
-        k = rope(heads(self.k_proj(x), self.kv_heads), positions)
+        q = heads(self.q_proj(x), self.heads)
+        k = heads(self.k_proj(x), self.kv_heads)
         v = heads(self.v_proj(x), self.kv_heads)
         if cache is None:
-            y = mlx_amd.window_attention(q, k, v, **self.visible)
-        else:
-            mlx_amd.paged_cache_update(k, v, cache.k[i], cache.v[i], cache.table, lengths)
-            y = mlx_amd.paged_attention(q, cache.k[i], cache.v[i], cache.table, lengths,
-                                        **self.visible)
+            y = mlx_amd.window_attention(mlx_amd.rope(q, positions), mlx_amd.rope(k, positions), v,
+                                         **self.visible)
+        else:  # (tokens turn by their places in the cache, which are their positions)
+            q, *pages = mlx_amd.rope_cache_update(q, k, v, cache.k[i], cache.v[i], cache.table,
+                                                  lengths)
+            y = mlx_amd.paged_attention(q, *pages, cache.table, lengths, **self.visible)
         return self.o_proj(y.transpose(1, 2).flatten(2))
 
     def forward(self, x, lengths, positions, cache, i):
