@@ -103,7 +103,7 @@ def adapter_matmul(
     ``a`` and ``b`` may be matrices.  ``scale``: a number, or one of each adapter ``[adapters]``.
 
     Sums are formed in 32 bits, ``x @ a.T`` is kept in 32 (float32) or twice the type's bits, and the
-    result is rounded once.  Up to 1024 adapters of rank up to 256; adapters of a lower rank than others
+    result is rounded once.  A request's values do not reach another's, whatever they are.  Up to 1024 adapters of rank up to 256; adapters of a lower rank than others
     are filled up with zeros.  Differentiable with respect to x, a, b and y (once, in reverse mode)."""
     out = ops._fast.adapter_matmul(x, a, b, indices, scale, y)
     if out is not None:
