@@ -240,67 +240,43 @@ __global__ __launch_bounds__(256) void shrink_kernel(const ShrinkArgs a) {
           rows[min(base + 16 * i + column, count - 1)] * a.x_stride;
     }
     floatx4 sum[kGroups][kChunks] = {};
-    // A wavefront's steps are neighbours, so that it reads whole lines; while one turn's operands
-    // are multiplied the next one's are on their way
-    constexpr int kAhead = kGroups * kChunks <= 2 ? 4 : 2;
+    // A wavefront's two steps are neighbours, so that it reads whole lines.  What others on the CU
+    // ask for meanwhile is enough: with the next turn's operands on their way, and with four steps
+    // in a turn, a call takes 64 us instead of 52 (8192 tokens of 14336 values to rank 16: 4.5 TB/s).
+    constexpr int kAhead = 2;
     constexpr int kTurn = kAhead * kStep<T>;
-    struct Turn {
-      uint4 x[kAhead][kGroups];
-      uint4 w[kAhead][kChunks];
-    };
-    const auto ask = [&](Turn& t, int k0, auto whole) {
+    const auto turn = [&](int k0, auto whole) {
+      uint4 xs[kAhead][kGroups];
+      uint4 ws[kAhead][kChunks];
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
         const int k = k0 + s * kStep<T> + quarter * kPer<T>;
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) {
-          t.x[s][i] = operand<T, kAligned, whole.value>(x_row[i], k, end);
+          xs[s][i] = operand<T, kAligned, whole.value>(x_row[i], k, end);
         }
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          t.w[s][c] = operand<T, kAligned, whole.value>(w_row[c], k, end);
+          ws[s][c] = operand<T, kAligned, whole.value>(w_row[c], k, end);
         }
       }
-    };
-    const auto add = [&](const Turn& t) {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
           for (int i = 0; i < kGroups; ++i) {
-            multiply<T>(t.w[s][c], t.x[s][i], sum[i][c]);
+            multiply<T>(ws[s][c], xs[s][i], sum[i][c]);
           }
         }
       }
     };
-    const int k0 = begin + wave * kTurn;
-    const int whole = k0 + kTurn > end ? 0 : (end - kTurn - k0) / (4 * kTurn) + 1;
-    const auto at = [&](int n) { return k0 + n * 4 * kTurn; };
-    // (no conditions between a turn's loads and its products: a wait then leaves the next one's
-    // in flight)
-    Turn one;
-    Turn two;
-    if (whole > 0) {
-      ask(one, at(0), std::true_type{});
-      int n = 0;
-      for (; n + 2 < whole; n += 2) {
-        ask(two, at(n + 1), std::true_type{});
-        add(one);
-        ask(one, at(n + 2), std::true_type{});
-        add(two);
-      }
-      if (n + 1 < whole) {
-        ask(two, at(n + 1), std::true_type{});
-        add(one);
-        add(two);
-      } else {
-        add(one);
-      }
+    int k = begin + wave * kTurn;
+    for (; k + kTurn <= end; k += 4 * kTurn) {
+      turn(k, std::true_type{});
     }
-    if (at(whole) < end) {
-      ask(one, at(whole), std::false_type{});
-      add(one);
+    if (k < end) {
+      turn(k, std::false_type{});
     }
     if (wave > 0) {
 #pragma unroll
@@ -1096,16 +1072,17 @@ Plan plan_of(const Sizes& s, bool gradients) {
       : s.T == s.n ? s.n
                     : s.T / p.tile + kinds;
   p.most_tiles = static_cast<int>(tiles);
-  // Parts of a sum until there are two workgroups a CU, if there is not one without.  us of 1, 2, 4, 8
-  // parts: 4 x 1024 tokens of 4096 values to rank 64 (132 tiles) 57, 57, 46, 50, 2000 tokens to rank 16
-  // (63 tiles) 24, 20, 18, 20, 7813 tokens of 14336 values (257 tiles) 114, 120, 122, 125.
+  // Parts of a sum until there are about two workgroups a CU.  us of a call with 16 outputs, with 1, 2,
+  // 4, 8 parts: 8192 tokens of 14336 values to rank 16 (257 tiles) 60, 52, 57, 60, 4096 tokens of 4096
+  // to rank 64 (132) 31, 32, 27, 24, 2000 tokens to rank 16 (63) 16, 11, 10, 10, 48 requests to rank 64
+  // 21, 14, 10, 10.
   const int sum_over = gradients ? s.N : s.K;
   int splits = 1;
-  while (splits < 16 && tiles * p.rank_blocks < 250 && tiles * p.rank_blocks * splits < 480 &&
+  while (splits < 16 && tiles * p.rank_blocks * splits < 480 &&
          sum_over >= 2 * splits * 4 * step * 2) {
     splits *= 2;
   }
-  p.per_split = round_up((sum_over + splits - 1) / splits, 4 * step);
+  p.per_split = round_up((sum_over + splits - 1) / splits, 8 * step);
   p.splits = (sum_over + p.per_split - 1) / p.per_split;
   const int out_columns = gradients ? s.K : s.N;
   p.columns = 256;
