@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
             c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
           }
         } else {
-          const float by = total > 0.0f ? 1.0f / total : 0.0f;
+          const float by = 1.0f / total; // (NaN, or nothing at all: no choice is known below)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             c[j] = above(l[j], most) * by;
@@ -660,6 +660,9 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
       if constexpr (kUnique) { // (its lower 13 bits are none again)
         const float v = value_of(static_cast<int>((mine[i] & ~0x1fffu) ^ 0x80000000u));
         logit[i] = __int_as_float(__float_as_int(v) & ~0x1fff);
+        if (logit[i] == -INFINITY) { // (or NaN)
+          logit[i] = to_f32(logits[index[i]]);
+        }
       } else {
         logit[i] = to_f32(logits[index[i]]);
       }

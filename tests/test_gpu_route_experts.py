@@ -222,6 +222,41 @@ def test_infinities_and_nan(gpu):
         assert indices.tolist() == [[3, 5, 0, 1, 2, 4] if row == 1 else [3, 5, 1, 0, 2, 4]]
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nan_of_every_type(gpu, dtype):
+    inf, nan = math.inf, math.nan
+    logits = torch.tensor([[nan] * 6, [0.0, nan, 1.0, 5.0, 2.0, 3.0], [-inf, nan, -inf, 1.0, -inf, -inf],
+                           [0.0, 1.0, 2.0, 3.0, 4.0, 5.0]], dtype=dtype).cuda().requires_grad_()
+    for scoring in ("softmax", "sigmoid"):
+        indices, weights = mlx_amd.route_experts(logits, 6, scoring=scoring)
+        assert indices.tolist() == [[0, 1, 2, 3, 4, 5], [3, 5, 4, 2, 0, 1], [3, 0, 1, 2, 4, 5],
+                                    [5, 4, 3, 2, 1, 0]]
+        assert weights[:3].isnan().all() and weights[3].isfinite().all()
+        dl, = torch.autograd.grad(weights.sum(), logits)
+        assert dl[:3].isnan().any(1).all() and dl[3].isfinite().all()
+        indices, weights = mlx_amd.route_experts(logits, 2, scoring=scoring)
+        assert weights[0].isnan().all() and weights[[1, 3]].isfinite().all()
+        assert weights[2].tolist() == [1.0, 0.0]  # the second is masked, index 0
+    weights = mlx_amd.route_experts(logits, 6, scoring="sigmoid", normalize=False)[1]
+    assert weights.isnan().tolist() == [[True] * 6, [False] * 5 + [True],
+                                        [False, False, True, False, False, False], [False] * 6]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_choices_that_all_are_nan_go_by_index(gpu, dtype):
+    """One NaN makes NaN of a softmax: no choice that has such a score is before another."""
+    logits = torch.tensor([[0.0, math.nan, 1.0, 5.0, 2.0, 3.0], [0.0, 1.0, 2.0, 3.0, 4.0, 5.0]],
+                          dtype=dtype).cuda()
+    bias = torch.tensor([0.0, 0.5, 3.0, 1.0, 4.0, 2.0], device="cuda")
+    for options in (dict(bias=bias), dict(bias=bias, groups=2, top_groups=1),
+                    dict(groups=2, top_groups=1, group_best=2)):
+        indices, _ = mlx_amd.route_experts(logits, 3, **options)
+        assert indices[0].tolist() == [0, 1, 2], options
+        indices, _ = mlx_amd.route_experts(logits[1:], 3, **options)
+        assert indices.tolist() == ([[4, 2, 5]] if options == dict(bias=bias) else
+                                    [[4, 5, 3]] if "bias" in options else [[5, 4, 3]])
+
+
 def test_shapes_strides_and_empties(gpu):
     wide = logits_of(2, 3, 5, 70, dtype=torch.bfloat16).cuda()
     want = reference(wide[..., 3:67], 4)
