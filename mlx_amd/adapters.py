@@ -2,7 +2,6 @@
 from __future__ import annotations
 
 import functools
-import math
 from typing import Optional, Union
 
 import torch
@@ -10,7 +9,7 @@ import torch
 from . import _lib, ops
 from ._copy import astype as _astype, contiguous as _contiguous
 from .attention import _int32, _tangents
-from .ops import _DTYPE_CODE, _FLOATING, _require_gpu, _require_one_device, _rows_of, _stream_ptr
+from .ops import _DTYPE_CODE, _FLOATING, _finite_scale, _require_gpu, _require_one_device, _rows_of, _stream_ptr
 
 __all__ = ["adapter_matmul"]
 
@@ -138,16 +137,14 @@ def adapter_matmul(
     if dtype not in _FLOATING:
         raise ValueError(f"[{tag}] Received unsupported type {dtype}.")
     scales = None
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"[{tag}] no gradients with respect to scale.")
     if isinstance(scale, torch.Tensor) and scale.dim() > 0:
         scales, scale = scale, 1.0
         if tuple(scales.shape) != (adapters,) or scales.dtype not in _FLOATING:
             raise ValueError(f"[{tag}] scale must be a number or {adapters} floating-point numbers but has "
                              f"shape {tuple(scales.shape)} and type {scales.dtype}.")
-        if scales.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError(f"[{tag}] no gradients with respect to scale.")
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"[{tag}] scale must be finite but got {scale}.")
+    scale = _finite_scale(tag, scale)
     if _tangents(*operands):
         raise NotImplementedError(f"[{tag}] no forward-mode gradients.")
     others = [t for t in (indices, scales) if t is not None]

@@ -72,6 +72,14 @@ def _require_one_device(tag: str, *tensors: torch.Tensor) -> None:
                          f"{', '.join(sorted(map(str, devices)))}.")
 
 
+def _finite_scale(tag: str, scale) -> float:
+    """A factor that the kernels hold in 32 bits"""
+    scale = float(scale)
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"[{tag}] scale must be finite in 32 bits but got {scale}.")
+    return scale
+
+
 def _rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """t as rows of its last dimension that are dense and evenly spaced, in place where it can be,
     and how many elements they are apart."""

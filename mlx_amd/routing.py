@@ -2,7 +2,6 @@
 which weights their results count."""
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -10,7 +9,7 @@ import torch
 from . import _lib, ops
 from ._copy import astype as _astype, contiguous as _contiguous
 from .attention import _tangents
-from .ops import _DTYPE_CODE, _FLOATING, _require_gpu, _require_one_device, _rows_of, _stream_ptr
+from .ops import _DTYPE_CODE, _FLOATING, _finite_scale, _require_gpu, _require_one_device, _rows_of, _stream_ptr
 
 __all__ = ["route_experts"]
 
@@ -111,9 +110,7 @@ def route_experts(
     if bias is not None and (bias.dtype not in _FLOATING or tuple(bias.shape) != (experts,)):
         raise ValueError(f"[{tag}] bias must hold {experts} floating-point numbers but has shape "
                          f"{tuple(bias.shape)} and type {bias.dtype}.")
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"[{tag}] scale must be finite but got {scale}.")
+    scale = _finite_scale(tag, scale)
     if _tangents(logits):
         raise NotImplementedError(f"[{tag}] no forward-mode gradients.")
     operands = [logits] if bias is None else [logits, bias]

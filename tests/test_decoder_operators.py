@@ -152,6 +152,20 @@ def test_no_forward_mode_and_no_gradients_through_the_cache():
         mlx_amd.adapter_matmul(**ADAPT, scale=torch.ones(4, requires_grad=True))
 
 
+def test_scales_of_a_single_number():
+    """Finite in the 32 bits that the kernels hold, and not what a graph would have to reach."""
+    for scale in (1e39, -float("inf"), 10 ** 60):
+        with pytest.raises(ValueError, match="finite in 32 bits"):
+            mlx_amd.route_experts(**ROUTE, scale=scale)
+        with pytest.raises(ValueError, match="finite in 32 bits"):
+            mlx_amd.adapter_matmul(**ADAPT, scale=scale)
+    scale = torch.tensor(2.0, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="scale"):
+        mlx_amd.adapter_matmul(**ADAPT, scale=scale)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+        mlx_amd.adapter_matmul(**ADAPT, scale=scale)
+
+
 def _status(name, *args):
     lib = _lib.load()
     return getattr(lib, name)(*args), lib.mlxrocm_last_error().decode()
