@@ -350,3 +350,16 @@ def test_beside_a_quantized_projection(gpu):
     assert (da[1] == 0).all() and (db[1] == 0).all() and (da[0] != 0).any()
     names = {n for n, p in layer.named_parameters()}
     assert names == {"lora_a", "lora_b"}  # the projection is frozen
+
+
+@pytest.mark.parametrize("dtype", (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64, torch.uint16,
+                                   torch.uint32, torch.uint64))
+def test_indices_of_every_type(gpu, dtype):
+    """No adapter is what lies outside of them in the indices' own type."""
+    args, _ = case(6, 2, 64, 48, 8, 3, torch.float32)
+    most = torch.iinfo(dtype).max
+    indices = [0, min(2 ** 32, most), 2, min(2 ** 32 + 1, most), min(2 ** 63, most), 1]
+    got = mlx_amd.adapter_matmul(**{**args, "indices": torch.tensor(indices, dtype=dtype).cuda()})
+    want = mlx_amd.adapter_matmul(
+        **{**args, "indices": torch.tensor([0, -1, 2, -1, -1, 1], dtype=torch.int32).cuda()})
+    assert torch.equal(got, want)
