@@ -16,12 +16,13 @@
 //   shrink   h or g, in 32 bits.  The four wavefronts of a workgroup and, for few tokens, several
 //            workgroups share a token's sum; the parts are added in one order by who reads them.
 //   expand   out or dx.  16-bit types: h as the sum of two numbers of the type, against the same
-//            operand of B twice (up to 16 ranks: in one instruction of 32).  So h keeps 16 bits (bfloat16) or 22, and the result's own
-//            rounding is all that is seen.  float16: h counts a power of two that brings the
-//            token's largest to 2^13.
+//            operand of B twice (up to 16 ranks: in one instruction of 32).  So h keeps 16 bits
+//            (bfloat16) or 22, and the result's own rounding is all that is seen.  float16: h
+//            counts a power of two that brings the token's largest to 2^13.
 //   turn     A and B with their two dimensions swapped, for the gradients: then g and dx are the
 //            same two products.
-//   tokens   dA and dB: sums over tokens, cut so that workgroups fill the card.
+//   tokens   dB and dA in one launch: sums over tokens, cut so that workgroups fill the card; dB
+//            first, whose dout the products before have just read (46 us of 235 MB then, 109 behind dx).
 //   join     their parts, in order; zeros for adapters without tokens.
 //
 // No atomics: the same inputs give the same bits.
@@ -333,6 +334,25 @@ struct ExpandArgs {
   int tile;
 };
 
+// Four ranks of the sum of a token's parts, in order
+__device__ __forceinline__ floatx4 sum_of_parts(const float* p, int splits, int64_t split_stride) {
+  floatx4 v = *reinterpret_cast<const floatx4*>(p);
+  for (int s = 1; s < splits; s += 5) { // (five asked for at once; 16 parts at most)
+    floatx4 part[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      part[i] = *reinterpret_cast<const floatx4*>(p + min(s + i, splits - 1) * split_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      if (s + i < splits) {
+        v += part[i];
+      }
+    }
+  }
+  return v;
+}
+
 // Eight ranks of a token's h times `by`, rounded, or what rounding took from them; float32: four
 template <typename T>
 __device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], bool lower, float by) {
@@ -474,21 +494,7 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
       const int t = n / quads;
       const int k = 4 * (n - t * quads);
       const int64_t at = static_cast<int64_t>(rows[base + t]) * a.padded + k;
-      const float* p = a.h + at;
-      floatx4 v = *reinterpret_cast<const floatx4*>(p);
-      for (int s = 1; s < a.splits; s += 5) { // (five asked for at once; 16 parts at most)
-        floatx4 part[5];
-#pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          part[i] = *reinterpret_cast<const floatx4*>(p + min(s + i, a.splits - 1) * a.split_stride);
-        }
-#pragma unroll
-        for (int i = 0; i < 5; ++i) {
-          if (s + i < a.splits) {
-            v += part[i];
-          }
-        }
-      }
+      const floatx4 v = sum_of_parts(a.h + at, a.splits, a.split_stride);
       *reinterpret_cast<floatx4*>(&held[t][k]) = v;
       if (a.h_sum != nullptr && blockIdx.y == 0) {
         *reinterpret_cast<floatx4*>(a.h_sum + at) = v;
@@ -779,17 +785,22 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a) {
 }
 
 // ---------------------------------------------------------------- sums over tokens
-struct TokenArgs {
-  Rows rows; // tiles: the segments
-  const float* p; // [splits, T, padded]: g or h
-  int64_t split_stride;
-  int splits, padded, r;
-  const void* q; // [T, W]: x or dout
+struct TokenSum {
+  const float* p; // [splits, T, padded]: h or g
+  int splits;
+  const void* q; // [T, W]: dout or x
   int64_t q_stride;
   int W;
+  int across;   // blocks of columns; 0: this sum is not wanted
   float* parts; // [slots, r, W]
   void* out;    // [adapters, r, W], or [adapters, W, r] (turned)
   int turned;
+};
+struct TokenArgs {
+  Rows rows; // tiles: the segments
+  int64_t split_stride;
+  int padded, r;
+  TokenSum of[2]; // dB, dA
 };
 
 constexpr int kTokens = 32;  // of a tile in LDS
@@ -810,11 +821,13 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
     return;
   }
   const Tile tile = a.rows.tiles[blockIdx.x];
+  const bool second = static_cast<int>(blockIdx.y) >= a.of[0].across;
+  const TokenSum& m = a.of[second];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15;
   const int quarter = lane >> 4;
-  const int c0 = blockIdx.y * kColumns;
+  const int c0 = (blockIdx.y - (second ? a.of[0].across : 0)) * kColumns;
   const int rank0 = blockIdx.z * kChunks * 16;
   for (int n = threadIdx.x; n < tile.rows; n += 256) {
     rows[n] = a.rows.row(tile.first + n);
@@ -834,9 +847,9 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
       const int t = first + n / kUnits;
       const int c = c0 + (n % kUnits) * kPer<T>;
       got[i] = uint4{0, 0, 0, 0};
-      if (t < tile.rows && c < a.W) {
+      if (t < tile.rows && c < m.W) {
         got[i] = operand<T, kAligned>(
-            static_cast<const T*>(a.q) + rows[t] * a.q_stride, c, a.W);
+            static_cast<const T*>(m.q) + rows[t] * m.q_stride, c, m.W);
       }
     }
 #pragma unroll
@@ -846,10 +859,8 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
       const int k = rank0 + n % (4 * kChunks) * 4;
       p_got[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
       if (n < kQuads && t < tile.rows && k < a.padded) {
-        const float* p = a.p + static_cast<int64_t>(rows[t]) * a.padded + k;
-        for (int s = 0; s < a.splits; ++s) {
-          p_got[i] += *reinterpret_cast<const floatx4*>(p + s * a.split_stride);
-        }
+        p_got[i] = sum_of_parts(
+            m.p + static_cast<int64_t>(rows[t]) * a.padded + k, m.splits, a.split_stride);
       }
     }
   };
@@ -974,25 +985,25 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
       const int n = c0 + 64 * wave + 4 * kPer<T> * (j / kTiles) + kPer<T> * quarter + 4 * (j % kTiles);
       const floatx4 v = sum[j][c];
       if (tile.slot >= 0) {
-        float* to = a.parts + (static_cast<int64_t>(tile.slot) * a.r + rank) * a.W + n;
-        if (kAligned && n < a.W) { // (W is a multiple of 4 at least, the parts are aligned)
+        float* to = m.parts + (static_cast<int64_t>(tile.slot) * a.r + rank) * m.W + n;
+        if (kAligned && n < m.W) { // (W is a multiple of 4 at least, the parts are aligned)
           *reinterpret_cast<floatx4*>(to) = v;
           continue;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (n + i < a.W) {
+          if (n + i < m.W) {
             to[i] = v[i];
           }
         }
         continue;
       }
-      T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tile.adapter) * a.r * a.W;
+      T* out = static_cast<T*>(m.out) + static_cast<int64_t>(tile.adapter) * a.r * m.W;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (n + i < a.W) {
-          out[a.turned ? static_cast<int64_t>(n + i) * a.r + rank
-                       : static_cast<int64_t>(rank) * a.W + n + i] = from_f32<T>(v[i]);
+        if (n + i < m.W) {
+          out[m.turned ? static_cast<int64_t>(n + i) * a.r + rank
+                       : static_cast<int64_t>(rank) * m.W + n + i] = from_f32<T>(v[i]);
         }
       }
     }
@@ -1000,29 +1011,31 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
 }
 
 struct JoinArgs {
-  const float* parts;
   const int32_t* slots;
-  void* out;
-  int r, W, turned;
+  int r;
+  TokenSum of[2];
 };
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
   const int adapter = blockIdx.z;
   const int first = a.slots[2 * adapter];
   const int count = a.slots[2 * adapter + 1];
-  const int n = blockIdx.x * 256 + threadIdx.x;
+  const bool second = static_cast<int>(blockIdx.x) >= a.of[0].across;
+  const TokenSum& m = a.of[second];
+  const int n = (blockIdx.x - (second ? a.of[0].across : 0)) * kColumns + threadIdx.x;
   const int rank = blockIdx.y;
-  if (first < 0 || n >= a.W) {
+  if (first < 0 || n >= m.W) {
     return;
   }
   float v = 0.0f;
   for (int s = 0; s < count; ++s) {
-    v += a.parts[(static_cast<int64_t>(first + s) * a.r + rank) * a.W + n];
+    v += m.parts[(static_cast<int64_t>(first + s) * a.r + rank) * m.W + n];
   }
-  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(adapter) * a.r * a.W;
-  out[a.turned ? static_cast<int64_t>(n) * a.r + rank : static_cast<int64_t>(rank) * a.W + n] =
+  T* out = static_cast<T*>(m.out) + static_cast<int64_t>(adapter) * a.r * m.W;
+  out[m.turned ? static_cast<int64_t>(n) * a.r + rank : static_cast<int64_t>(rank) * m.W + n] =
       from_f32<T>(v);
 }
+static_assert(kColumns == 256, "a workgroup of join_kernel has a block of columns");
 
 // ---------------------------------------------------------------- plans
 // Sizes of a call and where things lie in its workspace, in bytes
@@ -1036,7 +1049,7 @@ struct Plan {
   int splits, per_split; // of K (forward) or N (gradients)
   int columns;           // of a workgroup of expand
   int segment, most_segments, most_slots;
-  size_t order, tiles, counts, segments, slots, h, g_sum, turned_a, turned_b, parts, bytes;
+  size_t order, tiles, counts, segments, slots, h, turned_a, turned_b, parts_a, parts_b, bytes;
   int padded_n;
 };
 
@@ -1097,13 +1110,14 @@ Plan plan_of(const Sizes& s, bool gradients) {
   }
   p.h = claim(at, sizeof(float) * p.splits * s.T * p.padded); // (gradients: g)
   if (gradients) {
-    p.g_sum = claim(at, sizeof(float) * s.T * p.padded);
-  }
-  if (gradients) {
-    const int wide = s.K > s.N ? s.K : s.N;
-    const int64_t blocks = ((s.K + s.N - wide) + kColumns - 1) / kColumns; // of the narrower sums
-    int64_t segment = s.T * blocks * p.rank_blocks / 320 / kTokens * kTokens;
-    p.segment = static_cast<int>(segment < 64 ? 64 : segment > kMostSegment ? kMostSegment : segment);
+    const int64_t blocks = (s.K + kColumns - 1) / kColumns + (s.N + kColumns - 1) / kColumns;
+    // 640 workgroups, by tokens: 8192 tokens of 4096 values to 14336 by rank 16 290 us (320: 320, 1024: 302),
+    // 16384 of 8192 to 1024 by rank 32 292 (320: 306).  At least 64 tokens, as parts are written and read
+    // again: of rank 128 96 (4110 tokens of 1024 to 1001: 353, with 64 384, with 128 360).
+    const int64_t segment = s.T * blocks * p.rank_blocks / 640 / kTokens * kTokens;
+    const int least = p.chunks == 8 ? 96 : 64;
+    p.segment =
+        static_cast<int>(segment < least ? least : segment > kMostSegment ? kMostSegment : segment);
     p.most_segments = static_cast<int>(s.T / p.segment + kinds);
     p.most_slots = static_cast<int>(2 * (s.T / p.segment) + 1);
     p.segments = claim(at, sizeof(Tile) * p.most_segments);
@@ -1111,7 +1125,8 @@ Plan plan_of(const Sizes& s, bool gradients) {
     p.padded_n = round_up(s.N, 16);
     p.turned_a = claim(at, size * s.adapters * s.K * p.padded);
     p.turned_b = claim(at, size * s.adapters * s.r * p.padded_n);
-    p.parts = claim(at, sizeof(float) * p.most_slots * s.r * wide);
+    p.parts_a = claim(at, sizeof(float) * p.most_slots * s.r * s.K);
+    p.parts_b = claim(at, sizeof(float) * p.most_slots * s.r * s.N);
   }
   p.bytes = at;
   return p;
@@ -1204,12 +1219,36 @@ int expand(const ExpandArgs& a, const Plan& p, bool aligned, hipStream_t stream)
   return by_chunks(p.chunks, aligned, go);
 }
 
+// Both sums in one launch if either can have 16 bytes at a time or neither, and their joins in one
 template <typename T>
-int token_sums(const TokenArgs& a, const Plan& p, bool aligned, hipStream_t stream) {
-  const dim3 grid(p.most_segments, (a.W + kColumns - 1) / kColumns, p.rank_blocks);
-  return by_chunks(p.chunks, aligned, [&](auto chunks, auto is) {
-    token_kernel<T, decltype(chunks)::value, decltype(is)::value><<<grid, 256, 0, stream>>>(a);
-  });
+int token_sums(TokenArgs a, const Plan& p, const int32_t* slots, int adapters, hipStream_t stream) {
+  const auto aligned = [](const TokenSum& m) {
+    return aligned16(m.q, m.q_stride, sizeof(T)) && aligned16(nullptr, m.W, sizeof(T));
+  };
+  const auto launch = [&](const TokenArgs& k, bool is) {
+    const dim3 grid(p.most_segments, k.of[0].across + k.of[1].across, p.rank_blocks);
+    return by_chunks(p.chunks, is, [&](auto chunks, auto al) {
+      token_kernel<T, decltype(chunks)::value, decltype(al)::value><<<grid, 256, 0, stream>>>(k);
+    });
+  };
+  const bool is = aligned(a.of[a.of[0].across == 0]);
+  const bool together = a.of[1].across == 0 || aligned(a.of[1]) == is;
+  TokenArgs first = a;
+  TokenArgs second = a;
+  if (!together) {
+    first.of[1].across = second.of[0].across = 0;
+  }
+  int status = launch(first, is);
+  if (status == MLXROCM_OK && !together) {
+    status = launch(second, !is);
+  }
+  if (status != MLXROCM_OK) {
+    return status;
+  }
+  const JoinArgs j{slots, a.r, {a.of[0], a.of[1]}};
+  join_kernel<T><<<dim3(a.of[0].across + a.of[1].across, a.r, adapters), 256, 0, stream>>>(j);
+  MLXROCM_HIP_TRY(hipGetLastError());
+  return MLXROCM_OK;
 }
 
 int group(const GroupArgs& a, hipStream_t stream) {
@@ -1332,7 +1371,8 @@ extern "C" int mlxrocm_adapter_matmul(
     return rc;
   }
   const Plan p = plan_of(s, false);
-  if (out == nullptr || b == nullptr || x == nullptr || a == nullptr || (indices == nullptr && n_indices != 1) || (p.bytes > 0 && workspace == nullptr)) {
+  if (out == nullptr || b == nullptr || x == nullptr || a == nullptr ||
+      (indices == nullptr && n_indices != 1) || (p.bytes > 0 && workspace == nullptr)) {
     return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer", tag);
   }
   if (workspace_bytes < p.bytes) {
@@ -1425,7 +1465,8 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
     return rc;
   }
   const Plan p = plan_of(s, true);
-  if (x == nullptr || a == nullptr || b == nullptr || dout == nullptr || (indices == nullptr && n_indices != 1) || (db != nullptr && h == nullptr) ||
+  if (x == nullptr || a == nullptr || b == nullptr || dout == nullptr ||
+      (indices == nullptr && n_indices != 1) || (db != nullptr && h == nullptr) ||
       workspace == nullptr) {
     return fail(MLXROCM_INVALID_ARGUMENT, "[%s] null pointer", tag);
   }
@@ -1447,8 +1488,6 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
   runs.tiles = grouped.segments;
   runs.n_tiles = grouped.counts + 1;
   float* g = reinterpret_cast<float*>(ws + p.h);
-  float* g_sum = reinterpret_cast<float*>(ws + p.g_sum);
-  float* parts = reinterpret_cast<float*>(ws + p.parts);
   return dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const auto turn = [&](bool both) {
@@ -1464,31 +1503,6 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
       const dim3 grid(static_cast<unsigned>(ta.of[0].blocks + ta.of[1].blocks), adapters);
       turn_kernel<T><<<grid, 256, 0, st>>>(ta);
       return hipGetLastError();
-    };
-    const auto sums = [&](const float* from, int splits, const void* q, int64_t stride, int W,
-                          void* to, int turned) {
-      TokenArgs k{};
-      k.rows = runs;
-      k.p = from;
-      k.split_stride = rows * p.padded;
-      k.splits = splits;
-      k.padded = p.padded;
-      k.r = rank;
-      k.q = q;
-      k.q_stride = stride;
-      k.W = W;
-      k.parts = parts;
-      k.out = to;
-      k.turned = turned;
-      const int done = token_sums<T>(
-          k, p, aligned16(q, stride, size) && static_cast<size_t>(W) * size % 16 == 0, st);
-      if (done != MLXROCM_OK) {
-        return done;
-      }
-      const JoinArgs j{parts, grouped.slots, to, rank, W, turned};
-      join_kernel<T><<<dim3((W + 255) / 256, rank, adapters), 256, 0, st>>>(j);
-      MLXROCM_HIP_TRY(hipGetLastError());
-      return static_cast<int>(MLXROCM_OK);
     };
     const bool needs_g = dx != nullptr || da != nullptr;
     if (needs_g) {
@@ -1508,8 +1522,21 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
         return done;
       }
     }
-    if (db != nullptr) { // (right behind what has read dout already)
-      const int done = sums(h, 1, dout, dout_stride, N, db, 1);
+    // (right behind what has read dout already)
+    if (da != nullptr || db != nullptr) {
+      const auto across = [](const void* to, int W) {
+        return to == nullptr ? 0 : (W + kColumns - 1) / kColumns;
+      };
+      TokenArgs k{};
+      k.rows = runs;
+      k.split_stride = rows * p.padded;
+      k.padded = p.padded;
+      k.r = rank;
+      k.of[0] = {h, 1, dout, dout_stride, N, across(db, N), reinterpret_cast<float*>(ws + p.parts_b),
+                 db, 1};
+      k.of[1] = {g, p.splits, x, x_stride, K, across(da, K), reinterpret_cast<float*>(ws + p.parts_a),
+                 da, 0};
+      const int done = token_sums<T>(k, p, grouped.slots, adapters, st);
       if (done != MLXROCM_OK) {
         return done;
       }
@@ -1522,15 +1549,10 @@ extern "C" int mlxrocm_adapter_matmul_vjp(
       ea.N = K;
       ea.r = p.padded;
       ea.out = dx;
-      ea.h_sum = g_sum;
       const int done = expand<T>(ea, p, aligned16(dx, K, size), st);
       if (done != MLXROCM_OK) {
         return done;
       }
-    }
-    if (da != nullptr) {
-      return dx != nullptr ? sums(g_sum, 1, x, x_stride, K, da, 0)
-                           : sums(g, p.splits, x, x_stride, K, da, 0);
     }
     return static_cast<int>(MLXROCM_OK);
   });
