@@ -171,25 +171,28 @@ __device__ __forceinline__ void multiply(const uint4& a, const uint4& b, floatx4
 }
 
 // Elements k .. k + 15 / sizeof(T) of a row of n; what lies past its end is zero (kWhole: nothing
-// does)
+// does).  Sixteen bytes at once also where they are not aligned (4110 tokens of 1024 values to 1001 by
+// rank 128, float16 with gradients: 194 us; element by element 353).
 template <typename T, bool kAligned, bool kWhole = false>
 __device__ __forceinline__ uint4 operand(const T* row, int k, int n) {
+  union {
+    uint4 u;
+    T e[kPer<T>];
+  } raw;
   if constexpr (kAligned) { // (n is a multiple)
     if constexpr (kWhole) {
       return *reinterpret_cast<const uint4*>(row + k);
     }
     return k < n ? *reinterpret_cast<const uint4*>(row + k) : uint4{0, 0, 0, 0};
+  } else if (kWhole || k + kPer<T> <= n) {
+    __builtin_memcpy(&raw.u, row + k, 16);
   } else {
-    union {
-      uint4 u;
-      T e[kPer<T>];
-    } raw;
 #pragma unroll
     for (int i = 0; i < kPer<T>; ++i) {
       raw.e[i] = k + i < n ? row[k + i] : static_cast<T>(0.0f);
     }
-    return raw.u;
   }
+  return raw.u;
 }
 
 struct ShrinkArgs {
@@ -387,6 +390,8 @@ __device__ __forceinline__ void store_part(T* row, int n, int end, const Part<T>
     if (n < end) {
       *reinterpret_cast<uint4*>(row + n) = v.u;
     }
+  } else if (n + kPer<T> <= end) {
+    __builtin_memcpy(row + n, &v.u, 16);
   } else {
 #pragma unroll
     for (int k = 0; k < kPer<T>; ++k) {
@@ -1015,27 +1020,85 @@ struct JoinArgs {
   int r;
   TokenSum of[2];
 };
+// Of an adapter's sum 16 ranks of 64 columns a workgroup, through LDS where the result is turned, so
+// that a row's ranks are written side by side; zeros as they lie, 16 bytes a thread
+constexpr int kJoined = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+  __shared__ float held[kJoined][17];
   const int adapter = blockIdx.z;
   const int first = a.slots[2 * adapter];
   const int count = a.slots[2 * adapter + 1];
-  const bool second = static_cast<int>(blockIdx.x) >= a.of[0].across;
-  const TokenSum& m = a.of[second];
-  const int n = (blockIdx.x - (second ? a.of[0].across : 0)) * kColumns + threadIdx.x;
-  const int rank = blockIdx.y;
-  if (first < 0 || n >= m.W) {
+  if (first < 0) {
     return;
   }
-  float v = 0.0f;
-  for (int s = 0; s < count; ++s) {
-    v += m.parts[(static_cast<int64_t>(first + s) * a.r + rank) * m.W + n];
-  }
+  const int blocks = a.of[0].across * (kColumns / kJoined);
+  const bool second = static_cast<int>(blockIdx.x) >= blocks;
+  const TokenSum& m = a.of[second];
+  const int block = blockIdx.x - (second ? blocks : 0);
   T* out = static_cast<T*>(m.out) + static_cast<int64_t>(adapter) * a.r * m.W;
-  out[m.turned ? static_cast<int64_t>(n) * a.r + rank : static_cast<int64_t>(rank) * m.W + n] =
-      from_f32<T>(v);
+  if (count == 0) {
+    const int all = a.r * m.W; // (2^29 at most)
+    const int across = m.across * (kColumns / kJoined);
+    const int from = (blockIdx.y * across + block) * 16 * kJoined;
+    const int end = min(all, from + 16 * kJoined);
+    for (int n = from + kPer<T> * threadIdx.x; n < end; n += 256 * kPer<T>) {
+      Part<T> zero;
+      zero.u = uint4{0, 0, 0, 0};
+      store_part<T, false>(out, n, end, zero);
+    }
+    return;
+  }
+  const int c0 = block * kJoined;
+  const int rank0 = blockIdx.y * 16;
+  const int column = threadIdx.x & 63;
+  const int ranks = min(16, a.r - rank0);
+  const int wave = threadIdx.x >> 6;
+  if (c0 + column < m.W) {
+    // (four ranks a thread, of two parts at once)
+    const int64_t part = static_cast<int64_t>(a.r) * m.W;
+    const float* p = m.parts + first * part + static_cast<int64_t>(rank0) * m.W + c0 + column;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < count; s += 2) {
+      float one[4];
+      float two[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = static_cast<int64_t>(min(wave + 4 * j, ranks - 1)) * m.W;
+        one[j] = p[s * part + at];
+        two[j] = p[min(s + 1, count - 1) * part + at];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] += one[j];
+        v[j] += s + 1 < count ? two[j] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = wave + 4 * j;
+      if (i >= ranks) {
+        break;
+      }
+      if (m.turned) {
+        held[column][i] = v[j];
+      } else {
+        out[static_cast<int64_t>(rank0 + i) * m.W + c0 + column] = from_f32<T>(v[j]);
+      }
+    }
+  }
+  if (m.turned) {
+    __syncthreads();
+    for (int n = threadIdx.x; n < 16 * kJoined; n += 256) {
+      const int c = n / 16;
+      const int i = n % 16;
+      if (c0 + c < m.W && i < ranks) {
+        out[static_cast<int64_t>(c0 + c) * a.r + rank0 + i] = from_f32<T>(held[c][i]);
+      }
+    }
+  }
 }
-static_assert(kColumns == 256, "a workgroup of join_kernel has a block of columns");
+static_assert(kColumns % kJoined == 0);
 
 // ---------------------------------------------------------------- plans
 // Sizes of a call and where things lie in its workspace, in bytes
@@ -1246,7 +1309,8 @@ int token_sums(TokenArgs a, const Plan& p, const int32_t* slots, int adapters, h
     return status;
   }
   const JoinArgs j{slots, a.r, {a.of[0], a.of[1]}};
-  join_kernel<T><<<dim3(a.of[0].across + a.of[1].across, a.r, adapters), 256, 0, stream>>>(j);
+  const dim3 grid((a.of[0].across + a.of[1].across) * (kColumns / kJoined), (a.r + 15) / 16, adapters);
+  join_kernel<T><<<grid, 256, 0, stream>>>(j);
   MLXROCM_HIP_TRY(hipGetLastError());
   return MLXROCM_OK;
 }
