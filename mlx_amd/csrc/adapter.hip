@@ -25,6 +25,12 @@
 //            first, whose dout the products before have just read (46 us of 235 MB then, 109 behind dx).
 //   join     their parts, in order; zeros for adapters without tokens.
 //
+// Measured, bfloat16: 8192 tokens of 4096 values to 14336 by rank 16: shrink 19 us, expand 113 (470 MB,
+// 4.2 TB/s); backward group 5, turn 5, shrink 64 (235 MB, while the 235 MB before are still written back;
+// alone 48), tokens 63 (302 MB), join 6, expand 21.  13 x 601 tokens of 14336 to 4096 by rank 32, float16:
+// shrink 65 (224 MB, and as many bytes of A from L2), expand 42 (128 MB).  48 requests of 64 adapters of
+// rank 64, 4096 to 14336: 8 and 20, where their 86 MB take 17.
+//
 // No atomics: the same inputs give the same bits.
 #include <cmath>
 

