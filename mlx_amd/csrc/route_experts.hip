@@ -319,11 +319,17 @@ __device__ __forceinline__ bool exact_groups(
   for (int d = 1; d < a.group_lanes; d *= 2) {
     third = fmaxf(third, __shfl_xor(third, d, 64));
   }
-  // (equal ones cannot be told apart here)
   bool known = one - two > apart;
   // each lane the choices of those that it has; of a group's lanes one has the best, one the second
+  // (equal ones cannot be told apart here)
   double sum = l_of[0] == -INFINITY ? 0.0 : exact_choice(true, l_of[0], b_of[0]);
-  int has = (l_of[0] != -INFINITY) + 256 * (l_of[1] != -INFINITY);
+  // how many have the best, and the second: a lane may have more than one of them
+  constexpr int kSecond = 1 << 16;
+  int has = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    has += c[j] == one ? 1 : c[j] == two ? kSecond : 0;
+  }
   if (a.group_best == 2) {
     known = known && two - third > apart;
     sum += l_of[1] == -INFINITY ? 0.0 : exact_choice(true, l_of[1], b_of[1]);
@@ -332,7 +338,7 @@ __device__ __forceinline__ bool exact_groups(
     sum += __shfl_xor(sum, d, 64);
     has += __shfl_xor(has, d, 64);
   }
-  known = known && (has & 255) == 1 && (a.group_best == 1 || has >> 8 == 1);
+  known = known && has % kSecond == 1 && (a.group_best == 1 || has / kSecond == 1);
   // (a group whose two are not known: nor are the row's)
   const uint32_t not_known = static_cast<uint32_t>(
       __ballot(!known && p.group < a.groups) >> (threadIdx.x & 48));

@@ -330,3 +330,35 @@ def test_replays_and_experts(gpu):
         torch.cuda.synchronize()
         for got, ref in zip(out, want):
             assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("second, third", ((20.0, 18.0), (18.0, 20.0)))
+def test_second_choices_of_a_group_that_are_equal_in_32_bits(gpu, dtype, second, third):
+    """Sigmoids of 18, 19 and 20 are one number there: groups go by the larger of neighbours in 64."""
+    logits = torch.full((1, 32), -10.0, dtype=dtype)
+    logits[0, [0, 2, 3]] = torch.tensor([0.0, second, third], dtype=dtype)
+    logits[0, [16, 18]] = torch.tensor([0.0, 19.0], dtype=dtype)
+    bias = torch.zeros(32, device="cuda")
+    bias[[0, 16]] = 1.0
+    options = dict(scoring="sigmoid", bias=bias, groups=2, top_groups=1, group_best=2)
+    indices, *_ = check(logits, 1, **options)
+    assert indices.tolist() == [[0]]
+    check(logits, 5, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts, groups", ((32, 2), (48, 3), (256, 8), (240, 5), (1024, 4)))
+def test_saturated_choices_of_groups(gpu, dtype, experts, groups):
+    """One choice of each group stands out, the others are equal in 32 bits or masked out."""
+    g = torch.Generator().manual_seed(experts)
+    some = torch.tensor([-10.0, -10.0, -10.0, 17.0, 17.5, 18.0, 19.0, 20.0, -math.inf], dtype=dtype)
+    logits = some[torch.randint(0, len(some), (33, experts), generator=g)]
+    bias = torch.zeros(experts, device="cuda")
+    size = experts // groups
+    logits[:, ::size] = 0.0
+    bias[::size] = 1.0
+    for best in (1, 2):
+        for k in (1, 8):
+            check(logits, k, scoring="sigmoid", bias=bias, groups=groups, top_groups=groups // 2,
+                  group_best=best)
