@@ -524,9 +524,12 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
           keys[j] = j < p.n ? keys[j] : 0;
         }
       }
-      // both of them off, and both cut to whole numbers
-      const uint32_t apart = (static_cast<uint32_t>(2.0f * off * scale) + 3) * kPlaces;
-      known = known && fabsf(top) < INFINITY;
+      // both of them off, and both cut to whole numbers; choices as large as a bias of 2^21 are off by
+      // more than the keys reach, and no order is known
+      const float most_off = 2.0f * off * scale;
+      constexpr float kReach = 0x1p32f / kPlaces - 4.0f;
+      const uint32_t apart = (static_cast<uint32_t>(fminf(most_off, kReach)) + 3) * kPlaces;
+      known = known && most_off < kReach && fabsf(top) < INFINITY;
       bool in_order = take<V>(a.k, apart, keys, mine);
       // Where they are too near each other, but the first n >= k of sixteen are known to be the
       // largest: a lane each, their choices in 64 bits, and a place for each.

@@ -362,3 +362,20 @@ def test_saturated_choices_of_groups(gpu, dtype, experts, groups):
         for k in (1, 8):
             check(logits, k, scoring="sigmoid", bias=bias, groups=groups, top_groups=groups // 2,
                   group_best=best)
+
+
+@pytest.mark.parametrize("scoring", ("sigmoid", "softmax"))
+@pytest.mark.parametrize("experts", (16, 256, 1024))
+@pytest.mark.parametrize("size", (2.0 ** 17, 2097150.0, 2.0 ** 21, 3e6, 2.0 ** 24, 2.0 ** 33, 1e30))
+def test_large_biases_keep_the_order_of_64_bits(gpu, scoring, experts, size):
+    """A bias that forces experts leaves 32 bits nothing of their scores."""
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn((12, experts), generator=g)
+    bias = torch.zeros(experts, device="cuda")
+    bias[:6] = size
+    bias[6:9] = -size
+    logits[:, 0], logits[:, 1] = 0.49, 0.532  # sigmoids of 0.62 and 0.63
+    for k in (1, 2, 4, 9):
+        check(logits, k, scoring=scoring, bias=bias)
+    check(logits, 3, scoring=scoring, bias=bias, groups=4, top_groups=2, group_best=2)
+    check(logits, 3, scoring=scoring, bias=-bias)
