@@ -486,9 +486,9 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
         const bool stays = group_counts<V, float>(a, p, c, &gap);
         counts = stays && counts;
         if constexpr (kSums) {
-          float size = fmaxf(fabsf(c[0]), 1.0f); // (of what the choices are off by)
+          float size = 1.0f; // (of what the choices are off by; lanes may have none)
 #pragma unroll
-          for (int j = 1; j < V; ++j) {
+          for (int j = 0; j < V; ++j) {
             size = c[j] > -INFINITY ? fmaxf(size, fabsf(c[j])) : size;
           }
           const float apart = 4.0f * off * (1.0f + largest16(size));

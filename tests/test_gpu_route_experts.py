@@ -379,3 +379,28 @@ def test_large_biases_keep_the_order_of_64_bits(gpu, scoring, experts, size):
         check(logits, k, scoring=scoring, bias=bias)
     check(logits, 3, scoring=scoring, bias=bias, groups=4, top_groups=2, group_best=2)
     check(logits, 3, scoring=scoring, bias=-bias)
+
+
+@pytest.mark.parametrize("experts, groups, top", ((48, 3, 2), (9, 1, 1), (36, 4, 2), (45, 5, 3), (130, 13, 6),
+                                                  (96, 12, 5), (54, 6, 6)))
+def test_groups_that_leave_lanes_without_experts(gpu, experts, groups, top):
+    """No power of two of groups, or of experts of one; experts that are masked in front of a group."""
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn((24, experts), generator=g) * 2
+    logits[:8, 1::2] = logits[:8, :-1:2]  # pairs of one score
+    size = experts // groups
+    logits[6:12, ::size] = -math.inf
+    logits[10:14, 1::size] = math.nan
+    logits[12:18] += 20  # sigmoids that 32 bits do not tell apart
+    bias = (torch.randn((experts,), generator=g) * 0.1).cuda()
+    rows = [n for n in range(24) if not 10 <= n < 14]
+    for scoring in ("sigmoid", "softmax"):
+        for best in (1, 2):
+            for b in (bias, bias.round(), None):
+                options = dict(scoring=scoring, bias=b, groups=groups, top_groups=top, group_best=best)
+                check(logits[rows], min(5, top * size), **options)
+                # what is NaN is as if it were masked where others are left
+                if scoring == "sigmoid" and size > 5:
+                    got = mlx_amd.route_experts(logits.cuda(), 3, **options)[0]
+                    assert torch.equal(got.cpu(), reference(logits.nan_to_num(-math.inf, math.inf, -math.inf),
+                                                            3, **options)[0])
