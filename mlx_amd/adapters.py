@@ -139,15 +139,15 @@ def adapter_matmul(
     if dtype not in _FLOATING:
         raise ValueError(f"[{tag}] Received unsupported type {dtype}.")
     scales = None
-    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError(f"[{tag}] no gradients with respect to scale.")
     if isinstance(scale, torch.Tensor) and scale.dim() > 0:
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"[{tag}] no gradients with respect to scale.")
         scales, scale = scale, 1.0
         if tuple(scales.shape) != (adapters,) or scales.dtype not in _FLOATING:
             raise ValueError(f"[{tag}] scale must be a number or {adapters} floating-point numbers but has "
                              f"shape {tuple(scales.shape)} and type {scales.dtype}.")
     scale = _finite_scale(tag, scale)
-    if _tangents(*operands):
+    if _tangents(*operands) or (scales is not None and _tangents(scales)):
         raise NotImplementedError(f"[{tag}] no forward-mode gradients.")
     others = [t for t in (indices, scales) if t is not None]
     _require_gpu(tag, *operands, *others)

@@ -72,9 +72,18 @@ def _require_one_device(tag: str, *tensors: torch.Tensor) -> None:
                          f"{', '.join(sorted(map(str, devices)))}.")
 
 
+def _number(tag: str, name: str, value) -> float:
+    """A number of which no gradients are wanted: they would be lost without an error"""
+    if isinstance(value, torch.Tensor) and (
+            (value.requires_grad and torch.is_grad_enabled())
+            or torch.autograd.forward_ad.unpack_dual(value).tangent is not None):
+        raise NotImplementedError(f"[{tag}] no gradients with respect to {name}.")
+    return float(value)
+
+
 def _finite_scale(tag: str, scale) -> float:
     """A factor that the kernels hold in 32 bits"""
-    scale = float(scale)
+    scale = _number(tag, "scale", scale)
     if not abs(scale) <= torch.finfo(torch.float32).max:
         raise ValueError(f"[{tag}] scale must be finite in 32 bits but got {scale}.")
     return scale

@@ -21,7 +21,7 @@ from . import _lib, ops
 from ._copy import astype as _astype, contiguous as _contiguous, copy as _copy
 from .attention import (
     _array, _check_pages, _check_table, _empty_like, _int32, _strides, _table, _tangents)
-from .ops import _DTYPE_CODE, _FLOATING, _require_gpu, _require_one_device, _stream_ptr
+from .ops import _DTYPE_CODE, _FLOATING, _number, _require_gpu, _require_one_device, _stream_ptr
 
 __all__ = ["rope", "rope_cache_update"]
 
@@ -45,8 +45,8 @@ class _Rotation:
             raise ValueError(f"[{tag}] dims must be even and at most {min(D, _MOST_DIMS)} but is {dims}.")
         if base is not None and freqs is not None:
             raise ValueError(f"[{tag}] Only one of base or freqs can have a value.")
-        base = 10000.0 if base is None else float(base)
-        scale = float(scale)
+        base = 10000.0 if base is None else _number(tag, "base", base)
+        scale = _number(tag, "scale", scale)
         if not (math.isfinite(base) and base > 0 and math.isfinite(scale)):
             raise ValueError(f"[{tag}] base must be positive and scale finite but got {base}, {scale}.")
         shape = (batch, length)
@@ -147,7 +147,7 @@ def rope(
         raise ValueError(f"[{tag}] positions are needed.")
     rotation = _Rotation(tag, x.shape[3], x.shape[0], x.shape[2], positions, dims, traditional, base,
                          scale, freqs, sections)
-    if _tangents(x):
+    if _tangents(x) or (freqs is not None and _tangents(freqs)):
         raise NotImplementedError(f"[{tag}] no forward-mode gradients.")
     if freqs is not None and freqs.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"[{tag}] no gradients with respect to freqs.")

@@ -166,6 +166,36 @@ def test_scales_of_a_single_number():
         mlx_amd.adapter_matmul(**ADAPT, scale=scale)
 
 
+FACTORS = (
+    (mlx_amd.rope, ROPE, dict(freqs=torch.ones(32))),
+    (mlx_amd.rope, ROPE, dict(freqs=z(32))),
+    (mlx_amd.rope, ROPE, dict(scale=torch.tensor(2.0))),
+    (mlx_amd.rope, ROPE, dict(base=torch.tensor(500.0))),
+    (mlx_amd.rope_cache_update, UPDATE, dict(freqs=torch.ones(32))),
+    (mlx_amd.rope_cache_update, UPDATE, dict(scale=torch.tensor(2.0))),
+    (mlx_amd.rope_cache_update, UPDATE, dict(base=torch.tensor(500.0))),
+    (mlx_amd.route_experts, ROUTE, dict(scale=torch.tensor(2.0))),
+    (mlx_amd.adapter_matmul, ADAPT, dict(scale=torch.tensor(2.0))),
+    (mlx_amd.adapter_matmul, ADAPT, dict(scale=torch.ones(4))),
+)
+
+
+@pytest.mark.parametrize("call, args, factor", FACTORS)
+def test_gradients_of_factors_are_refused_not_dropped(call, args, factor):
+    import torch.autograd.forward_ad as fwad
+
+    (name, value), = factor.items()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        call(**args, **factor)
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match="gradients"):
+        call(**args, **{name: fwad.make_dual(value, torch.ones_like(value))})
+    leaf = value.clone().requires_grad_()
+    with pytest.raises(NotImplementedError, match="gradients"):
+        call(**args, **{name: leaf})
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+        call(**args, **{name: leaf})
+
+
 def _status(name, *args):
     lib = _lib.load()
     return getattr(lib, name)(*args), lib.mlxrocm_last_error().decode()
