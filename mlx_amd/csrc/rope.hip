@@ -475,7 +475,7 @@ extern "C" int mlxrocm_rope_cache_update(
   a.lengths = lengths;
   a.pages = pages;
   a.page = Divisor(page_size);
-  a.table_width = table_width;
+  a.table_width = pages == 0 ? 0 : table_width; // (no place is in a cache without pages)
   return dispatch_dtype(dtype, [&](auto t) {
     return launch<decltype(t), true>(tag, a, static_cast<hipStream_t>(stream));
   });

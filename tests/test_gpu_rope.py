@@ -1,10 +1,12 @@
 """rope and rope_cache_update against rotations in 64 bits."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import mlx_amd
+from mlx_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -273,6 +275,24 @@ def test_places_that_do_not_exist(gpu):
     case["block_table"][1, 0] = 1 << 20
     before = case["k_pages"].clone(), case["v_pages"].clone()
     check_update(case, mlx_amd.rope_cache_update(**case), before)
+
+
+def test_a_cache_without_pages(gpu):
+    """Queries turn, nothing is written, and neither table nor pages are read: they may be null."""
+    case = update_case(torch.bfloat16, 2, 4, 2, 3, 64, 16, [5, 3])
+    out = torch.full_like(case["q"], math.nan)
+    strides = (ctypes.c_int64 * 19)(*(s for t in (case["q"], case["k"], case["v"], out) for s in t.stride()[:3]))
+    at = case["lengths"][:, None].long() - 3 + torch.arange(3, device="cuda")
+    for pages, width in ((0, 7), (0, 0), (5, 0)):
+        status = _lib.load().mlxrocm_rope_cache_update(
+            *(case[n].data_ptr() for n in "qkv"), out.data_ptr(), None, None, None, case["lengths"].data_ptr(),
+            2, 4, 2, 3, 64, pages, 16, width, strides, None, None, 0, 1, None, 64, 0, 1e4, 1.0, None, 2,
+            torch.cuda.current_stream().cuda_stream)
+        assert status == _lib.OK
+        close(out, reference(case["q"], at))
+        out.fill_(math.nan)
+    empty = {**case, "k_pages": case["k_pages"][:0], "v_pages": case["v_pages"][:0]}
+    close(mlx_amd.rope_cache_update(**empty)[0], reference(case["q"], at))
 
 
 def test_strided_pages_and_tables(gpu):
