@@ -523,11 +523,12 @@ struct Adaption {
 struct AdapterVjp : torch::autograd::Function<AdapterVjp> {
   static at::Tensor forward(
       torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& a,
-      const at::Tensor& b, const at::Tensor& y, const Adaption* of) {
+      const at::Tensor& b, const std::optional<at::Tensor>& y, const Adaption* of) {
     at::Tensor out, h;
-    if (!of->run(x, a, b, y, &out, &h)) {
+    if (!of->run(x, a, b, y.value_or(at::Tensor()), &out, &h)) {
       throw NotPlainCall();
     }
+    ctx->saved_data["beside"] = y.has_value();
     ctx->save_for_backward(
         {x, a, b, h, of->indices == nullptr ? at::Tensor() : *of->indices});
     ctx->saved_data["scale"] = of->scale;
@@ -568,7 +569,7 @@ struct AdapterVjp : torch::autograd::Function<AdapterVjp> {
               stream_of(device)) == MLXROCM_OK,
           abi.last_error());
     }
-    if (ctx->needs_input_grad(3)) {
+    if (ctx->saved_data["beside"].toBool() && ctx->needs_input_grad(3)) {
       to[3] = grads[0];
       if (at::GradMode::is_enabled()) {
         to[3] = to[3].detach();
@@ -627,7 +628,9 @@ PyObject* adapter_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   of.sizes_of(*x, *a, *b);
   if (records_grad(*x) || records_grad(*a) || records_grad(*b) ||
       (y.defined() && records_grad(y))) {
-    return wrap(AdapterVjp::apply(*x, *a, *b, y, &of));
+    // (the graph has no place for a tensor that is none)
+    const std::optional<at::Tensor> beside = y.defined() ? std::optional(y) : std::nullopt;
+    return wrap(AdapterVjp::apply(*x, *a, *b, beside, &of));
   }
   at::Tensor out;
   bool done = false;
