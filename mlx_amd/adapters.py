@@ -101,9 +101,9 @@ def adapter_matmul(
     adapter's (-1, say) has none: ``y`` as it is.  Without ``indices`` there is one adapter for all, and
     ``a`` and ``b`` may be matrices.  ``scale``: a number, or one of each adapter ``[adapters]``.
 
-    Sums are formed in 32 bits, ``x @ a.T`` is kept in 32 (float32) or as the sum of two numbers of the
-    type, and the result is rounded once.  A request's values do not reach another's, whatever they are;
-    with an adapter that is not finite a request's own may be NaN where infinity is meant.  Up to 1024
+    Sums are formed in 32 bits, ``x @ a.T`` is kept in them (float16: in 23 bits of a token's largest), and
+    the result is rounded once.  A request's values do not reach another's, whatever they are; where
+    adapters or gradients are not finite a request's own may be NaN where infinity is meant.  Up to 1024
     adapters of rank up to 256; adapters of a lower rank than others are filled up with zeros.
     Differentiable with respect to x, a, b and y (once, in reverse mode)."""
     out = ops._fast.adapter_matmul(x, a, b, indices, scale, y)

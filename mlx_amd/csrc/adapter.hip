@@ -15,19 +15,22 @@
 //            none: every workgroup finds its tile by itself, an index a lane (13 prompts: 6 us less).
 //   shrink   h or g, in 32 bits.  The four wavefronts of a workgroup and, for few tokens, several
 //            workgroups share a token's sum; the parts are added in one order by who reads them.
-//   expand   out or dx.  16-bit types: h as the sum of two numbers of the type, against the same
-//            operand of B twice (up to 16 ranks: in one instruction of 32).  So h keeps 16 bits
-//            (bfloat16) or 22, and the result's own rounding is all that is seen.  float16: h
-//            counts a power of two that brings the token's largest to 2^13.
+//   expand   out or dx.  16-bit types: h as the sum of numbers of the type, against the same operand
+//            of B: three in bfloat16, all of float32's 24 bits; two in float16, 23 bits of the token's
+//            largest, which h is counted by a power of two to bring to 2^13 (a smaller rank keeps 23 of
+//            its own down to 2^-16 of that, then 2^-38 of it).  So sums that cancel keep what 32 bits
+//            have of them (with two numbers, 17 bits, in bfloat16 8192 tokens of 4096 to 14336 by rank 16
+//            take as long, 16384 of 8192 to 1024 by rank 32 with gradients 284 us instead of 288).
 //   turn     A and B with their two dimensions swapped, for the gradients: then g and dx are the
 //            same two products.
 //   tokens   dB and dA in one launch: sums over tokens, cut so that workgroups fill the card; dB
 //            first, whose dout the products before have just read (47 us of 235 MB then, 66 behind dx).
+//            h and g as three bfloat16 numbers, float16 activations as two.
 //   join     their parts, in order; zeros for adapters without tokens.
 //
 // Measured, bfloat16: 8192 tokens of 4096 values to 14336 by rank 16: shrink 19 us, expand 113 (470 MB,
 // 4.2 TB/s); backward group 5, turn 5, shrink 64 (235 MB, while the 235 MB before are still written back;
-// alone 48), tokens 63 (302 MB), join 6, expand 21.  13 x 601 tokens of 14336 to 4096 by rank 32, float16:
+// alone 48), tokens 64 (302 MB), join 6, expand 21.  13 x 601 tokens of 14336 to 4096 by rank 32, float16:
 // shrink 65 (224 MB, and as many bytes of A from L2), expand 42 (128 MB).  48 requests of 64 adapters of
 // rank 64, 4096 to 14336: 8 and 20, where their 86 MB take 17.
 //
@@ -362,24 +365,26 @@ __device__ __forceinline__ floatx4 sum_of_parts(const float* p, int splits, int6
   return v;
 }
 
-// Eight ranks of a token's h times `by`, rounded, or what rounding took from them; float32: four
+// Eight ranks of a token's h times `by`: the first, second or third of the numbers of the type whose
+// sum it is; float32: four, as they are
 template <typename T>
-__device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], bool lower, float by) {
+__device__ __forceinline__ uint4 rank_operand(const float (&v)[kPer<T>], int part, float by) {
   if constexpr (sizeof(T) == 4) {
     return __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3]));
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float part[2];
+      float of[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float x = v[2 * i + j] * by;
         const float upper = round_to<T>(x);
-        // (of what is not finite there is no lower part)
-        part[j] = !lower ? upper : fabsf(upper) < INFINITY ? x - upper : 0.0f;
+        const float rest = fabsf(upper) < INFINITY ? x - upper : 0.0f; // (of what is finite)
+        const float lower = round_to<T>(rest);
+        of[j] = part == 0 ? upper : part == 1 ? lower : rest - lower;
       }
-      w[i] = pack2<T>(part[0], part[1]);
+      w[i] = pack2<T>(of[0], of[1]);
     }
     return uint4{w[0], w[1], w[2], w[3]};
   }
@@ -408,8 +413,10 @@ __device__ __forceinline__ void store_part(T* row, int n, int end, const Part<T>
   }
 }
 
+// (128 ranks: within the registers of two workgroups a CU.  With one, 4110 tokens to 1001 columns in bfloat16
+// take 42 us instead of 31)
 template <typename T, int kGroups, int kChunks, bool kAligned, bool kAdd>
-__global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
+__global__ __launch_bounds__(256, kChunks == 8 ? 2 : 1) void expand_kernel(const ExpandArgs a) {
   constexpr int kPitch = 16 * kChunks + 4; // (rows of neighbouring tokens four banks apart)
   constexpr int kParts = 16 / kPer<T>;     // of a lane's results
   __shared__ int rows[kFew];
@@ -439,12 +446,14 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
     }
     return;
   }
-  // An instruction has 16 ranks (float32), 32, or 16 of the upper parts and the same of the lower
-  // ones; of those the lane has kPer from rank_of on
-  constexpr bool kPairs = sizeof(T) == 2 && kChunks > 1;
-  constexpr int kSteps = kPairs ? kChunks / 2 : kChunks;
-  constexpr int kRanks = kPairs ? 32 : 16;
-  const int rank_of = sizeof(T) == 4 ? 4 * quarter : kPairs ? 8 * quarter : 8 * (quarter & 1);
+  // An instruction has 16 ranks (float32), 32, or 16 of the first parts and the same of the second
+  // (bfloat16: then of the third, and nothing); of those the lane has kPer from rank_of on
+  constexpr bool kWhole = sizeof(T) == 2 && kChunks > 1;
+  constexpr int kParted = sizeof(T) == 4 ? 1 : std::is_same_v<T, bf16_t> ? 3 : 2;
+  constexpr int kTerms = sizeof(T) == 4 || kWhole ? kParted : kParted - 1;
+  constexpr int kSteps = kWhole ? kChunks / 2 : kChunks;
+  constexpr int kRanks = kWhole ? 32 : 16;
+  const int rank_of = sizeof(T) == 4 ? 4 * quarter : kWhole ? 8 * quarter : 8 * (quarter & 1);
   const T* b = static_cast<const T*>(a.b) + adapter * a.b_stride;
   const int n_begin = n_block + 64 * wave;
   // Of 64 columns a lane's results are 16 bytes of neighbours, the four quarters' side by side: row
@@ -512,8 +521,7 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
       }
     }
     __syncthreads();
-    uint4 h[kGroups][kSteps];
-    uint4 lower[kGroups][kPairs ? kSteps : 1];
+    uint4 h[kGroups][kSteps][kTerms];
     float back[kGroups]; // float16: what h was divided by
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -549,11 +557,12 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
       }
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
-        if constexpr (kPairs) {
-          h[i][c] = rank_operand<T>(v[c], false, by);
-          lower[i][c] = rank_operand<T>(v[c], true, by);
-        } else {
-          h[i][c] = rank_operand<T>(v[c], quarter >= 2, by);
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) {
+          h[i][c][t] = rank_operand<T>(v[c], kTerms == kParted ? t : t == 1 ? 2 : quarter >= 2, by);
+          if (kTerms < kParted && t == 1 && quarter >= 2) {
+            h[i][c][t] = uint4{0, 0, 0, 0};
+          }
         }
       }
     }
@@ -565,9 +574,9 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs a) {
         for (int c = 0; c < kSteps; ++c) {
 #pragma unroll
           for (int i = 0; i < kGroups; ++i) {
-            multiply<T>(weights[j][c], h[i][c], sum[i][j]);
-            if constexpr (kPairs) {
-              multiply<T>(weights[j][c], lower[i][c], sum[i][j]);
+#pragma unroll
+            for (int t = 0; t < kTerms; ++t) {
+              multiply<T>(weights[j][c], h[i][c][t], sum[i][j]);
             }
           }
         }
@@ -796,6 +805,35 @@ __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs a) {
 }
 
 // ---------------------------------------------------------------- sums over tokens
+// bfloat16 numbers whose sum n values are, of which the first of a pair is in the lower half: each is
+// what is left without its last 16 bits.  (Rounded ones take half as many instructions again.)
+template <int kParts, int n>
+__device__ __forceinline__ void cut(const float (&v)[n], uint32_t (&w)[kParts][n / 2]) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    most = fmaxf(most, fabsf(v[i]));
+  }
+  const bool infinite = __any(most == INFINITY); // (of infinity nothing is left; NaN stays NaN)
+#pragma unroll
+  for (int i = 0; i < n / 2; ++i) {
+    float x = v[2 * i];
+    float y = v[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      const uint32_t x_bits = __float_as_uint(x);
+      const uint32_t y_bits = __float_as_uint(y);
+      w[k][i] = __builtin_amdgcn_perm(y_bits, x_bits, 0x07060302);
+      x -= __uint_as_float(x_bits & 0xffff0000u);
+      y -= __uint_as_float(y_bits & 0xffff0000u);
+      if (k == 0 && infinite) {
+        x = fabsf(v[2 * i]) == INFINITY ? 0.0f : x;
+        y = fabsf(v[2 * i + 1]) == INFINITY ? 0.0f : y;
+      }
+    }
+  }
+}
+
 struct TokenSum {
   const float* p; // [splits, T, padded]: h or g
   int splits;
@@ -915,25 +953,9 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
         }
       }
     } else {
-      // In bfloat16, whose range is float32's: p as two numbers, a float16 q as two as well (exactly)
-      uint4 p[2][kChunks];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        uint32_t w[2][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = p_tile[which][8 * quarter + 2 * i][16 * c + column];
-          const float y = p_tile[which][8 * quarter + 2 * i + 1][16 * c + column];
-          const float x_upper = round_to<bf16_t>(x);
-          const float y_upper = round_to<bf16_t>(y);
-          w[0][i] = pack2<bf16_t>(x_upper, y_upper);
-          w[1][i] = pack2<bf16_t>(
-              fabsf(x_upper) < INFINITY ? x - x_upper : 0.0f,
-              fabsf(y_upper) < INFINITY ? y - y_upper : 0.0f);
-        }
-        p[0][c] = uint4{w[0][0], w[0][1], w[0][2], w[0][3]};
-        p[1][c] = uint4{w[1][0], w[1][1], w[1][2], w[1][3]};
-      }
+      // In bfloat16, whose range is float32's: p as three numbers, a float16 q as two (exactly; what the
+      // third and the second give is 2^-24 of the product)
+      uint4 q[4][std::is_same_v<T, bf16_t> ? 1 : 2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // A lane of sixteen gives the place of 4 columns of a token and gets 4 tokens of a column
@@ -951,33 +973,41 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
           w[2 * half + 1] = u.y;
         }
         if constexpr (std::is_same_v<T, bf16_t>) {
-          const uint4 q = uint4{w[0], w[1], w[2], w[3]};
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            sum[j][c] = mfma16<bf16_t>(q, p[0][c], sum[j][c]);
-            sum[j][c] = mfma16<bf16_t>(q, p[1][c], sum[j][c]);
-          }
+          q[j][0] = uint4{w[0], w[1], w[2], w[3]};
         } else {
-          uint32_t upper[4];
-          uint32_t lower[4];
+          float v[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = half_of<f16_t>(w[i], 0);
-            const float y = half_of<f16_t>(w[i], 1);
-            const float x_upper = round_to<bf16_t>(x);
-            const float y_upper = round_to<bf16_t>(y);
-            upper[i] = pack2<bf16_t>(x_upper, y_upper);
-            lower[i] = pack2<bf16_t>(
-                fabsf(x_upper) < INFINITY ? x - x_upper : 0.0f,
-                fabsf(y_upper) < INFINITY ? y - y_upper : 0.0f);
+          for (int i = 0; i < 8; ++i) {
+            v[i] = half_of<f16_t>(w[i / 2], i % 2);
           }
-          const uint4 q = uint4{upper[0], upper[1], upper[2], upper[3]};
-          const uint4 rest = uint4{lower[0], lower[1], lower[2], lower[3]};
+          uint32_t part[2][4];
+          cut(v, part);
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            sum[j][c] = mfma16<bf16_t>(q, p[0][c], sum[j][c]);
-            sum[j][c] = mfma16<bf16_t>(q, p[1][c], sum[j][c]);
-            sum[j][c] = mfma16<bf16_t>(rest, p[0][c], sum[j][c]);
+          for (int k = 0; k < 2; ++k) {
+            q[j][k] = uint4{part[k][0], part[k][1], part[k][2], part[k][3]};
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = p_tile[which][8 * quarter + i][16 * c + column];
+        }
+        uint32_t w[3][4];
+        cut(v, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const uint4 p = uint4{w[k][0], w[k][1], w[k][2], w[k][3]};
+            sum[j][c] = mfma16<bf16_t>(q[j][0], p, sum[j][c]);
+            if constexpr (std::is_same_v<T, f16_t>) {
+              if (k < 2) {
+                sum[j][c] = mfma16<bf16_t>(q[j][1], p, sum[j][c]);
+              }
+            }
           }
         }
       }

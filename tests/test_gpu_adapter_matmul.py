@@ -363,3 +363,70 @@ def test_indices_of_every_type(gpu, dtype):
     want = mlx_amd.adapter_matmul(
         **{**args, "indices": torch.tensor([0, -1, 2, -1, -1, 1], dtype=torch.int32).cuda()})
     assert torch.equal(got, want)
+
+
+def whole(*shape, most, g, dtype):
+    return torch.randint(0, most + 1, shape, generator=g).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T, r, odd", ((1, 8, 0), (3, 16, 1), (40, 16, 0), (40, 30, 0), (70, 64, 1), (70, 64, 0),
+                                       (40, 128, 0), (5, 130, 0), (40, 256, 1)))
+def test_sums_over_ranks_and_tokens_keep_their_32_bits(gpu, dtype, T, r, odd):
+    """Whole numbers whose sums 32 bits hold (below 2**24; 2**23, where float16 keeps 23 bits of a
+    token's h): what stays when they cancel is right to the last bit, and rounded once."""
+    g = torch.Generator().manual_seed(T + r)
+    half = dtype == torch.float16
+    K = (64 if half else 256) + odd
+    small, large = 255, 511 if half else 255
+
+    def exactly(got, want):
+        assert torch.equal(got.detach(), want.to(dtype)), float((got.detach().double() - want).abs().max())
+
+    # out: h[n % r] 2**-10 beside a y that is nearly its opposite
+    N = 2 * r + odd
+    x, a = whole(T, K, most=large, g=g, dtype=dtype), whole(1, r, K, most=small, g=g, dtype=dtype)
+    h = (x.double() @ a[0].double().T)[:, torch.arange(N) % r] * 2.0 ** -10
+    assert float(h.max()) < 2.0 ** (13 if half else 14) and float(h.max()) > 2.0 ** 10
+    b = torch.zeros((1, N, r), dtype=dtype, device="cuda")
+    b[0, torch.arange(N), torch.arange(N) % r] = 2.0 ** -10
+    y = -h.to(torch.bfloat16).to(dtype)
+    exactly(mlx_amd.adapter_matmul(x, a, b, y=y), h + y.double())
+    # h[2 j] - h[2 j + 1], whose rows of a differ in one place
+    even = r - r % 2
+    a = whole(1, r, K, most=small - 1, g=g, dtype=dtype)
+    a[0, 1:even:2] = a[0, :even:2]
+    a[0, 1:even:2, K // 3] += 1
+    b = torch.zeros((1, N, r), dtype=dtype, device="cuda")
+    b[0, torch.arange(N), torch.arange(N) % (even // 2) * 2] = 1.0
+    b[0, torch.arange(N), torch.arange(N) % (even // 2) * 2 + 1] = -1.0
+    exactly(mlx_amd.adapter_matmul(x, a, b), x.double() @ a[0].double().T @ b[0].double().T)
+    # dx: g[2 j] - g[2 j + 1], whose columns of b differ in one place
+    x, a = torch.ones((T, 2 * r + odd), dtype=dtype, device="cuda"), torch.zeros((1, r, 2 * r + odd), dtype=dtype)
+    n = torch.arange(even)
+    a[0, n, n // 2] = 1.0 - 2.0 * (n % 2).to(dtype)
+    b = whole(1, K, r, most=small - 1, g=g, dtype=dtype)
+    b[0, :, 1:even:2] = b[0, :, :even:2]
+    b[0, K // 3, 1:even:2] += 1
+    a = a.cuda()
+    dout = whole(T, K, most=large, g=g, dtype=dtype)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(mlx_amd.adapter_matmul(x, a, b), x, dout)
+    exactly(dx, dout.double() @ b[0].double() @ a[0].double())
+    # da and db: pairs of tokens that cancel but for one place; 16 tokens that are not zero, of 2**20 each
+    T = max(T, 16)
+    at = torch.randperm(T, generator=g)[:16].cuda()
+    sign = torch.zeros((T, 1), dtype=dtype, device="cuda")
+    sign[at[:8]], sign[at[8:]] = 1.0, -1.0
+    pairs = whole(T, 256, most=63, g=g, dtype=dtype)
+    pairs[at[8:]] = pairs[at[:8]]
+    pairs[at[8:], 7] += 1
+    weights = whole(1, 256, r, most=63, g=g, dtype=dtype)
+    x, a = (sign * torch.ones((1, 40 + odd), dtype=dtype, device="cuda")), whole(1, r, 40 + odd, most=3, g=g, dtype=dtype)
+    a.requires_grad_()
+    da, = torch.autograd.grad(mlx_amd.adapter_matmul(x, a, weights), a, pairs)
+    exactly(da[0], (pairs.double() @ weights[0].double()).T @ x.double())
+    b = torch.zeros((1, 40 + odd, r), dtype=dtype, device="cuda", requires_grad=True)
+    a = weights.transpose(1, 2).contiguous()
+    db, = torch.autograd.grad(mlx_amd.adapter_matmul(pairs, a, b), b, sign.expand(T, 40 + odd))
+    exactly(db[0], sign.expand(T, 40 + odd).double().T @ (pairs.double() @ a[0].double().T))
