@@ -163,5 +163,6 @@ def adapter_matmul(
         # (torch's own conversion: autograd converts the gradients back)
         operands = [t.to(dtype) for t in operands] + [None] * (4 - len(operands))
         return _AdapterVjp.apply(*operands, indices, scales, scale)
-    operands = [_astype(t, dtype) for t in operands] + [None] * (4 - len(operands))
+    with torch.cuda.device(x.device):
+        operands = [_astype(t, dtype) for t in operands] + [None] * (4 - len(operands))
     return _forward(*operands, indices, scales, scale, False)[0]

@@ -203,3 +203,53 @@ def test_twice_is_refused_and_unused_results_have_no_gradient(both):  # noqa: F8
         return indices, weights
 
     both(twice)
+
+
+def test_every_launch_is_on_the_tensors_device(monkeypatch):
+    """The bodies make the tensors' device the current one before they convert, copy or compute: an
+    operand may be on another."""
+    from mlx_amd import _copy, ops, rotary
+    from test_gpu_fast_ops import _Nothing
+
+    inside = []
+    device, copy, lib = torch.cuda.device, _copy.copy, _lib.load()
+
+    class Device(device):
+        def __enter__(self):
+            inside.append(self)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            inside.pop()
+            return super().__exit__(*args)
+
+    def copied(*args):
+        assert inside, "a copy"
+        return copy(*args)
+
+    class Checked:
+        def __getattr__(self, name):
+            if not name.endswith("_size") and name != "mlxrocm_last_error":
+                assert inside, name
+            return getattr(lib, name)
+
+    x, a, b, y = adapted(torch.bfloat16, 3)
+    q, k = _x(2, 7, 4, 64).transpose(1, 2), _x(2, 2, 64, 7).transpose(2, 3)
+    at = torch.arange(7, device="cuda").expand(2, 7)
+    pages = _x(7, 2, 16, 64), _x(7, 2, 16, 64)
+    freqs = torch.arange(1, 33, device="cuda").half()
+    logits = _x(5, 96)[:, ::2]
+    monkeypatch.setattr(ops, "_fast", _Nothing())
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_copy, "copy", copied)
+    monkeypatch.setattr(rotary, "_copy", copied)
+    monkeypatch.setattr(_lib, "load", Checked)
+    mlx_amd.adapter_matmul(x, a.float(), b, _int([1, 0, -1], torch.int64), y=y, scale=torch.ones(3, device="cuda").half())
+    mlx_amd.adapter_matmul(x[..., ::2].transpose(0, 1), a[..., :48], b, _int([1, 0, 1, 2, 0]))
+    mlx_amd.rope(k, at.to(torch.uint32), freqs=freqs)
+    mlx_amd.rope_cache_update(q, k, k, *pages, _int([[4, 0], [1, 6]], torch.int64), _int([7, 3], torch.int64), freqs=freqs)
+    mlx_amd.route_experts(logits, 4, bias=_x(48))
+    leaves = [t.requires_grad_() for t in (x, a, b, q, logits)]
+    out = (mlx_amd.adapter_matmul(x, a, b, _int([1, 0, 2], torch.int64)), mlx_amd.rope(q, at),
+           mlx_amd.route_experts(logits, 4)[1])
+    torch.autograd.grad(sum(t.float().sum() for t in out), leaves)
