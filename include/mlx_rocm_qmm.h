@@ -986,9 +986,11 @@ int mlxrocm_route_experts_vjp(
  * with x [rows, K], y (or NULL: zeros) and out [rows, N], a [adapters, rank, K], b [adapters, N,
  * rank]; rows whose index is no adapter's keep y.  indices NULL: all rows have adapter 0
  * (n_indices 1).  scales: on the device, or NULL.  adapters: 1024 at most, rank 256.  h: NULL, or
- * where x a^T stays for the gradients (h_size bytes).
+ * where scale scales[i] x a[i]^T stays for the gradients (h_size bytes): floats [rows, rank up to a
+ * multiple of 16], zeros past the rank; rows without an adapter are not written.
  * mlxrocm_adapter_matmul_vjp: dx [rows, K] (zeros where there is no adapter), da and db as a and b
- * (zeros for adapters without rows); each may be NULL.  y's gradient is dout.
+ * (zeros for adapters without rows); each may be NULL.  h is that of the forward, with the same scale
+ * and scales (db takes it as it is; not read where db is NULL).  y's gradient is dout.
  */
 size_t mlxrocm_adapter_matmul_workspace_size(
     int64_t rows, int n_indices, int adapters, int rank, int K, int N, int dtype);

@@ -180,8 +180,8 @@ __device__ __forceinline__ void multiply(const uint4& a, const uint4& b, floatx4
 }
 
 // Elements k .. k + 15 / sizeof(T) of a row of n; what lies past its end is zero (kWhole: nothing
-// does).  Sixteen bytes at once also where they are not aligned (4110 tokens of 1024 values to 1001 by
-// rank 128, float16 with gradients: 194 us; element by element 353).
+// does).  Sixteen bytes at once also where they are not aligned, as in store_part (4110 tokens of 1024
+// values to 1001 by rank 128, float16 with gradients: 181 us; both element by element 338).
 template <typename T, bool kAligned, bool kWhole = false>
 __device__ __forceinline__ uint4 operand(const T* row, int k, int n) {
   union {
@@ -1221,7 +1221,8 @@ Plan plan_of(const Sizes& s, bool gradients) {
     const int64_t blocks = (s.K + kColumns - 1) / kColumns + (s.N + kColumns - 1) / kColumns;
     // 640 workgroups, by tokens: 8192 tokens of 4096 values to 14336 by rank 16 290 us (320: 320, 1024: 302),
     // 16384 of 8192 to 1024 by rank 32 292 (320: 306).  At least 64 tokens, as parts are written and read
-    // again: of rank 128 96 (4110 tokens of 1024 to 1001: 353, with 64 384, with 128 360).
+    // again; of rank 128 96 (64, 96, 128: 4110 tokens of 1024 to 1001, float16 204, 181, 185, to 1024 149,
+    // 143, 141; 1400 of 2048 to 2048 by rank 256 192, 184, 185; 2048 of 2048 to 512 111, 101, 104).
     const int64_t segment = s.T * blocks * p.rank_blocks / 640 / kTokens * kTokens;
     const int least = p.chunks == 8 ? 96 : 64;
     p.segment =

@@ -283,9 +283,12 @@ int launch(const char* tag, RopeArgs& a, hipStream_t stream) {
   const int v = columns_of(a, kCache ? 3 : 1, sizeof(T));
   a.items = Divisor(a.D / (2 * v));
   a.rotated = a.pairs / v;
-  // Two tokens a workgroup where there are four workgroups a CU of them (16 ragged prompts of up to
-  // 1531 tokens, 36 heads of 128: one 77 us, two 72, four 75, eight 83); else one token, and its
-  // heads are cut until there are two workgroups a CU or a thread has one item.
+  // Two tokens a workgroup where there are four workgroups a CU of them; else one token, and its
+  // heads are cut until there are two workgroups a CU or a thread has one item.  us with one, two, four
+  // (bfloat16): into the cache 16 ragged prompts of up to 1531 tokens, 36 heads of 128 77, 72, 75, as many
+  // of 1531 89, 88, 93, 8 of 2000, 10 heads of 256 30, 27, 28; alone 4 x 2500, 28 of 128 25, 24, 25, 12000,
+  // 12 of 96 16.3, 12.6, 12.8, 4096, 8 of 256 9.1, 8.9, 8.9, 11200, 32 of 64 18.2, 17.2, 15.8, 4096, 64 of 128
+  // 22.2, 22.6, 22.8.
   const int heads = a.ends[2];
   const int64_t tokens = static_cast<int64_t>(a.B) * a.L;
   a.tokens = tokens >= 4 * 512 ? 2 : 1;

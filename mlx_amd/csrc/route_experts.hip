@@ -9,15 +9,16 @@
 // they have the scores' order (no bias, no sums), else of choices in 64 bits.  Those are formed in 32
 // bits first; where all that are chosen, and the first that is not, are further apart than 32 bits can be
 // off, the order is known.  Where they are not, the few that can be meant are formed in 64 (sigmoids: a
-// lane each), and only where that does not tell either, the whole row is.
+// lane each), and only where that does not tell either, the whole row is: softmaxes, equal choices,
+// and choices of 2^21 and more, of which 32 bits say nothing.
 //
 // What bounds it: the instructions of k searches for the largest.  Sixteen lanes have a row, one of
 // the rows of lanes that DPP instructions rotate within: the largest of sixteen lanes is four
 // instructions, for four rows of a wavefront at once.  A lane holds neighbouring experts of one
 // group, so that the lowest lane that has the largest value has the lowest index.  16384 tokens, 8 of
-// 256 experts in 4 of 8 groups by sigmoid and bias in float32 (17.8 MB): 14.7 us, with every choice in 64
-// bits 25.7; 32749 tokens, 4 of 60 by logits in float16: 6.8 (0.7 of it reading), gradient 7.2; one token
-// 2.1, the launch.
+// 256 experts in 4 of 8 groups by sigmoid and bias in float32 (17.8 MB): 15 us, with every choice in 64
+// bits 25.7; 8 of 192 in 2 of 3 groups by their best two 13.6, by softmax 24; 32749 tokens, 4 of 60 by
+// logits in float16: 6.9 (0.7 of it reading), gradient 7.2; one token 2.1, the launch.
 #include <type_traits>
 
 #include "common.h"

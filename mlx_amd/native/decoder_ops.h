@@ -499,7 +499,7 @@ struct Adaption {
   const int32_t* index() const {
     return indices == nullptr ? nullptr : static_cast<const int32_t*>(indices->data_ptr());
   }
-  // y and h may be undefined; h is where x a^T stays
+  // y may be undefined; h is where scale x a^T stays
   bool run(
       const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& y,
       at::Tensor* out, at::Tensor* h) const {

@@ -158,6 +158,29 @@ def test_logits_and_gradients_far_apart(gpu):
             assert torch.equal(one, two)
 
 
+def test_a_cache_beyond_32_bits(gpu):
+    """Pages, queries, keys and values that lie far apart hold what near ones do."""
+    g = torch.Generator().manual_seed(4)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g).to(torch.bfloat16).cuda()
+
+    def far(t):
+        apart = 8 * (2 ** 28 // (t.shape[0] - 1) + 131)  # (pages are aligned)
+        buffer = torch.empty(apart * t.shape[0], dtype=t.dtype, device="cuda")
+        return buffer.as_strided(t.shape, (apart, *t.stride()[1:])).copy_(t)
+
+    q, k, v = normal(3, 4, 5, 64), normal(3, 2, 5, 64), normal(3, 2, 5, 64)
+    pages = normal(6, 2, 16, 64), normal(6, 2, 16, 64)
+    table = torch.tensor([[5, 0], [1, 4], [3, 2]], dtype=torch.int32).cuda()
+    lengths = torch.tensor([18, 30, 3], dtype=torch.int32).cuda()
+    other = [far(t) for t in (q, k, v, *pages)]
+    assert other[3].stride(0) * 5 > 2 ** 31
+    near = mlx_amd.rope_cache_update(q, k, v, *pages, table, lengths)
+    for one, two in zip(near, mlx_amd.rope_cache_update(*other, table, lengths)):
+        assert torch.equal(one, two)
+
+
 @pytest.mark.parametrize("L", (1, 40))
 def test_rows_of_adapters_far_apart(gpu, L):
     args, dout = case(5, L, 96, 80, 16, 3, torch.bfloat16, [0, 2, -1, 2, 1])
