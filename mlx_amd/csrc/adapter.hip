@@ -181,7 +181,7 @@ __device__ __forceinline__ void multiply(const uint4& a, const uint4& b, floatx4
 
 // Elements k .. k + 15 / sizeof(T) of a row of n; what lies past its end is zero (kWhole: nothing
 // does).  Sixteen bytes at once also where they are not aligned, as in store_part (4110 tokens of 1024
-// values to 1001 by rank 128, float16 with gradients: 181 us; both element by element 338).
+// values to 1001 by rank 128, float16 with gradients: 182 us; both element by element 339).
 template <typename T, bool kAligned, bool kWhole = false>
 __device__ __forceinline__ uint4 operand(const T* row, int k, int n) {
   union {
@@ -953,8 +953,7 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
         }
       }
     } else {
-      // In bfloat16, whose range is float32's: p as three numbers, a float16 q as two (exactly; what the
-      // third and the second give is 2^-24 of the product)
+      // In bfloat16, whose range is float32's: p as three numbers, a float16 q as two, both exactly
       uint4 q[4][std::is_same_v<T, bf16_t> ? 1 : 2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1004,9 +1003,7 @@ __global__ __launch_bounds__(256) void token_kernel(const TokenArgs a) {
             const uint4 p = uint4{w[k][0], w[k][1], w[k][2], w[k][3]};
             sum[j][c] = mfma16<bf16_t>(q[j][0], p, sum[j][c]);
             if constexpr (std::is_same_v<T, f16_t>) {
-              if (k < 2) {
-                sum[j][c] = mfma16<bf16_t>(q[j][1], p, sum[j][c]);
-              }
+              sum[j][c] = mfma16<bf16_t>(q[j][1], p, sum[j][c]);
             }
           }
         }
@@ -1221,8 +1218,8 @@ Plan plan_of(const Sizes& s, bool gradients) {
     const int64_t blocks = (s.K + kColumns - 1) / kColumns + (s.N + kColumns - 1) / kColumns;
     // 640 workgroups, by tokens: 8192 tokens of 4096 values to 14336 by rank 16 290 us (320: 320, 1024: 302),
     // 16384 of 8192 to 1024 by rank 32 292 (320: 306).  At least 64 tokens, as parts are written and read
-    // again; of rank 128 96 (64, 96, 128: 4110 tokens of 1024 to 1001, float16 204, 181, 185, to 1024 149,
-    // 143, 141; 1400 of 2048 to 2048 by rank 256 192, 184, 185; 2048 of 2048 to 512 111, 101, 104).
+    // again; of rank 128 96 (64, 96, 128: 4110 tokens of 1024 to 1001, float16 204, 182, 185, to 1024 149,
+    // 144, 141; 1400 of 2048 to 2048 by rank 256 192, 184, 185; 2048 of 2048 to 512 111, 101, 104).
     const int64_t segment = s.T * blocks * p.rank_blocks / 640 / kTokens * kTokens;
     const int least = p.chunks == 8 ? 96 : 64;
     p.segment =

@@ -1,5 +1,6 @@
 """Rotary positions: ``rope`` (``mx.fast.rope`` with positions of each token in place of an offset, along
-one or several axes), and ``rope_cache_update``, which rotates queries and keys on their way to ``paged_attention``.
+one or several axes), and ``rope_cache_update``, which rotates queries and keys on their way to
+``paged_attention``.
 
 Pair ``i`` of the first ``dims`` columns of a head turns by ``scale * position / freqs[i]``, where
 ``freqs[i]`` is ``base ** (2 * i / dims)`` unless ``freqs`` is given.  The pair is the columns ``i``
